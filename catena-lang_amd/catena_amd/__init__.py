@@ -101,6 +101,18 @@ class Value(ctypes.Structure):
         return self.as_.mem
 
 
+class PagedKV(ctypes.Structure):
+    """catena_paged_kv_t: a cache in pages (device pointers and sizes)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("num_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("rows", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
+
+    @property
+    def slots(self) -> int:
+        return self.max_pages * self.page_size
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
@@ -147,6 +159,10 @@ SIGNATURES = {
     "catena_mi355x_rope_table_f32": (_int, [_vp, _vp, _u32, _u32]),
     "catena_mi355x_gemm_bf16_rope_qkv": (_int, [_vp] * 7 + [_u32] * 4 + [_u64]),
     "catena_mi355x_gemm_bf16_ksplit_f32": (_int, [_vp, _vp, _vp, _u64, _u64, _u64, _u32]),
+    "catena_mi355x_attn_paged_plan": (_int, [ctypes.POINTER(PagedKV), _u32, _int,
+                                             ctypes.POINTER(_u32), ctypes.POINTER(_u64)]),
+    "catena_mi355x_attn_paged_bf16": (_int, [ctypes.POINTER(PagedKV), _vp, _vp, _vp, _u32, _f32, _int,
+                                             _vp, _vp, _vp, _u64]),
     "catena_mi355x_argmax_f32": (_int, [_vp, _vp, _u64, _u64]),
     "catena_mi355x_broadcast_f32": (_int, [_vp, _u64, _f32]),
     "catena_mi355x_arange_f32": (_int, [_vp, _u64]),
@@ -451,6 +467,34 @@ def gemm_bf16_rope_qkv(a, w, rope_tab, lens, q, k_cache, v_cache, batch: int, tq
 def gemm_bf16_ksplit_f32(a, b, parts, n: int, m: int, k: int, splits: int) -> None:
     """parts[z][n][m] = A[:, kz] x B[kz, :] over the z-th of `splits` equal k ranges."""
     check(lib().catena_mi355x_gemm_bf16_ksplit_f32(_p(a), _p(b), _p(parts), n, m, k, splits))
+
+
+def _opt(x):
+    return None if x is None else _p(x)
+
+
+def _workspace(w):
+    """(pointer, bytes) of a workspace: a Buffer, such a pair, or None."""
+    if w is None:
+        return None, 0
+    return (w.ptr, w.nbytes) if isinstance(w, Buffer) else w
+
+
+def attn_paged_plan(kv: PagedKV, heads: int, weights: bool = False):
+    """(most runs a row is cut into, workspace bytes) of attn_paged_bf16 for
+    these sizes; needs no device."""
+    splits, nbytes = _u32(), _u64()
+    check(lib().catena_mi355x_attn_paged_plan(kv, heads, 1 if weights else 0, splits, nbytes))
+    return splits.value, nbytes.value
+
+
+def attn_paged_bf16(kv: PagedKV, q, lens, o, heads: int, scale: float, workspace=None,
+                    out_f32: bool = False, acc_in=None, acc_out=None) -> None:
+    """One new token per row over a cache in pages; workspace is a Buffer or a
+    (pointer, bytes) pair of attn_paged_plan's size."""
+    check(lib().catena_mi355x_attn_paged_bf16(kv, _p(q), _p(lens), _p(o), heads, scale,
+                                              1 if out_f32 else 0, _opt(acc_in), _opt(acc_out),
+                                              *_workspace(workspace)))
 
 
 def argmax_f32(x, idx, rows: int, n: int) -> None:

@@ -112,6 +112,18 @@ const KernelSpec kKernels[] = {
     {KernelId::AttnPrefillD128Bf16, "attn_prefill", "catena_attn_prefill_bf16_d128_bf16out"},
     {KernelId::AttnPrefillW8D128F32, "attn_prefill", "catena_attn_prefill_w8_bf16_d128_f32out"},
     {KernelId::AttnPrefillW8D128Bf16, "attn_prefill", "catena_attn_prefill_w8_bf16_d128_bf16out"},
+    {KernelId::AttnPagedD128F32, "attn_paged", "catena_attn_paged_d128_f32out"},
+    {KernelId::AttnPagedD128Bf16, "attn_paged", "catena_attn_paged_d128_bf16out"},
+    {KernelId::AttnPagedD64F32, "attn_paged", "catena_attn_paged_d64_f32out"},
+    {KernelId::AttnPagedD64Bf16, "attn_paged", "catena_attn_paged_d64_bf16out"},
+    {KernelId::AttnPagedWeightsD128F32, "attn_paged", "catena_attn_paged_weights_d128_f32out"},
+    {KernelId::AttnPagedWeightsD128Bf16, "attn_paged", "catena_attn_paged_weights_d128_bf16out"},
+    {KernelId::AttnPagedWeightsD64F32, "attn_paged", "catena_attn_paged_weights_d64_f32out"},
+    {KernelId::AttnPagedWeightsD64Bf16, "attn_paged", "catena_attn_paged_weights_d64_bf16out"},
+    {KernelId::AttnPagedJoinD128F32, "attn_paged", "catena_attn_paged_join_d128_f32out"},
+    {KernelId::AttnPagedJoinD128Bf16, "attn_paged", "catena_attn_paged_join_d128_bf16out"},
+    {KernelId::AttnPagedJoinD64F32, "attn_paged", "catena_attn_paged_join_d64_f32out"},
+    {KernelId::AttnPagedJoinD64Bf16, "attn_paged", "catena_attn_paged_join_d64_bf16out"},
     {KernelId::EmbedRowsBf16, "block", "catena_embed_rows_bf16"},
     {KernelId::RmsnormRows, "block", "catena_rmsnorm_rows"},
     {KernelId::RmsnormRows4, "block", "catena_rmsnorm_rows4"},

@@ -74,6 +74,18 @@ enum class KernelId : int {
   AttnPrefillD128Bf16,
   AttnPrefillW8D128F32,  // eight waves a workgroup (attn_prefill.hip)
   AttnPrefillW8D128Bf16,
+  AttnPagedD128F32,  // one token a row over a cache in pages (attn_paged.hip); D64, bf16 and
+  AttnPagedD128Bf16,  // the forms with weights in this order
+  AttnPagedD64F32,
+  AttnPagedD64Bf16,
+  AttnPagedWeightsD128F32,
+  AttnPagedWeightsD128Bf16,
+  AttnPagedWeightsD64F32,
+  AttnPagedWeightsD64Bf16,
+  AttnPagedJoinD128F32,
+  AttnPagedJoinD128Bf16,
+  AttnPagedJoinD64F32,
+  AttnPagedJoinD64Bf16,
   EmbedRowsBf16,
   RmsnormRows,
   RmsnormRows4,  // four rows a workgroup

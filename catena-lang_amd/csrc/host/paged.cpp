@@ -1,0 +1,147 @@
+// Kernel ABI of the key-value cache in pages (attn_paged.hip).
+//
+// Arguments are checked before the device is looked for, so a refused call is
+// refused without one.
+#include <algorithm>
+#include <cstdint>
+
+#include "../kernels/paged.h"
+#include "internal.h"
+
+using namespace catena;
+
+namespace {
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+uint64_t round_up(uint64_t a, uint64_t to) { return ceil_div(a, to) * to; }
+
+// The cache's sizes (and with `pools` its pointers) checked, as the kernels
+// take them.
+int paged_check(const catena_paged_kv_t* kv, bool pools, PagedKv* out) {
+  if (!kv) return fail(CATENA_ERR_INVALID_ARGUMENT, "null cache");
+  const uint32_t ps = kv->page_size;
+  if (ps < 16 || ps > 1024 || (ps & (ps - 1)) != 0)
+    return fail(CATENA_ERR_UNSUPPORTED, "page_size %u is not a power of two from 16 to 1024", ps);
+  if (kv->head_dim != 64 && kv->head_dim != 128)
+    return fail(CATENA_ERR_UNSUPPORTED, "paged cache head_dim %u unsupported (64 or 128)", kv->head_dim);
+  if (kv->kv_heads == 0 || kv->num_pages == 0 || kv->max_pages == 0)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "paged cache of %u heads, %u pages, %u table entries a row",
+                kv->kv_heads, kv->num_pages, kv->max_pages);
+  if (kv->kv_heads > 65535 || (uint64_t)kv->max_pages * ps > 0x7FFFFFFFull)
+    return fail(CATENA_ERR_UNSUPPORTED, "paged cache too large");
+  // bytes of a pool, so that no offset passes 64 bits
+  if ((uint64_t)kv->num_pages * kv->kv_heads > (1ull << 44))
+    return fail(CATENA_ERR_UNSUPPORTED, "paged cache too large");
+  if (pools && kv->rows > 0) {
+    if (!kv->k || !kv->v || !kv->table) return fail(CATENA_ERR_INVALID_ARGUMENT, "null page pool or table");
+    if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || !aligned(kv->table, 4))
+      return fail(CATENA_ERR_INVALID_ARGUMENT, "page pools must be 16-byte aligned");
+  }
+  uint32_t shift = 0;
+  while ((1u << shift) < ps) ++shift;
+  *out = PagedKv{kv->k, kv->v, kv->table, kv->num_pages, shift, kv->rows, kv->max_pages, kv->kv_heads, kv->head_dim};
+  return CATENA_OK;
+}
+
+// struct AttnPagedArgs of attn_paged.hip, field for field
+struct AttnPagedArgs {
+  PagedKv kv;
+  const uint16_t* q;
+  const uint32_t* lens;
+  void* o;
+  float* part_o;
+  float* part_ml;
+  float* scores;
+  const float* acc_in;
+  float* acc_out;
+  uint32_t group, head_tiles, splits;
+  float scale_log2;
+};
+
+struct AttnPagedPlan {
+  uint32_t group, head_tiles, splits;
+  uint64_t part_ml, part_o, scores, bytes;  // offsets and the sum
+};
+
+int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPlan* p) {
+  if (heads == 0 || heads % kv.kv_heads != 0)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "%u query heads over %u kv heads", heads, kv.kv_heads);
+  p->group = heads / kv.kv_heads;
+  p->head_tiles = (uint32_t)ceil_div(p->group, 16);
+  const uint64_t slots = paged_slots(kv), pairs = (uint64_t)kv.rows * kv.kv_heads, units = pairs * p->head_tiles;
+  if (units > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows and heads");
+  // two workgroups a CU, of no fewer than 128 slots each
+  const uint64_t want = units ? ceil_div(512, units) : 1;
+  p->splits = (uint32_t)std::min<uint64_t>(want, ceil_div(slots, 128));
+  const uint64_t parts = pairs * p->splits * p->group;
+  p->part_ml = 0;
+  p->part_o = p->splits > 1 || weights ? round_up(parts * 8, 256) : 0;
+  p->scores = p->part_o + (p->splits > 1 ? parts * kv.head_dim * 4 : 0);
+  p->bytes = p->scores + (weights ? pairs * p->group * slots * 4 : 0);
+  return CATENA_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int catena_mi355x_attn_paged_plan(const catena_paged_kv_t* kv, uint32_t heads, int weights, uint32_t* splits,
+                                  uint64_t* workspace_bytes) {
+  if (!splits || !workspace_bytes) return fail(CATENA_ERR_INVALID_ARGUMENT, "null output");
+  PagedKv c;
+  AttnPagedPlan p;
+  int st = paged_check(kv, false, &c);
+  if (!st) st = attn_paged_plan(c, heads, weights != 0, &p);
+  if (st) return st;
+  *splits = p.splits;
+  *workspace_bytes = p.bytes;
+  return CATENA_OK;
+}
+
+int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t* kv, const uint16_t* q, const uint32_t* lens, void* o,
+                                  uint32_t heads, float scale, int out_f32, const float* acc_in, float* acc_out,
+                                  void* workspace, uint64_t workspace_bytes) {
+  AttnPagedArgs a{};
+  AttnPagedPlan p;
+  int st = paged_check(kv, true, &a.kv);
+  if (!st) st = attn_paged_plan(a.kv, heads, acc_out != nullptr, &p);
+  if (st) return st;
+  if ((acc_in != nullptr) != (acc_out != nullptr))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "accumulated weights need an input and an output");
+  if (a.kv.rows == 0) return CATENA_OK;
+  if (!q || !lens || !o) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
+  if (!aligned(q, 16) || !aligned(o, 16) || !aligned(lens, 4) || !aligned(acc_in, 4) || !aligned(acc_out, 4))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "paged attention needs 16-byte aligned q and o");
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned(workspace, 16)))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "paged attention needs %llu bytes of 16-byte aligned workspace",
+                (unsigned long long)p.bytes);
+  st = ensure_init();
+  if (st) return st;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  a.q = q;
+  a.lens = lens;
+  a.o = o;
+  a.part_ml = reinterpret_cast<float*>(ws + p.part_ml);
+  a.part_o = reinterpret_cast<float*>(ws + p.part_o);
+  a.scores = reinterpret_cast<float*>(ws + p.scores);
+  a.acc_in = acc_in;
+  a.acc_out = acc_out;
+  a.group = p.group;
+  a.head_tiles = p.head_tiles;
+  a.splits = p.splits;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  // kernels in the order of their ids: D128 f32, D128 bf16, D64 f32, D64 bf16
+  const int form = (a.kv.head_dim == 64 ? 2 : 0) + (out_f32 ? 0 : 1);
+  const uint64_t pairs = (uint64_t)a.kv.rows * a.kv.kv_heads;
+  const KernelId first = acc_out ? KernelId::AttnPagedWeightsD128F32 : KernelId::AttnPagedD128F32;
+  void* args[] = {&a};
+  st = launch(static_cast<KernelId>(static_cast<int>(first) + form), dim3((unsigned)(pairs * p.head_tiles), p.splits),
+              dim3(256), 0, args);
+  if (st || (p.splits == 1 && !acc_out)) return st;
+  uint32_t join_blocks = p.splits > 1 ? (uint32_t)ceil_div(p.group, 4) : 0;
+  const uint64_t blocks = join_blocks + (acc_out ? ceil_div(paged_slots(a.kv), 1024) : 0);
+  void* jargs[] = {&a, &join_blocks};
+  return launch(static_cast<KernelId>(static_cast<int>(KernelId::AttnPagedJoinD128F32) + form),
+                dim3((unsigned)pairs, (unsigned)blocks), dim3(256), 0, jargs);
+}
+
+}  // extern "C"

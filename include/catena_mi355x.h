@@ -308,6 +308,52 @@ int catena_mi355x_silu_mul_bf16(const float *gu, uint16_t *out, uint64_t rows, u
 int catena_mi355x_gemm_bf16_silu(const uint16_t *a, const uint16_t *b, uint16_t *act, uint64_t n,
                                  uint64_t m, uint64_t k);
 
+/* -- a key-value cache in pages -- */
+
+/* A cache whose slots live in pages: k / v [num_pages][kv_heads][page_size]
+ * [head_dim] bf16, table[rows][max_pages] (device u32): slot j of a row is
+ * place j % page_size of page table[row][j / page_size].  page_size is a power
+ * of two from 16 to 1024, head_dim 64 or 128, max_pages * page_size < 2^31;
+ * k and v are 16-byte aligned.  A page number >= num_pages names no page: its
+ * slots are read as absent and written nowhere.  The struct itself is read by
+ * the call and not kept.  No reference counterpart. */
+typedef struct catena_paged_kv {
+  uint16_t *k;
+  uint16_t *v;
+  const uint32_t *table;
+  uint32_t num_pages;
+  uint32_t page_size;
+  uint32_t rows;
+  uint32_t max_pages; /* table entries per row */
+  uint32_t kv_heads;
+  uint32_t head_dim;
+} catena_paged_kv_t;
+
+/* How catena_mi355x_attn_paged_bf16 cuts a row (into at most `splits` runs of
+ * slots) and the bytes of workspace that it takes (0: none).  A function of
+ * the sizes alone (k, v and table are not looked at); needs no device. */
+int catena_mi355x_attn_paged_plan(const catena_paged_kv_t *kv, uint32_t heads, int weights,
+                                  uint32_t *splits, uint64_t *workspace_bytes);
+
+/* Attention of one new token per row over a cache in pages: q[rows][heads]
+ * [head_dim] bf16, lens[rows] (device u32: slots in use, the new token's among
+ * them; a length past the table counts as the table's), o[rows][heads]
+ * [head_dim] f32 (out_f32 != 0) or bf16 RNE.  Query head h reads kv head
+ * h / (heads / kv_heads); o = sum_j p_j v_j, p = softmax(scale * q . k_j) with
+ * the exponential itself (not math.exp-approx), sums in f32.  A row of no slots
+ * gives 0.  What the cache holds past a row's slots is never used.
+ * acc_in / acc_out[rows][kv_heads][max_pages * page_size] f32 (both or
+ * neither, may be the same): acc_out[j] = acc_in[j] + the sum of p_j over the
+ * query heads of a kv head, for the slots in use; others are left as they are.
+ * The result depends on the sizes and the inputs alone, bit by bit.
+ * workspace: 16-byte aligned, as many bytes as the plan says, used until the
+ * call's work has run; calls that may overlap (two captured graphs) take one
+ * each.  q and o 16-byte aligned.  Allocates nothing; may be captured. */
+int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q,
+                                  const uint32_t *lens, void *o, uint32_t heads, float scale,
+                                  int out_f32, const float *acc_in, float *acc_out,
+                                  void *workspace, uint64_t workspace_bytes);
+
 /* tensor.argmax-f32 per row (catena-lang/stdlib/tensor.hex:204-227):
  * idx[r] = first index of the maximum with the reference's NaN behaviour;
  * n = 0 gives 0xFFFFFFFF (the reference asserts n != 0). */
