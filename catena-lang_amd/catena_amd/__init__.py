@@ -163,6 +163,14 @@ SIGNATURES = {
                                              ctypes.POINTER(_u32), ctypes.POINTER(_u64)]),
     "catena_mi355x_attn_paged_bf16": (_int, [ctypes.POINTER(PagedKV), _vp, _vp, _vp, _u32, _f32, _int,
                                              _vp, _vp, _vp, _u64]),
+    "catena_mi355x_rope_qkv_paged_bf16": (_int, [ctypes.POINTER(PagedKV), _vp, _vp, _u32, _vp, _vp, _vp,
+                                                 _u32, _u32, _vp, _vp]),
+    "catena_mi355x_kv_evict_paged_plan": (_int, [ctypes.POINTER(PagedKV), _u32, ctypes.POINTER(_u64)]),
+    "catena_mi355x_kv_evict_paged_bf16": (_int, [ctypes.POINTER(PagedKV)] + [_vp] * 7 + [_u32, _u32, _vp, _u64]),
+    "catena_mi355x_beam_reorder_paged_bf16": (_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(_vp), _u32]
+                                              + [_vp] * 6),
+    "catena_mi355x_beam_select_plan": (_int, [_u32, _u32, _u32, ctypes.POINTER(_u64)]),
+    "catena_mi355x_beam_select_f32": (_int, [_vp] * 7 + [_u32] * 4 + [_vp, _u64]),
     "catena_mi355x_argmax_f32": (_int, [_vp, _vp, _u64, _u64]),
     "catena_mi355x_broadcast_f32": (_int, [_vp, _u64, _f32]),
     "catena_mi355x_arange_f32": (_int, [_vp, _u64]),
@@ -494,6 +502,59 @@ def attn_paged_bf16(kv: PagedKV, q, lens, o, heads: int, scale: float, workspace
     (pointer, bytes) pair of attn_paged_plan's size."""
     check(lib().catena_mi355x_attn_paged_bf16(kv, _p(q), _p(lens), _p(o), heads, scale,
                                               1 if out_f32 else 0, _opt(acc_in), _opt(acc_out),
+                                              *_workspace(workspace)))
+
+
+def rope_qkv_paged_bf16(kv: PagedKV, qkv, rope_tab, table_positions: int, lens, seen, q, tq: int,
+                        heads: int, acc=None, slot_pos=None) -> None:
+    """RoPE of tq tokens a row and their append into pages; lens / seen count
+    slots / positions after the append (seen None: as lens)."""
+    check(lib().catena_mi355x_rope_qkv_paged_bf16(kv, _p(qkv), _p(rope_tab), table_positions, _p(lens),
+                                                  _opt(seen), _p(q), tq, heads, _opt(acc),
+                                                  _opt(slot_pos)))
+
+
+def kv_evict_paged_plan(kv: PagedKV, budget: int) -> int:
+    """Workspace bytes of kv_evict_paged_bf16; needs no device."""
+    nbytes = _u64()
+    check(lib().catena_mi355x_kv_evict_paged_plan(kv, budget, nbytes))
+    return nbytes.value
+
+
+def kv_evict_paged_bf16(kv: PagedKV, lens, seen, acc_in, slot_pos_in, lens_out, acc_out, slot_pos_out,
+                        budget: int, recent: int, workspace) -> None:
+    """Keeps `budget` slots per (row, kv head): the last `recent` positions,
+    then the largest accumulated weights."""
+    check(lib().catena_mi355x_kv_evict_paged_bf16(kv, _p(lens), _p(seen), _p(acc_in), _p(slot_pos_in),
+                                                  _p(lens_out), _p(acc_out), _p(slot_pos_out), budget,
+                                                  recent, *_workspace(workspace)))
+
+
+def beam_reorder_paged_bf16(kv: PagedKV, pools, lens, parents, spare, table_out, lens_out,
+                            spare_out) -> None:
+    """Row r goes on as row parents[r] was; pools: the K and V pools of every
+    layer under kv's table."""
+    arr = (_vp * len(pools))(*[_p(x) for x in pools])
+    check(lib().catena_mi355x_beam_reorder_paged_bf16(kv, arr, len(pools), _p(lens), _p(parents),
+                                                      _p(spare), _p(table_out), _p(lens_out),
+                                                      _p(spare_out)))
+
+
+BEAM_NO_EOS = 0xFFFFFFFF  # no token ends a beam
+
+
+def beam_select_plan(groups: int, beams: int, vocab: int) -> int:
+    """Workspace bytes of beam_select_f32; needs no device."""
+    nbytes = _u64()
+    check(lib().catena_mi355x_beam_select_plan(groups, beams, vocab, nbytes))
+    return nbytes.value
+
+
+def beam_select_f32(logits, scores, done, tokens, parents, scores_out, done_out, groups: int, beams: int,
+                    vocab: int, eos: int, workspace) -> None:
+    """The best `beams` continuations of every group over beams and vocabulary."""
+    check(lib().catena_mi355x_beam_select_f32(_p(logits), _p(scores), _opt(done), _p(tokens), _p(parents),
+                                              _p(scores_out), _opt(done_out), groups, beams, vocab, eos,
                                               *_workspace(workspace)))
 
 

@@ -124,6 +124,12 @@ const KernelSpec kKernels[] = {
     {KernelId::AttnPagedJoinD128Bf16, "attn_paged", "catena_attn_paged_join_d128_bf16out"},
     {KernelId::AttnPagedJoinD64F32, "attn_paged", "catena_attn_paged_join_d64_f32out"},
     {KernelId::AttnPagedJoinD64Bf16, "attn_paged", "catena_attn_paged_join_d64_bf16out"},
+    {KernelId::RopeQkvPaged, "kv_paged", "catena_rope_qkv_paged"},
+    {KernelId::KvEvictChoose, "kv_paged", "catena_kv_evict_choose"},
+    {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
+    {KernelId::KvReorder, "kv_paged", "catena_kv_reorder"},
+    {KernelId::BeamRuns, "beam", "catena_beam_runs"},
+    {KernelId::BeamJoin, "beam", "catena_beam_join"},
     {KernelId::EmbedRowsBf16, "block", "catena_embed_rows_bf16"},
     {KernelId::RmsnormRows, "block", "catena_rmsnorm_rows"},
     {KernelId::RmsnormRows4, "block", "catena_rmsnorm_rows4"},

@@ -86,6 +86,12 @@ enum class KernelId : int {
   AttnPagedJoinD128Bf16,
   AttnPagedJoinD64F32,
   AttnPagedJoinD64Bf16,
+  RopeQkvPaged,  // upkeep of a cache in pages (kv_paged.hip)
+  KvEvictChoose,
+  KvEvictMove,
+  KvReorder,
+  BeamRuns,  // beam search's selection (beam.hip)
+  BeamJoin,
   EmbedRowsBf16,
   RmsnormRows,
   RmsnormRows4,  // four rows a workgroup

@@ -1,4 +1,5 @@
-// Kernel ABI of the key-value cache in pages (attn_paged.hip).
+// Kernel ABI of the key-value cache in pages (attn_paged.hip,
+// kv_paged.hip).
 //
 // Arguments are checked before the device is looked for, so a refused call is
 // refused without one.
@@ -80,6 +81,27 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   p->bytes = p->scores + (weights ? pairs * p->group * slots * 4 : 0);
   return CATENA_OK;
 }
+
+constexpr uint32_t kEvictMoves = 64;  // a workgroup of catena_kv_evict_move
+// Most moves of a (row, kv head): slots below the budget, and slots from it on
+uint32_t evict_most(const PagedKv& kv, uint32_t budget) {
+  const uint32_t slots = paged_slots(kv);
+  return budget >= slots ? 0 : std::min(budget, slots - budget);
+}
+// count[pairs], holes[pairs][most], sources[pairs][most]
+int evict_plan(const PagedKv& kv, uint32_t budget, uint64_t* bytes) {
+  if (budget == 0) return fail(CATENA_ERR_INVALID_ARGUMENT, "a budget of no slots");
+  const uint64_t pairs = (uint64_t)kv.rows * kv.kv_heads;
+  if (pairs > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows and heads");
+  if (evict_most(kv, budget) > 65535 * kEvictMoves) return fail(CATENA_ERR_UNSUPPORTED, "eviction of too many slots");
+  *bytes = pairs * 4 * (1 + 2ull * evict_most(kv, budget));
+  return CATENA_OK;
+}
+
+// struct ReorderPools of kv_paged.hip
+struct ReorderPools {
+  uint16_t* p[128];
+};
 }  // namespace
 
 extern "C" {
@@ -142,6 +164,106 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t* kv, const uint16_t* q
   void* jargs[] = {&a, &join_blocks};
   return launch(static_cast<KernelId>(static_cast<int>(KernelId::AttnPagedJoinD128F32) + form),
                 dim3((unsigned)pairs, (unsigned)blocks), dim3(256), 0, jargs);
+}
+
+int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t* kv, const float* qkv, const float* rope_tab,
+                                      uint32_t table_positions, const uint32_t* lens, const uint32_t* seen,
+                                      uint16_t* q, uint32_t tq, uint32_t heads, float* acc, uint32_t* slot_pos) {
+  PagedKv c;
+  int st = paged_check(kv, true, &c);
+  if (st) return st;
+  if (heads == 0 || heads % c.kv_heads != 0)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "%u query heads over %u kv heads", heads, c.kv_heads);
+  if ((acc != nullptr) != (slot_pos != nullptr))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "a tracked cache has weights and positions");
+  const uint64_t tokens = (uint64_t)c.rows * tq;
+  if (tokens == 0) return CATENA_OK;
+  if (!qkv || !rope_tab || !lens || !q) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
+  if (table_positions == 0) return fail(CATENA_ERR_INVALID_ARGUMENT, "empty rotation table");
+  if (!aligned(qkv, 16) || !aligned(rope_tab, 16) || !aligned(q, 16) || !aligned(lens, 4) || !aligned(seen, 4) ||
+      !aligned(acc, 4) || !aligned(slot_pos, 4))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "paged append needs 16-byte aligned qkv, rope_tab and q");
+  const uint64_t blocks = ceil_div(((uint64_t)heads + 2ull * c.kv_heads) * (c.head_dim / 8), 256);
+  if (tokens > 0x7FFFFFFFull || blocks > 65535) return fail(CATENA_ERR_UNSUPPORTED, "paged append too large");
+  st = ensure_init();
+  if (st) return st;
+  void* args[] = {&c, &qkv, &rope_tab, &table_positions, &lens, &seen, &q, &tq, &heads, &acc, &slot_pos};
+  return launch(KernelId::RopeQkvPaged, dim3((unsigned)tokens, (unsigned)blocks), dim3(256), 0, args);
+}
+
+int catena_mi355x_kv_evict_paged_plan(const catena_paged_kv_t* kv, uint32_t budget, uint64_t* workspace_bytes) {
+  if (!workspace_bytes) return fail(CATENA_ERR_INVALID_ARGUMENT, "null output");
+  PagedKv c;
+  int st = paged_check(kv, false, &c);
+  if (!st) st = evict_plan(c, budget, workspace_bytes);
+  return st;
+}
+
+int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_t* lens, const uint32_t* seen,
+                                      const float* acc_in, const uint32_t* slot_pos_in, uint32_t* lens_out,
+                                      float* acc_out, uint32_t* slot_pos_out, uint32_t budget, uint32_t recent,
+                                      void* workspace, uint64_t workspace_bytes) {
+  PagedKv c;
+  uint64_t need = 0;
+  int st = paged_check(kv, true, &c);
+  if (!st) st = evict_plan(c, budget, &need);
+  if (st) return st;
+  if (c.rows == 0) return CATENA_OK;
+  if (!lens || !seen || !acc_in || !slot_pos_in || !lens_out || !acc_out || !slot_pos_out)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
+  const void* words[] = {lens, seen, acc_in, slot_pos_in, lens_out, acc_out, slot_pos_out};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(CATENA_ERR_INVALID_ARGUMENT, "misaligned operand");
+  if (lens_out == lens) return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction's new lengths may not replace the old");
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction needs %llu bytes of 16-byte aligned workspace",
+                (unsigned long long)need);
+  st = ensure_init();
+  if (st) return st;
+  const uint32_t pairs = c.rows * c.kv_heads;
+  uint32_t most = evict_most(c, budget);
+  uint32_t* count = static_cast<uint32_t*>(workspace);
+  uint32_t* holes = count + pairs;
+  uint32_t* sources = holes + (uint64_t)pairs * most;
+  void* args[] = {&c,       &lens,  &seen,  &acc_in,  &slot_pos_in, &lens_out, &acc_out,
+                  &slot_pos_out, &count, &holes, &sources, &most,        &budget,   &recent};
+  st = launch(KernelId::KvEvictChoose, dim3(pairs), dim3(1024), 0, args);
+  if (st || most == 0) return st;
+  void* margs[] = {&c, &acc_in, &slot_pos_in, &acc_out, &slot_pos_out, &count, &holes, &sources, &most};
+  return launch(KernelId::KvEvictMove, dim3(pairs, (unsigned)ceil_div(most, kEvictMoves)), dim3(256), 0, margs);
+}
+
+int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t* kv, uint16_t* const* pools, uint32_t n_pools,
+                                          const uint32_t* lens, const uint32_t* parents, const uint32_t* spare,
+                                          uint32_t* table_out, uint32_t* lens_out, uint32_t* spare_out) {
+  PagedKv c;
+  int st = paged_check(kv, false, &c);
+  if (st) return st;
+  if (c.rows == 0) return CATENA_OK;
+  if (!c.table || (n_pools > 0 && !pools) || !lens || !parents || !spare || !table_out || !lens_out || !spare_out)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
+  const void* words[] = {c.table, lens, parents, spare, table_out, lens_out, spare_out};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(CATENA_ERR_INVALID_ARGUMENT, "misaligned operand");
+  for (uint32_t i = 0; i < n_pools; ++i)
+    if (!pools[i] || !aligned(pools[i], 16))
+      return fail(CATENA_ERR_INVALID_ARGUMENT, "page pools must be 16-byte aligned");
+  if (table_out == c.table || lens_out == lens || spare_out == spare)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "reorder's outputs may not replace its inputs");
+  if (c.rows > 0x7FFFFFFFu) return fail(CATENA_ERR_UNSUPPORTED, "too many rows");
+  st = ensure_init();
+  if (st) return st;
+  // 128 pools a launch (their pointers are kernel arguments); the table once
+  for (uint32_t first = 0; first == 0 || first < n_pools; first += 128) {
+    uint32_t n = std::min(n_pools - first, 128u);
+    ReorderPools p{};
+    for (uint32_t i = 0; i < n; ++i) p.p[i] = pools[first + i];
+    uint32_t tables = first == 0;
+    void* args[] = {&c, &p, &n, &tables, &lens, &parents, &spare, &table_out, &lens_out, &spare_out};
+    st = launch(KernelId::KvReorder, dim3(c.rows, n ? c.kv_heads : 1, n ? n : 1), dim3(256), 0, args);
+    if (st) return st;
+  }
+  return CATENA_OK;
 }
 
 }  // extern "C"

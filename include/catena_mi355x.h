@@ -354,6 +354,98 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q
                                   int out_f32, const float *acc_in, float *acc_out,
                                   void *workspace, uint64_t workspace_bytes);
 
+/* RoPE + append into pages, catena_mi355x_rope_qkv_bf16's twin for a cache in
+ * pages and grouped heads: qkv[rows * tq][(heads + 2 kv_heads) * head_dim] f32
+ * (columns: q heads | k heads | v heads), rope_tab[table_positions]
+ * [head_dim / 2] (cos, sin) f32 (catena_mi355x_rope_table_f32's, or any).
+ * lens[rows] (device u32) counts a row's slots after the append: token t goes
+ * to slot lens[row] - tq + t.  seen[rows] counts its positions after the
+ * append, given-up ones among them: token t is at position seen[row] - tq + t;
+ * NULL: as lens.  Writes q[rows * tq][heads * head_dim] bf16 (rotated) and the
+ * bf16 rotated k and v into the slots.  acc and slot_pos ([rows][kv_heads]
+ * [max_pages * page_size] f32 and u32, both or neither): the new slots' weight
+ * 0 and their position.  A token whose slot lies outside the table or whose
+ * position outside rope_tab writes q (rotated by rope_tab's first position)
+ * and nothing else, one whose page does not exist q alone.  qkv, rope_tab and q
+ * 16-byte aligned.  No reference counterpart. */
+int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t *kv, const float *qkv,
+                                      const float *rope_tab, uint32_t table_positions,
+                                      const uint32_t *lens, const uint32_t *seen, uint16_t *q,
+                                      uint32_t tq, uint32_t heads, float *acc, uint32_t *slot_pos);
+
+/* Bytes of workspace that catena_mi355x_kv_evict_paged_bf16 takes (0: none).
+ * A function of the sizes alone; needs no device. */
+int catena_mi355x_kv_evict_paged_plan(const catena_paged_kv_t *kv, uint32_t budget,
+                                      uint64_t *workspace_bytes);
+
+/* Bounds a cache in pages: per (row, kv head), of the lens[row] slots in use
+ * min(lens[row], budget) are kept -- those of the last `recent` of the
+ * seen[row] positions, then those of the largest accumulated weight, the lower
+ * slot where two are equal, a NaN weight behind every number -- and become the
+ * first slots: the i-th slot given up below the budget takes K, V, weight and
+ * position of the i-th slot kept from the budget on; the others stay where
+ * they are.  (Attention does not depend on the order of slots; RoPE is applied
+ * before the append.)  lens_out[rows] is the new length.  acc_in / acc_out and
+ * slot_pos_in / slot_pos_out ([rows][kv_heads][max_pages * page_size]) are each
+ * two buffers or the same one; entries past the new length are left as they
+ * are.  lens_out is not lens.  The pages must be the row's own (a page that
+ * catena_mi355x_beam_reorder_paged_bf16 shares changes for all its rows).
+ * workspace as for catena_mi355x_attn_paged_bf16.  No reference counterpart. */
+int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t *kv, const uint32_t *lens,
+                                      const uint32_t *seen, const float *acc_in,
+                                      const uint32_t *slot_pos_in, uint32_t *lens_out,
+                                      float *acc_out, uint32_t *slot_pos_out, uint32_t budget,
+                                      uint32_t recent, void *workspace, uint64_t workspace_bytes);
+
+/* Row r of a cache in pages goes on as row parents[r] was (beam search): the
+ * pages that the parent has filled are shared, the partly filled one is copied
+ * into page spare[r].  kv gives the sizes and the table (k and v are not
+ * used); pools[n_pools] (host array of device pointers, 16-byte aligned) are
+ * the K and V pools of every layer, all under this table.  lens[rows],
+ * parents[rows] (row numbers), spare[rows] (device u32).  table_out[rows]
+ * [max_pages]: the parent's filled pages, then spare[r] where a page was
+ * copied, then r's own; lens_out[rows]; spare_out[rows]: r's own partly filled
+ * page where spare[r] took its place, else spare[r].  A row that is its own
+ * parent keeps its pages and copies nothing.  So rows that begin with
+ * max_pages pages and one spare page of their own need no allocator: filled
+ * pages are never written again, and the page that a row writes next is its
+ * own.  A row whose parent does not exist, has another length than the row, or
+ * one past the table comes out with length 0 and page numbers 0xFFFFFFFF.
+ * The outputs are not the inputs; spare pages are distinct and in no table.
+ * No reference counterpart. */
+int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t *kv, uint16_t *const *pools,
+                                          uint32_t n_pools, const uint32_t *lens,
+                                          const uint32_t *parents, const uint32_t *spare,
+                                          uint32_t *table_out, uint32_t *lens_out,
+                                          uint32_t *spare_out);
+
+/* Bytes of workspace that catena_mi355x_beam_select_f32 takes.  A function of
+ * the sizes alone; needs no device. */
+int catena_mi355x_beam_select_plan(uint32_t groups, uint32_t beams, uint32_t vocab,
+                                   uint64_t *workspace_bytes);
+
+/* Beam search's selection: of logits[groups][beams][vocab] f32 and scores
+ * [groups][beams] f32 (log probabilities so far) the `beams` largest
+ *   scores[w] + logits[w][v] - log sum_u exp(logits[w][u])
+ * over a group's beams w and tokens v, larger first; equal scores: the lower
+ * beam, then the larger logit, then the lower token.  done[groups][beams] u32
+ * (NULL: none): a beam that is not 0 there offers only token eos, at its own
+ * score.  Writes per place tokens, parents (rows: group * beams + w), scores_out
+ * (computed in f64, rounded to f32) and done_out (may be NULL): 1 where the
+ * parent was done or the token is eos.  eos 0xFFFFFFFF: no token ends a beam
+ * (done must then be NULL).  A continuation whose score is not finite is not
+ * offered; NaN or +inf among a beam's logits take all of them.  A place that
+ * nothing fills has its own row as parent, token 0, score -inf and done 0.
+ * For the first step after a prompt give all beams but a group's first the
+ * score -inf.  scores_out may be scores, done_out may be done.  1 <= beams <=
+ * 32, 1 <= vocab <= 2^26.  workspace as for catena_mi355x_attn_paged_bf16.  No
+ * reference counterpart (catena_mi355x_argmax_f32 is the greedy choice). */
+int catena_mi355x_beam_select_f32(const float *logits, const float *scores, const uint32_t *done,
+                                  uint32_t *tokens, uint32_t *parents, float *scores_out,
+                                  uint32_t *done_out, uint32_t groups, uint32_t beams,
+                                  uint32_t vocab, uint32_t eos, void *workspace,
+                                  uint64_t workspace_bytes);
+
 /* tensor.argmax-f32 per row (catena-lang/stdlib/tensor.hex:204-227):
  * idx[r] = first index of the maximum with the reference's NaN behaviour;
  * n = 0 gives 0xFFFFFFFF (the reference asserts n != 0). */

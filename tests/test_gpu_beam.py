@@ -1,0 +1,220 @@
+"""Beam search's selection against the formula in 64 bits.  Places are whole
+numbers: inputs are drawn until neighbouring scores differ by more than the
+calculation can be off, so that the order is the formula's."""
+import numpy as np
+import pytest
+
+import catena_amd as ca
+from gpu_util import captured, say
+from paged_util import U
+
+pytestmark = pytest.mark.gpu
+EOS = 2
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    say("init device 0")
+    ca.init(0)
+
+
+class Select:
+    def __init__(self, logits, scores, done, eos=EOS):
+        self.logits, self.scores, self.done, self.eos = logits, scores, done, eos
+        self.groups, self.beams, self.vocab = logits.shape
+        self.lb, self.sb = ca.Buffer.from_array(logits), ca.Buffer.from_array(scores)
+        self.db = None if done is None else ca.Buffer.from_array(done)
+        self.out = [ca.Buffer.from_array(np.full(scores.shape, 0xABABABAB, np.uint32)) for _ in range(4)]
+        self.work = ca.Buffer.from_array(np.full(ca.beam_select_plan(*logits.shape), 0xFF, np.uint8))
+
+    def __call__(self):
+        t, p, s, d = self.out
+        ca.beam_select_f32(self.lb, self.sb, self.db, t, p, s, d, self.groups, self.beams, self.vocab, self.eos, self.work)
+
+    def read(self):
+        t, p, s, d = self.out
+        shape = self.scores.shape
+        return t.read(np.uint32, shape), p.read(np.uint32, shape), s.read(np.float32, shape), d.read(np.uint32, shape)
+
+    def want(self):
+        """(tokens, parents, scores, done, smallest distance of a chosen score to
+        the next of another beam)."""
+        g, w, v = self.logits.shape
+        x = self.logits.astype(np.float64)
+        with np.errstate(all="ignore"):
+            top = x.max(-1, keepdims=True)
+            lse = top + np.log(np.exp(x - top).sum(-1, keepdims=True))
+            total = self.scores.astype(np.float64)[..., None] + (x - lse)
+            total[~np.isfinite(lse[..., 0])] = -np.inf
+        total[~np.isfinite(total)] = -np.inf
+        if self.done is not None:
+            over = self.done != 0
+            total[over] = -np.inf
+            total[over, self.eos] = np.where(np.isfinite(self.scores), self.scores, -np.inf)[over]
+        tokens, parents, done = (np.zeros((g, w), np.uint32) for _ in range(3))
+        scores = np.full((g, w), -np.inf)
+        near = np.inf
+        for i in range(g):
+            flat = total[i].reshape(-1)
+            few = np.argpartition(-flat, min(w + 1, flat.size - 1))[: w + 2] if flat.size > 4 * w else np.arange(flat.size)
+            # equal ones at the edge belong too
+            edge = np.sort(flat[few])[::-1][min(w, len(few)) - 1]
+            few = np.flatnonzero(flat >= edge) if np.isfinite(edge) else np.flatnonzero(np.isfinite(flat))
+            order = few[np.lexsort((few, -flat[few]))]
+            rest = flat[np.setdiff1d(np.argpartition(-flat, min(2 * w, flat.size - 1))[: 2 * w + 1], order[:w])]
+            chosen = flat[order[:w]]
+            beams = order[:w] // v
+            for a in range(len(chosen)):
+                others = np.concatenate([chosen[(np.arange(len(chosen)) != a) & (beams != beams[a])], rest])
+                gaps = np.abs(others[np.isfinite(others)] - chosen[a])
+                near = min(near, gaps[gaps > 0].min(initial=np.inf))
+            for j in range(w):
+                parents[i, j] = i * w + j
+                if j < len(order):
+                    b, t = divmod(int(order[j]), v)
+                    tokens[i, j], parents[i, j], scores[i, j] = t, i * w + b, flat[order[j]]
+                    done[i, j] = t == self.eos or (self.done is not None and self.done[i, b] != 0)
+        return tokens, parents, scores, done, near
+
+    def check(self, tied=False):
+        tokens, parents, scores, done, near = self.want()
+        if not tied:
+            assert near > 1e-6, near  # ten times what the log sum can be off
+        got = self.read()
+        assert np.array_equal(got[0], tokens)
+        assert np.array_equal(got[1], parents)
+        assert np.array_equal(got[3], done)
+        fine = np.isfinite(scores)
+        assert np.array_equal(np.isfinite(got[2]), fine) and np.all(got[2][~fine] == -np.inf)
+        # an exponential and a sum of 16 are off by 18 u at most, its log by as much; one rounding
+        assert np.all(np.abs(got[2][fine] - scores[fine]) <= 20 * U + U * np.abs(scores[fine]))
+
+
+def _draw(seed, groups, beams, vocab, done_share=0.2, scale=2.5, eos=EOS):
+    """Inputs whose order the calculation cannot miss."""
+    for trial in range(20):
+        rng = np.random.default_rng(1000 * seed + trial)
+        logits = (scale * rng.standard_normal((groups, beams, vocab))).astype(np.float32)
+        scores = (-4 - 8 * rng.random((groups, beams))).astype(np.float32)
+        done = (rng.random((groups, beams)) < done_share).astype(np.uint32) if eos != ca.BEAM_NO_EOS else None
+        case = Select(logits, scores, done, eos)
+        if case.want()[4] > 1e-6:
+            return case
+    raise AssertionError("no such inputs")
+
+
+@pytest.mark.parametrize("groups,beams,vocab", [
+    (1, 1, 1), (1, 4, 3), (2, 32, 40), (3, 4, 32000), (1, 8, 4096), (1, 8, 4097), (2, 5, 4095), (1, 32, 12289), (7, 3, 1000),
+    (1, 1, 300000), (2, 2, 64), (64, 2, 33), (1, 16, 50021),
+])
+def test_against_the_formula(groups, beams, vocab):
+    say(f"beam_select {groups} x {beams} x {vocab}")
+    case = _draw(beams + vocab, groups, beams, vocab, eos=min(EOS, vocab - 1))
+    case()
+    case.check()
+
+
+def test_no_end_token():
+    say("beam_select without an end token")
+    case = _draw(5, 2, 4, 5000, eos=ca.BEAM_NO_EOS)
+    case()
+    case.check()
+    assert not case.read()[3].any()
+
+
+def test_first_step():
+    """Every beam but the first at -inf: the first one's best tokens."""
+    say("beam_select first step")
+    case = _draw(6, 3, 6, 9000)
+    scores = np.full((3, 6), -np.inf, np.float32)
+    scores[:, 0] = 0
+    case = Select(case.logits, scores, np.zeros((3, 6), np.uint32))
+    case()
+    case.check()
+    assert np.all(case.read()[1] == 6 * np.arange(3)[:, None])
+
+
+@pytest.mark.parametrize("vocab", [50, 4096, 9001])
+def test_equal_logits(vocab):
+    """Whole rows of one value, more equal logits than the list holds, and few
+    values: the lower beam, then the lower token."""
+    say(f"beam_select equal logits {vocab}")
+    rng = np.random.default_rng(vocab)
+    logits = np.zeros((4, 5, vocab), np.float32)
+    logits[1] = rng.integers(0, 3, (5, vocab))
+    logits[2, :, ::2] = -0.0
+    logits[3] = np.where(rng.random((5, vocab)) < 0.5, 7.0, -3.0)
+    scores = np.zeros((4, 5), np.float32)
+    scores[3] = [-1, -1, -2, -1, -1]
+    # rows of groups 1 and 3 must not tie between beams by rounding alone
+    case = Select(logits[[0, 2]], scores[[0, 2]], None, ca.BEAM_NO_EOS)
+    case()
+    case.check(tied=True)
+    for i in (1, 3):
+        one = Select(np.repeat(logits[i:i + 1, :1], 5, 1), scores[i:i + 1], None, ca.BEAM_NO_EOS)  # equal sums too
+        one()
+        one.check(tied=True)
+
+
+def test_masked_and_odd_logits():
+    """-inf offers nothing; fewer offered than beams leave places empty; NaN, +inf
+    or -inf alone take a beam out; so does a score that is not finite."""
+    say("beam_select masked logits")
+    case = _draw(8, 8, 4, 6000, done_share=0)
+    x, s, d = case.logits.copy(), case.scores.copy(), case.done.copy()
+    x[0, :, 10:] = -np.inf               # ten tokens a beam are allowed
+    x[1] = -np.inf                       # none
+    x[2] = -np.inf
+    x[2, 1, 77], x[2, 3, 5000] = 1.0, -2.0  # two in all
+    x[3, 0, 4500] = np.nan
+    x[4, 2, 3] = np.inf
+    x[5, 0], x[5, 1, 5] = np.nan, -np.inf
+    s[6] = [np.nan, -np.inf, np.inf, -1]
+    d[7] = [1, 1, 0, 1]
+    s[7] = [-3, -np.inf, -90, np.nan]    # a done beam far ahead, two of no score
+    case = Select(x, s, d)
+    case()
+    case.check()
+    tokens, parents, scores, done = case.read()
+    assert np.array_equal(parents[1], 4 + np.arange(4)) and np.all(scores[1] == -np.inf) and not tokens[1].any()
+    assert np.sum(np.isfinite(scores[2])) == 2
+    assert tokens[7, 0] == EOS and done[7, 0] == 1 and scores[7, 0] == -3
+
+
+def test_every_beam_done():
+    say("beam_select all done")
+    case = _draw(9, 2, 4, 3000)
+    case = Select(case.logits, case.scores, np.full((2, 4), 7, np.uint32))
+    case()
+    case.check()
+    assert np.all(case.read()[3] == 1) and np.all(case.read()[0] == EOS)
+    assert np.array_equal(-np.sort(-case.scores, -1), case.read()[2])
+
+
+def test_in_place_and_replayed():
+    """scores_out = scores and done_out = done, step after step; and a graph that
+    is replayed on new logits."""
+    say("beam_select in place, graph")
+    first = _draw(10, 2, 4, 5000)
+    first.out[2], first.out[3] = first.sb, first.db
+    for seed in (11, 12):
+        first()
+        first.check()
+        _, _, s, d = first.read()
+        nxt = _draw(seed, 2, 4, 5000)
+        first.logits, first.scores, first.done = nxt.logits, s, d
+        first.lb.write(nxt.logits)
+    case = _draw(13, 2, 4, 5000)
+    replay = captured(case)
+    other = _draw(14, 1, 8, 2000)
+    for seed in (13, 15, 16):
+        nxt = _draw(seed, 2, 4, 5000)
+        case.logits, case.scores, case.done = nxt.logits, nxt.scores, nxt.done
+        for buf, value in ((case.lb, nxt.logits), (case.sb, nxt.scores), (case.db, nxt.done)):
+            buf.write(value)
+        for o in case.out:
+            o.write(np.full(o.nbytes, 0xEE, np.uint8))
+        replay()
+        other()
+        case.check()
+        other.check()

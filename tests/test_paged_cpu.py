@@ -96,3 +96,73 @@ def test_slot_to_address(tmp_path):
                     str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout
+
+
+def append(kv, qkv=P, tab=P, positions=64, lens=P, seen=None, q=P, tq=1, heads=8, acc=None, slot_pos=None):
+    ca.rope_qkv_paged_bf16(kv, qkv, tab, positions, lens, seen, q, tq, heads, acc, slot_pos)
+
+
+def evict(kv, lens=P, seen=P, acc=P, pos=P, lens_out=2 * P, acc_out=P, pos_out=P, budget=8, recent=2, work=(P, 1 << 40)):
+    ca.kv_evict_paged_bf16(kv, lens, seen, acc, pos, lens_out, acc_out, pos_out, budget, recent, work)
+
+
+def reorder(kv, pools=(P, P), lens=P, parents=P, spare=P, table_out=P, lens_out=2 * P, spare_out=2 * P):
+    ca.beam_reorder_paged_bf16(kv, list(pools), lens, parents, spare, table_out, lens_out, spare_out)
+
+
+@pytest.mark.parametrize("call", [append, evict, reorder])
+@pytest.mark.parametrize("status,over", BAD_GEOMETRY)
+def test_upkeep_refuses_a_bad_cache(call, status, over):
+    if call is reorder and ("k" in over or "v" in over):
+        return  # reads the sizes and the table alone
+    refused(status, call, geometry(**over))
+
+
+def test_append_refuses_bad_arguments():
+    kv = geometry()
+    for over in (dict(heads=0), dict(heads=6), dict(qkv=0), dict(tab=0), dict(lens=0), dict(q=0), dict(positions=0),
+                 dict(qkv=P + 4), dict(tab=P + 8), dict(q=P + 2), dict(lens=P + 2), dict(seen=P + 1), dict(acc=P),
+                 dict(slot_pos=P), dict(acc=P + 2, slot_pos=P), dict(acc=P, slot_pos=P + 2)):
+        refused(INVALID, append, kv, **over)
+    refused(UNSUPPORTED, append, geometry(rows=1 << 20), tq=1 << 12)
+
+
+def test_evict_refuses_bad_arguments():
+    kv = geometry()
+    need = ca.kv_evict_paged_plan(kv, 8)
+    assert need == 16 * 4 * (1 + 2 * 8)
+    for name in ("lens", "seen", "acc", "pos", "lens_out", "acc_out", "pos_out"):
+        refused(INVALID, evict, kv, **{name: 0})
+        refused(INVALID, evict, kv, **{name: P + 2})
+    for over in (dict(budget=0), dict(lens_out=P), dict(work=None), dict(work=(0, need)), dict(work=(P, need - 1)), dict(work=(P + 4, need))):
+        refused(INVALID, evict, kv, **over)
+    refused(INVALID, ca.kv_evict_paged_plan, kv, 0)
+    refused(UNSUPPORTED, ca.kv_evict_paged_plan, geometry(max_pages=1 << 24), 1 << 26)
+    # a budget of the whole table needs the counts alone
+    assert ca.kv_evict_paged_plan(kv, 1 << 20) == 16 * 4
+
+
+def test_reorder_refuses_bad_arguments():
+    kv = geometry()
+    for name in ("lens", "parents", "spare", "table_out", "lens_out", "spare_out"):
+        refused(INVALID, reorder, kv, **{name: 0})
+        refused(INVALID, reorder, kv, **{name: P + 1})
+    for over in (dict(pools=(P, 0)), dict(pools=(P, P + 8)), dict(table_out=1 << 22), dict(lens_out=P), dict(spare_out=P)):
+        refused(INVALID, reorder, kv, **over)
+
+
+def test_beam_selection_refuses_bad_arguments():
+    good = dict(logits=P, scores=P, done=P, tokens=P, parents=P, scores_out=P, done_out=P, groups=2, beams=4, vocab=100, eos=2,
+                workspace=(P, 1 << 30))
+    need = ca.beam_select_plan(2, 4, 100)
+    assert need >= 8 * (4 * 8 + 8 + 4)
+    for name in ("logits", "scores", "tokens", "parents", "scores_out"):
+        refused(INVALID, ca.beam_select_f32, **{**good, name: 0})
+    for name in ("logits", "scores", "done", "tokens", "parents", "scores_out", "done_out"):
+        refused(INVALID, ca.beam_select_f32, **{**good, name: P + 1})
+    for over in (dict(beams=0), dict(vocab=0), dict(eos=100), dict(eos=ca.BEAM_NO_EOS), dict(workspace=None),
+                 dict(workspace=(P, need - 1)), dict(workspace=(P + 8, need)), dict(workspace=(0, need))):
+        refused(INVALID, ca.beam_select_f32, **{**good, **over})
+    for over in (dict(beams=33), dict(vocab=(1 << 26) + 1), dict(groups=1 << 29)):
+        refused(UNSUPPORTED, ca.beam_select_f32, **{**good, **over})
+        refused(UNSUPPORTED, ca.beam_select_plan, *({**good, **over}[n] for n in ("groups", "beams", "vocab")))
