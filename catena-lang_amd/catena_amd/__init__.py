@@ -489,11 +489,11 @@ def _workspace(w):
 
 
 def attn_paged_plan(kv: PagedKV, heads: int, weights: bool = False):
-    """(most runs a row is cut into, workspace bytes) of attn_paged_bf16 for
-    these sizes; needs no device."""
-    splits, nbytes = _u32(), _u64()
-    check(lib().catena_mi355x_attn_paged_plan(kv, heads, 1 if weights else 0, splits, nbytes))
-    return splits.value, nbytes.value
+    """(parts that all rows' slots are cut into or 0, workspace bytes) of
+    attn_paged_bf16 for these sizes; needs no device."""
+    parts, nbytes = _u32(), _u64()
+    check(lib().catena_mi355x_attn_paged_plan(kv, heads, 1 if weights else 0, parts, nbytes))
+    return parts.value, nbytes.value
 
 
 def attn_paged_bf16(kv: PagedKV, q, lens, o, heads: int, scale: float, workspace=None,

@@ -74,8 +74,9 @@ enum class KernelId : int {
   AttnPrefillD128Bf16,
   AttnPrefillW8D128F32,  // eight waves a workgroup (attn_prefill.hip)
   AttnPrefillW8D128Bf16,
-  AttnPagedD128F32,  // one token a row over a cache in pages (attn_paged.hip); D64, bf16 and
-  AttnPagedD128Bf16,  // the forms with weights in this order
+  // one token a row over a cache in pages (attn_paged.hip)
+  AttnPagedD128F32,
+  AttnPagedD128Bf16,
   AttnPagedD64F32,
   AttnPagedD64Bf16,
   AttnPagedWeightsD128F32,

@@ -52,16 +52,17 @@ struct AttnPagedArgs {
   void* o;
   float* part_o;
   float* part_ml;
+  float* whole_ml;
   float* scores;
   const float* acc_in;
   float* acc_out;
-  uint32_t group, head_tiles, splits;
+  uint32_t group, head_tiles, blocks;
   float scale_log2;
 };
 
 struct AttnPagedPlan {
-  uint32_t group, head_tiles, splits;
-  uint64_t part_ml, part_o, scores, bytes;  // offsets and the sum
+  uint32_t group, head_tiles, blocks, pieces;
+  uint64_t part_ml, whole_ml, scores, bytes;  // offsets and the sum; part_o comes first
 };
 
 int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPlan* p) {
@@ -70,14 +71,27 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   p->group = heads / kv.kv_heads;
   p->head_tiles = (uint32_t)ceil_div(p->group, 16);
   const uint64_t slots = paged_slots(kv), pairs = (uint64_t)kv.rows * kv.kv_heads, units = pairs * p->head_tiles;
-  if (units > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows and heads");
-  // two workgroups a CU, of no fewer than 128 slots each
-  const uint64_t want = units ? ceil_div(512, units) : 1;
-  p->splits = (uint32_t)std::min<uint64_t>(want, ceil_div(slots, 128));
-  const uint64_t parts = pairs * p->splits * p->group;
-  p->part_ml = 0;
-  p->part_o = p->splits > 1 || weights ? round_up(parts * 8, 256) : 0;
-  p->scores = p->part_o + (p->splits > 1 ? parts * kv.head_dim * 4 : 0);
+  const uint64_t tiles = units * ceil_div(slots, 32);
+  if (units > 0x3FFFFFFFull || tiles > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows, heads and slots");
+  // A workgroup per unit while a row's slots take no longer than cutting them
+  // costs: half a row at one CU's 38 GB/s (rows of a batch are taken to be half
+  // full) against 5.5 us of a second kernel and 1/128 us a unit of short parts.
+  // Units x slots of 128, a unit each / cut: 16 x 640 8.9 / 8.9 us, x 1280 17.7 /
+  // 9.7; 64 x 1024 14.7 / 12.6; 512 x 512 17.9 / 28.4, x 1024 32.6 / 37.6, x 2048 57
+  // / 54, x 4096 119 / 90; 2048 x 640 57 / 102.  With weights only where a unit is
+  // all of its kv head, whose weights it then adds itself.
+  // Cut: two workgroups a CU, no fewer than four tiles each; one a CU once those
+  // are long (32768 tiles: 83.1 us against 85.3).
+  const uint64_t row_bytes = slots * kv.head_dim * 4;
+  if (row_bytes <= 418000 + 594 * units && !(weights && p->head_tiles > 1))
+    p->blocks = 0;
+  else
+    p->blocks = (uint32_t)std::min<uint64_t>(tiles >= 16384 ? 256 : 512, ceil_div(tiles, 4));
+  p->pieces = p->blocks > 16 * units ? 4 : 1;
+  const uint64_t parts = 2ull * p->blocks * std::min(p->group, 16u);
+  p->part_ml = parts * kv.head_dim * 4;
+  p->whole_ml = p->part_ml + parts * 8;
+  p->scores = round_up(p->whole_ml + (weights && p->blocks ? pairs * p->group * 8 : 0), 16);
   p->bytes = p->scores + (weights ? pairs * p->group * slots * 4 : 0);
   return CATENA_OK;
 }
@@ -106,15 +120,15 @@ struct ReorderPools {
 
 extern "C" {
 
-int catena_mi355x_attn_paged_plan(const catena_paged_kv_t* kv, uint32_t heads, int weights, uint32_t* splits,
+int catena_mi355x_attn_paged_plan(const catena_paged_kv_t* kv, uint32_t heads, int weights, uint32_t* parts,
                                   uint64_t* workspace_bytes) {
-  if (!splits || !workspace_bytes) return fail(CATENA_ERR_INVALID_ARGUMENT, "null output");
+  if (!parts || !workspace_bytes) return fail(CATENA_ERR_INVALID_ARGUMENT, "null output");
   PagedKv c;
   AttnPagedPlan p;
   int st = paged_check(kv, false, &c);
   if (!st) st = attn_paged_plan(c, heads, weights != 0, &p);
   if (st) return st;
-  *splits = p.splits;
+  *parts = p.blocks;
   *workspace_bytes = p.bytes;
   return CATENA_OK;
 }
@@ -142,26 +156,26 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t* kv, const uint16_t* q
   a.q = q;
   a.lens = lens;
   a.o = o;
+  a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float*>(ws + p.part_ml);
-  a.part_o = reinterpret_cast<float*>(ws + p.part_o);
+  a.whole_ml = reinterpret_cast<float*>(ws + p.whole_ml);
   a.scores = reinterpret_cast<float*>(ws + p.scores);
   a.acc_in = acc_in;
   a.acc_out = acc_out;
   a.group = p.group;
   a.head_tiles = p.head_tiles;
-  a.splits = p.splits;
+  a.blocks = p.blocks;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   // kernels in the order of their ids: D128 f32, D128 bf16, D64 f32, D64 bf16
   const int form = (a.kv.head_dim == 64 ? 2 : 0) + (out_f32 ? 0 : 1);
   const uint64_t pairs = (uint64_t)a.kv.rows * a.kv.kv_heads;
   const KernelId first = acc_out ? KernelId::AttnPagedWeightsD128F32 : KernelId::AttnPagedD128F32;
   void* args[] = {&a};
-  st = launch(static_cast<KernelId>(static_cast<int>(first) + form), dim3((unsigned)(pairs * p.head_tiles), p.splits),
-              dim3(256), 0, args);
-  if (st || (p.splits == 1 && !acc_out)) return st;
-  uint32_t join_blocks = p.splits > 1 ? (uint32_t)ceil_div(p.group, 4) : 0;
-  const uint64_t blocks = join_blocks + (acc_out ? ceil_div(paged_slots(a.kv), 1024) : 0);
-  void* jargs[] = {&a, &join_blocks};
+  st = launch(static_cast<KernelId>(static_cast<int>(first) + form), dim3(p.blocks ? p.blocks : (unsigned)(pairs * p.head_tiles)), dim3(256), 0, args);
+  if (st || p.blocks == 0) return st;
+  uint32_t pieces = p.pieces;
+  const uint64_t blocks = (uint64_t)p.group * pieces + (acc_out ? ceil_div(paged_slots(a.kv), 1024) : 0);
+  void* jargs[] = {&a, &pieces};
   return launch(static_cast<KernelId>(static_cast<int>(KernelId::AttnPagedJoinD128F32) + form),
                 dim3((unsigned)pairs, (unsigned)blocks), dim3(256), 0, jargs);
 }

@@ -8,9 +8,16 @@
 //
 // Bound: the cache is read once, 4 D bytes per (slot, kv head), against 4 D
 // flops per query head, so HBM.  One pass: the running maximum and sum of the
-// softmax beside the running o.  The slots of a row are cut into `splits` runs,
-// one workgroup each, and joined by a second kernel; a run's bounds follow from
-// the row's own length, so a short row of a long table is spread as wide.
+// softmax beside the running o.
+//
+// Work is dealt out in one of two ways.  A workgroup per unit ((row, kv head) and
+// up to 16 query heads) while rows are short; it needs no join.  One CU brings in
+// about 38 GB/s, so long rows are cut: all units' tiles form one line in the
+// order of rows, every workgroup takes an equal stretch of it (ends of units in
+// it and all), and a second kernel joins the units that were cut.  The stretches
+// follow from the rows' own lengths, so ragged batches are even: 64 rows of 1 ..
+// 4096 slots x 8 kv heads of 128 take 88 us (6.1 TB/s), against 112 with the
+// rows cut alike; 131072 slots x 8 heads in one row 80 us (6.7 TB/s).
 //
 // A wave takes 32 slots at a time (two runs of 16, each inside one page).
 // Products on the matrix cores with the cache as the A operand, straight from
@@ -43,21 +50,39 @@ namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// The slots [beg, end) of split s, in whole tiles of 32
-struct Run {
-  uint32_t beg, end;  // tiles
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then rows to rows
+CATENA_DEV uint32_t wave_prefix(uint32_t x) {
+#define CATENA_DPP_ADD(ctrl, rows) \
+  x = x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, (ctrl), (rows), 0xF, false)
+  CATENA_DPP_ADD(0x111, 0xF);
+  CATENA_DPP_ADD(0x112, 0xF);
+  CATENA_DPP_ADD(0x114, 0xF);
+  CATENA_DPP_ADD(0x118, 0xF);
+  CATENA_DPP_ADD(0x142, 0xA);
+  CATENA_DPP_ADD(0x143, 0xC);
+#undef CATENA_DPP_ADD
+  return x;
+}
+CATENA_DEV uint32_t lane_of(uint32_t x, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane); }
+
+// A uniform word that no workgroup of this kernel writes: by a scalar load, which
+// the compiler does not choose by itself behind the kernel's own stores, and
+// which leaves the order of the cache's vector loads alone
+CATENA_DEV uint32_t scalar_word(const uint32_t* p, uint32_t i) {
+  typedef const uint32_t __attribute__((address_space(4))) * word;
+  return ((word)(uintptr_t)p)[i];
+}
+
+// The work in one line: rows one after the other, a row's units (kv head and 16
+// query heads) one after the other, a unit's tiles of 32 slots in order.
+struct Line {
+  uint32_t tiles;  // in all
+  uint32_t per;    // a workgroup's
 };
-CATENA_DEV Run run_of(uint32_t len, uint32_t splits, uint32_t s) {
-  const uint32_t tiles = (len + 31) / 32;
-  const uint32_t per = ((tiles + splits - 1) / splits + 3) & ~3u;  // every wave of a run has as many
-  const uint32_t beg = s * per;
-  return Run{beg < tiles ? beg : tiles, beg + per < tiles ? beg + per : tiles};
-}
-CATENA_DEV uint32_t runs_of(uint32_t len, uint32_t splits) {
-  const uint32_t tiles = (len + 31) / 32;
-  const uint32_t per = ((tiles + splits - 1) / splits + 3) & ~3u;
-  return per == 0 ? 0 : (tiles + per - 1) / per;
-}
+// A row on it
+struct RowOnLine {
+  uint32_t row, len, tiles, first;  // tiles of one unit; place of the row's first
+};
 
 CATENA_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // the reference point of exponents: 0 while no score is above -inf
@@ -69,112 +94,218 @@ struct AttnPagedArgs {
   const uint16_t* q;      // [rows][heads][D]
   const uint32_t* lens;   // [rows]
   void* o;                // [rows][heads][D], written here where splits == 1
-  float* part_o;          // [rows][kv_heads][splits][group][D]
-  float* part_ml;         // [rows][kv_heads][splits][group][2]: maximum (base 2), sum
+  float* part_o;          // [blocks][2][min(group, 16)][D]
+  float* part_ml;         // [blocks][2][min(group, 16)][2]: maximum (base 2), sum
+  float* whole_ml;        // [rows][heads][2]: of units that one workgroup of the line had, with weights only
   float* scores;          // [rows][heads][slots] base-2 scores, with weights only
   const float* acc_in;    // [rows][kv_heads][slots]
   float* acc_out;
-  uint32_t group, head_tiles, splits;
+  uint32_t group, head_tiles;
+  uint32_t blocks;        // workgroups of the line; 0: one a unit
   float scale_log2;       // scale * log2(e)
 };
+
+CATENA_DEV uint32_t tiles_of(const AttnPagedArgs& a, uint32_t row) {
+  return row < a.kv.rows ? (paged_len(a.kv, a.lens[row]) + 31) / 32 : 0u;
+}
+// Lane r's row among the first 64, kept for the look-ups that follow
+struct FirstRows {
+  uint32_t n, upto;  // its tiles, and those of the rows up to it
+};
+CATENA_DEV FirstRows first_rows(const AttnPagedArgs& a) {
+  const uint32_t n = tiles_of(a, threadIdx.x & 63u);
+  return FirstRows{n, wave_prefix(n)};
+}
+CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
+  uint32_t all = lane_of(f.upto, 63);
+  if (a.kv.rows > 64) {
+    uint32_t n = 0;
+    for (uint32_t r = 64 + (threadIdx.x & 63u); r < a.kv.rows; r += 64) n += tiles_of(a, r);
+    all += lane_of(wave_prefix(n), 63);
+  }
+  all *= a.kv.kv_heads * a.head_tiles;
+  return Line{all, (all + a.blocks - 1) / a.blocks};
+}
+// The row that place `at` of the line (below its end) belongs to
+CATENA_DEV RowOnLine row_at_place(const AttnPagedArgs& a, const FirstRows& f, uint32_t at) {
+  const uint32_t lane = threadIdx.x & 63u, units = a.kv.kv_heads * a.head_tiles;
+  uint32_t n = f.n, upto = f.upto, r0 = 0;
+  uint64_t past = __ballot(upto * units > at);
+  while (!past && r0 + 64 < a.kv.rows) {
+    r0 += 64;
+    n = tiles_of(a, r0 + lane);
+    upto = lane_of(upto, 63) + wave_prefix(n);
+    past = __ballot(upto * units > at);
+  }
+  const uint32_t j = (uint32_t)__ffsll((unsigned long long)past) - 1, row = r0 + j, tiles = lane_of(n, j);
+  return RowOnLine{row, paged_len(a.kv, scalar_word(a.lens, row)), tiles, (lane_of(upto, j) - tiles) * units};
+}
+CATENA_DEV RowOnLine row_on_line(const AttnPagedArgs& a, const FirstRows& f, uint32_t row) {
+  const uint32_t len = paged_len(a.kv, scalar_word(a.lens, row)), tiles = (len + 31) / 32;
+  uint32_t before = lane_of(f.upto, row < 64 ? row : 63);
+  if (row >= 64) {
+    uint32_t n = 0;
+    for (uint32_t r = 64 + (threadIdx.x & 63u); r <= row; r += 64) n += tiles_of(a, r);
+    before += lane_of(wave_prefix(n), 63);
+  }
+  return RowOnLine{row, len, tiles, (before - tiles) * a.kv.kv_heads * a.head_tiles};
+}
+
+// p of heads h0 .. + hn - 1 (of 2^(score - base[h]) share[h]) summed over them, four
+// slots at a time from `slot` on, and added to the slots' weights
+CATENA_DEV void add_weights(const AttnPagedArgs& a, uint32_t row, uint32_t kvh, uint32_t h0, uint32_t hn, uint32_t len,
+                            uint32_t slot, uint32_t step, const float* base, const float* share) {
+  const uint32_t slots = paged_slots(a.kv);
+  const uint64_t pair = (uint64_t)row * a.kv.kv_heads + kvh;
+  const float* scores = a.scores + (pair * a.group + h0) * slots;
+  const float* in = (h0 ? a.acc_out : a.acc_in) + pair * slots;
+  float* out = a.acc_out + pair * slots;
+  for (; slot < len; slot += step) {  // slots come in whole pages of 16 or more
+    f32x4_t w = f32x4_t{0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t h = 0; h < hn; ++h) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(scores + (uint64_t)h * slots + slot);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = w[i] + exp2_fast(x[i] - base[h]) * share[h];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (slot + i < len) out[slot + i] = in[slot + i] + w[i];
+  }
+}
+
+// Two runs of 16 slots of a tile, as a wave holds them
+template <int D>
+struct Tile {
+  uint32_t n[2];            // slots that count
+  u32x4_t k[2][D / 32];     // slot c, d = 32 i + 8 g ..
+  uint32_t v[8][D / 32];    // slot 4 g + j % 4 of run j / 4, columns (D / 16) c ..
+};
+
+constexpr int kWaves = 4;
+
+// What a workgroup's waves hand over to each other; rows of o are padded, which
+// keeps the lanes of a 16-byte store off each other's banks
+template <int D>
+struct Shared {
+  float m[kWaves][16], l[kWaves][16];
+  __attribute__((aligned(16))) float o[kWaves][16][D + 4];
+  float base[16], share[16];
+};
+
+// A workgroup's part of a unit: tiles [beg, end) of query heads 16 ht .. + gn - 1 of
+// a (row, kv head)
+struct Part {
+  uint32_t row, len, tiles, kvh, ht, gn, beg, end;
+};
+CATENA_DEV Part part_from(const AttnPagedArgs& a, uint32_t row, uint32_t len, uint32_t unit, uint32_t beg,
+                          uint32_t most) {
+  Part p;
+  p.row = row;
+  p.len = len;
+  p.tiles = (len + 31) / 32;
+  p.kvh = unit / a.head_tiles;
+  p.ht = unit % a.head_tiles;
+  p.gn = a.group - 16 * p.ht < 16 ? a.group - 16 * p.ht : 16;
+  p.beg = beg;
+  p.end = p.tiles - beg < most ? p.tiles : beg + most;
+  return p;
+}
+// The part behind p, of at most `most` tiles; there is one
+CATENA_DEV Part part_behind(const AttnPagedArgs& a, const Part& p, uint32_t most) {
+  const uint32_t unit = p.kvh * a.head_tiles + p.ht + 1;
+  if (unit < a.kv.kv_heads * a.head_tiles) return part_from(a, p.row, p.len, unit, 0, most);
+  uint32_t row = p.row, len = 0;
+  while (len == 0 && ++row < a.kv.rows) len = paged_len(a.kv, scalar_word(a.lens, row));
+  return part_from(a, row, len, 0, 0, most);
+}
 
 template <int D, bool F32, bool WEIGHTS>
 CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
   constexpr int KC = D / 32;  // K loads of 8 values, products of S
   constexpr int VC = D / 16;  // columns of V a lane takes
+  constexpr int kNonTemporal = 2;
+  __shared__ Shared<D> sh;
   const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t unit = blockIdx.x, split = blockIdx.y;
-  const uint32_t ht = unit % a.head_tiles, pair = unit / a.head_tiles;  // pair: (row, kv head)
-  const uint32_t row = pair / a.kv.kv_heads, kvh = pair % a.kv.kv_heads;
-  const uint32_t heads = a.group * a.kv.kv_heads;
-  const uint32_t gn = a.group - 16 * ht < 16 ? a.group - 16 * ht : 16;
-  const uint32_t slots = paged_slots(a.kv);
-  const uint32_t len = paged_len(a.kv, a.lens[row]);
-  const Run run = run_of(len, a.splits, split);
-  if (a.splits > 1 && run.beg >= run.end) return;  // the join knows how many runs a length has
-
-  // Q as the B operand: lane = head c, 8 values of each 32-wide block of d
-  bf16x8_t qf[KC];
-  {
-    const uint16_t* q = a.q + ((uint64_t)row * heads + kvh * a.group + 16 * ht + (c < gn ? c : 0)) * D;
-#pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + 32 * i + 8 * g);
-      if (c >= gn) w = u32x4_t{0, 0, 0, 0};
-      qf[i] = __builtin_bit_cast(bf16x8_t, w);
-    }
-  }
-
-  float m = kNegInf, l = 0.0f;
-  f32x4_t acc[VC];
-#pragma unroll
-  for (int e = 0; e < VC; ++e) acc[e] = f32x4_t{0, 0, 0, 0};
-
-  const uint32_t* table = a.kv.table + (uint64_t)row * a.kv.max_pages;
+  const uint32_t heads = a.group * a.kv.kv_heads, slots = paged_slots(a.kv);
+  const uint32_t part_heads = a.group < 16 ? a.group : 16;
   const uint32_t mask = (1u << a.kv.page_shift) - 1u;
-  for (uint32_t t = run.beg + wave; t < run.end; t += 4) {
-    // two runs of 16 slots: where they live and how many count
-    uint64_t at[2];
-    uint32_t n[2];
+  const int koff = (int)(c * D + 8 * g) * 2, voff = (int)(4 * g * D + VC * c) * 2;
+
+  // The rows of a tile, through descriptors that end with those that count:
+  // what lies behind the row's end (it may be anything), or in a page that is
+  // not there, is not read and comes as 0.
+  auto request = [&](Tile<D>& x, const Part& p, uint32_t t) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t slot = 32 * t + 16 * u;
-      uint32_t page = slot < len ? table[slot >> a.kv.page_shift] : 0u;
-      const bool here = slot < len && page < a.kv.num_pages;
-      n[u] = !here ? 0u : len - slot < 16 ? len - slot : 16u;
-      if (!here) page = 0;  // read and left out
-      at[u] = paged_offset(a.kv, page, kvh, slot & mask);
-    }
-    // K and V of the tile
-    u32x4_t kr[2][KC];
+      const bool in = t < p.end && slot < p.len;
+      const uint32_t page =
+          in ? scalar_word(a.kv.table + (uint64_t)p.row * a.kv.max_pages, slot >> a.kv.page_shift) : 0xFFFFFFFFu;
+      const bool here = page < a.kv.num_pages;
+      x.n[u] = !here ? 0u : p.len - slot < 16 ? p.len - slot : 16u;
+      const uint64_t at = here ? paged_offset(a.kv, page, p.kvh, slot & mask) : 0ull;
+      const int bytes = (int)(x.n[u] * D * 2);
+      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kv.k + at), (short)0, bytes, 0x00020000);
+      const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kv.v + at), (short)0, bytes, 0x00020000);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int i = 0; i < KC; ++i) x.k[u][i] = __builtin_amdgcn_raw_buffer_load_b128(kr, koff, 64 * i, kNonTemporal);
 #pragma unroll
-      for (int i = 0; i < KC; ++i)
-        kr[u][i] = *reinterpret_cast<const u32x4_t*>(a.kv.k + at[u] + c * D + 32 * i + 8 * g);
-    uint32_t vr[8][VC / 2];  // slot (j < 4: 4 g + j of the first run, else of the second), columns VC c ..
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (VC == 8) {
+          const u32x4_t w = __builtin_amdgcn_raw_buffer_load_b128(vr, voff, j * D * 2, kNonTemporal);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t* p = a.kv.v + at[j / 4] + (4 * g + j % 4) * D + VC * c;
-      if constexpr (VC == 8) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) vr[j][x] = w[x];
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        vr[j][0] = w.x;
-        vr[j][1] = w.y;
+          for (int y = 0; y < 4; ++y) x.v[4 * u + j][y] = w[y];
+        } else {
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, voff, j * D * 2, kNonTemporal);
+          x.v[4 * u + j][0] = w[0];
+          x.v[4 * u + j][1] = w[1];
+        }
       }
     }
+  };
+  bf16x8_t qf[KC];
+  float m, l;
+  f32x4_t acc[VC];
+  auto begin = [&](const Part& p) {
+    // Q as the B operand: lane = head c, 8 values of each 32-wide block of d
+    const uint16_t* q = a.q + ((uint64_t)p.row * heads + p.kvh * a.group + 16 * p.ht + (c < p.gn ? c : 0)) * D;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + 32 * i + 8 * g);
+      if (c >= p.gn) w = u32x4_t{0, 0, 0, 0};
+      qf[i] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    m = kNegInf;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VC; ++e) acc[e] = f32x4_t{0, 0, 0, 0};
+  };
+
+  auto take = [&](Tile<D>& x, const Part& w, uint32_t t) {
     // scores in base 2: s[j] is slot (g, j) of head c
     float s[8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      f32x4_t x = f32x4_t{0, 0, 0, 0};
+      f32x4_t y = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KC; ++i)
-        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kr[u][i]), qf[i], x, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[u][i]), qf[i], y, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[4 * u + j] = x[j] * a.scale_log2;
+      for (int j = 0; j < 4; ++j) s[4 * u + j] = y[j] * a.scale_log2;
     }
-    if (n[0] < 16 || n[1] < 16) {
-      // what the tile holds past the row's end (or of a page that is not there)
-      // may be anything: no score, and zeros in V's place
+    if (x.n[0] < 16 || x.n[1] < 16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = 4 * g + j % 4 < n[j / 4];
-        s[j] = in ? s[j] : kNegInf;
-#pragma unroll
-        for (int x = 0; x < VC / 2; ++x) vr[j][x] = in ? vr[j][x] : 0u;
-      }
+      for (int j = 0; j < 8; ++j) s[j] = 4 * g + j % 4 < x.n[j / 4] ? s[j] : kNegInf;
     }
     if constexpr (WEIGHTS) {
-      if (c < gn) {
-        float* dst = a.scores + ((uint64_t)row * heads + kvh * a.group + 16 * ht + c) * slots + 32 * t + 4 * g;
+      if (c < w.gn && t < w.end) {  // an empty tile's slots are another part's
+        float* dst = a.scores + ((uint64_t)w.row * heads + w.kvh * a.group + 16 * w.ht + c) * slots + 32 * t + 4 * g;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (32 * t + 16 * u < len)
+          if (32 * t + 16 * u < w.len)
             *reinterpret_cast<f32x4_t*>(dst + 16 * u) = f32x4_t{s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]};
       }
     }
@@ -204,20 +335,20 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     constexpr int TERMS = F32 ? 3 : 2;
     bf16x8_t pt[TERMS];
 #pragma unroll
-    for (int x = 0; x < TERMS; ++x) {
-      u32x4_t w;
+    for (int y = 0; y < TERMS; ++y) {
+      u32x4_t word;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (x + 1 < TERMS) {
+        if (y + 1 < TERMS) {
           const uint32_t b0 = __float_as_uint(p[2 * j]), b1 = __float_as_uint(p[2 * j + 1]);
-          w[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+          word[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
           p[2 * j] = __builtin_fmaxf(p[2 * j] - __uint_as_float(b0 & 0xFFFF0000u), 0x1p-126f);
           p[2 * j + 1] = __builtin_fmaxf(p[2 * j + 1] - __uint_as_float(b1 & 0xFFFF0000u), 0x1p-126f);
         } else {
-          w[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
+          word[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
         }
       }
-      pt[x] = __builtin_bit_cast(bf16x8_t, w);
+      pt[y] = __builtin_bit_cast(bf16x8_t, word);
     }
 #pragma unroll
     for (int e = 0; e < VC; ++e) {
@@ -225,158 +356,268 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
       u32x4_t col;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        col[j] = __builtin_amdgcn_perm(vr[2 * j + 1][e / 2], vr[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        col[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][e / 2], x.v[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
       const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, col);
 #pragma unroll
-      for (int x = 0; x < TERMS; ++x)
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pt[x], acc[e], 0, 0, 0);
+      for (int y = 0; y < TERMS; ++y)
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pt[y], acc[e], 0, 0, 0);
     }
-  }
+  };
 
-  // The four waves' (m, l, o) to one
-  l = l + __shfl_xor(l, 16);
-  l = l + __shfl_xor(l, 32);
-  constexpr int OS = D + 4;  // keeps the lanes of a 16-byte store off each other's banks
-  __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ __attribute__((aligned(16))) float s_o[4][16][OS];
-  if (g == 0) {
-    s_m[wave][c] = m;
-    s_l[wave][c] = l;
-  }
-  if (c < gn) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < VC; e += 4)
-        *reinterpret_cast<f32x4_t*>(&s_o[wave][c][4 * VC * g + VC * i + e]) =
-            f32x4_t{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
-  }
-  __syncthreads();
-  for (uint32_t id = threadIdx.x; id < gn * (D / 4); id += 256) {
-    const uint32_t h = id / (D / 4), d = id % (D / 4) * 4;
-    float mm = kNegInf;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = __builtin_fmaxf(mm, s_m[w][h]);
-    float ll = 0.0f;
-    f32x4_t o = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2_fast(s_m[w][h] - anchor(mm));
-      ll = ll + s_l[w][h] * f;
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(&s_o[w][h][d]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] + x[i] * f;
+  auto finish = [&](const Part& p) {
+    // The waves' (m, l, o) to one
+    l = l + __shfl_xor(l, 16);
+    l = l + __shfl_xor(l, 32);
+    __syncthreads();  // the last unit's values have been read
+    if (g == 0) {
+      sh.m[wave][c] = m;
+      sh.l[wave][c] = l;
     }
-    const uint32_t head = 16 * ht + h;
-    if (a.splits > 1 || WEIGHTS) {
-      const uint64_t at = ((uint64_t)pair * a.splits + split) * a.group + head;
-      if (d == 0) {
-        a.part_ml[2 * at] = mm;
-        a.part_ml[2 * at + 1] = ll;
+    if (c < p.gn) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VC; e += 4)
+          *reinterpret_cast<f32x4_t*>(&sh.o[wave][c][4 * VC * g + VC * i + e]) =
+              f32x4_t{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
+    }
+    __syncthreads();
+    for (uint32_t id = threadIdx.x; id < p.gn * (D / 4); id += 64 * kWaves) {
+      const uint32_t h = id / (D / 4), d = id % (D / 4) * 4;
+      float mm = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh.m[w][h]);
+      float ll = 0.0f;
+      f32x4_t o = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = exp2_fast(sh.m[w][h] - anchor(mm));
+        ll = ll + sh.l[w][h] * f;
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(&sh.o[w][h][d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = o[i] + x[i] * f;
       }
-      if (a.splits > 1) {
+      const uint32_t head = p.kvh * a.group + 16 * p.ht + h;
+      if (p.beg != 0 || p.end != p.tiles) {
+        // the first part of a unit in the workgroup's second place, else the first
+        const uint64_t at = ((uint64_t)blockIdx.x * 2 + (p.beg == 0)) * part_heads + h;
+        if (d == 0) {
+          a.part_ml[2 * at] = mm;
+          a.part_ml[2 * at + 1] = ll;
+        }
         *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = o;
         continue;
       }
-    }
-    const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + d;
+      const uint64_t to = (uint64_t)p.row * heads + head, at = to * D + d;
+      if constexpr (WEIGHTS) {
+        if (d == 0 && a.blocks != 0) {
+          a.whole_ml[2 * to] = mm;
+          a.whole_ml[2 * to + 1] = ll;
+        }
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = len ? o[i] / ll : 0.0f;
-    if constexpr (F32) {
-      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + at) = o;
-    } else {
-      uint2 w;
-      w.x = pack_bf16x2(o[0], o[1]);
-      w.y = pack_bf16x2(o[2], o[3]);
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w;
+      for (int i = 0; i < 4; ++i) o[i] = p.len ? o[i] / ll : 0.0f;
+      if constexpr (F32) {
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + at) = o;
+      } else {
+        uint2 w;
+        w.x = pack_bf16x2(o[0], o[1]);
+        w.y = pack_bf16x2(o[2], o[3]);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w;
+      }
     }
+  };
+
+  uint32_t at = 0, last = 0;  // what is left of the line behind `now`
+  Part now;
+  if (a.blocks == 0) {
+    const uint32_t units = a.kv.kv_heads * a.head_tiles, row = blockIdx.x / units;
+    now = part_from(a, row, paged_len(a.kv, scalar_word(a.lens, row)), blockIdx.x % units, 0, 0xFFFFFFFFu);
+  } else {
+    const FirstRows rows = first_rows(a);
+    const Line line = line_of(a, rows);
+    at = blockIdx.x * line.per;
+    if (at >= line.tiles) return;
+    last = line.tiles - at < line.per ? line.tiles : at + line.per;
+    const RowOnLine r = row_at_place(a, rows, at);
+    now = part_from(a, r.row, r.len, (at - r.first) / r.tiles, (at - r.first) % r.tiles, last - at);
+    at += now.end - now.beg;
+  }
+
+  // The workgroup's parts one after the other, a wave's tiles of each kWaves
+  // apart (one without any takes an empty one).  A tile's rows are requested
+  // while the tile before it is worked on, across the border of two parts too.
+  uint32_t t = now.beg + wave;
+  Tile<D> one, two;
+  request(one, now, t);
+  begin(now);
+  auto step = [&](Tile<D>& x, Tile<D>& y) {
+    const bool ends = t + kWaves >= now.end, more = at < last;
+    Part next = now;
+    uint32_t tn = t + kWaves;  // past the end where nothing is left
+    if (ends && more) {
+      next = part_behind(a, now, last - at);
+      at += next.end - next.beg;
+      tn = next.beg + wave;
+    }
+    request(y, next, tn);
+    __builtin_amdgcn_sched_barrier(0);
+    take(x, now, t);
+    __builtin_amdgcn_sched_barrier(0);
+    if (ends) {
+      finish(now);
+      if (!more) return false;
+      begin(next);
+    }
+    now = next;
+    t = tn;
+    return true;
+  };
+  while (step(one, two) && step(two, one)) {
+  }
+
+  if constexpr (WEIGHTS) {
+    // a whole unit's weights, where it is its kv head's only one: the scores are
+    // this workgroup's own, behind the barriers of finish()
+    if (a.blocks != 0) return;
+    if (threadIdx.x < now.gn) {
+      float mm = kNegInf, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh.m[w][threadIdx.x]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) ll = ll + sh.l[w][threadIdx.x] * exp2_fast(sh.m[w][threadIdx.x] - anchor(mm));
+      sh.base[threadIdx.x] = anchor(mm);
+      sh.share[threadIdx.x] = 1.0f / ll;
+    }
+    __syncthreads();
+    add_weights(a, now.row, now.kvh, 0, now.gn, now.len, 4 * threadIdx.x, 1024, sh.base, sh.share);
   }
 }
 
-// Joins the runs of a row and adds the weights.  grid.x = (row, kv head);
-// blockIdx.y < join_blocks: four query heads' o, else 1024 slots' weights.
+// Where the parts of a unit are: the workgroups that have one are numbered on
+struct Parts {
+  uint32_t first, n;  // n < 2: one workgroup had the unit
+};
+CATENA_DEV Parts parts_of(const Line& line, const RowOnLine& r, uint32_t unit) {
+  if (r.tiles == 0) return Parts{0, 0};
+  const uint32_t beg = r.first + unit * r.tiles, first = beg / line.per;
+  return Parts{first, (beg + r.tiles - 1) / line.per - first + 1};
+}
+
+// Joins the parts of units, writes 0 for rows without slots, and adds the
+// weights.  grid.x = (row, kv head); blockIdx.y < group * pieces: D / pieces
+// columns of one query head's o, several parts at a time; else 1024 slots'
+// weights.
 template <int D, bool F32>
-CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t join_blocks) {
+CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
   const uint32_t pair = blockIdx.x, row = pair / a.kv.kv_heads, kvh = pair % a.kv.kv_heads;
-  const uint32_t len = paged_len(a.kv, a.lens[row]);
-  const uint32_t runs = runs_of(len, a.splits);
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t heads = a.group * a.kv.kv_heads, slots = paged_slots(a.kv);
-  const float* ml = a.part_ml + 2 * (uint64_t)pair * a.splits * a.group;
-  if (blockIdx.y < join_blocks) {
-    const uint32_t head = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63u;
-    if (head >= a.group) return;
-    const float* po = a.part_o + ((uint64_t)pair * a.splits * a.group + head) * D;
-    constexpr int PER = D / 64;
-    float mm = kNegInf;
-    for (uint32_t s = 0; s < runs; ++s) mm = __builtin_fmaxf(mm, ml[2 * ((uint64_t)s * a.group + head)]);
-    float ll = 0.0f, o[PER] = {};
-    for (uint32_t s = 0; s < runs; ++s) {
-      const uint64_t at = (uint64_t)s * a.group + head;
-      const float f = exp2_fast(ml[2 * at] - anchor(mm));
-      ll = ll + ml[2 * at + 1] * f;
+  const uint32_t part_heads = a.group < 16 ? a.group : 16;
+  const FirstRows rows = first_rows(a);
+  const Line line = line_of(a, rows);
+  const RowOnLine r = row_on_line(a, rows, row);
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml);
+  // place of a unit's part i for its head h: the unit's first part lies in the
+  // second of its workgroup's places
+  auto part = [&](const Parts& p, uint32_t i, uint32_t h) {
+    return ((uint64_t)(p.first + i) * 2 + (i == 0)) * part_heads + h;
+  };
+  if (blockIdx.y < a.group * pieces) {
+    const uint32_t head = blockIdx.y / pieces, piece = blockIdx.y % pieces;
+    const Parts p = parts_of(line, r, kvh * a.head_tiles + head / 16);
+    if (p.n == 1) return;
+    const uint32_t lanes = D / 4 / pieces;  // a part's columns, 16 bytes each
+    const uint32_t col = piece * lanes * 4 + tid % lanes * 4, mine = tid / lanes, step = 256 / lanes;
+    __shared__ float s_red[4][2];
+    __shared__ __attribute__((aligned(16))) float s_o[256 * 4];
+    float m = kNegInf;
+    for (uint32_t i = tid; i < p.n; i += 256) m = __builtin_fmaxf(m, ml[part(p, i, head % 16)][0]);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] = o[i] + po[(uint64_t)s * a.group * D + PER * lane + i] * f;
-    }
-    const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + PER * lane;
+    for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) s_red[wave][0] = m;
+    __syncthreads();
+    m = __builtin_fmaxf(__builtin_fmaxf(s_red[0][0], s_red[1][0]), __builtin_fmaxf(s_red[2][0], s_red[3][0]));
+    const float base = anchor(m);
+    float l = 0.0f;
+    f32x4_t o = f32x4_t{0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t i = mine; i < p.n; i += step) {
+      const uint64_t at = part(p, i, head % 16);
+      const f32x2 x = ml[at];
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + col);
+      const float f = exp2_fast(x[0] - base);
+      l = l + x[1] * f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float x = len ? o[i] / ll : 0.0f;
-      if constexpr (F32)
-        static_cast<float*>(a.o)[at + i] = x;
-      else
-        static_cast<uint16_t*>(a.o)[at + i] = (uint16_t)f32_to_bf16_bits(x);
+      for (int j = 0; j < 4; ++j) o[j] = o[j] + y[j] * f;
     }
+    // over the parts: lanes of one column are `lanes` apart
+    *reinterpret_cast<f32x4_t*>(&s_o[4 * tid]) = o;
+    l = tid % lanes == 0 ? l : 0.0f;  // each part once
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) l = l + __shfl_xor(l, d);
+    if (lane == 0) s_red[wave][1] = l;
+    __syncthreads();
+    if (tid >= lanes * 4) return;
+    l = (s_red[0][1] + s_red[1][1]) + (s_red[2][1] + s_red[3][1]);
+    float sum = 0.0f;
+    for (uint32_t i = 0; i < step; ++i) sum = sum + s_o[i * lanes * 4 + tid];
+    const float x = r.len ? sum / l : 0.0f;
+    const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + piece * lanes * 4 + tid;
+    if constexpr (F32)
+      static_cast<float*>(a.o)[at] = x;
+    else
+      static_cast<uint16_t*>(a.o)[at] = (uint16_t)f32_to_bf16_bits(x);
     return;
   }
-  const uint32_t slot0 = (blockIdx.y - join_blocks) * 1024;
-  if (slot0 >= len) return;
-  __shared__ float s_m[256], s_r[256];  // of up to 256 heads of the group at a time
-  f32x4_t w = f32x4_t{0, 0, 0, 0};
-  const uint32_t slot = slot0 + 4 * threadIdx.x;  // slots come in whole pages of 16 or more
-  for (uint32_t h0 = 0; h0 < a.group; h0 += 256) {
-    const uint32_t hn = a.group - h0 < 256 ? a.group - h0 : 256;
+  const uint32_t slot0 = (blockIdx.y - a.group * pieces) * 1024;
+  if (slot0 >= r.len) return;
+  __shared__ float s_m[16], s_r[16];
+  for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
+    const uint32_t hn = a.group - h0 < 16 ? a.group - h0 : 16;
+    const Parts p = parts_of(line, r, kvh * a.head_tiles + h0 / 16);
     if (h0) __syncthreads();
-    if (threadIdx.x < hn) {
-      const uint32_t head = h0 + threadIdx.x;
-      float mm = kNegInf;
-      for (uint32_t s = 0; s < runs; ++s) mm = __builtin_fmaxf(mm, ml[2 * ((uint64_t)s * a.group + head)]);
-      float ll = 0.0f;
-      for (uint32_t s = 0; s < runs; ++s) {
-        const uint64_t at = (uint64_t)s * a.group + head;
-        ll = ll + ml[2 * at + 1] * exp2_fast(ml[2 * at] - anchor(mm));
+    // 16 lanes a head, a part each
+    for (uint32_t h = tid / 16; h < hn; h += 16) {
+      float m = kNegInf, l = 0.0f;
+      if (p.n == 1) {
+        const float* x = a.whole_ml + 2 * ((uint64_t)row * heads + kvh * a.group + h0 + h);
+        m = x[0];
+        l = x[1];
+      } else {
+        for (uint32_t i = tid % 16; i < p.n; i += 16) m = __builtin_fmaxf(m, ml[part(p, i, h)][0]);
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+        for (uint32_t i = tid % 16; i < p.n; i += 16) {
+          const f32x2 x = ml[part(p, i, h)];
+          l = l + x[1] * exp2_fast(x[0] - anchor(m));
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) l = l + __shfl_xor(l, d);
       }
-      s_m[threadIdx.x] = anchor(mm);
-      s_r[threadIdx.x] = 1.0f / ll;
+      if (tid % 16 == 0) {
+        s_m[h] = anchor(m);
+        s_r[h] = 1.0f / l;
+      }
     }
     __syncthreads();
-    if (slot < len) {
-      const float* sc = a.scores + ((uint64_t)row * heads + kvh * a.group + h0) * slots + slot;
-      for (uint32_t h = 0; h < hn; ++h) {
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sc + (uint64_t)h * slots);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = w[i] + exp2_fast(x[i] - s_m[h]) * s_r[h];
-      }
-    }
+    add_weights(a, row, kvh, h0, hn, r.len, slot0 + 4 * tid, 0x80000000u, s_m, s_r);  // slots < 2^31: once
   }
-  if (slot >= len) return;
-  const uint64_t at = (uint64_t)pair * slots + slot;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (slot + i < len) a.acc_out[at + i] = a.acc_in[at + i] + w[i];
 }
 
 }  // namespace
 
-#define CATENA_ATTN_PAGED(D, OUT, F32)                                                                  \
-  extern "C" __global__ __launch_bounds__(256) void catena_attn_paged_d##D##_##OUT(AttnPagedArgs a) {         \
-    attn_paged_run<D, F32, false>(a);                                                                         \
-  }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(256) void catena_attn_paged_weights_d##D##_##OUT(AttnPagedArgs a) { \
-    attn_paged_run<D, F32, true>(a);                                                                          \
-  }                                                                                                           \
+#define CATENA_ATTN_PAGED(D, OUT, F32)                                                                      \
+  extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_d##D##_##OUT(AttnPagedArgs a) {      \
+    attn_paged_run<D, F32, false>(a);                                                                      \
+  }                                                                                                         \
+  extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_weights_d##D##_##OUT(AttnPagedArgs a) { \
+    attn_paged_run<D, F32, true>(a);                                                                       \
+  }                                                                                                         \
   extern "C" __global__ __launch_bounds__(256) void catena_attn_paged_join_d##D##_##OUT(AttnPagedArgs a,      \
-                                                                                        uint32_t join_blocks) { \
-    attn_paged_join<D, F32>(a, join_blocks);                                                                  \
+                                                                                        uint32_t pieces) {    \
+    attn_paged_join<D, F32>(a, pieces);                                                                       \
   }
 CATENA_ATTN_PAGED(128, f32out, true)
 CATENA_ATTN_PAGED(128, bf16out, false)

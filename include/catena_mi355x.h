@@ -329,11 +329,12 @@ typedef struct catena_paged_kv {
   uint32_t head_dim;
 } catena_paged_kv_t;
 
-/* How catena_mi355x_attn_paged_bf16 cuts a row (into at most `splits` runs of
- * slots) and the bytes of workspace that it takes (0: none).  A function of
- * the sizes alone (k, v and table are not looked at); needs no device. */
+/* How catena_mi355x_attn_paged_bf16 deals out its work -- into `parts` equal
+ * parts of all rows' slots, joined by a second kernel, or (0) a row and kv head
+ * at a time -- and the bytes of workspace that it takes (0: none).  A function
+ * of the sizes alone (k, v and table are not looked at); needs no device. */
 int catena_mi355x_attn_paged_plan(const catena_paged_kv_t *kv, uint32_t heads, int weights,
-                                  uint32_t *splits, uint64_t *workspace_bytes);
+                                  uint32_t *parts, uint64_t *workspace_bytes);
 
 /* Attention of one new token per row over a cache in pages: q[rows][heads]
  * [head_dim] bf16, lens[rows] (device u32: slots in use, the new token's among

@@ -29,7 +29,7 @@ class Call:
         self.o = ca.Buffer(rows * heads * cache.dim * 4)
         self.acc = None if acc is None else ca.Buffer.from_array(acc)
         self.acc_out = None if acc is None else ca.Buffer.from_array(np.full_like(acc, -7.0))
-        self.splits, nbytes = ca.attn_paged_plan(self.kv, heads, acc is not None)
+        self.parts, nbytes = ca.attn_paged_plan(self.kv, heads, acc is not None)
         # no byte of the workspace counts before it is written
         self.work = ca.Buffer.from_array(np.full(max(nbytes, 16), 0xFF, np.uint8))
 
@@ -90,6 +90,9 @@ CASES = [
     (3, 3, 64, 16, 700, [11200, 1, 40, 10000]),          # short rows of a long table
     (1, 1, 128, 16, 1, [16]),
     (5, 5, 128, 16, 3, [33] * 130),                      # more pairs than workgroups a round
+    (2, 1, 64, 16, 200, [(37 * i) % 211 for i in range(149)] + [3200]),  # many rows on one line, some without slots
+    (34, 2, 64, 32, 100, [3200, 1777, 0]),               # cut rows of 17 query heads a kv head
+    (4, 2, 128, 32, 60, [1920] * 3 + [64, 32, 31, 96]),  # parts that end with units
 ]
 
 
@@ -234,7 +237,7 @@ def test_captured_and_replayed():
     one = Call(Cache(rng, [900, 17, 0], 2, 128, 16, 60), bf16(rng.standard_normal((3, 8, 128))), 8, 0.1, True,
                np.zeros((3, 2, 960), np.float32))
     two = Call(Cache(rng, [4000], 1, 128, 32, 125), bf16(rng.standard_normal((1, 4, 128))), 4, 0.1, False)
-    assert one.splits > 1 and two.splits > 1
+    assert one.parts > 1 and two.parts > 1
     want = []
     for call in (one, two):
         call()

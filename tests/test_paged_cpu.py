@@ -37,23 +37,27 @@ def test_attention_refuses_bad_arguments():
     for over in (dict(heads=0), dict(heads=6), dict(q=0), dict(lens=0), dict(o=0), dict(q=P + 8), dict(o=P + 4),
                  dict(lens=P + 1), dict(acc_in=P), dict(acc_out=P), dict(acc_in=P + 2, acc_out=P)):
         refused(INVALID, attn, kv, **over)
-    need = ca.attn_paged_plan(kv, 8)[1]
+    long = geometry(rows=1, max_pages=8192)
+    need = ca.attn_paged_plan(long, 8)[1]
     assert need > 0
     for work in (None, (0, need), (P, need - 1), (P + 8, need)):
-        refused(INVALID, attn, kv, work=work)
+        refused(INVALID, attn, long, work=work)
     refused(UNSUPPORTED, attn, geometry(rows=1 << 31, kv_heads=4))
+    refused(UNSUPPORTED, attn, geometry(rows=1 << 16, kv_heads=64, max_pages=1 << 14), heads=64)
 
 
 def test_attention_plan():
     kv = geometry(rows=1, max_pages=8192, kv_heads=8)
-    splits, nbytes = ca.attn_paged_plan(kv, 32)
-    assert splits > 1 and nbytes >= splits * 32 * (128 + 2) * 4
+    parts, nbytes = ca.attn_paged_plan(kv, 32)
+    assert parts > 1 and nbytes >= parts * 2 * 4 * (128 + 2) * 4
     # the scores of every head and slot beside it, where weights are wanted
     assert ca.attn_paged_plan(kv, 32, True)[1] >= nbytes + 32 * kv.slots * 4
-    # many rows: whole, without a workspace
-    assert ca.attn_paged_plan(geometry(rows=1024, kv_heads=8), 8) == (1, 0)
+    # short rows: whole, without a workspace but for the scores
+    short = geometry(rows=1024, kv_heads=8)
+    assert ca.attn_paged_plan(short, 8) == (0, 0)
+    assert ca.attn_paged_plan(short, 8, True)[0] == 0 and ca.attn_paged_plan(short, 8, True)[1] >= 8 * 1024 * short.slots * 4
     # neither the pointers nor a device matter
-    assert ca.attn_paged_plan(geometry(rows=1, max_pages=8192, kv_heads=8, k=0, v=0, table=0), 32) == (splits, nbytes)
+    assert ca.attn_paged_plan(geometry(rows=1, max_pages=8192, kv_heads=8, k=0, v=0, table=0), 32) == (parts, nbytes)
     refused(INVALID, ca.attn_paged_plan, kv, 12)
     refused(UNSUPPORTED, ca.attn_paged_plan, geometry(page_size=24), 8)
 
