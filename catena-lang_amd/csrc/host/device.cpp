@@ -128,7 +128,8 @@ const KernelSpec kKernels[] = {
     {KernelId::KvEvictChoose, "kv_paged", "catena_kv_evict_choose"},
     {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
     {KernelId::KvReorder, "kv_paged", "catena_kv_reorder"},
-    {KernelId::BeamRuns, "beam", "catena_beam_runs"},
+    {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},
+    {KernelId::BeamRuns16, "beam", "catena_beam_runs_16"},
     {KernelId::BeamJoin, "beam", "catena_beam_join"},
     {KernelId::EmbedRowsBf16, "block", "catena_embed_rows_bf16"},
     {KernelId::RmsnormRows, "block", "catena_rmsnorm_rows"},

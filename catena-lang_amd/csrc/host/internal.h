@@ -91,7 +91,8 @@ enum class KernelId : int {
   KvEvictChoose,
   KvEvictMove,
   KvReorder,
-  BeamRuns,  // beam search's selection (beam.hip)
+  BeamRuns8,  // beam search's selection (beam.hip)
+  BeamRuns16,
   BeamJoin,
   EmbedRowsBf16,
   RmsnormRows,

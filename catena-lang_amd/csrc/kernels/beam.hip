@@ -13,20 +13,26 @@
 // latency of two launches.  First kernel: a workgroup keeps a run of a row's
 // logits in registers, takes their maximum, the sum of their exponentials and
 // their W largest.  Second kernel: a workgroup per group joins the runs of
-// its rows and merges the W sorted lists.
+// its rows and merges the W sorted lists.  Per
+// logit the first one issues a maximum, a subtraction, a product, an exponential
+// (four times an add), an add and a comparison; exponentials by exp2, keys only
+// for logits that reach the bound, loads without address arithmetic: 32 beams x 8
+// x 128000 in 22.7 us (5.8 TB/s), against 38 with keys for all and exponentials
+// in two steps.
 //
-// Scores of different beams meet in 64 bits: within a beam the logits decide, but
-// between beams the sums may lie closer than 32 bits can tell.  Exponentials and
-// a thread's sum of 16 are f32 (each off by 2^-23 of itself), sums of those and
-// all that follows f64.
+// Accuracy: an exponential is off by 2^-24 of |x - m| log2 e + 2 (log2 e in f32
+// among it), either way from term to term; sums of a thread's terms are f32.
+// Sums of those, and scores, which meet those of other beams, are f64: within a
+// beam the logits decide, but between beams the scores may lie closer than 32
+// bits can tell.
 #include "common.h"
 
 namespace {
 
-constexpr int PER = 16;             // logits a thread holds
-constexpr uint32_t RUN = 256 * PER;  // and a workgroup
 constexpr uint32_t LIST = 1024;      // candidates it can sort at once
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kNonTemporal = 2;
+constexpr float kLog2e = 1.44269502f;
 
 // Orders offered logits (larger first, lower token where equal); 0: not offered
 CATENA_DEV uint32_t offer(float x) { return x > kNegInf ? mono_bits(__float_as_uint(x)) : 0u; }
@@ -35,35 +41,59 @@ CATENA_DEV float offered(uint32_t mono) {
 }
 CATENA_DEV uint64_t with_token(uint32_t mono, uint32_t token) { return mono ? ((uint64_t)mono << 32) | ~token : 0ull; }
 
-// The largest of the wave's values
+// The largest of the wave's values; the lower halves meet only where the upper
+// ones are equal
 CATENA_DEV uint64_t wave_max64(uint64_t x) {
   const uint32_t hi = wave_umax((uint32_t)(x >> 32));
-  const uint32_t lo = wave_umax((uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
+  const uint64_t have = __ballot((uint32_t)(x >> 32) == hi);
+  uint32_t lo;
+  if ((have & (have - 1)) == 0)
+    lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, __ffsll((unsigned long long)have) - 1);
+  else
+    lo = wave_umax((uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
   return ((uint64_t)hi << 32) | lo;
 }
 
-}  // namespace
+// A bound that at least `beams` of the wave's 64 values reach (of those that are
+// not 0; 0 where there are fewer), near the largest such one
+CATENA_DEV uint32_t wave_bound(uint32_t x, uint32_t beams) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int b = 31; b >= 14; --b) {
+    const uint32_t t = bound | (1u << b);
+    if ((uint32_t)__popcll(__ballot(x >= t)) >= beams) bound = t;
+  }
+  return bound;
+}
 
 // Run blockIdx.y of row blockIdx.x: part_m its maximum, part_s the sum of
-// exp(logit - maximum), best[W] its largest (with_token, 0 where there are fewer).
-// The W-th largest of one wave's 64 lane maxima is a bound that W logits reach:
-// what reaches the largest such bound of the four waves is listed and
-// sorted by counting.  Where more do than the list holds (equal logits), the W
-// are taken one after the other.
-extern "C" __global__ __launch_bounds__(256) void catena_beam_runs(
-    const float* __restrict__ logits, const uint32_t* __restrict__ done, float* __restrict__ part_m,
-    double* __restrict__ part_s, uint64_t* __restrict__ best, uint32_t vocab, uint32_t beams) {
+// exp(logit - maximum), best[W] its largest (with_token, 0 where there are
+// fewer).  The W-th largest of one wave's 64 lane maxima, cut to 18 bits, is a
+// bound that W logits reach: what reaches the largest such bound of the four
+// waves is listed and sorted by counting.  Where more do than the list holds
+// (equal logits), the W are taken one after the other.
+template <int PER>
+CATENA_DEV void beam_runs(const float* __restrict__ logits, const uint32_t* __restrict__ done,
+                          float* __restrict__ part_m, double* __restrict__ part_s, uint64_t* __restrict__ best,
+                          uint32_t vocab, uint32_t beams) {
   __shared__ float s_max[4];
   __shared__ double s_sum[4];
   __shared__ uint32_t s_bound[4], s_count;
   __shared__ uint64_t s_key[LIST], s_wave[4];
   const uint32_t row = blockIdx.x, run = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   if (done && done[row]) return;
-  const float* x = logits + (uint64_t)row * vocab;
-  const uint32_t first = run * RUN + tid;
+  const uint32_t first = run * 256 * PER + tid;
+  const int bytes = (int)(vocab * 4u);  // at most 2^28
+  const __amdgpu_buffer_rsrc_t x =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(logits + (uint64_t)row * vocab), (short)0, bytes, 0x00020000);
   float v[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) v[k] = first + 256 * k < vocab ? x[first + 256 * k] : kNegInf;
+  for (int k = 0; k < PER; ++k)
+    v[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(x, (int)(first * 4), 1024 * k, kNonTemporal));
+  if (first - tid + 256 * PER > vocab) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[k] = first + 256 * k < vocab ? v[k] : kNegInf;
+  }
   if (tid == 0) s_count = 0;
 
   float top = v[0];
@@ -71,13 +101,8 @@ extern "C" __global__ __launch_bounds__(256) void catena_beam_runs(
   for (int k = 1; k < PER; ++k) top = __builtin_fmaxf(top, v[k]);  // of the numbers: a NaN shows in the sum
   const uint32_t mine = offer(top);
   // the maximum, and the wave's bound
-  uint32_t bound = 0;
-#pragma unroll 1
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t t = bound | (1u << b);
-    if ((uint32_t)__popcll(__ballot(mine >= t)) >= beams) bound = t;
-  }
   const uint32_t wmax = wave_umax(mine);
+  uint32_t bound = wave_bound(mine, beams);
   if (lane == 0) {
     s_max[wave] = wmax ? offered(wmax) : kNegInf;
     s_bound[wave] = bound;
@@ -85,29 +110,28 @@ extern "C" __global__ __launch_bounds__(256) void catena_beam_runs(
   __syncthreads();
   const float m = __builtin_fmaxf(__builtin_fmaxf(s_max[0], s_max[1]), __builtin_fmaxf(s_max[2], s_max[3]));
   bound = max(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])), 1u);
-  // exp(x - m) = 2^(x log2e - m log2e), the product's rounding made good by a
-  // second one; no reference point while nothing is above -inf
-  const float ref = m == kNegInf ? 0.0f : m;
-  float sum = 0.0f;
+  // nothing to refer to while nothing is above -inf
+  const float c = m == kNegInf ? 0.0f : m;
+  float sum[4] = {};
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const float d = v[k] - ref;
-    const float hi = d * 1.44269502f;
-    const float lo = __builtin_fmaf(d, 1.44269502f, -hi) + d * 1.92596303e-8f;
-    float e = __builtin_amdgcn_exp2f(hi);
-    if (d > -__builtin_huge_valf()) e = __builtin_fmaf(e, lo * 0.693147182f, e);
-    sum = sum + e;
-  }
-  double total = (double)sum;
+  for (int k = 0; k < PER; ++k) sum[k % 4] = sum[k % 4] + __builtin_amdgcn_exp2f((v[k] - c) * kLog2e);
+  double total = (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) total = total + __shfl_xor(total, d);
   if (lane == 0) s_sum[wave] = total;
+  if (mine >= bound) {
+    const float least = bound == 1u ? -__FLT_MAX__ : offered(bound);
+    uint32_t which = 0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const uint32_t key = offer(v[k]);
-    if (key >= bound) {
+    for (int k = 0; k < PER; ++k) which |= v[k] >= least ? 1u << k : 0u;
+    while (which) {
+      const uint32_t one = (uint32_t)__ffs((int)which) - 1;
+      which &= which - 1;
+      float value = v[0];
+#pragma unroll
+      for (int k = 1; k < PER; ++k) value = one == (uint32_t)k ? v[k] : value;
       const uint32_t at = atomicAdd(&s_count, 1u);
-      if (at < LIST) s_key[at] = with_token(key, first + 256 * k);
+      if (at < LIST) s_key[at] = with_token(offer(value), first + 256 * one);
     }
   }
   __syncthreads();
@@ -147,116 +171,154 @@ extern "C" __global__ __launch_bounds__(256) void catena_beam_runs(
   }
 }
 
-// Group blockIdx.x: a wave joins a row's runs (its log sum in f64) and takes the
-// W largest of their lists, each lane at the head of lists of its own; then the
-// first wave merges the rows' lists, lane w at the head of beam w's.
-// W <= 32.  A place that no offered continuation fills: its own beam as
-// parent, token 0, score -inf, not done.
+// The `beams` largest of n keys (and of those in best, where there are any) into
+// best in order, by one wave: PER keys a lane in registers (the keys are sorted lists of
+// `beams`; shifted, so that a lane has entries of several ranks and few keys reach
+// the bound that half the lanes' largest do).  Those that reach the
+// wave's bound are listed and sorted by counting; where they are more than the
+// list holds, the largest is taken out time after time.
+constexpr uint32_t WLIST = 128;
+template <int PER>
+CATENA_DEV void largest_of(const uint64_t* keys, uint32_t n, bool more, uint64_t* best, uint32_t beams,
+                           uint64_t* list) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint64_t k[PER + 1];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t at = 64 * i + ((lane + 5 * i) & 63u);
+    k[i] = at < n ? keys[at] : 0ull;
+  }
+  k[PER] = more && lane < beams ? best[lane] : 0ull;
+  uint64_t mine = 0;
+#pragma unroll
+  for (int i = 0; i <= PER; ++i) mine = k[i] > mine ? k[i] : mine;
+  const uint32_t least = max(wave_bound((uint32_t)(mine >> 32), beams), 1u);
+  uint32_t count = 0;
+#pragma unroll
+  for (int i = 0; i <= PER; ++i) {
+    const bool in = (uint32_t)(k[i] >> 32) >= least;
+    const uint64_t have = __ballot(in);
+    const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
+    if (in && at < WLIST) list[at] = k[i];
+    count += (uint32_t)__popcll(have);
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (count <= WLIST) {
+    const uint64_t a = lane < count ? list[lane] : 0ull, b = lane + 64 < count ? list[lane + 64] : 0ull;
+    uint32_t above_a = 0, above_b = 0;
+    for (uint32_t j = 0; j < count; ++j) {
+      const uint64_t x = list[j];
+      above_a += x > a;
+      above_b += x > b;
+    }
+    if (a && above_a < beams) best[above_a] = a;
+    if (b && above_b < beams) best[above_b] = b;
+    if (lane >= count && lane < beams) best[lane] = 0;
+    return;
+  }
+  uint64_t kept = 0;
+  for (uint32_t r = 0; r < beams; ++r) {
+    const uint64_t top = wave_max64(mine);
+    if (lane == r) kept = top;
+    if (mine == top) {
+      mine = 0;
+#pragma unroll
+      for (int i = 0; i <= PER; ++i) mine = k[i] < top && k[i] > mine ? k[i] : mine;
+    }
+  }
+  if (lane < beams) best[lane] = kept;
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void catena_beam_runs_8(
+    const float* logits, const uint32_t* done, float* part_m, double* part_s, uint64_t* best, uint32_t vocab,
+    uint32_t beams) {
+  beam_runs<8>(logits, done, part_m, part_s, best, vocab, beams);
+}
+extern "C" __global__ __launch_bounds__(256) void catena_beam_runs_16(
+    const float* logits, const uint32_t* done, float* part_m, double* part_s, uint64_t* best, uint32_t vocab,
+    uint32_t beams) {
+  beam_runs<16>(logits, done, part_m, part_s, best, vocab, beams);
+}
+// Group blockIdx.x: a wave joins a row's runs (their log sum in f64) and takes
+// the W largest of their lists; then the first wave merges the rows' lists, lane
+// w at the head of beam w's.  W <= 32; 64 threads a beam, up to 16.  A place that
+// no offered continuation fills: its own beam as parent, token 0, score -inf, not
+// done.
 extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
     const float* __restrict__ part_m, const double* __restrict__ part_s, const uint64_t* __restrict__ best,
     const float* scores, const uint32_t* done, uint32_t* tokens, uint32_t* parents, float* scores_out,
     uint32_t* done_out, uint32_t runs, uint32_t beams, uint32_t eos) {
-  __shared__ uint64_t s_best[32][32];
-  __shared__ double s_shift[32];
+  __shared__ uint64_t s_best[32][32];  // with_token, then the scores as ordered integers
+  __shared__ uint32_t s_token[32][32];
+  __shared__ uint64_t s_list[16][WLIST];
   __shared__ uint32_t s_done[32];
   const uint32_t group = blockIdx.x, lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (uint32_t w = wave; w < beams; w += 16) {
+  for (uint32_t w = wave; w < beams; w += blockDim.x / 64) {
     const uint32_t row = group * beams + w;
+    // a done beam's parts were not written: read all the same, so that nothing
+    // waits for the flag, and not used
     const double score = (double)scores[row];
-    if (done && done[row]) {
-      if (lane == 0) {
-        s_done[w] = 1;
-        s_shift[w] = score;
-      }
-      continue;
-    }
+    const bool over = done && done[row] != 0;
     const float* pm = part_m + (uint64_t)row * runs;
     const double* ps = part_s + (uint64_t)row * runs;
-    float m = kNegInf;
-    for (uint32_t r = lane; r < runs; r += 64) m = __builtin_fmaxf(m, pm[r]);
+    const uint64_t* keys = best + (uint64_t)row * runs * beams;
+    const uint32_t n = runs * beams;
+    // a run of nothing above -inf adds 0 (or its NaN)
+    float m = lane < runs ? pm[lane] : kNegInf;
+    double sum = lane < runs ? ps[lane] : 0.0;
+    if (n <= 256) {
+      largest_of<4>(keys, n, false, s_best[w], beams, s_list[wave]);
+    } else {
+      for (uint32_t i = 0; i < n; i += 1024)
+        largest_of<16>(keys + i, n - i < 1024 ? n - i : 1024, i != 0, s_best[w], beams, s_list[wave]);
+    }
+    const float mine = m;
+    for (uint32_t r = lane + 64; r < runs; r += 64) m = __builtin_fmaxf(m, pm[r]);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-    const double ref = m == kNegInf ? 0.0 : (double)m;
-    double sum = 0.0;
-    for (uint32_t r = lane; r < runs; r += 64) sum = sum + ps[r] * exp((double)pm[r] - ref);
+    sum = lane < runs ? sum * exp((double)mine - (double)m) : 0.0;
+    for (uint32_t r = lane + 64; r < runs; r += 64) sum = sum + ps[r] * exp((double)pm[r] - (double)m);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum = sum + __shfl_xor(sum, d);
-    if (lane == 0) {
-      s_done[w] = 0;
-      s_shift[w] = score - (ref + log(sum));
-    }
-    const uint64_t* lists = best + (uint64_t)row * runs * beams;
-    uint64_t last = ~0ull;
-    uint64_t head = 0;  // the largest of this lane's lists below `last`
-    bool stale = true;
-    for (uint32_t r = 0; r < beams; ++r) {
-      if (stale) {
-        head = 0;
-        for (uint32_t q = lane; q < runs; q += 64) {
-          const uint64_t* list = lists + (uint64_t)q * beams;
-          for (uint32_t i = 0; i < beams; ++i) {
-            const uint64_t key = list[i];
-            if (key < last) {
-              head = key > head ? key : head;
-              break;
-            }
-          }
-        }
-      }
-      const uint64_t top = wave_max64(head);
-      if (lane == 0) s_best[w][r] = top;
-      last = top;
-      stale = head == top;
+    const double shift = over ? score : score - ((double)m + log(sum));
+    // the row's continuations: 0 where it has no more, or offers none
+    if (lane == 0) s_done[w] = over;
+    if (lane < beams) {
+      const uint64_t b = over ? (lane == 0 ? 1ull : 0ull) : s_best[w][lane];
+      const double s = over ? shift : (double)offered((uint32_t)(b >> 32)) + shift;
+      const uint64_t bits = (uint64_t)__double_as_longlong(s + 0.0);  // -0 as +0
+      s_token[w][lane] = over ? eos : ~(uint32_t)b;
+      s_best[w][lane] = b == 0 || !(shift - shift == 0.0) ? 0ull : (bits >> 63) ? ~bits : bits | (1ull << 63);
     }
   }
   __syncthreads();
   if (wave != 0) return;
-  const uint32_t w = lane;
-  const bool here = w < beams;
-  const double shift = here ? s_shift[w] : 0.0;
-  const bool over = here && s_done[w] != 0;
-  const bool offers = here && shift - shift == 0.0;  // finite
-  uint32_t at = 0;
+  uint32_t at = 0, won = 0xFFFFFFFFu;  // lane w: its list's head; lane r: place r's (beam, entry)
+  uint64_t head = lane < beams ? s_best[lane][0] : 0ull, score = 0;
   for (uint32_t r = 0; r < beams; ++r) {
-    // this beam's next continuation as an ordered integer: 0 where it has none
-    uint64_t key = 0;
-    uint32_t token = 0;
-    double s = 0.0;
-    if (offers && at < (over ? 1u : beams)) {
-      if (over) {
-        s = shift;
-        token = eos;
-        key = 1;
-      } else if (s_best[w][at]) {
-        const uint64_t b = s_best[w][at];
-        s = (double)offered((uint32_t)(b >> 32)) + shift;
-        token = ~(uint32_t)b;
-        key = 1;
-      }
-      if (key) {
-        const uint64_t bits = (uint64_t)__double_as_longlong(s + 0.0);  // -0 as +0
-        key = (bits >> 63) ? ~bits : bits | (1ull << 63);
-      }
+    const uint64_t top = wave_max64(head);
+    if (top == 0) break;
+    const uint32_t w = (uint32_t)__ffsll((unsigned long long)__ballot(head == top)) - 1;
+    const uint32_t entry = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)w);
+    if (lane == r) {
+      won = w * 32 + entry;
+      score = top;
     }
-    const uint64_t top = wave_max64(key);
-    const uint32_t out = group * beams + r;
-    if (top == 0) {
-      if (lane == 0) {
-        tokens[out] = 0;
-        parents[out] = out;
-        scores_out[out] = kNegInf;
-        if (done_out) done_out[out] = 0;
-      }
-      continue;
-    }
-    const uint32_t winner = (uint32_t)__ffsll((unsigned long long)__ballot(key == top)) - 1;
-    if (lane == winner) {
-      tokens[out] = token;
-      parents[out] = group * beams + w;
-      scores_out[out] = (float)s;
-      if (done_out) done_out[out] = over || token == eos;
+    if (lane == w) {
       ++at;
+      head = at < beams ? s_best[w][at] : 0ull;
     }
   }
+  if (lane >= beams) return;
+  const uint32_t out = group * beams + lane;
+  const bool filled = won != 0xFFFFFFFFu;
+  const uint32_t w = won / 32 % 32, token = filled ? s_token[w][won % 32] : 0u;
+  const uint64_t bits = (score >> 63) ? score & ~(1ull << 63) : ~score;
+  tokens[out] = token;
+  parents[out] = filled ? group * beams + w : out;
+  scores_out[out] = filled ? (float)__longlong_as_double((long long)bits) : kNegInf;
+  if (done_out) done_out[out] = filled && (s_done[w] != 0 || token == eos);
 }

@@ -79,15 +79,17 @@ class Select:
     def check(self, tied=False):
         tokens, parents, scores, done, near = self.want()
         if not tied:
-            assert near > 1e-6, near  # ten times what the log sum can be off
+            assert near > 1e-6, near  # between beams; far beyond what their log sums, off alike, differ by
         got = self.read()
         assert np.array_equal(got[0], tokens)
         assert np.array_equal(got[1], parents)
         assert np.array_equal(got[3], done)
         fine = np.isfinite(scores)
         assert np.array_equal(np.isfinite(got[2]), fine) and np.all(got[2][~fine] == -np.inf)
-        # an exponential and a sum of 16 are off by 18 u at most, its log by as much; one rounding
-        assert np.all(np.abs(got[2][fine] - scores[fine]) <= 20 * U + U * np.abs(scores[fine]))
+        # an exponential is off by u of |x - max| log2 e (below 2^6 where it counts, log2 e in f32 and the
+        # product's rounding each) and 2 of itself, a sum of 16 by 16 u; one rounding of the result
+        bound = (2 * 64 + 18) * U
+        assert np.all(np.abs(got[2][fine] - scores[fine]) <= bound + U * np.abs(scores[fine]))
 
 
 def _draw(seed, groups, beams, vocab, done_share=0.2, scale=2.5, eos=EOS):
@@ -179,6 +181,21 @@ def test_masked_and_odd_logits():
     assert np.array_equal(parents[1], 4 + np.arange(4)) and np.all(scores[1] == -np.inf) and not tokens[1].any()
     assert np.sum(np.isfinite(scores[2])) == 2
     assert tokens[7, 0] == EOS and done[7, 0] == 1 and scores[7, 0] == -3
+
+
+def test_far_logits_beside_a_masked_run():
+    """Logits near -2000, and near +2000, in a row of which whole runs are masked:
+    the references of the other runs alone count."""
+    say("beam_select far logits")
+    case = _draw(17, 2, 3, 40000, done_share=0)
+    x = case.logits.copy()
+    x[0] -= 2000
+    x[1] += 2000
+    x[:, :, :9000] = -np.inf
+    x[:, 1, 17000:] = -np.inf
+    case = Select(x, case.scores, case.done)
+    case()
+    case.check()
 
 
 def test_every_beam_done():
