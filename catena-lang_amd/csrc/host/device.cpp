@@ -125,7 +125,8 @@ const KernelSpec kKernels[] = {
     {KernelId::AttnPagedJoinD64F32, "attn_paged", "catena_attn_paged_join_d64_f32out"},
     {KernelId::AttnPagedJoinD64Bf16, "attn_paged", "catena_attn_paged_join_d64_bf16out"},
     {KernelId::RopeQkvPaged, "kv_paged", "catena_rope_qkv_paged"},
-    {KernelId::KvEvictChoose, "kv_paged", "catena_kv_evict_choose"},
+    {KernelId::KvEvictChoose1k, "kv_paged", "catena_kv_evict_choose_1k"},
+    {KernelId::KvEvictChoose8k, "kv_paged", "catena_kv_evict_choose_8k"},
     {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
     {KernelId::KvReorder, "kv_paged", "catena_kv_reorder"},
     {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},

@@ -88,7 +88,8 @@ enum class KernelId : int {
   AttnPagedJoinD64F32,
   AttnPagedJoinD64Bf16,
   RopeQkvPaged,  // upkeep of a cache in pages (kv_paged.hip)
-  KvEvictChoose,
+  KvEvictChoose1k,
+  KvEvictChoose8k,
   KvEvictMove,
   KvReorder,
   BeamRuns8,  // beam search's selection (beam.hip)

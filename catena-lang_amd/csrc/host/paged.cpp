@@ -96,6 +96,7 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   return CATENA_OK;
 }
 
+constexpr uint32_t kEvictAtOnce = 64;  // moves that its lists in LDS hold
 constexpr uint32_t kEvictMoves = 64;  // a workgroup of catena_kv_evict_move
 // Most moves of a (row, kv head): slots below the budget, and slots from it on
 uint32_t evict_most(const PagedKv& kv, uint32_t budget) {
@@ -111,6 +112,22 @@ int evict_plan(const PagedKv& kv, uint32_t budget, uint64_t* bytes) {
   *bytes = pairs * 4 * (1 + 2ull * evict_most(kv, budget));
   return CATENA_OK;
 }
+
+// struct EvictArgs of kv_paged.hip, field for field
+struct EvictArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* seen;
+  const float* acc_in;
+  const uint32_t* pos_in;
+  uint32_t* lens_out;
+  float* acc_out;
+  uint32_t* pos_out;
+  uint32_t* count;
+  uint32_t* holes;
+  uint32_t* sources;
+  uint32_t most, budget, recent, at_once;
+};
 
 // struct ReorderPools of kv_paged.hip
 struct ReorderPools {
@@ -217,7 +234,8 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_
                                       const float* acc_in, const uint32_t* slot_pos_in, uint32_t* lens_out,
                                       float* acc_out, uint32_t* slot_pos_out, uint32_t budget, uint32_t recent,
                                       void* workspace, uint64_t workspace_bytes) {
-  PagedKv c;
+  EvictArgs a{};
+  PagedKv& c = a.kv;
   uint64_t need = 0;
   int st = paged_check(kv, true, &c);
   if (!st) st = evict_plan(c, budget, &need);
@@ -228,23 +246,36 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_
   const void* words[] = {lens, seen, acc_in, slot_pos_in, lens_out, acc_out, slot_pos_out};
   for (const void* p : words)
     if (!aligned(p, 4)) return fail(CATENA_ERR_INVALID_ARGUMENT, "misaligned operand");
+  if (!aligned(acc_in, 16) || !aligned(slot_pos_in, 16) || !aligned(acc_out, 16) || !aligned(slot_pos_out, 16))
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction needs 16-byte aligned weights and positions");
   if (lens_out == lens) return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction's new lengths may not replace the old");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction needs %llu bytes of 16-byte aligned workspace",
                 (unsigned long long)need);
   st = ensure_init();
   if (st) return st;
-  const uint32_t pairs = c.rows * c.kv_heads;
-  uint32_t most = evict_most(c, budget);
-  uint32_t* count = static_cast<uint32_t*>(workspace);
-  uint32_t* holes = count + pairs;
-  uint32_t* sources = holes + (uint64_t)pairs * most;
-  void* args[] = {&c,       &lens,  &seen,  &acc_in,  &slot_pos_in, &lens_out, &acc_out,
-                  &slot_pos_out, &count, &holes, &sources, &most,        &budget,   &recent};
-  st = launch(KernelId::KvEvictChoose, dim3(pairs), dim3(1024), 0, args);
-  if (st || most == 0) return st;
-  void* margs[] = {&c, &acc_in, &slot_pos_in, &acc_out, &slot_pos_out, &count, &holes, &sources, &most};
-  return launch(KernelId::KvEvictMove, dim3(pairs, (unsigned)ceil_div(most, kEvictMoves)), dim3(256), 0, margs);
+  const uint32_t pairs = c.rows * c.kv_heads, slots = paged_slots(c);
+  a.lens = lens;
+  a.seen = seen;
+  a.acc_in = acc_in;
+  a.pos_in = slot_pos_in;
+  a.lens_out = lens_out;
+  a.acc_out = acc_out;
+  a.pos_out = slot_pos_out;
+  a.most = evict_most(c, budget);
+  a.count = static_cast<uint32_t*>(workspace);
+  a.holes = a.count + pairs;
+  a.sources = a.holes + (uint64_t)pairs * a.most;
+  a.budget = budget;
+  a.recent = recent;
+  // Few moves are made by the workgroup that chose them, which saves a launch;
+  // more by workgroups of 64 each.
+  a.at_once = a.most <= kEvictAtOnce;
+  void* args[] = {&a};
+  st = slots <= 1024 ? launch(KernelId::KvEvictChoose1k, dim3(pairs), dim3(256), 0, args)
+                     : launch(KernelId::KvEvictChoose8k, dim3(pairs), dim3(1024), 0, args);
+  if (st || a.at_once) return st;
+  return launch(KernelId::KvEvictMove, dim3(pairs, (unsigned)ceil_div(a.most, kEvictMoves)), dim3(256), 0, args);
 }
 
 int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t* kv, uint16_t* const* pools, uint32_t n_pools,

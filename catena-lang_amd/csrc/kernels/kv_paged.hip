@@ -89,21 +89,31 @@ CATENA_DEV uint32_t keep_key(float weight, uint32_t pos, uint32_t late) {
   return weight != weight ? 0u : mono_bits(__float_as_uint(weight));
 }
 
-// Exclusive prefix sum over the workgroup's 1024 threads, and the total
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then rows to rows
+CATENA_DEV uint32_t wave_prefix(uint32_t x) {
+#define CATENA_DPP_ADD(ctrl, rows) \
+  x = x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, (ctrl), (rows), 0xF, false)
+  CATENA_DPP_ADD(0x111, 0xF);
+  CATENA_DPP_ADD(0x112, 0xF);
+  CATENA_DPP_ADD(0x114, 0xF);
+  CATENA_DPP_ADD(0x118, 0xF);
+  CATENA_DPP_ADD(0x142, 0xA);
+  CATENA_DPP_ADD(0x143, 0xC);
+#undef CATENA_DPP_ADD
+  return x;
+}
+
+// Exclusive prefix sum over the workgroup's threads, and the total.  s_wave[2]:
+// the caller alternates between the two, so that one barrier is enough.
+template <int WAVES>
 CATENA_DEV uint32_t block_prefix(uint32_t x, uint32_t* s_wave, uint32_t* total) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t in = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t y = __shfl_up(in, d);
-    if (lane >= (uint32_t)d) in += y;
-  }
-  __syncthreads();  // s_wave is free again
+  const uint32_t in = wave_prefix(x);
   if (lane == 63) s_wave[wave] = in;
   __syncthreads();
   uint32_t before = 0, sum = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < 16; ++w) {
+  for (uint32_t w = 0; w < WAVES; ++w) {
     const uint32_t v = s_wave[w];
     before += w < wave ? v : 0u;
     sum += v;
@@ -112,132 +122,240 @@ CATENA_DEV uint32_t block_prefix(uint32_t x, uint32_t* s_wave, uint32_t* total) 
   return before + in - x;
 }
 
-}  // namespace
+struct EvictArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* seen;
+  const float* acc_in;
+  const uint32_t* pos_in;
+  uint32_t* lens_out;
+  float* acc_out;
+  uint32_t* pos_out;
+  uint32_t* count;    // [pairs]
+  uint32_t* holes;    // [pairs][most]
+  uint32_t* sources;  // [pairs][most]
+  uint32_t most, budget, recent;
+  uint32_t at_once;   // the choosing workgroup makes the moves itself
+};
+
+// Moves first, first + step, ... of a (row, kv head), four at a time: a row of K and
+// of V (16 bytes a lane), the slot's weight and position.  Sources lie from the
+// budget on and are never written, so the order does not matter.
+CATENA_DEV void evict_moves(const EvictArgs& a, uint32_t pair, const uint32_t* holes, const uint32_t* sources,
+                            uint32_t first, uint32_t end, uint32_t step) {
+  constexpr int AT = 4;
+  const uint32_t row = pair / a.kv.kv_heads, h = pair % a.kv.kv_heads;
+  const uint32_t lane = threadIdx.x % (a.kv.head_dim / 8);
+  const uint64_t base = (uint64_t)pair * paged_slots(a.kv);
+  for (uint32_t i = first; i < end; i += AT * step) {
+    uint32_t to[AT], from[AT];
+    uint64_t dst[AT], src[AT];
+    bool there[AT];
+    u32x4_t k[AT], v[AT];
+#pragma unroll
+    for (int j = 0; j < AT; ++j) {
+      const bool in = i + j * step < end;
+      to[j] = in ? holes[i + j * step] : 0xFFFFFFFFu;
+      from[j] = in ? sources[i + j * step] : 0xFFFFFFFFu;
+    }
+#pragma unroll
+    for (int j = 0; j < AT; ++j)
+      there[j] = paged_place(a.kv, row, h, to[j], &dst[j]) && paged_place(a.kv, row, h, from[j], &src[j]);
+#pragma unroll
+    for (int j = 0; j < AT; ++j)
+      if (there[j]) {
+        k[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(a.kv.k + src[j] + 8 * lane));
+        v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(a.kv.v + src[j] + 8 * lane));
+      }
+#pragma unroll
+    for (int j = 0; j < AT; ++j) {
+      if (there[j]) {
+        *reinterpret_cast<u32x4_t*>(a.kv.k + dst[j] + 8 * lane) = k[j];
+        *reinterpret_cast<u32x4_t*>(a.kv.v + dst[j] + 8 * lane) = v[j];
+      }
+      if (lane == 0 && to[j] != 0xFFFFFFFFu) {
+        a.acc_out[base + to[j]] = a.acc_in[base + from[j]];
+        a.pos_out[base + to[j]] = a.pos_in[base + from[j]];
+      }
+    }
+  }
+}
 
 // What a (row, kv head) keeps: the lists of slots to fill and of slots to fill
-// them from, and the weights and positions of the slots that stay in place.
-// The budget-th largest key is found digit by digit (12, 12 and 8 bits, a
-// histogram in LDS each), then a thread walks a run of slots of its own.
-// One workgroup of 1024 per (row, kv head); lists: count[pairs], holes
-// [pairs][most], sources[pairs][most].
-extern "C" __global__ __launch_bounds__(1024) void catena_kv_evict_choose(
-    PagedKv kv, const uint32_t* lens, const uint32_t* seen, const float* acc_in, const uint32_t* pos_in,
-    uint32_t* lens_out, float* acc_out, uint32_t* pos_out, uint32_t* count, uint32_t* holes, uint32_t* sources,
-    uint32_t most, uint32_t budget, uint32_t recent) {
-  __shared__ uint32_t hist[4096];
-  __shared__ uint32_t s_wave[16], s_bin, s_left;
-  const uint32_t pair = blockIdx.x, row = pair / kv.kv_heads, tid = threadIdx.x;
-  const uint32_t n = paged_len(kv, lens[row]), kept = n < budget ? n : budget;
-  const uint64_t base = (uint64_t)pair * paged_slots(kv);
-  const float* acc = acc_in + base;
-  const uint32_t* pos = pos_in + base;
-  if (tid == 0 && pair % kv.kv_heads == 0) lens_out[row] = kept;
-  const bool moved = acc_out != acc_in, moved_pos = pos_out != pos_in;
-  if (n <= budget) {
-    for (uint32_t j = tid; j < n; j += 1024) {
-      if (moved) acc_out[base + j] = acc[j];
-      if (moved_pos) pos_out[base + j] = pos[j];
+// them from, and the weights and positions of the slots that stay in place.  A
+// thread has KEYS slots in a row of every THREADS * KEYS; a row that is no longer
+// stays in registers, a longer one is read again for each pass.  The budget-th
+// largest key is found digit by digit from the top, a histogram in LDS each, until
+// a digit's keys are all kept; prefix sums over the threads then order both lists.
+// Bound: latency (two dependent loads, a dozen barriers), so short rows take a
+// small workgroup.
+template <int THREADS, int KEYS>
+CATENA_DEV void evict_choose(const EvictArgs& a) {
+  constexpr int WAVES = THREADS / 64, DIGIT = THREADS == 256 ? 8 : 12, STEPS = THREADS == 256 ? 4 : 3;
+  constexpr uint32_t BINS = 1u << DIGIT, OWN = BINS / THREADS, TILE = THREADS * KEYS;
+  constexpr uint32_t LISTS = 64;
+  __shared__ uint32_t hist[BINS];
+  __shared__ uint32_t s_wave[2][WAVES], s_bin, s_left, s_in_bin, s_holes[LISTS], s_sources[LISTS];
+  const uint32_t pair = blockIdx.x, row = pair / a.kv.kv_heads, tid = threadIdx.x, budget = a.budget;
+  const uint32_t slots = paged_slots(a.kv);
+  const uint64_t base = (uint64_t)pair * slots;
+
+  // the thread's slots of a tile up to `upto`; what is read behind the row's end
+  // is table, in whole vectors, and its keys do not count
+  f32x4_t w[KEYS / 4];
+  u32x4_t p[KEYS / 4];
+  uint32_t beg = 0;
+  auto load = [&](uint32_t tile, uint32_t upto) {
+    beg = tile * TILE + tid * KEYS;
+#pragma unroll
+    for (int i = 0; i < KEYS / 4; ++i) {
+      const bool in = beg + 4 * i < upto;
+      w[i] = in ? *reinterpret_cast<const f32x4_t*>(a.acc_in + base + beg + 4 * i) : f32x4_t{0, 0, 0, 0};
+      p[i] = in ? *reinterpret_cast<const u32x4_t*>(a.pos_in + base + beg + 4 * i) : u32x4_t{0, 0, 0, 0};
     }
-    if (tid == 0) count[pair] = 0;
+  };
+  // a table of one tile is read before the row's length is known
+  const bool single = slots <= TILE;
+  if (single) load(0, slots);
+  const uint32_t n = paged_len(a.kv, a.lens[row]), total_seen = a.seen[row], kept = n < budget ? n : budget;
+  const uint32_t late = total_seen - (a.recent < total_seen ? a.recent : total_seen);
+  const uint32_t tiles = (n + TILE - 1) / TILE;
+  if (!single && tiles == 1) load(0, n);
+  if (tid == 0 && pair % a.kv.kv_heads == 0) a.lens_out[row] = kept;
+  auto each = [&](auto what) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      if (beg + i < n) what(beg + i, keep_key(w[i / 4][i % 4], p[i / 4][i % 4], late));
+  };
+  // the slots below the budget as they are; the moves overwrite those given up
+  auto copy = [&]() {
+#pragma unroll
+    for (int i = 0; i < KEYS / 4; ++i) {
+      const uint32_t j = beg + 4 * i;
+      if (j + 4 <= kept) {
+        if (a.acc_out != a.acc_in) *reinterpret_cast<f32x4_t*>(a.acc_out + base + j) = w[i];
+        if (a.pos_out != a.pos_in) *reinterpret_cast<u32x4_t*>(a.pos_out + base + j) = p[i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < kept) {
+            if (a.acc_out != a.acc_in) a.acc_out[base + j + e] = w[i][e];
+            if (a.pos_out != a.pos_in) a.pos_out[base + j + e] = p[i][e];
+          }
+      }
+    }
+  };
+  if (n <= budget) {
+    for (uint32_t tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load(tile, n);
+      copy();
+    }
+    if (tid == 0 && !a.at_once) a.count[pair] = 0;
     return;
   }
-  const uint32_t total_seen = seen[row], late = total_seen - (recent < total_seen ? recent : total_seen);
-  // the budget-th largest key: its bits from the top
-  uint32_t prefix = 0, left = budget;
+
+  uint32_t prefix = 0, left = budget, shift = 32, total;
+  bool ties = true;  // more keys in the prefix's range than are kept
 #pragma unroll 1
-  for (int step = 0; step < 3; ++step) {
-    const uint32_t shift = step == 0 ? 20 : step == 1 ? 8 : 0, bins = step == 2 ? 256 : 4096;
-    const uint32_t above = step == 0 ? 0u : 0xFFFFFFFFu << (step == 1 ? 20 : 8);  // bits already known
-    for (uint32_t b = tid; b < bins; b += 1024) hist[b] = 0;
+  for (int step = 0; step < STEPS && ties; ++step) {
+    const uint32_t known = step == 0 ? 0u : 0xFFFFFFFFu << shift;
+    const uint32_t bits = shift < DIGIT ? shift : DIGIT, bins = 1u << bits;
+    shift -= bits;
+#pragma unroll
+    for (uint32_t b = 0; b < OWN; ++b) hist[tid + b * THREADS] = 0;
     __syncthreads();
-    for (uint32_t j = tid; j < n; j += 1024) {
-      const uint32_t key = keep_key(acc[j], pos[j], late);
-      if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load(tile, n);
+      each([&](uint32_t, uint32_t key) {
+        if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+      });
     }
     __syncthreads();
-    // thread t's bins from the top: the keys above them, then bin by bin
-    const uint32_t per = bins / 1024 ? bins / 1024 : 1;
-    uint32_t mine = 0;
-    for (uint32_t b = 0; b < per; ++b) {
-      const uint32_t at = tid * per + b;
-      if (at < bins) mine += hist[bins - 1 - at];
+    // the thread's bins from the top: the keys above them, then bin by bin (a
+    // digit of fewer bits leaves the upper bins empty)
+    uint32_t own[OWN], mine = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < OWN; ++b) {
+      own[b] = hist[BINS - 1 - (tid * OWN + b)];
+      mine += own[b];
     }
-    uint32_t total;
-    uint32_t over = block_prefix(mine, s_wave, &total);
+    uint32_t over = block_prefix<WAVES>(mine, s_wave[step & 1], &total);
     if (over < left && over + mine >= left) {
-      for (uint32_t b = 0; b < per; ++b) {
-        const uint32_t bin = bins - 1 - (tid * per + b), c = hist[bin];
-        if (over + c >= left) {
-          s_bin = bin;
+#pragma unroll
+      for (uint32_t b = 0; b < OWN; ++b) {
+        if (over < left && over + own[b] >= left) {
+          s_bin = BINS - 1 - (tid * OWN + b);
           s_left = left - over;
-          break;
+          s_in_bin = own[b];
         }
-        over += c;
+        over += own[b];
       }
     }
     __syncthreads();
     prefix |= s_bin << shift;
     left = s_left;
+    ties = s_in_bin != left;
   }
-  // Slots of that very key: the first `left` of them are kept.  A thread's run
-  // of slots, so that one prefix sum orders them all.
-  const uint32_t per = (n + 1023) / 1024, beg = tid * per < n ? tid * per : n, end = beg + per < n ? beg + per : n;
-  uint32_t equal = 0;
-  for (uint32_t j = beg; j < end; ++j) equal += keep_key(acc[j], pos[j], late) == prefix;
-  uint32_t total;
-  const uint32_t equal0 = block_prefix(equal, s_wave, &total);
-  uint32_t seen_eq = equal0, n_hole = 0, n_src = 0;
-  for (uint32_t j = beg; j < end; ++j) {
-    const uint32_t key = keep_key(acc[j], pos[j], late);
-    const bool keep = key > prefix || (key == prefix && seen_eq++ < left);
-    n_hole += !keep && j < budget;
-    n_src += keep && j >= budget;
-  }
-  uint32_t holes_all, src_all;
-  uint32_t hole = block_prefix(n_hole, s_wave, &holes_all), src = block_prefix(n_src, s_wave, &src_all);
-  seen_eq = equal0;
-  for (uint32_t j = beg; j < end; ++j) {
-    const uint32_t key = keep_key(acc[j], pos[j], late);
-    const bool keep = key > prefix || (key == prefix && seen_eq++ < left);
-    if (j < budget) {
-      if (!keep) {
-        holes[(uint64_t)pair * most + hole++] = j;
-      } else {
-        if (moved) acc_out[base + j] = acc[j];
-        if (moved_pos) pos_out[base + j] = pos[j];
-      }
-    } else if (keep) {
-      sources[(uint64_t)pair * most + src++] = j;
+
+  // Kept: keys above the prefix's range, and in it all or, of that very key, the
+  // first `left`.  Both lists in the order of slots; few moves stay in LDS for
+  // this workgroup.
+  const uint32_t range = 0xFFFFFFFFu << shift;
+  const bool here = a.at_once != 0;
+  uint32_t* holes = here ? s_holes : a.holes + (uint64_t)pair * a.most;
+  uint32_t* sources = here ? s_sources : a.sources + (uint64_t)pair * a.most;
+  uint32_t equal_before = 0, holes_before = 0, sources_before = 0;
+#pragma unroll 1
+  for (uint32_t tile = 0; tile < tiles; ++tile) {
+    if (tiles > 1) load(tile, n);
+    uint32_t passed = 0;
+    if (ties) {
+      uint32_t equal = 0;
+      each([&](uint32_t, uint32_t key) { equal += (key & range) == prefix; });
+      if (tile) __syncthreads();  // the last tile's sums have been read
+      passed = equal_before + block_prefix<WAVES>(equal, s_wave[0], &total);
+      equal_before += total;
     }
+    uint32_t given = 0, taken = 0;  // a bit a slot: given up below the budget, kept from it on
+    each([&](uint32_t j, uint32_t key) {
+      const bool keep = (key & range) > prefix || ((key & range) == prefix && (!ties || passed++ < left));
+      const uint32_t bit = 1u << (j - beg);
+      given |= !keep && j < budget ? bit : 0u;
+      taken |= keep && j >= budget ? bit : 0u;
+    });
+    if (tile) __syncthreads();
+    // a tile's counts fit 16 bits each
+    const uint32_t before =
+        block_prefix<WAVES>(((uint32_t)__popc(taken) << 16) | (uint32_t)__popc(given), s_wave[1], &total);
+    uint32_t hole = holes_before + (before & 0xFFFFu), src = sources_before + (before >> 16);
+    holes_before += total & 0xFFFFu;
+    sources_before += total >> 16;
+    for (; given; given &= given - 1) holes[hole++] = beg + (uint32_t)__ffs((int)given) - 1;
+    for (; taken; taken &= taken - 1) sources[src++] = beg + (uint32_t)__ffs((int)taken) - 1;
+    copy();
   }
-  if (tid == 0) count[pair] = holes_all;
+  if (here) {
+    __syncthreads();
+    const uint32_t lanes = a.kv.head_dim / 8;
+    evict_moves(a, pair, s_holes, s_sources, tid / lanes, holes_before, THREADS / lanes);
+  } else if (tid == 0) {
+    a.count[pair] = holes_before;
+  }
 }
 
-// The moves: a row of K and of V (16 bytes a lane), the slot's weight and
-// position.  Sources lie from the budget on and are never written, so the order
-// does not matter.  grid = (pairs, ceil(most / 64)); 64 moves a workgroup.
-extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_move(
-    PagedKv kv, const float* acc_in, const uint32_t* pos_in, float* acc_out, uint32_t* pos_out,
-    const uint32_t* count, const uint32_t* holes, const uint32_t* sources, uint32_t most) {
-  const uint32_t pair = blockIdx.x, row = pair / kv.kv_heads, h = pair % kv.kv_heads;
-  const uint32_t n = count[pair], lanes = kv.head_dim / 8;
-  const uint32_t lane = threadIdx.x % lanes, first = blockIdx.y * 64 + threadIdx.x / lanes;
-  const uint32_t end = blockIdx.y * 64 + 64 < n ? blockIdx.y * 64 + 64 : n;
-  const uint64_t base = (uint64_t)pair * paged_slots(kv), list = (uint64_t)pair * most;
-  for (uint32_t i = first; i < end; i += 256 / lanes) {
-    const uint32_t to = holes[list + i], from = sources[list + i];
-    uint64_t dst, src;
-    if (paged_place(kv, row, h, to, &dst) && paged_place(kv, row, h, from, &src)) {
-      const u32x4_t k = *reinterpret_cast<const u32x4_t*>(kv.k + src + 8 * lane);
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(kv.v + src + 8 * lane);
-      *reinterpret_cast<u32x4_t*>(kv.k + dst + 8 * lane) = k;
-      *reinterpret_cast<u32x4_t*>(kv.v + dst + 8 * lane) = v;
-    }
-    if (lane == 0) {
-      acc_out[base + to] = acc_in[base + from];
-      pos_out[base + to] = pos_in[base + from];
-    }
-  }
+}  // namespace
+
+// One workgroup per (row, kv head)
+extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_choose_1k(EvictArgs a) { evict_choose<256, 4>(a); }
+extern "C" __global__ __launch_bounds__(1024) void catena_kv_evict_choose_8k(EvictArgs a) { evict_choose<1024, 8>(a); }
+
+// grid = (pairs, ceil(most / 64)); 64 moves a workgroup
+extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_move(EvictArgs a) {
+  const uint32_t pair = blockIdx.x, lanes = a.kv.head_dim / 8, first = blockIdx.y * 64, n = a.count[pair];
+  if (first >= n) return;
+  evict_moves(a, pair, a.holes + (uint64_t)pair * a.most, a.sources + (uint64_t)pair * a.most,
+              first + threadIdx.x / lanes, n - first < 64 ? n : first + 64, 256 / lanes);
 }
 
 // ------------------------------------------------------------------ reorder

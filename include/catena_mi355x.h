@@ -388,8 +388,8 @@ int catena_mi355x_kv_evict_paged_plan(const catena_paged_kv_t *kv, uint32_t budg
  * they are.  (Attention does not depend on the order of slots; RoPE is applied
  * before the append.)  lens_out[rows] is the new length.  acc_in / acc_out and
  * slot_pos_in / slot_pos_out ([rows][kv_heads][max_pages * page_size]) are each
- * two buffers or the same one; entries past the new length are left as they
- * are.  lens_out is not lens.  The pages must be the row's own (a page that
+ * two buffers or the same one, 16-byte aligned; entries past the new length are
+ * left as they are.  lens_out is not lens.  The pages must be the row's own (a page that
  * catena_mi355x_beam_reorder_paged_bf16 shares changes for all its rows).
  * workspace as for catena_mi355x_attn_paged_bf16.  No reference counterpart. */
 int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t *kv, const uint32_t *lens,

@@ -138,6 +138,8 @@ def test_evict_refuses_bad_arguments():
     for name in ("lens", "seen", "acc", "pos", "lens_out", "acc_out", "pos_out"):
         refused(INVALID, evict, kv, **{name: 0})
         refused(INVALID, evict, kv, **{name: P + 2})
+    for name in ("acc", "pos", "acc_out", "pos_out"):
+        refused(INVALID, evict, kv, **{name: P + 8})
     for over in (dict(budget=0), dict(lens_out=P), dict(work=None), dict(work=(0, need)), dict(work=(P, need - 1)), dict(work=(P + 4, need))):
         refused(INVALID, evict, kv, **over)
     refused(INVALID, ca.kv_evict_paged_plan, kv, 0)
