@@ -74,16 +74,19 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   const uint64_t tiles = units * ceil_div(slots, 32);
   if (units > 0x3FFFFFFFull || tiles > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows, heads and slots");
   // A workgroup per unit while a row's slots take no longer than cutting them
-  // costs: half a row at one CU's 38 GB/s (rows of a batch are taken to be half
-  // full) against 5.5 us of a second kernel and 1/128 us a unit of short parts.
-  // Units x slots of 128, a unit each / cut: 16 x 640 8.9 / 8.9 us, x 1280 17.7 /
-  // 9.7; 64 x 1024 14.7 / 12.6; 512 x 512 17.9 / 28.4, x 1024 32.6 / 37.6, x 2048 57
-  // / 54, x 4096 119 / 90; 2048 x 640 57 / 102.  With weights only where a unit is
-  // all of its kv head, whose weights it then adds itself.
+  // costs: a row at one CU's 38 GB/s against a second kernel and, the more units
+  // there are, their short parts.  Units x slots of 128 (ragged from 256 on), a unit
+  // each / cut, us: 16 x 384 6.7 / 8.0, x 512 7.9 / 8.0, x 2048 28.5 / 9.4; 64 x 512
+  // 10.1 / 9.0; 128 x 640 12.8 / 13.0; 256 x 1024 18.0 / 25.5, x 1536 25.9 / 32.9
+  // (a unit for every CU); 512 x 1024 32.6 / 37, x 1536 47.7 / 44.7, x 4096 119 / 89;
+  // 1024 x 2048 97 / 101, x 4096 209 / 178; 2048 x 2048 191 / 214, x 4096 364 / 356.
+  // With weights only where a unit is all of its kv head, whose weights it then
+  // adds itself.
   // Cut: two workgroups a CU, no fewer than four tiles each; one a CU once those
   // are long (32768 tiles: 83.1 us against 85.3).
   const uint64_t row_bytes = slots * kv.head_dim * 4;
-  if (row_bytes <= 418000 + 594 * units && !(weights && p->head_tiles > 1))
+  const uint64_t short_row = units > 128 && units <= 256 ? 1000000 : 230000 + 850 * units;
+  if (row_bytes <= short_row && !(weights && p->head_tiles > 1))
     p->blocks = 0;
   else
     p->blocks = (uint32_t)std::min<uint64_t>(tiles >= 16384 ? 256 : 512, ceil_div(tiles, 4));

@@ -105,22 +105,22 @@ struct AttnPagedArgs {
   float scale_log2;       // scale * log2(e)
 };
 
-CATENA_DEV uint32_t tiles_of(const AttnPagedArgs& a, uint32_t row) {
-  return row < a.kv.rows ? (paged_len(a.kv, a.lens[row]) + 31) / 32 : 0u;
-}
 // Lane r's row among the first 64, kept for the look-ups that follow
 struct FirstRows {
-  uint32_t n, upto;  // its tiles, and those of the rows up to it
+  uint32_t len, upto;  // its slots, and the tiles of the rows up to it
 };
+CATENA_DEV uint32_t len_of(const AttnPagedArgs& a, uint32_t row) {
+  return row < a.kv.rows ? paged_len(a.kv, a.lens[row]) : 0u;
+}
 CATENA_DEV FirstRows first_rows(const AttnPagedArgs& a) {
-  const uint32_t n = tiles_of(a, threadIdx.x & 63u);
-  return FirstRows{n, wave_prefix(n)};
+  const uint32_t len = len_of(a, threadIdx.x & 63u);
+  return FirstRows{len, wave_prefix((len + 31) / 32)};
 }
 CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
   uint32_t all = lane_of(f.upto, 63);
   if (a.kv.rows > 64) {
     uint32_t n = 0;
-    for (uint32_t r = 64 + (threadIdx.x & 63u); r < a.kv.rows; r += 64) n += tiles_of(a, r);
+    for (uint32_t r = 64 + (threadIdx.x & 63u); r < a.kv.rows; r += 64) n += (len_of(a, r) + 31) / 32;
     all += lane_of(wave_prefix(n), 63);
   }
   all *= a.kv.kv_heads * a.head_tiles;
@@ -129,23 +129,24 @@ CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
 // The row that place `at` of the line (below its end) belongs to
 CATENA_DEV RowOnLine row_at_place(const AttnPagedArgs& a, const FirstRows& f, uint32_t at) {
   const uint32_t lane = threadIdx.x & 63u, units = a.kv.kv_heads * a.head_tiles;
-  uint32_t n = f.n, upto = f.upto, r0 = 0;
+  uint32_t len = f.len, upto = f.upto, r0 = 0;
   uint64_t past = __ballot(upto * units > at);
   while (!past && r0 + 64 < a.kv.rows) {
     r0 += 64;
-    n = tiles_of(a, r0 + lane);
-    upto = lane_of(upto, 63) + wave_prefix(n);
+    len = len_of(a, r0 + lane);
+    upto = lane_of(upto, 63) + wave_prefix((len + 31) / 32);
     past = __ballot(upto * units > at);
   }
-  const uint32_t j = (uint32_t)__ffsll((unsigned long long)past) - 1, row = r0 + j, tiles = lane_of(n, j);
-  return RowOnLine{row, paged_len(a.kv, scalar_word(a.lens, row)), tiles, (lane_of(upto, j) - tiles) * units};
+  const uint32_t j = (uint32_t)__ffsll((unsigned long long)past) - 1, n = lane_of(len, j), tiles = (n + 31) / 32;
+  return RowOnLine{r0 + j, n, tiles, (lane_of(upto, j) - tiles) * units};
 }
 CATENA_DEV RowOnLine row_on_line(const AttnPagedArgs& a, const FirstRows& f, uint32_t row) {
-  const uint32_t len = paged_len(a.kv, scalar_word(a.lens, row)), tiles = (len + 31) / 32;
+  const uint32_t len = row < 64 ? lane_of(f.len, row) : paged_len(a.kv, scalar_word(a.lens, row));
+  const uint32_t tiles = (len + 31) / 32;
   uint32_t before = lane_of(f.upto, row < 64 ? row : 63);
   if (row >= 64) {
     uint32_t n = 0;
-    for (uint32_t r = 64 + (threadIdx.x & 63u); r <= row; r += 64) n += tiles_of(a, r);
+    for (uint32_t r = 64 + (threadIdx.x & 63u); r <= row; r += 64) n += (len_of(a, r) + 31) / 32;
     before += lane_of(wave_prefix(n), 63);
   }
   return RowOnLine{row, len, tiles, (before - tiles) * a.kv.kv_heads * a.head_tiles};
@@ -512,8 +513,7 @@ template <int D, bool F32>
 CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const uint32_t pair = blockIdx.x, row = pair / a.kv.kv_heads, kvh = pair % a.kv.kv_heads;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t heads = a.group * a.kv.kv_heads, slots = paged_slots(a.kv);
+  const uint32_t tid = threadIdx.x, heads = a.group * a.kv.kv_heads;
   const uint32_t part_heads = a.group < 16 ? a.group : 16;
   const FirstRows rows = first_rows(a);
   const Line line = line_of(a, rows);
@@ -530,39 +530,34 @@ CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
     if (p.n == 1) return;
     const uint32_t lanes = D / 4 / pieces;  // a part's columns, 16 bytes each
     const uint32_t col = piece * lanes * 4 + tid % lanes * 4, mine = tid / lanes, step = 256 / lanes;
-    __shared__ float s_red[4][2];
+    // a thread's parts with a running maximum, then the threads' sums of a column
+    __shared__ f32x2 s_ml[64];
     __shared__ __attribute__((aligned(16))) float s_o[256 * 4];
-    float m = kNegInf;
-    for (uint32_t i = tid; i < p.n; i += 256) m = __builtin_fmaxf(m, ml[part(p, i, head % 16)][0]);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-    if (lane == 0) s_red[wave][0] = m;
-    __syncthreads();
-    m = __builtin_fmaxf(__builtin_fmaxf(s_red[0][0], s_red[1][0]), __builtin_fmaxf(s_red[2][0], s_red[3][0]));
-    const float base = anchor(m);
-    float l = 0.0f;
+    float m = kNegInf, l = 0.0f;
     f32x4_t o = f32x4_t{0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t i = mine; i < p.n; i += step) {
       const uint64_t at = part(p, i, head % 16);
       const f32x2 x = ml[at];
       const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + col);
-      const float f = exp2_fast(x[0] - base);
-      l = l + x[1] * f;
+      const float m2 = __builtin_fmaxf(m, x[0]), f = exp2_fast(m - anchor(m2)), e = exp2_fast(x[0] - anchor(m2));
+      m = m2;
+      l = l * f + x[1] * e;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = o[j] + y[j] * f;
+      for (int j = 0; j < 4; ++j) o[j] = o[j] * f + y[j] * e;
     }
-    // over the parts: lanes of one column are `lanes` apart
     *reinterpret_cast<f32x4_t*>(&s_o[4 * tid]) = o;
-    l = tid % lanes == 0 ? l : 0.0f;  // each part once
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) l = l + __shfl_xor(l, d);
-    if (lane == 0) s_red[wave][1] = l;
+    if (tid % lanes == 0) s_ml[mine] = f32x2{m, l};
     __syncthreads();
     if (tid >= lanes * 4) return;
-    l = (s_red[0][1] + s_red[1][1]) + (s_red[2][1] + s_red[3][1]);
+    for (uint32_t i = 0; i < step; ++i) m = __builtin_fmaxf(m, s_ml[i][0]);
+    l = 0.0f;
     float sum = 0.0f;
-    for (uint32_t i = 0; i < step; ++i) sum = sum + s_o[i * lanes * 4 + tid];
+    for (uint32_t i = 0; i < step; ++i) {
+      const float f = exp2_fast(s_ml[i][0] - anchor(m));
+      l = l + s_ml[i][1] * f;
+      sum = sum + s_o[i * lanes * 4 + tid] * f;
+    }
     const float x = r.len ? sum / l : 0.0f;
     const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + piece * lanes * 4 + tid;
     if constexpr (F32)
