@@ -54,6 +54,28 @@ CATENA_DEV uint64_t wave_max64(uint64_t x) {
   return ((uint64_t)hi << 32) | lo;
 }
 
+// The sum of the wave's values in f64: within rows of 16 lanes, then rows to rows
+CATENA_DEV double wave_sum64(double x) {
+#define CATENA_DPP_ADD64(ctrl, rows)                                                                        \
+  {                                                                                                         \
+    const uint64_t b = (uint64_t)__double_as_longlong(x);                                                     \
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, (ctrl), (rows), 0xF, false); \
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), (ctrl), (rows), 0xF, false);   \
+    x = x + __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));                                     \
+  }
+  CATENA_DPP_ADD64(0x111, 0xF);
+  CATENA_DPP_ADD64(0x112, 0xF);
+  CATENA_DPP_ADD64(0x114, 0xF);
+  CATENA_DPP_ADD64(0x118, 0xF);
+  CATENA_DPP_ADD64(0x142, 0xA);
+  CATENA_DPP_ADD64(0x143, 0xC);
+#undef CATENA_DPP_ADD64
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+
 // A bound that at least `beams` of the wave's 64 values reach (of those that are
 // not 0; 0 where there are fewer), near the largest such one
 CATENA_DEV uint32_t wave_bound(uint32_t x, uint32_t beams) {
@@ -79,7 +101,7 @@ CATENA_DEV void beam_runs(const float* __restrict__ logits, const uint32_t* __re
   __shared__ float s_max[4];
   __shared__ double s_sum[4];
   __shared__ uint32_t s_bound[4], s_count;
-  __shared__ uint64_t s_key[LIST], s_wave[4];
+  __shared__ uint64_t s_key[LIST + 8], s_wave[4];
   const uint32_t row = blockIdx.x, run = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   if (done && done[row]) return;
   const uint32_t first = run * 256 * PER + tid;
@@ -115,9 +137,7 @@ CATENA_DEV void beam_runs(const float* __restrict__ logits, const uint32_t* __re
   float sum[4] = {};
 #pragma unroll
   for (int k = 0; k < PER; ++k) sum[k % 4] = sum[k % 4] + __builtin_amdgcn_exp2f((v[k] - c) * kLog2e);
-  double total = (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) total = total + __shfl_xor(total, d);
+  const double total = wave_sum64((double)((sum[0] + sum[1]) + (sum[2] + sum[3])));
   if (lane == 0) s_sum[wave] = total;
   if (mine >= bound) {
     const float least = bound == 1u ? -__FLT_MAX__ : offered(bound);
@@ -143,10 +163,14 @@ CATENA_DEV void beam_runs(const float* __restrict__ logits, const uint32_t* __re
   const uint32_t n = s_count;
   uint64_t* out = best + part * beams;
   if (n <= LIST) {
+    if (tid < 8) s_key[n + tid] = 0;  // eight at a time
+    __syncthreads();
     for (uint32_t i = tid; i < n; i += 256) {
       const uint64_t key = s_key[i];
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; ++j) rank += s_key[j] > key;
+      for (uint32_t j = 0; j < n; j += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += s_key[j + e] > key;
       if (rank < beams) out[rank] = key;
     }
     if (tid >= n && tid < beams) out[tid] = 0;
@@ -202,15 +226,18 @@ CATENA_DEV void largest_of(const uint64_t* keys, uint32_t n, bool more, uint64_t
     if (in && at < WLIST) list[at] = k[i];
     count += (uint32_t)__popcll(have);
   }
+  if (count <= WLIST && lane < 8) list[count + lane] = 0;  // eight at a time
   __builtin_amdgcn_wave_barrier();
   if (count <= WLIST) {
     const uint64_t a = lane < count ? list[lane] : 0ull, b = lane + 64 < count ? list[lane + 64] : 0ull;
     uint32_t above_a = 0, above_b = 0;
-    for (uint32_t j = 0; j < count; ++j) {
-      const uint64_t x = list[j];
-      above_a += x > a;
-      above_b += x > b;
-    }
+    for (uint32_t j = 0; j < count; j += 8)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint64_t x = list[j + e];
+        above_a += x > a;
+        above_b += x > b;
+      }
     if (a && above_a < beams) best[above_a] = a;
     if (b && above_b < beams) best[above_b] = b;
     if (lane >= count && lane < beams) best[lane] = 0;
@@ -252,7 +279,7 @@ extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
     uint32_t* done_out, uint32_t runs, uint32_t beams, uint32_t eos) {
   __shared__ uint64_t s_best[32][32];  // with_token, then the scores as ordered integers
   __shared__ uint32_t s_token[32][32];
-  __shared__ uint64_t s_list[16][WLIST];
+  __shared__ uint64_t s_list[16][WLIST + 8];
   __shared__ uint32_t s_done[32];
   const uint32_t group = blockIdx.x, lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -277,12 +304,11 @@ extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
     }
     const float mine = m;
     for (uint32_t r = lane + 64; r < runs; r += 64) m = __builtin_fmaxf(m, pm[r]);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+    const uint32_t top = wave_umax(offer(m));
+    m = top ? offered(top) : kNegInf;
     sum = lane < runs ? sum * exp((double)mine - (double)m) : 0.0;
     for (uint32_t r = lane + 64; r < runs; r += 64) sum = sum + ps[r] * exp((double)pm[r] - (double)m);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum = sum + __shfl_xor(sum, d);
+    sum = wave_sum64(sum);
     const double shift = over ? score : score - ((double)m + log(sum));
     // the row's continuations: 0 where it has no more, or offers none
     if (lane == 0) s_done[w] = over;
