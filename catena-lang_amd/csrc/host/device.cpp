@@ -128,7 +128,8 @@ const KernelSpec kKernels[] = {
     {KernelId::KvEvictChoose1k, "kv_paged", "catena_kv_evict_choose_1k"},
     {KernelId::KvEvictChoose8k, "kv_paged", "catena_kv_evict_choose_8k"},
     {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
-    {KernelId::KvReorder, "kv_paged", "catena_kv_reorder"},
+    {KernelId::KvReorder8, "kv_paged", "catena_kv_reorder_8"},
+    {KernelId::KvReorder128, "kv_paged", "catena_kv_reorder_128"},
     {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},
     {KernelId::BeamRuns16, "beam", "catena_beam_runs_16"},
     {KernelId::BeamJoin, "beam", "catena_beam_join"},

@@ -91,7 +91,8 @@ enum class KernelId : int {
   KvEvictChoose1k,
   KvEvictChoose8k,
   KvEvictMove,
-  KvReorder,
+  KvReorder8,
+  KvReorder128,
   BeamRuns8,  // beam search's selection (beam.hip)
   BeamRuns16,
   BeamJoin,

@@ -132,9 +132,20 @@ struct EvictArgs {
   uint32_t most, budget, recent, at_once;
 };
 
-// struct ReorderPools of kv_paged.hip
+// structs ReorderArgs and ReorderPools of kv_paged.hip, field for field
+struct ReorderArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* parents;
+  const uint32_t* spare;
+  uint32_t* table_out;
+  uint32_t* lens_out;
+  uint32_t* spare_out;
+  uint32_t n_pools, tables;
+};
+constexpr uint32_t kReorderFew = 8, kReorderMost = 128;
 struct ReorderPools {
-  uint16_t* p[128];
+  uint16_t* p[kReorderMost];
 };
 }  // namespace
 
@@ -301,14 +312,17 @@ int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t* kv, uint16_t*
   if (c.rows > 0x7FFFFFFFu) return fail(CATENA_ERR_UNSUPPORTED, "too many rows");
   st = ensure_init();
   if (st) return st;
-  // 128 pools a launch (their pointers are kernel arguments); the table once
-  for (uint32_t first = 0; first == 0 || first < n_pools; first += 128) {
-    uint32_t n = std::min(n_pools - first, 128u);
-    ReorderPools p{};
-    for (uint32_t i = 0; i < n; ++i) p.p[i] = pools[first + i];
-    uint32_t tables = first == 0;
-    void* args[] = {&c, &p, &n, &tables, &lens, &parents, &spare, &table_out, &lens_out, &spare_out};
-    st = launch(KernelId::KvReorder, dim3(c.rows, n ? c.kv_heads : 1, n ? n : 1), dim3(256), 0, args);
+  // the pools in as many launches as their pointers need; the table once
+  for (uint32_t first = 0; first == 0 || first < n_pools; first += kReorderMost) {
+    ReorderArgs a{c, lens, parents, spare, table_out, lens_out, spare_out, std::min(n_pools - first, kReorderMost),
+                  first == 0};
+    ReorderPools p;
+    const bool few = a.n_pools <= kReorderFew;
+    for (uint32_t i = 0; i < (few ? kReorderFew : kReorderMost); ++i)
+      p.p[i] = i < a.n_pools ? pools[first + i] : nullptr;
+    void* args[] = {&a, &p};
+    st = launch(few ? KernelId::KvReorder8 : KernelId::KvReorder128,
+                dim3(c.rows, a.n_pools ? c.kv_heads : 1, a.n_pools ? a.n_pools : 1), dim3(256), 0, args);
     if (st) return st;
   }
   return CATENA_OK;

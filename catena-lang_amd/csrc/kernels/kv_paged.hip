@@ -196,6 +196,7 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
   constexpr uint32_t LISTS = 64;
   __shared__ uint32_t hist[BINS];
   __shared__ uint32_t s_wave[2][WAVES], s_bin, s_left, s_in_bin, s_holes[LISTS], s_sources[LISTS];
+  __shared__ uint64_t s_low[WAVES];
   const uint32_t pair = blockIdx.x, row = pair / a.kv.kv_heads, tid = threadIdx.x, budget = a.budget;
   const uint32_t slots = paged_slots(a.kv);
   const uint64_t base = (uint64_t)pair * slots;
@@ -250,6 +251,32 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
       if (tiles > 1) load(tile, n);
       copy();
     }
+    if (tid == 0 && !a.at_once) a.count[pair] = 0;
+    return;
+  }
+
+  // One slot too many, as behind every step of a full cache: the smallest key, the
+  // higher slot of equal ones, is given up, and the last slot takes its place.
+  if (n - budget == 1) {
+    uint64_t low = ~0ull;
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load(tile, n);
+      each([&](uint32_t j, uint32_t key) {
+        const uint64_t x = ((uint64_t)key << 32) | ~j;
+        low = x < low ? x : low;
+      });
+      copy();
+    }
+    const uint32_t hi = ~wave_umax(~(uint32_t)(low >> 32));
+    const uint32_t lo = ~wave_umax((uint32_t)(low >> 32) == hi ? ~(uint32_t)low : 0u);
+    if (tid % 64 == 0) s_low[tid / 64] = ((uint64_t)hi << 32) | lo;
+    __syncthreads();
+    low = s_low[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) low = s_low[i] < low ? s_low[i] : low;
+    const uint32_t to = ~(uint32_t)low;
+    if (to < budget && tid < a.kv.head_dim / 8) evict_moves(a, pair, &to, &budget, 0, 1, 1);
     if (tid == 0 && !a.at_once) a.count[pair] = 0;
     return;
   }
@@ -370,35 +397,57 @@ extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_move(EvictArgs
 //
 // grid = (rows, kv_heads, pools): one (row, head, pool)'s slots of the last page;
 // the workgroups of head 0 and pool 0 write the row's table.
-struct ReorderPools {
-  uint16_t* p[128];
+struct ReorderArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* parents;
+  const uint32_t* spare;
+  uint32_t* table_out;
+  uint32_t* lens_out;
+  uint32_t* spare_out;
+  uint32_t n_pools, tables;
 };
-extern "C" __global__ __launch_bounds__(256) void catena_kv_reorder(
-    PagedKv kv, ReorderPools pools, uint32_t n_pools, uint32_t tables, const uint32_t* lens, const uint32_t* parents,
-    const uint32_t* spare, uint32_t* table_out, uint32_t* lens_out, uint32_t* spare_out) {
+template <int MOST>
+struct ReorderPools {
+  uint16_t* p[MOST];
+};
+
+namespace {
+CATENA_DEV void kv_reorder(const ReorderArgs& a, uint16_t* const* pools) {
+  const PagedKv& kv = a.kv;
   const uint32_t r = blockIdx.x, h = blockIdx.y, mask = (1u << kv.page_shift) - 1u;
-  const uint32_t p = parents[r];
-  const uint32_t n = p < kv.rows ? lens[p] : 0u;
-  const bool good = p < kv.rows && n == lens[r] && n <= paged_slots(kv);
+  const uint32_t p = a.parents[r];
+  const uint32_t n = p < kv.rows ? a.lens[p] : 0u;
+  const bool good = p < kv.rows && n == a.lens[r] && n <= paged_slots(kv);
   const uint32_t last = n >> kv.page_shift, used = n & mask;
   const bool copies = good && p != r && used != 0;
   const uint32_t* mine = kv.table + (uint64_t)r * kv.max_pages;
   const uint32_t* theirs = kv.table + (uint64_t)(good ? p : r) * kv.max_pages;
-  if (tables && h == 0 && blockIdx.z == 0) {
-    uint32_t* out = table_out + (uint64_t)r * kv.max_pages;
+  if (a.tables && h == 0 && blockIdx.z == 0) {
+    uint32_t* out = a.table_out + (uint64_t)r * kv.max_pages;
     for (uint32_t j = threadIdx.x; j < kv.max_pages; j += 256)
-      out[j] = !good ? 0xFFFFFFFFu : j < last ? theirs[j] : j == last && copies ? spare[r] : mine[j];
+      out[j] = !good ? 0xFFFFFFFFu : j < last ? theirs[j] : j == last && copies ? a.spare[r] : mine[j];
     if (threadIdx.x == 0) {
-      lens_out[r] = good ? n : 0u;
-      spare_out[r] = copies ? mine[last] : spare[r];
+      a.lens_out[r] = good ? n : 0u;
+      a.spare_out[r] = copies ? mine[last] : a.spare[r];
     }
   }
-  if (!copies || blockIdx.z >= n_pools) return;
-  const uint32_t from = theirs[last], to = spare[r];
+  if (!copies || blockIdx.z >= a.n_pools) return;
+  const uint32_t from = theirs[last], to = a.spare[r];
   if (from >= kv.num_pages || to >= kv.num_pages) return;
-  uint16_t* pool = pools.p[blockIdx.z];
+  uint16_t* pool = pools[blockIdx.z];
   const u32x4_t* src = reinterpret_cast<const u32x4_t*>(pool + paged_offset(kv, from, h, 0));
   u32x4_t* dst = reinterpret_cast<u32x4_t*>(pool + paged_offset(kv, to, h, 0));
   const uint32_t chunks = used * (kv.head_dim / 8);
   for (uint32_t i = threadIdx.x; i < chunks; i += 256) dst[i] = src[i];
+}
+}  // namespace
+
+// The pools' pointers are kernel arguments: up to 8 (a few layers) or up to 128,
+// whose 1 KiB takes 0.5 us longer to hand over.
+extern "C" __global__ __launch_bounds__(256) void catena_kv_reorder_8(ReorderArgs a, ReorderPools<8> pools) {
+  kv_reorder(a, pools.p);
+}
+extern "C" __global__ __launch_bounds__(256) void catena_kv_reorder_128(ReorderArgs a, ReorderPools<128> pools) {
+  kv_reorder(a, pools.p);
 }

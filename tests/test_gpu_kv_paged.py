@@ -208,6 +208,7 @@ def _weights(rng, kind, shape, slots):
     (4, 128, 64, 10, 511, 100, [640, 512, 513]),   # one slot, and many
     (1, 64, 16, 200, 1000, 64, [3200, 1500]),
     (2, 128, 16, 3, 48, 4, [48, 20]),              # a budget of the whole table
+    (2, 64, 16, 100, 1200, 7, [1201, 1600, 1202]), # one slot, two and many of a longer row
 ])
 def test_evict(kvh, dim, page, pages, budget, recent, lens, kind, in_place):
     say(f"evict budget {budget} recent {recent} {kind} in place {in_place}")
@@ -221,13 +222,14 @@ def test_evict(kvh, dim, page, pages, budget, recent, lens, kind, in_place):
     case.check()
 
 
-def test_evict_long_row():
-    """More slots than a workgroup has threads by far, heads that differ."""
-    say("evict long row")
+@pytest.mark.parametrize("budget", [50000, 70000])
+def test_evict_long_row(budget):
+    """More slots than a workgroup holds, heads that differ; one slot too many."""
+    say(f"evict long row {budget}")
     rng = np.random.default_rng(21)
     cache = Cache(rng, [70001], 2, 64, 1024, 69)
     pos = np.stack([rng.permutation(cache.slots) for _ in range(2)])[None].astype(np.uint32)
-    case = Evict(cache, _weights(rng, "spread", (1, 2, cache.slots), cache.slots), pos, np.array([cache.slots], np.uint32), 50000, 3000, False)
+    case = Evict(cache, _weights(rng, "spread", (1, 2, cache.slots), cache.slots), pos, np.array([cache.slots], np.uint32), budget, 3000, False)
     case()
     case.check()
 
