@@ -309,6 +309,11 @@ class Buffer:
         return self.mem.data or 0
 
     @property
+    def _as_parameter_(self):
+        """What ctypes passes for a buffer: its device pointer (None if empty)."""
+        return self.mem.data
+
+    @property
     def nbytes(self) -> int:
         return self.mem.len
 
@@ -477,15 +482,14 @@ def gemm_bf16_ksplit_f32(a, b, parts, n: int, m: int, k: int, splits: int) -> No
     check(lib().catena_mi355x_gemm_bf16_ksplit_f32(_p(a), _p(b), _p(parts), n, m, k, splits))
 
 
-def _opt(x):
-    return None if x is None else _p(x)
-
-
+# The calls below pass Buffers, pointers (int) and None to ctypes as they are: a
+# decode step makes many small ones, and a conversion of each argument here would
+# cost as much as the launch leaves.
 def _workspace(w):
-    """(pointer, bytes) of a workspace: a Buffer, such a pair, or None."""
-    if w is None:
-        return None, 0
-    return (w.ptr, w.nbytes) if isinstance(w, Buffer) else w
+    """(pointer, bytes) of a workspace: such a pair, a Buffer, or None."""
+    if type(w) is tuple:
+        return w
+    return (None, 0) if w is None else (w.ptr, w.nbytes)
 
 
 def attn_paged_plan(kv: PagedKV, heads: int, weights: bool = False):
@@ -500,8 +504,8 @@ def attn_paged_bf16(kv: PagedKV, q, lens, o, heads: int, scale: float, workspace
                     out_f32: bool = False, acc_in=None, acc_out=None) -> None:
     """One new token per row over a cache in pages; workspace is a Buffer or a
     (pointer, bytes) pair of attn_paged_plan's size."""
-    check(lib().catena_mi355x_attn_paged_bf16(kv, _p(q), _p(lens), _p(o), heads, scale,
-                                              1 if out_f32 else 0, _opt(acc_in), _opt(acc_out),
+    check(lib().catena_mi355x_attn_paged_bf16(kv, q, lens, o, heads, scale,
+                                              1 if out_f32 else 0, acc_in, acc_out,
                                               *_workspace(workspace)))
 
 
@@ -509,9 +513,9 @@ def rope_qkv_paged_bf16(kv: PagedKV, qkv, rope_tab, table_positions: int, lens, 
                         heads: int, acc=None, slot_pos=None) -> None:
     """RoPE of tq tokens a row and their append into pages; lens / seen count
     slots / positions after the append (seen None: as lens)."""
-    check(lib().catena_mi355x_rope_qkv_paged_bf16(kv, _p(qkv), _p(rope_tab), table_positions, _p(lens),
-                                                  _opt(seen), _p(q), tq, heads, _opt(acc),
-                                                  _opt(slot_pos)))
+    check(lib().catena_mi355x_rope_qkv_paged_bf16(kv, qkv, rope_tab, table_positions, lens,
+                                                  seen, q, tq, heads, acc,
+                                                  slot_pos))
 
 
 def kv_evict_paged_plan(kv: PagedKV, budget: int) -> int:
@@ -525,8 +529,8 @@ def kv_evict_paged_bf16(kv: PagedKV, lens, seen, acc_in, slot_pos_in, lens_out, 
                         budget: int, recent: int, workspace) -> None:
     """Keeps `budget` slots per (row, kv head): the last `recent` positions,
     then the largest accumulated weights."""
-    check(lib().catena_mi355x_kv_evict_paged_bf16(kv, _p(lens), _p(seen), _p(acc_in), _p(slot_pos_in),
-                                                  _p(lens_out), _p(acc_out), _p(slot_pos_out), budget,
+    check(lib().catena_mi355x_kv_evict_paged_bf16(kv, lens, seen, acc_in, slot_pos_in,
+                                                  lens_out, acc_out, slot_pos_out, budget,
                                                   recent, *_workspace(workspace)))
 
 
@@ -534,10 +538,10 @@ def beam_reorder_paged_bf16(kv: PagedKV, pools, lens, parents, spare, table_out,
                             spare_out) -> None:
     """Row r goes on as row parents[r] was; pools: the K and V pools of every
     layer under kv's table."""
-    arr = (_vp * len(pools))(*[_p(x) for x in pools])
-    check(lib().catena_mi355x_beam_reorder_paged_bf16(kv, arr, len(pools), _p(lens), _p(parents),
-                                                      _p(spare), _p(table_out), _p(lens_out),
-                                                      _p(spare_out)))
+    arr = (_vp * len(pools))(*[x.ptr if isinstance(x, Buffer) else x for x in pools])
+    check(lib().catena_mi355x_beam_reorder_paged_bf16(kv, arr, len(pools), lens, parents,
+                                                      spare, table_out, lens_out,
+                                                      spare_out))
 
 
 BEAM_NO_EOS = 0xFFFFFFFF  # no token ends a beam
@@ -553,8 +557,8 @@ def beam_select_plan(groups: int, beams: int, vocab: int) -> int:
 def beam_select_f32(logits, scores, done, tokens, parents, scores_out, done_out, groups: int, beams: int,
                     vocab: int, eos: int, workspace) -> None:
     """The best `beams` continuations of every group over beams and vocabulary."""
-    check(lib().catena_mi355x_beam_select_f32(_p(logits), _p(scores), _opt(done), _p(tokens), _p(parents),
-                                              _p(scores_out), _opt(done_out), groups, beams, vocab, eos,
+    check(lib().catena_mi355x_beam_select_f32(logits, scores, done, tokens, parents,
+                                              scores_out, done_out, groups, beams, vocab, eos,
                                               *_workspace(workspace)))
 
 
