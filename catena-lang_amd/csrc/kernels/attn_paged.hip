@@ -450,8 +450,8 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
   // while the tile before it is worked on, across the border of two parts too.
   uint32_t t = now.beg + wave;
   Tile<D> one, two;
-  request(one, now, t);
   begin(now);
+  request(one, now, t);
   auto step = [&](Tile<D>& x, Tile<D>& y) {
     const bool ends = t + kWaves >= now.end, more = at < last;
     Part next = now;
