@@ -111,14 +111,10 @@ CATENA_DEV uint32_t block_prefix(uint32_t x, uint32_t* s_wave, uint32_t* total) 
   const uint32_t in = wave_prefix(x);
   if (lane == 63) s_wave[wave] = in;
   __syncthreads();
-  uint32_t before = 0, sum = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < WAVES; ++w) {
-    const uint32_t v = s_wave[w];
-    before += w < wave ? v : 0u;
-    sum += v;
-  }
-  *total = sum;
+  const uint32_t sums = wave_prefix(lane < WAVES ? s_wave[lane] : 0u);
+  const uint32_t w = __builtin_amdgcn_readfirstlane(wave);
+  *total = (uint32_t)__builtin_amdgcn_readlane((int)sums, WAVES - 1);
+  const uint32_t before = w ? (uint32_t)__builtin_amdgcn_readlane((int)sums, (int)w - 1) : 0u;
   return before + in - x;
 }
 
@@ -223,10 +219,14 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
   const uint32_t tiles = (n + TILE - 1) / TILE;
   if (!single && tiles == 1) load(0, n);
   if (tid == 0 && pair % a.kv.kv_heads == 0) a.lens_out[row] = kept;
-  auto each = [&](auto what) {
+  // the tile's keys; 0, the last of all, behind the row's end
+  uint32_t keys[KEYS];
+  auto rate = [&]() {
 #pragma unroll
-    for (int i = 0; i < KEYS; ++i)
-      if (beg + i < n) what(beg + i, keep_key(w[i / 4][i % 4], p[i / 4][i % 4], late));
+    for (int i = 0; i < KEYS; ++i) {
+      const uint32_t key = keep_key(w[i / 4][i % 4], p[i / 4][i % 4], late);
+      keys[i] = beg + i < n ? key : 0u;
+    }
   };
   // the slots below the budget as they are; the moves overwrite those given up
   auto copy = [&]() {
@@ -254,6 +254,7 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
     if (tid == 0 && !a.at_once) a.count[pair] = 0;
     return;
   }
+  if (tiles == 1) rate();
 
   // One slot too many, as behind every step of a full cache: the smallest key, the
   // higher slot of equal ones, is given up, and the last slot takes its place.
@@ -261,11 +262,12 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
     uint64_t low = ~0ull;
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; ++tile) {
-      if (tiles > 1) load(tile, n);
-      each([&](uint32_t j, uint32_t key) {
-        const uint64_t x = ((uint64_t)key << 32) | ~j;
-        low = x < low ? x : low;
-      });
+      if (tiles > 1) load(tile, n), rate();
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) {
+        const uint64_t x = ((uint64_t)keys[i] << 32) | ~(beg + i);
+        if (beg + i < n) low = x < low ? x : low;
+      }
       copy();
     }
     const uint32_t hi = ~wave_umax(~(uint32_t)(low >> 32));
@@ -293,10 +295,12 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
     __syncthreads();
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; ++tile) {
-      if (tiles > 1) load(tile, n);
-      each([&](uint32_t, uint32_t key) {
-        if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
-      });
+      if (tiles > 1) load(tile, n), rate();
+      if (beg < n) {
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i)
+          if ((keys[i] & known) == prefix) atomicAdd(&hist[(keys[i] >> shift) & (bins - 1)], 1u);
+      }
     }
     __syncthreads();
     // the thread's bins from the top: the keys above them, then bin by bin (a
@@ -328,6 +332,8 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
   // Kept: keys above the prefix's range, and in it all or, of that very key, the
   // first `left`.  Both lists in the order of slots; few moves stay in LDS for
   // this workgroup.
+  // (What lies behind the row's end has the lowest key and the highest slots: it
+  // is counted among equals, never kept.)
   const uint32_t range = 0xFFFFFFFFu << shift;
   const bool here = a.at_once != 0;
   uint32_t* holes = here ? s_holes : a.holes + (uint64_t)pair * a.most;
@@ -335,22 +341,31 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
   uint32_t equal_before = 0, holes_before = 0, sources_before = 0;
 #pragma unroll 1
   for (uint32_t tile = 0; tile < tiles; ++tile) {
-    if (tiles > 1) load(tile, n);
+    if (tiles > 1) load(tile, n), rate();
     uint32_t passed = 0;
     if (ties) {
       uint32_t equal = 0;
-      each([&](uint32_t, uint32_t key) { equal += (key & range) == prefix; });
+      if (beg < n) {
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) equal += (keys[i] & range) == prefix;
+      }
       if (tile) __syncthreads();  // the last tile's sums have been read
       passed = equal_before + block_prefix<WAVES>(equal, s_wave[0], &total);
       equal_before += total;
     }
-    uint32_t given = 0, taken = 0;  // a bit a slot: given up below the budget, kept from it on
-    each([&](uint32_t j, uint32_t key) {
-      const bool keep = (key & range) > prefix || ((key & range) == prefix && (!ties || passed++ < left));
-      const uint32_t bit = 1u << (j - beg);
-      given |= !keep && j < budget ? bit : 0u;
-      taken |= keep && j >= budget ? bit : 0u;
-    });
+    uint32_t kept_bits = 0;  // a bit a slot
+    if (beg < n) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) {
+        const uint32_t key = keys[i] & range;
+        const bool same = key == prefix, keep = key > prefix || (same && (!ties || passed < left));
+        passed += same;
+        kept_bits |= keep ? 1u << i : 0u;
+      }
+    }
+    // given up below the budget, kept from it on
+    const uint32_t below = beg >= budget ? 0u : budget - beg >= KEYS ? (1u << KEYS) - 1u : (1u << (budget - beg)) - 1u;
+    uint32_t given = ~kept_bits & below, taken = kept_bits & ~below;
     if (tile) __syncthreads();
     // a tile's counts fit 16 bits each
     const uint32_t before =
