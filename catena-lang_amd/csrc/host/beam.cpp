@@ -19,7 +19,8 @@ int beam_plan(uint32_t groups, uint32_t beams, uint32_t vocab, BeamPlan* p) {
   if (beams > 32 || vocab > (1u << 26))
     return fail(CATENA_ERR_UNSUPPORTED, "beam selection of %u beams over %u tokens", beams, vocab);
   p->rows = (uint64_t)groups * beams;
-  if (p->rows > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many beams");
+  // (a grid's first side, whose threads may not pass 32 bits)
+  if (p->rows > 0xFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many beams");
   // 16 logits a thread; 8 while that gives less than a workgroup for each CU
   // (4 x 32000: 4.3 us against 4.7; 256 x 128000: 31.8 against 22.7)
   p->per = p->rows * ((vocab + 4095) / 4096) < 256 ? 8 : 16;

@@ -15,6 +15,8 @@ namespace {
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 uint64_t round_up(uint64_t a, uint64_t to) { return ceil_div(a, to) * to; }
+// a grid's first side, whose threads may not pass 32 bits
+constexpr uint64_t grid_most(uint32_t threads) { return 0xFFFFFFFFull / threads; }
 
 // The cache's sizes (and with `pools` its pointers) checked, as the kernels
 // take them.
@@ -56,12 +58,13 @@ struct AttnPagedArgs {
   float* scores;
   const float* acc_in;
   float* acc_out;
-  uint32_t group, head_tiles, blocks;
+  uint32_t group, head_tiles, blocks, short_slots;
   float scale_log2;
 };
 
+constexpr uint64_t kJoinBlocks = 2048;  // eight a CU; they take several rows each
 struct AttnPagedPlan {
-  uint32_t group, head_tiles, blocks, pieces;
+  uint32_t group, head_tiles, blocks, short_slots, pieces;
   uint64_t part_ml, whole_ml, scores, bytes;  // offsets and the sum; part_o comes first
 };
 
@@ -72,25 +75,33 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   p->head_tiles = (uint32_t)ceil_div(p->group, 16);
   const uint64_t slots = paged_slots(kv), pairs = (uint64_t)kv.rows * kv.kv_heads, units = pairs * p->head_tiles;
   const uint64_t tiles = units * ceil_div(slots, 32);
-  if (units > 0x3FFFFFFFull || tiles > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows, heads and slots");
-  // A workgroup per unit while a row's slots take no longer than cutting them
-  // costs: a row at one CU's 38 GB/s against a second kernel and, the more units
-  // there are, their short parts.  Units x slots of 128 (ragged from 256 on), a unit
-  // each / cut, us: 16 x 384 6.7 / 8.0, x 512 7.9 / 8.0, x 2048 28.5 / 9.4; 64 x 512
-  // 10.1 / 9.0; 128 x 640 12.8 / 13.0; 256 x 1024 18.0 / 25.5, x 1536 25.9 / 32.9
-  // (a unit for every CU); 512 x 1024 32.6 / 37, x 1536 47.7 / 44.7, x 4096 119 / 89;
-  // 1024 x 2048 97 / 101, x 4096 209 / 178; 2048 x 2048 191 / 214, x 4096 364 / 356.
-  // With weights only where a unit is all of its kv head, whose weights it then
-  // adds itself.
-  // Cut: two workgroups a CU, no fewer than four tiles each; one a CU once those
-  // are long (32768 tiles: 83.1 us against 85.3).
-  const uint64_t row_bytes = slots * kv.head_dim * 4;
+  // (a grid's second side is 65535 at most: 4 pieces a head of a kv head, and with
+  // weights a strip for every 1024 slots)
+  if (units > 0x7FFFFFFull || tiles > 0x7FFFFFFFull || 4ull * p->group + (weights ? slots / 1024 + 1 : 0) > 65535)
+    return fail(CATENA_ERR_UNSUPPORTED, "too many rows, heads and slots");
+  // Whole units while a row's slots take no longer than cutting them costs: a row
+  // at one CU's 38 GB/s against a join and, the more units there are, their short
+  // parts.  Units x slots of 128 (ragged from 256 on), a workgroup a unit / cut, us:
+  // 16 x 384 6.7 / 8.0, x 512 7.9 / 8.0, x 2048 28.5 / 9.4; 64 x 512 10.1 / 9.0; 128 x
+  // 640 12.8 / 13.0; 256 x 1024 18.0 / 25.5, x 1536 25.9 / 32.9 (a unit for every CU);
+  // 512 x 1024 32.6 / 37, x 1536 47.7 / 44.7, x 4096 119 / 89; 1024 x 2048 97 / 101, x
+  // 4096 209 / 178; 2048 x 2048 191 / 214, x 4096 364 / 356.
+  // Where a full table is that short, a workgroup per unit and no second kernel
+  // (which weights of several units of one kv head need all the same); else two
+  // workgroups a CU at most (one where a long table's few units fill no more), no
+  // fewer than four tiles each, and both kernels apply the rule to the longest row
+  // that they find: 64 rows x 8 heads in tables of 4096 slots, 1 .. 100 of them in
+  // use 8.6 us (cut 16), 1 .. 300 14.3 (27), 1 .. 600 22 (32).
   const uint64_t short_row = units > 128 && units <= 256 ? 1000000 : 230000 + 850 * units;
-  if (row_bytes <= short_row && !(weights && p->head_tiles > 1))
+  p->short_slots = (uint32_t)std::min<uint64_t>(short_row / (kv.head_dim * 4), slots);
+  if (p->short_slots == slots && !(weights && p->head_tiles > 1))
     p->blocks = 0;
   else
-    p->blocks = (uint32_t)std::min<uint64_t>(tiles >= 16384 ? 256 : 512, ceil_div(tiles, 4));
-  p->pieces = p->blocks > 16 * units ? 4 : 1;
+    p->blocks = (uint32_t)std::min<uint64_t>(tiles >= 16384 && units <= 256 ? 256 : 512, ceil_div(tiles, 4));
+  // the join by a unit's number of parts: a thread takes all of them, or some, or
+  // some of a quarter of the columns (1 part a unit 5.0 / 6.6 us, 5 parts 4.5 / 3.7 /
+  // 4.6, 64 parts - / 26 / 5)
+  p->pieces = p->blocks <= 2 * units ? 0 : p->blocks <= 16 * units ? 1 : 4;
   const uint64_t parts = 2ull * p->blocks * std::min(p->group, 16u);
   p->part_ml = parts * kv.head_dim * 4;
   p->whole_ml = p->part_ml + parts * 8;
@@ -106,11 +117,13 @@ uint32_t evict_most(const PagedKv& kv, uint32_t budget) {
   const uint32_t slots = paged_slots(kv);
   return budget >= slots ? 0 : std::min(budget, slots - budget);
 }
+// a workgroup for a (row, kv head): small while that holds the table
+uint32_t evict_threads(const PagedKv& kv) { return paged_slots(kv) <= 1024 ? 256 : 1024; }
 // count[pairs], holes[pairs][most], sources[pairs][most]
 int evict_plan(const PagedKv& kv, uint32_t budget, uint64_t* bytes) {
   if (budget == 0) return fail(CATENA_ERR_INVALID_ARGUMENT, "a budget of no slots");
   const uint64_t pairs = (uint64_t)kv.rows * kv.kv_heads;
-  if (pairs > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many rows and heads");
+  if (pairs > grid_most(evict_threads(kv))) return fail(CATENA_ERR_UNSUPPORTED, "too many rows and heads");
   if (evict_most(kv, budget) > 65535 * kEvictMoves) return fail(CATENA_ERR_UNSUPPORTED, "eviction of too many slots");
   *bytes = pairs * 4 * (1 + 2ull * evict_most(kv, budget));
   return CATENA_OK;
@@ -196,19 +209,23 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t* kv, const uint16_t* q
   a.group = p.group;
   a.head_tiles = p.head_tiles;
   a.blocks = p.blocks;
+  a.short_slots = p.short_slots;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   // kernels in the order of their ids: D128 f32, D128 bf16, D64 f32, D64 bf16
   const int form = (a.kv.head_dim == 64 ? 2 : 0) + (out_f32 ? 0 : 1);
   const uint64_t pairs = (uint64_t)a.kv.rows * a.kv.kv_heads;
   const KernelId first = acc_out ? KernelId::AttnPagedWeightsD128F32 : KernelId::AttnPagedD128F32;
   void* args[] = {&a};
-  st = launch(static_cast<KernelId>(static_cast<int>(first) + form), dim3(p.blocks ? p.blocks : (unsigned)(pairs * p.head_tiles)), dim3(256), 0, args);
+  st = launch(static_cast<KernelId>(static_cast<int>(first) + form),
+              dim3(p.blocks ? p.blocks : (unsigned)std::min(pairs * p.head_tiles, grid_most(256))), dim3(256), 0, args);
   if (st || p.blocks == 0) return st;
   uint32_t pieces = p.pieces;
-  const uint64_t blocks = (uint64_t)p.group * pieces + (acc_out ? ceil_div(paged_slots(a.kv), 1024) : 0);
+  const uint64_t joins = pieces ? (uint64_t)p.group * pieces : ceil_div((uint64_t)p.group * a.kv.head_dim, 1024);
+  const uint64_t items = joins + (acc_out ? ceil_div(paged_slots(a.kv), 1024) : 0);
+  const uint64_t rows = std::min<uint64_t>(a.kv.rows, std::max<uint64_t>(1, kJoinBlocks / (items * a.kv.kv_heads)));
   void* jargs[] = {&a, &pieces};
   return launch(static_cast<KernelId>(static_cast<int>(KernelId::AttnPagedJoinD128F32) + form),
-                dim3((unsigned)pairs, (unsigned)blocks), dim3(256), 0, jargs);
+                dim3(a.kv.kv_heads, (unsigned)items, (unsigned)rows), dim3(256), 0, jargs);
 }
 
 int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t* kv, const float* qkv, const float* rope_tab,
@@ -229,7 +246,7 @@ int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t* kv, const float* 
       !aligned(acc, 4) || !aligned(slot_pos, 4))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "paged append needs 16-byte aligned qkv, rope_tab and q");
   const uint64_t blocks = ceil_div(((uint64_t)heads + 2ull * c.kv_heads) * (c.head_dim / 8), 256);
-  if (tokens > 0x7FFFFFFFull || blocks > 65535) return fail(CATENA_ERR_UNSUPPORTED, "paged append too large");
+  if (tokens > grid_most(256) || blocks > 65535) return fail(CATENA_ERR_UNSUPPORTED, "paged append too large");
   st = ensure_init();
   if (st) return st;
   void* args[] = {&c, &qkv, &rope_tab, &table_positions, &lens, &seen, &q, &tq, &heads, &acc, &slot_pos};
@@ -262,13 +279,14 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_
     if (!aligned(p, 4)) return fail(CATENA_ERR_INVALID_ARGUMENT, "misaligned operand");
   if (!aligned(acc_in, 16) || !aligned(slot_pos_in, 16) || !aligned(acc_out, 16) || !aligned(slot_pos_out, 16))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction needs 16-byte aligned weights and positions");
-  if (lens_out == lens) return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction's new lengths may not replace the old");
+  if (lens_out == lens || lens_out == seen)
+    return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction's new lengths may not replace the old or the positions' count");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "eviction needs %llu bytes of 16-byte aligned workspace",
                 (unsigned long long)need);
   st = ensure_init();
   if (st) return st;
-  const uint32_t pairs = c.rows * c.kv_heads, slots = paged_slots(c);
+  const uint32_t pairs = c.rows * c.kv_heads, threads = evict_threads(c);
   a.lens = lens;
   a.seen = seen;
   a.acc_in = acc_in;
@@ -286,8 +304,8 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_
   // more by workgroups of 64 each.
   a.at_once = a.most <= kEvictAtOnce;
   void* args[] = {&a};
-  st = slots <= 1024 ? launch(KernelId::KvEvictChoose1k, dim3(pairs), dim3(256), 0, args)
-                     : launch(KernelId::KvEvictChoose8k, dim3(pairs), dim3(1024), 0, args);
+  st = launch(threads == 256 ? KernelId::KvEvictChoose1k : KernelId::KvEvictChoose8k, dim3(pairs), dim3(threads), 0,
+              args);
   if (st || a.at_once) return st;
   return launch(KernelId::KvEvictMove, dim3(pairs, (unsigned)ceil_div(a.most, kEvictMoves)), dim3(256), 0, args);
 }
@@ -309,7 +327,7 @@ int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t* kv, uint16_t*
       return fail(CATENA_ERR_INVALID_ARGUMENT, "page pools must be 16-byte aligned");
   if (table_out == c.table || lens_out == lens || spare_out == spare)
     return fail(CATENA_ERR_INVALID_ARGUMENT, "reorder's outputs may not replace its inputs");
-  if (c.rows > 0x7FFFFFFFu) return fail(CATENA_ERR_UNSUPPORTED, "too many rows");
+  if (c.rows > grid_most(256)) return fail(CATENA_ERR_UNSUPPORTED, "too many rows");
   st = ensure_init();
   if (st) return st;
   // the pools in as many launches as their pointers need; the table once

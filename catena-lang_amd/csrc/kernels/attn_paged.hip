@@ -10,14 +10,16 @@
 // flops per query head, so HBM.  One pass: the running maximum and sum of the
 // softmax beside the running o.
 //
-// Work is dealt out in one of two ways.  A workgroup per unit ((row, kv head) and
-// up to 16 query heads) while rows are short; it needs no join.  One CU brings in
-// about 38 GB/s, so long rows are cut: all units' tiles form one line in the
-// order of rows, every workgroup takes an equal stretch of it (ends of units in
-// it and all), and a second kernel joins the units that were cut.  The stretches
+// Work is dealt out in one of two ways.  A workgroup takes whole units ((row, kv
+// head) and up to 16 query heads) while rows are short; they need no join.  One CU
+// brings in about 38 GB/s, so long rows are cut: all units' tiles form one line in
+// the order of rows, every workgroup takes an equal stretch of it (ends of units
+// in it and all), and a second kernel joins the units that were cut.  The stretches
 // follow from the rows' own lengths, so ragged batches are even: 64 rows of 1 ..
-// 4096 slots x 8 kv heads of 128 take 88 us (6.1 TB/s), against 112 with the
-// rows cut alike; 131072 slots x 8 heads in one row 80 us (6.7 TB/s).
+// 4096 slots x 8 kv heads of 128 take 84 us (6.3 TB/s) and 5 to join, against 112
+// with the rows cut alike; 131072 slots x 8 heads in one row 80 us (6.7 TB/s).
+// Where even a full table is short, the host launches a workgroup per unit and no
+// join; else both kernels see by the rows' lengths which it is.
 //
 // A wave takes 32 slots at a time (two runs of 16, each inside one page).
 // Products on the matrix cores with the cache as the A operand, straight from
@@ -32,7 +34,7 @@
 //     registers; product e then gives columns VC m + e, m = 0 .. 15, so that
 //     lane (c, g) ends with o of head c, columns 4 VC g .. + 4 VC - 1.
 // Heads past the group's last fill the 16 columns with zeros; the matrix cores
-// have time for that (one slot's 32 x D x 16 flop against 4 D bytes).
+// have time for that (64 D flop of one slot against its 4 D bytes).
 //
 // Rounding: scores and sums in f32.  p goes into the product as bf16 terms,
 // each the upper half of what the one before left over: three (all 24 bits) for
@@ -50,19 +52,6 @@ namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// Inclusive prefix sum over the wave: within rows of 16 lanes, then rows to rows
-CATENA_DEV uint32_t wave_prefix(uint32_t x) {
-#define CATENA_DPP_ADD(ctrl, rows) \
-  x = x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, (ctrl), (rows), 0xF, false)
-  CATENA_DPP_ADD(0x111, 0xF);
-  CATENA_DPP_ADD(0x112, 0xF);
-  CATENA_DPP_ADD(0x114, 0xF);
-  CATENA_DPP_ADD(0x118, 0xF);
-  CATENA_DPP_ADD(0x142, 0xA);
-  CATENA_DPP_ADD(0x143, 0xC);
-#undef CATENA_DPP_ADD
-  return x;
-}
 CATENA_DEV uint32_t lane_of(uint32_t x, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane); }
 
 // A uniform word that no workgroup of this kernel writes: by a scalar load, which
@@ -78,6 +67,7 @@ CATENA_DEV uint32_t scalar_word(const uint32_t* p, uint32_t i) {
 struct Line {
   uint32_t tiles;  // in all
   uint32_t per;    // a workgroup's
+  bool whole;      // not cut: a workgroup takes whole units in turn
 };
 // A row on it
 struct RowOnLine {
@@ -88,22 +78,37 @@ CATENA_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // the reference point of exponents: 0 while no score is above -inf
 CATENA_DEV float anchor(float m) { return m == kNegInf ? 0.0f : m; }
 
-
 struct AttnPagedArgs {
   PagedKv kv;
   const uint16_t* q;      // [rows][heads][D]
   const uint32_t* lens;   // [rows]
-  void* o;                // [rows][heads][D], written here where splits == 1
+  void* o;                // [rows][heads][D]
   float* part_o;          // [blocks][2][min(group, 16)][D]
   float* part_ml;         // [blocks][2][min(group, 16)][2]: maximum (base 2), sum
-  float* whole_ml;        // [rows][heads][2]: of units that one workgroup of the line had, with weights only
+  float* whole_ml;        // [rows][heads][2]: of units that were not cut, with weights that the join adds
   float* scores;          // [rows][heads][slots] base-2 scores, with weights only
   const float* acc_in;    // [rows][kv_heads][slots]
   float* acc_out;
   uint32_t group, head_tiles;
-  uint32_t blocks;        // workgroups of the line; 0: one a unit
+  uint32_t blocks;        // workgroups; 0: one a unit
+  uint32_t short_slots;   // whole units while no row is longer
   float scale_log2;       // scale * log2(e)
 };
+
+// Four columns of o / l
+template <bool F32>
+CATENA_DEV void store_o(const AttnPagedArgs& a, uint64_t at, f32x4_t o, float l) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = o[i] / l;
+  if constexpr (F32) {
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + at) = o;
+  } else {
+    uint2 w;
+    w.x = pack_bf16x2(o[0], o[1]);
+    w.y = pack_bf16x2(o[2], o[3]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w;
+  }
+}
 
 // Lane r's row among the first 64, kept for the look-ups that follow
 struct FirstRows {
@@ -118,13 +123,21 @@ CATENA_DEV FirstRows first_rows(const AttnPagedArgs& a) {
 }
 CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
   uint32_t all = lane_of(f.upto, 63);
+  bool whole = f.len <= a.short_slots;
   if (a.kv.rows > 64) {
     uint32_t n = 0;
-    for (uint32_t r = 64 + (threadIdx.x & 63u); r < a.kv.rows; r += 64) n += (len_of(a, r) + 31) / 32;
+#pragma unroll 4
+    for (uint32_t r = 64 + (threadIdx.x & 63u); r < a.kv.rows; r += 64) {
+      const uint32_t len = len_of(a, r);
+      n += (len + 31) / 32;
+      whole = whole && len <= a.short_slots;
+    }
     all += lane_of(wave_prefix(n), 63);
   }
   all *= a.kv.kv_heads * a.head_tiles;
-  return Line{all, (all + a.blocks - 1) / a.blocks};
+  // long parts: one workgroup a CU (32768 tiles: 83.1 us against 85.3 with two)
+  const uint32_t blocks = all >= 16384 && a.blocks > 256 ? 256 : a.blocks;
+  return Line{all, (all + blocks - 1) / blocks, __all(whole) != 0};
 }
 // The row that place `at` of the line (below its end) belongs to
 CATENA_DEV RowOnLine row_at_place(const AttnPagedArgs& a, const FirstRows& f, uint32_t at) {
@@ -163,7 +176,7 @@ CATENA_DEV void add_weights(const AttnPagedArgs& a, uint32_t row, uint32_t kvh, 
   float* out = a.acc_out + pair * slots;
   for (; slot < len; slot += step) {  // slots come in whole pages of 16 or more
     f32x4_t w = f32x4_t{0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 2
     for (uint32_t h = 0; h < hn; ++h) {
       const f32x4_t x = *reinterpret_cast<const f32x4_t*>(scores + (uint64_t)h * slots + slot);
 #pragma unroll
@@ -205,8 +218,8 @@ CATENA_DEV Part part_from(const AttnPagedArgs& a, uint32_t row, uint32_t len, ui
   p.row = row;
   p.len = len;
   p.tiles = (len + 31) / 32;
-  p.kvh = unit / a.head_tiles;
-  p.ht = unit % a.head_tiles;
+  p.kvh = a.head_tiles == 1 ? unit : unit / a.head_tiles;
+  p.ht = unit - p.kvh * a.head_tiles;
   p.gn = a.group - 16 * p.ht < 16 ? a.group - 16 * p.ht : 16;
   p.beg = beg;
   p.end = p.tiles - beg < most ? p.tiles : beg + most;
@@ -365,6 +378,7 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     }
   };
 
+  bool whole = a.blocks == 0;  // units are not cut
   auto finish = [&](const Part& p) {
     // The waves' (m, l, o) to one
     l = l + __shfl_xor(l, 16);
@@ -411,38 +425,54 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
       }
       const uint64_t to = (uint64_t)p.row * heads + head, at = to * D + d;
       if constexpr (WEIGHTS) {
-        if (d == 0 && a.blocks != 0) {
+        if (d == 0 && whole && a.head_tiles == 1) {
+          sh.base[h] = anchor(mm);
+          sh.share[h] = 1.0f / ll;
+        } else if (d == 0) {
           a.whole_ml[2 * to] = mm;
           a.whole_ml[2 * to + 1] = ll;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = p.len ? o[i] / ll : 0.0f;
-      if constexpr (F32) {
-        *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + at) = o;
-      } else {
-        uint2 w;
-        w.x = pack_bf16x2(o[0], o[1]);
-        w.y = pack_bf16x2(o[2], o[3]);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w;
+      store_o<F32>(a, at, o, p.len ? ll : 1.0f);  // no slots: 0 / 1
+    }
+    if constexpr (WEIGHTS) {
+      // weights of whole units that are all of their kv head (of the line's the
+      // second kernel adds them, strip by strip): the scores are this workgroup's
+      // own, behind two barriers
+      if (whole && a.head_tiles == 1) {
+        __syncthreads();
+        add_weights(a, p.row, p.kvh, 0, p.gn, p.len, 4 * threadIdx.x, 1024, sh.base, sh.share);
       }
     }
   };
 
-  uint32_t at = 0, last = 0;  // what is left of the line behind `now`
+  // what is left behind `now`: places of the line, or whole units
+  const uint32_t units = a.kv.kv_heads * a.head_tiles;
+  uint32_t at, last;
   Part now;
-  if (a.blocks == 0) {
-    const uint32_t units = a.kv.kv_heads * a.head_tiles, row = blockIdx.x / units;
-    now = part_from(a, row, paged_len(a.kv, scalar_word(a.lens, row)), blockIdx.x % units, 0, 0xFFFFFFFFu);
-  } else {
+  auto unit_from = [&](uint32_t u) {
+    const uint32_t row = u / units;
+    return part_from(a, row, paged_len(a.kv, scalar_word(a.lens, row)), u % units, 0, 0xFFFFFFFFu);
+  };
+  if (!whole) {
     const FirstRows rows = first_rows(a);
     const Line line = line_of(a, rows);
-    at = blockIdx.x * line.per;
-    if (at >= line.tiles) return;
-    last = line.tiles - at < line.per ? line.tiles : at + line.per;
-    const RowOnLine r = row_at_place(a, rows, at);
-    now = part_from(a, r.row, r.len, (at - r.first) / r.tiles, (at - r.first) % r.tiles, last - at);
-    at += now.end - now.beg;
+    whole = line.whole;
+    if (!whole) {
+      at = blockIdx.x * line.per;
+      if (at >= line.tiles) return;
+      last = line.tiles - at < line.per ? line.tiles : at + line.per;
+      const RowOnLine r = row_at_place(a, rows, at);
+      now = part_from(a, r.row, r.len, (at - r.first) / r.tiles, (at - r.first) % r.tiles, last - at);
+      at += now.end - now.beg;
+    }
+  }
+  if (whole) {
+    at = blockIdx.x;
+    last = a.kv.rows * units;
+    if (at >= last) return;
+    now = unit_from(at);
+    at += gridDim.x;
   }
 
   // The workgroup's parts one after the other, a wave's tiles of each kWaves
@@ -457,8 +487,13 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     Part next = now;
     uint32_t tn = t + kWaves;  // past the end where nothing is left
     if (ends && more) {
-      next = part_behind(a, now, last - at);
-      at += next.end - next.beg;
+      if (whole) {
+        next = unit_from(at);
+        at += gridDim.x;
+      } else {
+        next = part_behind(a, now, last - at);
+        at += next.end - next.beg;
+      }
       tn = next.beg + wave;
     }
     request(y, next, tn);
@@ -476,23 +511,6 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
   };
   while (step(one, two) && step(two, one)) {
   }
-
-  if constexpr (WEIGHTS) {
-    // a whole unit's weights, where it is its kv head's only one: the scores are
-    // this workgroup's own, behind the barriers of finish()
-    if (a.blocks != 0) return;
-    if (threadIdx.x < now.gn) {
-      float mm = kNegInf, ll = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh.m[w][threadIdx.x]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) ll = ll + sh.l[w][threadIdx.x] * exp2_fast(sh.m[w][threadIdx.x] - anchor(mm));
-      sh.base[threadIdx.x] = anchor(mm);
-      sh.share[threadIdx.x] = 1.0f / ll;
-    }
-    __syncthreads();
-    add_weights(a, now.row, now.kvh, 0, now.gn, now.len, 4 * threadIdx.x, 1024, sh.base, sh.share);
-  }
 }
 
 // Where the parts of a unit are: the workgroups that have one are numbered on
@@ -505,99 +523,126 @@ CATENA_DEV Parts parts_of(const Line& line, const RowOnLine& r, uint32_t unit) {
   return Parts{first, (beg + r.tiles - 1) / line.per - first + 1};
 }
 
-// Joins the parts of units, writes 0 for rows without slots, and adds the
-// weights.  grid.x = (row, kv head); blockIdx.y < group * pieces: D / pieces
-// columns of one query head's o, several parts at a time; else 1024 slots'
-// weights.
+// Place of a unit's part i for head h of its 16: the unit's first part lies in the
+// second of its workgroup's places
+CATENA_DEV uint64_t part_place(const AttnPagedArgs& a, const Parts& p, uint32_t i, uint32_t h) {
+  return ((uint64_t)(p.first + i) * 2 + (i == 0)) * (a.group < 16 ? a.group : 16) + h;
+}
+
+// One thread's parts i = first, first + step, ... of a unit's head, with a running
+// maximum: four columns of o from `col` on
+struct Joined {
+  f32x4_t o;
+  float m, l;
+};
+template <int D>
+CATENA_DEV Joined join_parts(const AttnPagedArgs& a, const Parts& p, uint32_t h, uint32_t col, uint32_t first,
+                             uint32_t step) {
+  Joined j{f32x4_t{0, 0, 0, 0}, kNegInf, 0.0f};
+#pragma unroll 4
+  for (uint32_t i = first; i < p.n; i += step) {
+    const uint64_t at = part_place(a, p, i, h);
+    const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
+    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + col);
+    const float m = __builtin_fmaxf(j.m, pm), f = exp2_fast(j.m - anchor(m)), e = exp2_fast(pm - anchor(m));
+    j.m = m;
+    j.l = j.l * f + pl * e;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) j.o[c] = j.o[c] * f + y[c] * e;
+  }
+  return j;
+}
+
+// Joins the units that were cut, writes 0 for rows without slots, and adds the
+// weights that the first kernel could not.  blockIdx.x: the kv head, blockIdx.z:
+// rows in turn; blockIdx.y < joins: the o of 1024 / D query heads, a thread four
+// columns (pieces 0, for units of few parts), or D / pieces columns of one head, a
+// thread some of the parts; else 1024 slots' weights.
 template <int D, bool F32>
 CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const uint32_t pair = blockIdx.x, row = pair / a.kv.kv_heads, kvh = pair % a.kv.kv_heads;
-  const uint32_t tid = threadIdx.x, heads = a.group * a.kv.kv_heads;
-  const uint32_t part_heads = a.group < 16 ? a.group : 16;
+  __shared__ f32x2 s_ml[64];
+  __shared__ __attribute__((aligned(16))) float s_o[256 * 4];
+  __shared__ float s_m[16], s_r[16];
+  const uint32_t tid = threadIdx.x, heads = a.group * a.kv.kv_heads, kvh = blockIdx.x;
   const FirstRows rows = first_rows(a);
   const Line line = line_of(a, rows);
-  const RowOnLine r = row_on_line(a, rows, row);
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml);
-  // place of a unit's part i for its head h: the unit's first part lies in the
-  // second of its workgroup's places
-  auto part = [&](const Parts& p, uint32_t i, uint32_t h) {
-    return ((uint64_t)(p.first + i) * 2 + (i == 0)) * part_heads + h;
-  };
-  if (blockIdx.y < a.group * pieces) {
-    const uint32_t head = blockIdx.y / pieces, piece = blockIdx.y % pieces;
-    const Parts p = parts_of(line, r, kvh * a.head_tiles + head / 16);
-    if (p.n == 1) return;
-    const uint32_t lanes = D / 4 / pieces;  // a part's columns, 16 bytes each
-    const uint32_t col = piece * lanes * 4 + tid % lanes * 4, mine = tid / lanes, step = 256 / lanes;
-    // a thread's parts with a running maximum, then the threads' sums of a column
-    __shared__ f32x2 s_ml[64];
-    __shared__ __attribute__((aligned(16))) float s_o[256 * 4];
-    float m = kNegInf, l = 0.0f;
-    f32x4_t o = f32x4_t{0, 0, 0, 0};
-#pragma unroll 4
-    for (uint32_t i = mine; i < p.n; i += step) {
-      const uint64_t at = part(p, i, head % 16);
-      const f32x2 x = ml[at];
-      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + col);
-      const float m2 = __builtin_fmaxf(m, x[0]), f = exp2_fast(m - anchor(m2)), e = exp2_fast(x[0] - anchor(m2));
-      m = m2;
-      l = l * f + x[1] * e;
+  if (line.whole && (!a.acc_out || a.head_tiles == 1)) return;
+  constexpr uint32_t LANES = D / 4;
+  const uint32_t joins = pieces ? a.group * pieces : (a.group * LANES + 255) / 256;
+  const uint32_t quarters = pieces == 4 ? 2 : 0;  // pieces: 0, 1 or 4
+  if (blockIdx.y < joins) {
+    if (line.whole) return;
+    const uint32_t lanes = LANES >> quarters;  // of a head's columns, 16 bytes each
+    const uint32_t head = pieces ? blockIdx.y >> quarters : blockIdx.y * (256 / LANES) + tid / LANES;
+    const uint32_t col = (pieces == 4 ? blockIdx.y % 4 * lanes * 4 : 0u) + tid % lanes * 4;
+    const uint32_t mine = tid / lanes, step = 256 / lanes;
+    for (uint32_t row = blockIdx.z; row < a.kv.rows; row += gridDim.z) {
+      const RowOnLine r = row_on_line(a, rows, row);
+      const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + col;
+      const Parts p = parts_of(line, r, kvh * a.head_tiles + head / 16);
+      if (!pieces) {
+        if (head >= a.group || p.n == 1) continue;
+        const Joined j = join_parts<D>(a, p, head % 16, col, 0, 1);
+        store_o<F32>(a, at, j.o, r.len ? j.l : 1.0f);
+        continue;
+      }
+      if (p.n == 1) continue;
+      const Joined j = join_parts<D>(a, p, head % 16, col, mine, step);
+      __syncthreads();  // the last one's values have been read
+      *reinterpret_cast<f32x4_t*>(&s_o[4 * tid]) = j.o;
+      if (tid % lanes == 0) s_ml[mine] = f32x2{j.m, j.l};
+      __syncthreads();
+      if (tid < lanes) {
+        float m = kNegInf, l = 0.0f;
+        f32x4_t o = f32x4_t{0, 0, 0, 0};
+        for (uint32_t i = 0; i < step; ++i) m = __builtin_fmaxf(m, s_ml[i][0]);
+        for (uint32_t i = 0; i < step; ++i) {
+          const float f = exp2_fast(s_ml[i][0] - anchor(m));
+          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&s_o[4 * (i * lanes + tid)]);
+          l = l + s_ml[i][1] * f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = o[j] * f + y[j] * e;
+          for (int c = 0; c < 4; ++c) o[c] = o[c] + y[c] * f;
+        }
+        store_o<F32>(a, at, o, r.len ? l : 1.0f);
+      }
     }
-    *reinterpret_cast<f32x4_t*>(&s_o[4 * tid]) = o;
-    if (tid % lanes == 0) s_ml[mine] = f32x2{m, l};
-    __syncthreads();
-    if (tid >= lanes * 4) return;
-    for (uint32_t i = 0; i < step; ++i) m = __builtin_fmaxf(m, s_ml[i][0]);
-    l = 0.0f;
-    float sum = 0.0f;
-    for (uint32_t i = 0; i < step; ++i) {
-      const float f = exp2_fast(s_ml[i][0] - anchor(m));
-      l = l + s_ml[i][1] * f;
-      sum = sum + s_o[i * lanes * 4 + tid] * f;
-    }
-    const float x = r.len ? sum / l : 0.0f;
-    const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + piece * lanes * 4 + tid;
-    if constexpr (F32)
-      static_cast<float*>(a.o)[at] = x;
-    else
-      static_cast<uint16_t*>(a.o)[at] = (uint16_t)f32_to_bf16_bits(x);
     return;
   }
-  const uint32_t slot0 = (blockIdx.y - a.group * pieces) * 1024;
-  if (slot0 >= r.len) return;
-  __shared__ float s_m[16], s_r[16];
-  for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
-    const uint32_t hn = a.group - h0 < 16 ? a.group - h0 : 16;
-    const Parts p = parts_of(line, r, kvh * a.head_tiles + h0 / 16);
-    if (h0) __syncthreads();
-    // 16 lanes a head, a part each
-    for (uint32_t h = tid / 16; h < hn; h += 16) {
-      float m = kNegInf, l = 0.0f;
-      if (p.n == 1) {
-        const float* x = a.whole_ml + 2 * ((uint64_t)row * heads + kvh * a.group + h0 + h);
-        m = x[0];
-        l = x[1];
-      } else {
-        for (uint32_t i = tid % 16; i < p.n; i += 16) m = __builtin_fmaxf(m, ml[part(p, i, h)][0]);
+  const uint32_t slot0 = (blockIdx.y - joins) * 1024;
+  for (uint32_t row = blockIdx.z; row < a.kv.rows; row += gridDim.z) {
+    const RowOnLine r = row_on_line(a, rows, row);
+    if (slot0 >= r.len) continue;
+    for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
+      const uint32_t hn = a.group - h0 < 16 ? a.group - h0 : 16;
+      const Parts p = parts_of(line, r, kvh * a.head_tiles + h0 / 16);
+      __syncthreads();  // the last heads' values have been read
+      // 16 lanes a head, a part each
+      for (uint32_t h = tid / 16; h < hn; h += 16) {
+        float m = kNegInf, l = 0.0f;
+        if (line.whole || p.n == 1) {
+          const float* x = a.whole_ml + 2 * ((uint64_t)row * heads + kvh * a.group + h0 + h);
+          m = x[0];
+          l = x[1];
+        } else {
+          for (uint32_t i = tid % 16; i < p.n; i += 16) m = __builtin_fmaxf(m, a.part_ml[2 * part_place(a, p, i, h)]);
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-        for (uint32_t i = tid % 16; i < p.n; i += 16) {
-          const f32x2 x = ml[part(p, i, h)];
-          l = l + x[1] * exp2_fast(x[0] - anchor(m));
+          for (int d = 1; d < 16; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+          for (uint32_t i = tid % 16; i < p.n; i += 16) {
+            const float* x = a.part_ml + 2 * part_place(a, p, i, h);
+            l = l + x[1] * exp2_fast(x[0] - anchor(m));
+          }
+#pragma unroll
+          for (int d = 1; d < 16; d *= 2) l = l + __shfl_xor(l, d);
         }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) l = l + __shfl_xor(l, d);
+        if (tid % 16 == 0) {
+          s_m[h] = anchor(m);
+          s_r[h] = 1.0f / l;
+        }
       }
-      if (tid % 16 == 0) {
-        s_m[h] = anchor(m);
-        s_r[h] = 1.0f / l;
-      }
+      __syncthreads();
+      add_weights(a, row, kvh, h0, hn, r.len, slot0 + 4 * tid, 0x80000000u, s_m, s_r);  // slots < 2^31: once
     }
-    __syncthreads();
-    add_weights(a, row, kvh, h0, hn, r.len, slot0 + 4 * tid, 0x80000000u, s_m, s_r);  // slots < 2^31: once
   }
 }
 

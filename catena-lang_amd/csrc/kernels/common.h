@@ -611,6 +611,20 @@ CATENA_DEV uint64_t max_key(float v, uint32_t t) {
   return make_key(mono_bits(bits), t, bits);
 }
 
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then rows to rows
+CATENA_DEV uint32_t wave_prefix(uint32_t x) {
+#define CATENA_DPP_ADD(ctrl, rows) \
+  x = x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, (ctrl), (rows), 0xF, false)
+  CATENA_DPP_ADD(0x111, 0xF);
+  CATENA_DPP_ADD(0x112, 0xF);
+  CATENA_DPP_ADD(0x114, 0xF);
+  CATENA_DPP_ADD(0x118, 0xF);
+  CATENA_DPP_ADD(0x142, 0xA);
+  CATENA_DPP_ADD(0x143, 0xC);
+#undef CATENA_DPP_ADD
+  return x;
+}
+
 // Maximum over the wave of an unsigned value (0 is the identity): inclusive
 // max scans within rows of 16 lanes (row_shr 1, 2, 4, 8), rows joined
 // through row_bcast 15 and 31, lane 63's result returned uniformly.

@@ -89,20 +89,6 @@ CATENA_DEV uint32_t keep_key(float weight, uint32_t pos, uint32_t late) {
   return weight != weight ? 0u : mono_bits(__float_as_uint(weight));
 }
 
-// Inclusive prefix sum over the wave: within rows of 16 lanes, then rows to rows
-CATENA_DEV uint32_t wave_prefix(uint32_t x) {
-#define CATENA_DPP_ADD(ctrl, rows) \
-  x = x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, (ctrl), (rows), 0xF, false)
-  CATENA_DPP_ADD(0x111, 0xF);
-  CATENA_DPP_ADD(0x112, 0xF);
-  CATENA_DPP_ADD(0x114, 0xF);
-  CATENA_DPP_ADD(0x118, 0xF);
-  CATENA_DPP_ADD(0x142, 0xA);
-  CATENA_DPP_ADD(0x143, 0xC);
-#undef CATENA_DPP_ADD
-  return x;
-}
-
 // Exclusive prefix sum over the workgroup's threads, and the total.  s_wave[2]:
 // the caller alternates between the two, so that one barrier is enough.
 template <int WAVES>

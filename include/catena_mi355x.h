@@ -342,7 +342,8 @@ int catena_mi355x_attn_paged_plan(const catena_paged_kv_t *kv, uint32_t heads, i
  * [head_dim] f32 (out_f32 != 0) or bf16 RNE.  Query head h reads kv head
  * h / (heads / kv_heads); o = sum_j p_j v_j, p = softmax(scale * q . k_j) with
  * the exponential itself (not math.exp-approx), sums in f32.  A row of no slots
- * gives 0.  What the cache holds past a row's slots is never used.
+ * gives 0, one of whose slots no page is there NaN.  What the cache holds past a
+ * row's slots is never used.
  * acc_in / acc_out[rows][kv_heads][max_pages * page_size] f32 (both or
  * neither, may be the same): acc_out[j] = acc_in[j] + the sum of p_j over the
  * query heads of a kv head, for the slots in use; others are left as they are.
@@ -389,8 +390,9 @@ int catena_mi355x_kv_evict_paged_plan(const catena_paged_kv_t *kv, uint32_t budg
  * before the append.)  lens_out[rows] is the new length.  acc_in / acc_out and
  * slot_pos_in / slot_pos_out ([rows][kv_heads][max_pages * page_size]) are each
  * two buffers or the same one, 16-byte aligned; entries past the new length are
- * left as they are.  lens_out is not lens.  The pages must be the row's own (a page that
- * catena_mi355x_beam_reorder_paged_bf16 shares changes for all its rows).
+ * left as they are.  lens_out is neither lens nor seen.  The pages must be the
+ * row's own (one that catena_mi355x_beam_reorder_paged_bf16 shares changes for
+ * all its rows); K and V of a slot without a page are not moved.
  * workspace as for catena_mi355x_attn_paged_bf16.  No reference counterpart. */
 int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t *kv, const uint32_t *lens,
                                       const uint32_t *seen, const float *acc_in,

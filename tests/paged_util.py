@@ -19,17 +19,20 @@ def f64(bits) -> np.ndarray:
 
 
 class Cache:
-    """rows of `lens` slots in pages, each row's pages anywhere in the pool."""
+    """rows of `lens` slots in pages, each row's pages anywhere in the pool; lazy:
+    pages for the slots in use alone, table entries behind them name none."""
 
-    def __init__(self, rng, lens, kv_heads, dim, page, max_pages, spare=0, scale=1.0):
+    def __init__(self, rng, lens, kv_heads, dim, page, max_pages, spare=0, scale=1.0, lazy=False):
         self.lens = np.asarray(lens, np.uint32)
         rows = len(self.lens)
         self.page, self.max_pages, self.kv_heads, self.dim = page, max_pages, kv_heads, dim
         self.slots = page * max_pages
-        num = rows * max_pages + spare
+        used = np.minimum(-(-self.lens // page), max_pages) if lazy else np.full(rows, max_pages)
+        num = max(int(used.sum()) + spare, 1)
         order = rng.permutation(num).astype(np.uint32)
-        self.table = order[: rows * max_pages].reshape(rows, max_pages).copy()
-        self.spare = order[rows * max_pages:].copy()
+        self.table = np.full((rows, max_pages), 0xFFFFFFFF, np.uint32)
+        self.table[np.arange(max_pages) < used[:, None]] = order[: int(used.sum())]
+        self.spare = order[int(used.sum()):].copy()
         self.num_pages = num
         self.k = np.full((num, kv_heads, page, dim), NAN16, np.uint16)
         self.v = self.k.copy()

@@ -94,6 +94,13 @@ CASES = [
     (34, 2, 64, 32, 100, [3200, 1777, 0]),               # cut rows of 17 query heads a kv head
     (4, 2, 128, 32, 60, [1920] * 3 + [64, 32, 31, 96]),  # parts that end with units
 ]
+SHORT_ROWS = [  # of long tables: whole units, more than there are workgroups, or fewer; none
+    (8, 8, 64, 16, 256, [(13 * i) % 91 for i in range(70)]),
+    (34, 2, 64, 32, 64, [900, 1, 0, 513]),               # two tiles of heads
+    (8, 2, 128, 64, 1024, [400, 33]),
+    (4, 4, 128, 16, 512, [0, 0, 0]),
+]
+CASES += SHORT_ROWS
 
 
 @pytest.mark.parametrize("weights", [False, True])
@@ -103,7 +110,7 @@ def test_against_the_formula(case, out_f32, weights):
     heads, kvh, dim, page, pages, lens = CASES[case]
     say(f"attn_paged case {case} heads {heads}/{kvh} dim {dim} page {page} slots {page * pages} f32 {out_f32} weights {weights}")
     rng = np.random.default_rng(100 + case)
-    cache = Cache(rng, lens, kvh, dim, page, pages)
+    cache = Cache(rng, lens, kvh, dim, page, pages, lazy=CASES[case] in SHORT_ROWS)
     q = bf16(rng.standard_normal((len(lens), heads, dim)))
     acc = rng.random((len(lens), kvh, cache.slots)).astype(np.float32) if weights else None
     scale = dim ** -0.5

@@ -44,6 +44,12 @@ def test_attention_refuses_bad_arguments():
         refused(INVALID, attn, long, work=work)
     refused(UNSUPPORTED, attn, geometry(rows=1 << 31, kv_heads=4))
     refused(UNSUPPORTED, attn, geometry(rows=1 << 16, kv_heads=64, max_pages=1 << 14), heads=64)
+    # more slots than the strips of weights in a grid cover; without weights there are none
+    long = geometry(rows=1, kv_heads=1, page_size=1024, max_pages=1 << 16)
+    assert ca.attn_paged_plan(long, 1)[0] > 0
+    refused(UNSUPPORTED, ca.attn_paged_plan, long, 1, True)
+    refused(UNSUPPORTED, attn, long, heads=1, acc_in=P, acc_out=P)
+    refused(UNSUPPORTED, ca.attn_paged_plan, geometry(rows=1, kv_heads=1), 1 << 14)  # heads of one kv head
 
 
 def test_attention_plan():
@@ -128,7 +134,8 @@ def test_append_refuses_bad_arguments():
                  dict(qkv=P + 4), dict(tab=P + 8), dict(q=P + 2), dict(lens=P + 2), dict(seen=P + 1), dict(acc=P),
                  dict(slot_pos=P), dict(acc=P + 2, slot_pos=P), dict(acc=P, slot_pos=P + 2)):
         refused(INVALID, append, kv, **over)
-    refused(UNSUPPORTED, append, geometry(rows=1 << 20), tq=1 << 12)
+    for rows, tq in ((1 << 20, 1 << 12), (1 << 12, 1 << 12), (1 << 24, 1)):
+        refused(UNSUPPORTED, append, geometry(rows=rows), tq=tq)
 
 
 def test_evict_refuses_bad_arguments():
@@ -140,6 +147,10 @@ def test_evict_refuses_bad_arguments():
         refused(INVALID, evict, kv, **{name: P + 2})
     for name in ("acc", "pos", "acc_out", "pos_out"):
         refused(INVALID, evict, kv, **{name: P + 8})
+    refused(INVALID, evict, kv, seen=2 * P)  # the new lengths' place
+    for rows, pages in ((1 << 22, 16), (1 << 20, 80)):  # more workgroups than a grid takes
+        refused(UNSUPPORTED, evict, geometry(rows=rows, max_pages=pages))
+        refused(UNSUPPORTED, ca.kv_evict_paged_plan, geometry(rows=rows, max_pages=pages), 8)
     for over in (dict(budget=0), dict(lens_out=P), dict(work=None), dict(work=(0, need)), dict(work=(P, need - 1)), dict(work=(P + 4, need))):
         refused(INVALID, evict, kv, **over)
     refused(INVALID, ca.kv_evict_paged_plan, kv, 0)
@@ -153,6 +164,7 @@ def test_reorder_refuses_bad_arguments():
     for name in ("lens", "parents", "spare", "table_out", "lens_out", "spare_out"):
         refused(INVALID, reorder, kv, **{name: 0})
         refused(INVALID, reorder, kv, **{name: P + 1})
+    refused(UNSUPPORTED, reorder, geometry(rows=1 << 24))
     for over in (dict(pools=(P, 0)), dict(pools=(P, P + 8)), dict(table_out=1 << 22), dict(lens_out=P), dict(spare_out=P)):
         refused(INVALID, reorder, kv, **over)
 
@@ -169,6 +181,6 @@ def test_beam_selection_refuses_bad_arguments():
     for over in (dict(beams=0), dict(vocab=0), dict(eos=100), dict(eos=ca.BEAM_NO_EOS), dict(workspace=None),
                  dict(workspace=(P, need - 1)), dict(workspace=(P + 8, need)), dict(workspace=(0, need))):
         refused(INVALID, ca.beam_select_f32, **{**good, **over})
-    for over in (dict(beams=33), dict(vocab=(1 << 26) + 1), dict(groups=1 << 29)):
+    for over in (dict(beams=33), dict(vocab=(1 << 26) + 1), dict(groups=1 << 29), dict(groups=1 << 22)):
         refused(UNSUPPORTED, ca.beam_select_f32, **{**good, **over})
         refused(UNSUPPORTED, ca.beam_select_plan, *({**good, **over}[n] for n in ("groups", "beams", "vocab")))
