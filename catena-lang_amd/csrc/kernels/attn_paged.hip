@@ -135,8 +135,9 @@ CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
     all += lane_of(wave_prefix(n), 63);
   }
   all *= a.kv.kv_heads * a.head_tiles;
-  // long parts: one workgroup a CU (32768 tiles: 83.1 us against 85.3 with two)
-  const uint32_t blocks = all >= 16384 && a.blocks > 256 ? 256 : a.blocks;
+  // long parts: one workgroup a CU (D = 128, 32768 tiles: 83.1 us against 85.3 with
+  // two; D = 64, whose tiles are half as long, ragged rows: 59.6 against 57.3)
+  const uint32_t blocks = all >= 16384 && a.blocks > 256 && a.kv.head_dim == 128 ? 256 : a.blocks;
   return Line{all, (all + blocks - 1) / blocks, __all(whole) != 0};
 }
 // The row that place `at` of the line (below its end) belongs to
