@@ -13,11 +13,11 @@
 // latency of two launches.  First kernel: a workgroup keeps a run of a row's
 // logits in registers, takes their maximum, the sum of their exponentials and
 // their W largest.  Second kernel: a workgroup per group joins the runs of
-// its rows and merges the W sorted lists.  Per
+// its rows and takes the W largest of their lists.  Per
 // logit the first one issues a maximum, a subtraction, a product, an exponential
 // (four times an add), an add and a comparison; exponentials by exp2, keys only
 // for logits that reach the bound, loads without address arithmetic: 32 beams x 8
-// x 128000 in 22.7 us (5.8 TB/s), against 38 with keys for all and exponentials
+// x 128000 in 22.0 us (6.0 TB/s), against 38 with keys for all and exponentials
 // in two steps.
 //
 // Accuracy: an exponential is off by 2^-24 of |x - m| log2 e + 2 (log2 e in f32
@@ -202,6 +202,27 @@ CATENA_DEV void beam_runs(const float* __restrict__ logits, const uint32_t* __re
 // wave's bound are listed and sorted by counting; where they are more than the
 // list holds, the largest is taken out time after time.
 constexpr uint32_t WLIST = 128;
+// Each of the list's count keys to its place, by the number of larger ones; behind
+// them the list has eight zeros
+template <int PER>
+CATENA_DEV void place(const uint64_t* list, uint32_t count, uint64_t* best, uint32_t beams) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint64_t mine[PER];
+  uint32_t above[PER] = {};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine[i] = lane + 64 * i < count ? list[lane + 64 * i] : 0ull;
+  for (uint32_t j = 0; j < count; j += 8)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint64_t x = list[j + e];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) above[i] += x > mine[i];
+    }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (mine[i] && above[i] < beams) best[above[i]] = mine[i];
+}
+
 template <int PER>
 CATENA_DEV void largest_of(const uint64_t* keys, uint32_t n, bool more, uint64_t* best, uint32_t beams,
                            uint64_t* list) {
@@ -216,7 +237,8 @@ CATENA_DEV void largest_of(const uint64_t* keys, uint32_t n, bool more, uint64_t
   uint64_t mine = 0;
 #pragma unroll
   for (int i = 0; i <= PER; ++i) mine = k[i] > mine ? k[i] : mine;
-  const uint32_t least = max(wave_bound((uint32_t)(mine >> 32), beams), 1u);
+  // (few keys are sorted sooner than bounded)
+  const uint32_t least = !more && n <= 32 ? 1u : max(wave_bound((uint32_t)(mine >> 32), beams), 1u);
   uint32_t count = 0;
 #pragma unroll
   for (int i = 0; i <= PER; ++i) {
@@ -229,17 +251,11 @@ CATENA_DEV void largest_of(const uint64_t* keys, uint32_t n, bool more, uint64_t
   if (count <= WLIST && lane < 8) list[count + lane] = 0;  // eight at a time
   __builtin_amdgcn_wave_barrier();
   if (count <= WLIST) {
-    const uint64_t a = lane < count ? list[lane] : 0ull, b = lane + 64 < count ? list[lane + 64] : 0ull;
-    uint32_t above_a = 0, above_b = 0;
-    for (uint32_t j = 0; j < count; j += 8)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint64_t x = list[j + e];
-        above_a += x > a;
-        above_b += x > b;
-      }
-    if (a && above_a < beams) best[above_a] = a;
-    if (b && above_b < beams) best[above_b] = b;
+    if (count <= 64) {
+      place<1>(list, count, best, beams);
+    } else {
+      place<2>(list, count, best, beams);
+    }
     if (lane >= count && lane < beams) best[lane] = 0;
     return;
   }
@@ -269,10 +285,13 @@ extern "C" __global__ __launch_bounds__(256) void catena_beam_runs_16(
   beam_runs<16>(logits, done, part_m, part_s, best, vocab, beams);
 }
 // Group blockIdx.x: a wave joins a row's runs (their log sum in f64) and takes
-// the W largest of their lists; then the first wave merges the rows' lists, lane
-// w at the head of beam w's.  W <= 32; 64 threads a beam, up to 16.  A place that
-// no offered continuation fills: its own beam as parent, token 0, score -inf, not
-// done.
+// the W largest of their lists; then the first wave takes the W largest of all
+// rows', as f64 scores in ordered integers whose last ten bits give way to the
+// entry's number, so that no two are equal and a lower beam goes first.  (Merging
+// the rows' lists entry by entry takes 0.2 us each: 4, 8, 16, 32 beams 4.2, 5.5,
+// 8.7, 16.6 us against 3.7, 4.6, 6.4, 11.4.)  W <= 32; 64 threads a beam, up to 16.
+// A place that no offered continuation fills: its own beam as parent, token 0,
+// score -inf, not done.
 extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
     const float* __restrict__ part_m, const double* __restrict__ part_s, const uint64_t* __restrict__ best,
     const float* scores, const uint32_t* done, uint32_t* tokens, uint32_t* parents, float* scores_out,
@@ -281,6 +300,7 @@ extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
   __shared__ uint32_t s_token[32][32];
   __shared__ uint64_t s_list[16][WLIST + 8];
   __shared__ uint32_t s_done[32];
+  __shared__ uint64_t s_key[32 * 32], s_won[32];
   const uint32_t group = blockIdx.x, lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (uint32_t w = wave; w < beams; w += blockDim.x / 64) {
@@ -296,7 +316,9 @@ extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
     // a run of nothing above -inf adds 0 (or its NaN)
     float m = lane < runs ? pm[lane] : kNegInf;
     double sum = lane < runs ? ps[lane] : 0.0;
-    if (n <= 256) {
+    if (n <= 64) {
+      largest_of<1>(keys, n, false, s_best[w], beams, s_list[wave]);
+    } else if (n <= 256) {
       largest_of<4>(keys, n, false, s_best[w], beams, s_list[wave]);
     } else {
       for (uint32_t i = 0; i < n; i += 1024)
@@ -317,31 +339,28 @@ extern "C" __global__ __launch_bounds__(1024) void catena_beam_join(
       const double s = over ? shift : (double)offered((uint32_t)(b >> 32)) + shift;
       const uint64_t bits = (uint64_t)__double_as_longlong(s + 0.0);  // -0 as +0
       s_token[w][lane] = over ? eos : ~(uint32_t)b;
-      s_best[w][lane] = b == 0 || !(shift - shift == 0.0) ? 0ull : (bits >> 63) ? ~bits : bits | (1ull << 63);
+      const uint64_t key = (bits >> 63) ? ~bits : bits | (1ull << 63);
+      s_best[w][lane] = key;
+      s_key[w * beams + lane] =
+          b == 0 || !(shift - shift == 0.0) ? 0ull : (key & ~1023ull) | (1023u - (32 * w + lane));
     }
   }
   __syncthreads();
   if (wave != 0) return;
-  uint32_t at = 0, won = 0xFFFFFFFFu;  // lane w: its list's head; lane r: place r's (beam, entry)
-  uint64_t head = lane < beams ? s_best[lane][0] : 0ull, score = 0;
-  for (uint32_t r = 0; r < beams; ++r) {
-    const uint64_t top = wave_max64(head);
-    if (top == 0) break;
-    const uint32_t w = (uint32_t)__ffsll((unsigned long long)__ballot(head == top)) - 1;
-    const uint32_t entry = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)w);
-    if (lane == r) {
-      won = w * 32 + entry;
-      score = top;
-    }
-    if (lane == w) {
-      ++at;
-      head = at < beams ? s_best[w][at] : 0ull;
-    }
-  }
+  const uint32_t n = beams * beams;
+  if (n <= 64)
+    largest_of<1>(s_key, n, false, s_won, beams, s_list[0]);
+  else if (n <= 256)
+    largest_of<4>(s_key, n, false, s_won, beams, s_list[0]);
+  else
+    largest_of<16>(s_key, n, false, s_won, beams, s_list[0]);
+  __builtin_amdgcn_wave_barrier();
   if (lane >= beams) return;
   const uint32_t out = group * beams + lane;
-  const bool filled = won != 0xFFFFFFFFu;
-  const uint32_t w = won / 32 % 32, token = filled ? s_token[w][won % 32] : 0u;
+  const uint64_t won = s_won[lane];
+  const bool filled = won != 0;
+  const uint32_t place = 1023u - (uint32_t)(won & 1023u), w = place / 32, token = filled ? s_token[w][place % 32] : 0u;
+  const uint64_t score = s_best[w][place % 32];
   const uint64_t bits = (score >> 63) ? score & ~(1ull << 63) : ~score;
   tokens[out] = token;
   parents[out] = filled ? group * beams + w : out;

@@ -430,8 +430,8 @@ int catena_mi355x_beam_select_plan(uint32_t groups, uint32_t beams, uint32_t voc
 /* Beam search's selection: of logits[groups][beams][vocab] f32 and scores
  * [groups][beams] f32 (log probabilities so far) the `beams` largest
  *   scores[w] + logits[w][v] - log sum_u exp(logits[w][u])
- * over a group's beams w and tokens v, larger first; equal scores: the lower
- * beam, then the larger logit, then the lower token.  done[groups][beams] u32
+ * over a group's beams w and tokens v, larger first; equal scores (of two beams:
+ * to 2^-42 of them): the lower beam, then the larger logit, then the lower token.  done[groups][beams] u32
  * (NULL: none): a beam that is not 0 there offers only token eos, at its own
  * score.  Writes per place tokens, parents (rows: group * beams + w), scores_out
  * (computed in f64, rounded to f32) and done_out (may be NULL): 1 where the
