@@ -110,14 +110,15 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   return CATENA_OK;
 }
 
-constexpr uint32_t kEvictAtOnce = 64;  // moves that its lists in LDS hold
+constexpr uint32_t kEvictAtOnce = 128;  // moves that its lists in LDS hold
 constexpr uint32_t kEvictMoves = 64;  // a workgroup of catena_kv_evict_move
 // Most moves of a (row, kv head): slots below the budget, and slots from it on
 uint32_t evict_most(const PagedKv& kv, uint32_t budget) {
   const uint32_t slots = paged_slots(kv);
   return budget >= slots ? 0 : std::min(budget, slots - budget);
 }
-// a workgroup for a (row, kv head): small while that holds the table
+// a workgroup for a (row, kv head): small while that holds the table (tables of 528
+// slots, one too many, 8 rows x 16 heads 4.3 us against 4.6, 64 rows 5.0 / 15.7)
 uint32_t evict_threads(const PagedKv& kv) { return paged_slots(kv) <= 1024 ? 256 : 1024; }
 // count[pairs], holes[pairs][most], sources[pairs][most]
 int evict_plan(const PagedKv& kv, uint32_t budget, uint64_t* bytes) {
@@ -301,7 +302,9 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t* kv, const uint32_
   a.budget = budget;
   a.recent = recent;
   // Few moves are made by the workgroup that chose them, which saves a launch;
-  // more by workgroups of 64 each.
+  // more by workgroups of 64 each (8 rows x 16 heads of 128, at most 128 moves, of 32
+  // slots too many 6.9 us against 9.1, of 64 8.3 / 10.7, of 96 11.0 / 11.2; at most
+  // 144, of 128 slots 12.8 / 11.5).
   a.at_once = a.most <= kEvictAtOnce;
   void* args[] = {&a};
   st = launch(threads == 256 ? KernelId::KvEvictChoose1k : KernelId::KvEvictChoose8k, dim3(pairs), dim3(threads), 0,

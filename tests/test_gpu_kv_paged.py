@@ -209,6 +209,8 @@ def _weights(rng, kind, shape, slots):
     (1, 64, 16, 200, 1000, 64, [3200, 1500]),
     (2, 128, 16, 3, 48, 4, [48, 20]),              # a budget of the whole table
     (2, 64, 16, 100, 1200, 7, [1201, 1600, 1202]), # one slot, two and many of a longer row
+    (2, 128, 16, 20, 128, 16, [320, 250, 140]),    # as many moves as the choosing workgroup makes
+    (1, 64, 32, 50, 1472, 9, [1600, 1500]),
 ])
 def test_evict(kvh, dim, page, pages, budget, recent, lens, kind, in_place):
     say(f"evict budget {budget} recent {recent} {kind} in place {in_place}")
