@@ -184,6 +184,27 @@ def test_infinities_and_nan_in_use():
         assert np.all(np.abs(got[r] - o) <= attention_slack(es, 70) * pv + U * np.abs(o))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("out_f32", [True, False])
+def test_values_of_the_largest_size_that_weigh_nothing(dim, out_f32):
+    """Slots far below the maximum (e^-300), their values near the type's largest:
+    nothing of them is in the sum."""
+    say(f"attn_paged large values dim {dim} f32 {out_f32}")
+    rng = np.random.default_rng(13)
+    cache = Cache(rng, [80], 1, dim, 16, 5)
+    q = np.zeros((1, 3, dim), np.float32)
+    q[..., 0] = 1
+    k = 0.5 * rng.standard_normal((1, 80, dim))
+    light = np.arange(3, 80, 7)
+    k[:, light, 0] = -300
+    v = rng.standard_normal((1, 80, dim))
+    v[:, light] = 3e38
+    cache.put(cache.k, 0, np.arange(80), bf16(k))
+    cache.put(cache.v, 0, np.arange(80), bf16(v))
+    got, _ = Call(cache, bf16(q), 3, 1.0, out_f32).run()
+    check(cache, bf16(q), 3, 1.0, got, out_f32)
+
+
 def test_offsets_past_32_bits():
     """Pages behind 2^32 elements of a pool."""
     say("attn_paged large pool")
