@@ -9,6 +9,8 @@ Layout mirrors the C header:
   * device/pool:   init, Buffer (catena_mem_t), synchronize, stream
   * kernel ABI:    gemm_f32_exact, gemm_bf16, attn_decode_bf16, softmax_f32, ...
                    and the decoder-block pieces (rmsnorm, rope, silu_mul, argmax, ...)
+  * paged cache:   PagedKV, attn_paged_bf16, rope_qkv_paged_bf16, kv_evict_paged_bf16,
+                   beam_select_f32, beam_reorder_paged_bf16 and their plans
   * decoder:       Decoder (catena_mi355x_decoder_*)
   * program ABI:   program_* functions (fail-stop: they trap on bad input)
   * runtime:       Runtime (catena_runtime_*), mirrors Runtime::from_sources /

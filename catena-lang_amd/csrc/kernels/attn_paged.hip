@@ -16,7 +16,7 @@
 // the order of rows, every workgroup takes an equal stretch of it (ends of units
 // in it and all), and a second kernel joins the units that were cut.  The stretches
 // follow from the rows' own lengths, so ragged batches are even: 64 rows of 1 ..
-// 4096 slots x 8 kv heads of 128 take 84 us (6.3 TB/s) and 5 to join, against 112
+// 4096 slots x 8 kv heads of 128 take 85 us (6.3 TB/s) and 5 to join, against 112
 // with the rows cut alike; 131072 slots x 8 heads in one row 80 us (6.7 TB/s).
 // Where even a full table is short, the host launches a workgroup per unit and no
 // join; else both kernels see by the rows' lengths which it is.
