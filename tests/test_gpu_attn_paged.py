@@ -280,3 +280,26 @@ def test_captured_and_replayed():
             got_o, got_acc = call.bits()
             assert np.array_equal(got_o, o)
             assert acc is None or np.array_equal(got_acc, acc)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_replayed_with_other_lengths(weights):
+    """One graph, lengths that change between replays: cut rows, whole units of
+    short rows, no slots at all."""
+    say(f"attn_paged graph, lengths change, weights {weights}")
+    rng = np.random.default_rng(14)
+    cache = Cache(rng, [4096, 4096, 4096], 2, 64, 32, 128)
+    q = bf16(rng.standard_normal((3, 8, 64)))
+    acc = rng.random((3, 2, cache.slots)).astype(np.float32) if weights else None
+    call = Call(cache, q, 8, 0.125, True, acc)
+    assert call.parts > 0
+    replay = captured(call)
+    for lens in ([4096, 1, 2000], [90, 0, 33], [0, 0, 0], [31, 4096, 700], [4096, 1, 2000]):
+        cache.lens = np.array(lens, np.uint32)
+        cache.lb.write(cache.lens)
+        if weights:
+            call.acc_out.write(np.full_like(acc, -7.0))
+        call.o.write(np.full(call.o.nbytes, 0xEE, np.uint8))
+        replay()
+        o, got_acc = call.bits()
+        check(cache, q, 8, 0.125, o.view(np.float32).astype(np.float64), True, acc, got_acc)
