@@ -189,3 +189,32 @@ def test_beam_search_over_shared_pages():
         tokens_now = t[:, None]
         history = np.concatenate([history[p], tokens_now], 1)
     assert shared > 0
+
+
+def test_prompt_attends_over_pages():
+    """A prompt's tokens as rows of their own whose tables are the sequence's: causal
+    attention over the pages that the append has just filled."""
+    say("prompt over pages")
+    rng = np.random.default_rng(43)
+    heads, kvh, dim, page, pages, tq, old = 6, 2, 128, 32, 5, 70, 33
+    cache = Cache(rng, [old + tq], kvh, dim, page, pages)
+    kv = cache.upload()
+    tab = _rope_tab(old + tq, dim)
+    q, o = ca.Buffer(tq * heads * dim * 2), ca.Buffer(tq * heads * dim * 2)
+    qkv = ca.Buffer.from_array(rng.standard_normal((tq, (heads + 2 * kvh) * dim)).astype(np.float32))
+    ca.rope_qkv_paged_bf16(kv, qkv, tab, old + tq, cache.lb, None, q, tq, heads)
+    tables = ca.Buffer.from_array(np.repeat(cache.table, tq, 0))
+    lens = ca.Buffer.from_array(np.arange(old + 1, old + tq + 1, dtype=np.uint32))
+    each = ca.PagedKV(kv.k, kv.v, tables.ptr, kv.num_pages, page, tq, pages, kvh, dim)
+    work = ca.Buffer(max(ca.attn_paged_plan(each, heads)[1], 16))
+    ca.attn_paged_bf16(each, q, lens, o, heads, dim ** -0.5, work)
+    got, q16 = f64(o.read(np.uint16, (tq, heads, dim))), f64(q.read(np.uint16, (tq, heads, dim)))
+    k, v = (f64(cache.get(pool, 0, old + tq)) for pool in cache.download())
+    group = heads // kvh
+    for t in range(tq):
+        n = old + t + 1
+        for h in range(kvh):
+            mine = slice(h * group, (h + 1) * group)
+            want, _, pv, es = attention(q16[t, mine], k[h, :n], v[h, :n], dim ** -0.5)
+            slack = attention_slack(es, n)
+            assert np.all(np.abs(got[t, mine] - want) <= (slack + 2.0 ** -16) * pv + UB * (np.abs(want) + slack * pv)), (t, h)
