@@ -368,8 +368,9 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q
  * [max_pages * page_size] f32 and u32, both or neither): the new slots' weight
  * 0 and their position.  A token whose slot lies outside the table or whose
  * position outside rope_tab writes q (rotated by rope_tab's first position)
- * and nothing else, one whose page does not exist q alone.  qkv, rope_tab and q
- * 16-byte aligned.  No reference counterpart. */
+ * and nothing else, one whose page does not exist q alone.  No two rows append
+ * into the same page.  qkv, rope_tab and q 16-byte aligned.  No reference
+ * counterpart. */
 int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t *kv, const float *qkv,
                                       const float *rope_tab, uint32_t table_positions,
                                       const uint32_t *lens, const uint32_t *seen, uint16_t *q,
