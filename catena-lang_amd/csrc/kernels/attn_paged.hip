@@ -45,6 +45,12 @@
 // The maximum is raised only where a score passes it by more than 8 in base 2,
 // for all lanes of a head at once: until then p stays below 2^8, which costs no
 // accuracy, and most tiles need no exchange between lanes.
+//
+// Range: the sums of p v are divided by that of p at the end alone.  p enters the
+// products times a power of two below 2^-8 / n, so that no sum passes half the
+// largest |v| and any finite values give a finite mean; the division takes the
+// power back.  (What it costs lies at the other end: products below f32's smallest, of
+// values below some 2^-80.)
 #include "common.h"
 #include "paged.h"
 
@@ -77,6 +83,8 @@ struct RowOnLine {
 CATENA_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // the reference point of exponents: 0 while no score is above -inf
 CATENA_DEV float anchor(float m) { return m == kNegInf ? 0.0f : m; }
+// p's power of two in the products of a row of n > 0 slots: n of p < 2^8 stay below 1/2
+CATENA_DEV float ease_of(uint32_t n) { return __uint_as_float((uint32_t)(127 - 41 + __builtin_clz(n)) << 23); }
 
 struct AttnPagedArgs {
   PagedKv kv;
@@ -95,9 +103,11 @@ struct AttnPagedArgs {
   float scale_log2;       // scale * log2(e)
 };
 
-// Four columns of o / l
+// Four columns of o / l of a row of n slots, whose o is the eased sum; 0 where there are
+// none
 template <bool F32>
-CATENA_DEV void store_o(const AttnPagedArgs& a, uint64_t at, f32x4_t o, float l) {
+CATENA_DEV void store_o(const AttnPagedArgs& a, uint64_t at, f32x4_t o, float l, uint32_t n) {
+  l = n ? l * ease_of(n) : 1.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = o[i] / l;
   if constexpr (F32) {
@@ -282,7 +292,7 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     }
   };
   bf16x8_t qf[KC];
-  float m, l;
+  float m, l, ease;
   f32x4_t acc[VC];
   auto begin = [&](const Part& p) {
     // Q as the B operand: lane = head c, 8 values of each 32-wide block of d
@@ -295,6 +305,7 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     }
     m = kNegInf;
     l = 0.0f;
+    ease = ease_of(p.len | 1u);
 #pragma unroll
     for (int e = 0; e < VC; ++e) acc[e] = f32x4_t{0, 0, 0, 0};
   };
@@ -345,6 +356,7 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     for (int j = 0; j < 8; ++j) {
       p[j] = exp2_fast(s[j] - base);
       l = l + p[j];
+      p[j] = p[j] * ease;
     }
     // p's bf16 terms
     constexpr int TERMS = F32 ? 3 : 2;
@@ -435,7 +447,7 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
           a.whole_ml[2 * to + 1] = ll;
         }
       }
-      store_o<F32>(a, at, o, p.len ? ll : 1.0f);  // no slots: 0 / 1
+      store_o<F32>(a, at, o, ll, p.len);
     }
     if constexpr (WEIGHTS) {
       // weights of whole units that are all of their kv head (of the line's the
@@ -586,7 +598,7 @@ CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
       if (!pieces) {
         if (head >= a.group || p.n == 1) continue;
         const Joined j = join_parts<D>(a, p, head % 16, col, 0, 1);
-        store_o<F32>(a, at, j.o, r.len ? j.l : 1.0f);
+        store_o<F32>(a, at, j.o, j.l, r.len);
         continue;
       }
       if (p.n == 1) continue;
@@ -606,7 +618,7 @@ CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) o[c] = o[c] + y[c] * f;
         }
-        store_o<F32>(a, at, o, r.len ? l : 1.0f);
+        store_o<F32>(a, at, o, l, r.len);
       }
     }
     return;

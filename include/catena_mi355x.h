@@ -341,8 +341,9 @@ int catena_mi355x_attn_paged_plan(const catena_paged_kv_t *kv, uint32_t heads, i
  * them; a length past the table counts as the table's), o[rows][heads]
  * [head_dim] f32 (out_f32 != 0) or bf16 RNE.  Query head h reads kv head
  * h / (heads / kv_heads); o = sum_j p_j v_j, p = softmax(scale * q . k_j) with
- * the exponential itself (not math.exp-approx), sums in f32.  A row of no slots
- * gives 0, a row whose pages are all unknown NaN.  What the cache holds past a
+ * the exponential itself (not math.exp-approx), sums in f32 that finite values of
+ * any size do not overflow.  A row of no slots gives 0, a row whose pages are all
+ * unknown NaN.  What the cache holds past a
  * row's slots is never used.
  * acc_in / acc_out[rows][kv_heads][max_pages * page_size] f32 (both or
  * neither, may be the same): acc_out[j] = acc_in[j] + the sum of p_j over the

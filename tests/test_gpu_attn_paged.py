@@ -303,3 +303,51 @@ def test_replayed_with_other_lengths(weights):
         replay()
         o, got_acc = call.bits()
         check(cache, q, 8, 0.125, o.view(np.float32).astype(np.float64), True, acc, got_acc)
+
+
+LARGE = [
+    # heads, kv heads, dim, page, max pages, lens
+    (3, 1, 128, 16, 5, [2, 80]),                    # whole units
+    (34, 2, 64, 16, 5, [80, 33, 16]),               # two tiles of heads
+    (2, 1, 64, 16, 1024, [16384]),                  # cut rows, by the parts a unit has: many,
+    (4, 4, 128, 32, 128, [4096] * 8 + [70, 5]),     # some,
+    (8, 8, 64, 32, 128, [4096] * 8 + [31] * 60),    # few
+]
+
+
+@pytest.mark.parametrize("out_f32", [True, False])
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_values_near_the_largest_that_weigh(case, out_f32):
+    """Values near the type's largest, all of one sign in a column and all of
+    weight: their mean is as large as they are, no sum on the way larger.  Scores
+    rise along the row, so that many weights are formed below their maximum."""
+    heads, kvh, dim, page, pages, lens = LARGE[case]
+    say(f"attn_paged values of weight near the largest, case {case} f32 {out_f32}")
+    rng = np.random.default_rng(200 + case)
+    cache = Cache(rng, lens, kvh, dim, page, pages, lazy=True)
+    q = np.zeros((len(lens), heads, dim), np.float32)
+    q[..., 0] = 1
+    sign = np.where(rng.random((kvh, 1, dim)) < 0.5, -1.0, 1.0)
+    for r, n in enumerate(lens):
+        k = 0.1 * rng.standard_normal((kvh, n, dim))
+        k[:, :, 0] += np.linspace(0, 6, n)
+        cache.put(cache.k, r, np.arange(n), bf16(k))
+        cache.put(cache.v, r, np.arange(n), bf16(sign * (3.2e38 + 1e37 * rng.random((kvh, n, dim)))))
+    call = Call(cache, bf16(q), heads, 1.0, out_f32, rng.random((len(lens), kvh, cache.slots)).astype(np.float32))
+    assert (call.parts > 0) == (case >= 2 or case == 1)  # weights of two tiles of heads are joined
+    got, acc = call.run()
+    assert np.all(np.isfinite(got))
+    check(cache, bf16(q), heads, 1.0, got, out_f32, call.acc.read(np.float32, acc.shape), acc)
+
+
+@pytest.mark.parametrize("size", [1e-33, 1e-25, 1e18, 1e35])
+@pytest.mark.parametrize("lens", [[80], [16384]])
+def test_values_of_any_size(lens, size):
+    """The mean of small values and of large ones, over few slots and many."""
+    say(f"attn_paged values near {size}, {lens[0]} slots")
+    rng = np.random.default_rng(15)
+    cache = Cache(rng, lens, 1, 64, 16, lens[0] // 16)
+    cache.put(cache.v, 0, np.arange(lens[0]), bf16(size * rng.standard_normal((1, lens[0], 64))))
+    q = bf16(rng.standard_normal((1, 3, 64)))
+    got, _ = Call(cache, q, 3, 0.125, True).run()
+    check(cache, q, 3, 0.125, got, True)
