@@ -399,7 +399,9 @@ extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_move(EvictArgs
 // past it stay r's own.  Nothing that is read here is written: the tables are
 // two, and a spare page is in no table.  A row that is its own parent keeps its
 // pages.  A row whose parent does not exist, has another length than the row
-// or one past the table is given up: length 0, no pages, its spare kept.
+// or one past the table is given up: length 0, no pages, its spare kept.  Where the
+// parent's partly filled page is none of the pool's, r's is none either: neither its
+// spare page nor its own has those rows.
 //
 // Bound: HBM, two passes over the used part of a page for each (row, head, pool); a
 // launch where that is little.  64 rows x 8 heads of 128, 32 pools, 49 slots each: 65.6
@@ -429,21 +431,22 @@ CATENA_DEV void kv_reorder(const ReorderArgs& a, uint16_t* const* pools) {
   const uint32_t n = p < kv.rows ? a.lens[p] : 0u;
   const bool good = p < kv.rows && n == a.lens[r] && n <= paged_slots(kv);
   const uint32_t last = n >> kv.page_shift, used = n & mask;
-  const bool copies = good && p != r && used != 0;
+  const bool partly = good && p != r && used != 0;
   const uint32_t* mine = kv.table + (uint64_t)r * kv.max_pages;
   const uint32_t* theirs = kv.table + (uint64_t)(good ? p : r) * kv.max_pages;
+  const uint32_t from = theirs[partly ? last : 0u], to = a.spare[r];
+  const bool copies = partly && from < kv.num_pages;
   if (a.tables && h == 0 && blockIdx.z == 0) {
     uint32_t* out = a.table_out + (uint64_t)r * kv.max_pages;
     for (uint32_t j = threadIdx.x; j < kv.max_pages; j += 256)
-      out[j] = !good ? 0xFFFFFFFFu : j < last ? theirs[j] : j == last && copies ? a.spare[r] : mine[j];
+      out[j] = !good ? 0xFFFFFFFFu : j < last ? theirs[j] : j == last && partly ? (copies ? to : from) : mine[j];
     if (threadIdx.x == 0) {
       a.lens_out[r] = good ? n : 0u;
-      a.spare_out[r] = copies ? mine[last] : a.spare[r];
+      a.spare_out[r] = copies ? mine[last] : to;
     }
   }
   if (!copies || blockIdx.z >= a.n_pools) return;
-  const uint32_t from = theirs[last], to = a.spare[r];
-  if (from >= kv.num_pages || to >= kv.num_pages) return;
+  if (to >= kv.num_pages) return;
   uint16_t* pool = pools[blockIdx.z];
   const u32x4_t* src = reinterpret_cast<const u32x4_t*>(pool + paged_offset(kv, from, h, 0));
   u32x4_t* dst = reinterpret_cast<u32x4_t*>(pool + paged_offset(kv, to, h, 0));

@@ -415,7 +415,10 @@ int catena_mi355x_kv_evict_paged_bf16(const catena_paged_kv_t *kv, const uint32_
  * max_pages pages and one spare page of their own need no allocator: filled
  * pages are never written again, and the page that a row writes next is its
  * own.  A row whose parent does not exist, has another length than the row, or
- * one past the table comes out with length 0 and page numbers 0xFFFFFFFF.
+ * one past the table comes out with length 0 and page numbers 0xFFFFFFFF.  A
+ * partly filled page of the parent that does not exist is passed on as it is (and
+ * r keeps spare[r]); one that was to go into a spare page that does not exist is
+ * absent.
  * The outputs are not the inputs; spare pages are distinct and in no table.
  * No reference counterpart. */
 int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t *kv, uint16_t *const *pools,

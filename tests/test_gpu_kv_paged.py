@@ -353,3 +353,36 @@ def test_reorder_captured_and_replayed():
             dev.write(pool)
         replay()
         case.check()
+
+
+# ---------------------------------------------------------------- reorder, pages that are not there
+
+def test_reorder_of_pages_that_are_not_there():
+    """A parent whose partly filled page does not exist: absent for its children too,
+    and their own pages' old rows are not in its place.  A spare page that does not
+    exist takes no rows."""
+    say("reorder unknown pages")
+    rng = np.random.default_rng(33)
+    parents = [0, 0, 1, 0, 4]
+    case = Reorder(rng, 5, 2, 64, 16, 4, [37] * 5, parents, 3)
+    table, spare = case.c.table.copy(), case.c.spare.copy()
+    table[1, 2], table[4, 2] = case.c.num_pages, 0xFFFFFFFF  # the parent of 2; its own parent
+    table[0, 1] = 0xFFFFFFFF                                 # a filled page: of 0, 1 and 3
+    spare[3] = case.c.num_pages + 5
+    case.c.tb.write(table)
+    case.sb.write(spare)
+    case()
+    got, num = case.t2.read(np.uint32, table.shape), case.c.num_pages
+    want, want_spare, pools = table.copy(), spare.copy(), [p.copy() for p in case.pools]
+    want[1, :2], want[1, 2], want_spare[1] = table[0, :2], spare[1], table[1, 2]
+    want[2, :2] = table[1, :2]
+    want[3, :2], want[3, 2], want_spare[3] = table[0, :2], spare[3], table[3, 2]
+    for pool in pools:
+        pool[spare[1], :, :5] = pool[table[0, 2], :, :5]
+    assert got[2, 2] >= num
+    got[2, 2] = want[2, 2]
+    assert np.array_equal(got, want)
+    assert np.array_equal(case.s2.read(np.uint32), want_spare)
+    assert np.array_equal(case.l2.read(np.uint32), [37] * 5)
+    for pool, dev in zip(pools, case.dev):
+        assert np.array_equal(dev.read(np.uint16, pool.shape), pool)
