@@ -126,7 +126,9 @@ const KernelSpec kKernels[] = {
     {KernelId::AttnPagedJoinD64Bf16, "attn_paged", "catena_attn_paged_join_d64_bf16out"},
     {KernelId::RopeQkvPaged, "kv_paged", "catena_rope_qkv_paged"},
     {KernelId::KvEvictChoose1k, "kv_paged", "catena_kv_evict_choose_1k"},
+    {KernelId::KvEvictChoose1kManyRecent, "kv_paged", "catena_kv_evict_choose_1k_many_recent"},
     {KernelId::KvEvictChoose8k, "kv_paged", "catena_kv_evict_choose_8k"},
+    {KernelId::KvEvictChoose8kManyRecent, "kv_paged", "catena_kv_evict_choose_8k_many_recent"},
     {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
     {KernelId::KvReorder8, "kv_paged", "catena_kv_reorder_8"},
     {KernelId::KvReorder128, "kv_paged", "catena_kv_reorder_128"},

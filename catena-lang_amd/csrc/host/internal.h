@@ -89,7 +89,9 @@ enum class KernelId : int {
   AttnPagedJoinD64Bf16,
   RopeQkvPaged,  // upkeep of a cache in pages (kv_paged.hip)
   KvEvictChoose1k,
+  KvEvictChoose1kManyRecent,
   KvEvictChoose8k,
+  KvEvictChoose8kManyRecent,
   KvEvictMove,
   KvReorder8,
   KvReorder128,

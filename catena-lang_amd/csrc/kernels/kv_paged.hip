@@ -77,7 +77,8 @@ extern "C" __global__ __launch_bounds__(256) void catena_rope_qkv_paged(
 //
 // Keeps min(n, budget) of a row's n slots, per kv head: those of the last
 // `recent` positions, then those of the largest accumulated weight, the lower
-// slot where two are equal; a NaN weight goes first.  The i-th slot given up
+// slot where two are equal; a NaN weight goes first.  Where more slots than the
+// budget are recent, the newest are kept.  The i-th slot given up
 // below the budget takes the i-th kept slot from the budget on, so that the
 // kept slots are the first ones: attention does not depend on the slots' order,
 // and only as many rows move as were given up there.
@@ -88,6 +89,12 @@ namespace {
 CATENA_DEV uint32_t keep_key(float weight, uint32_t pos, uint32_t late) {
   if (pos >= late) return 0xFFFFFFFFu;
   return weight != weight ? 0u : mono_bits(__float_as_uint(weight));
+}
+
+// The same where the recent slots alone are more than the budget
+CATENA_DEV uint32_t newest_key(uint32_t pos, uint32_t late) {
+  const uint32_t after = pos - late;
+  return pos < late ? 0u : after < 0xFFFFFFFFu ? after + 1 : after;
 }
 
 // Exclusive prefix sum over the workgroup's threads, and the total.  s_wave[2]:
@@ -173,7 +180,9 @@ CATENA_DEV void evict_moves(const EvictArgs& a, uint32_t pair, const uint32_t* h
 // Bound: latency (two dependent loads, a dozen barriers), so short rows take a
 // small workgroup: 32 x 8 rows of 5120 slots, 4096 kept, 12.6 us; 8 x 16 of 513 slots,
 // 512 kept, 4.0 with the move.
-template <int THREADS, int KEYS>
+// MANY: recent > budget.  Positions differ, so that only then more slots than the budget
+// can be recent, which is counted first.
+template <int THREADS, int KEYS, bool MANY>
 CATENA_DEV void evict_choose(const EvictArgs& a) {
   constexpr int WAVES = THREADS / 64, DIGIT = THREADS == 256 ? 8 : 12, STEPS = THREADS == 256 ? 4 : 3;
   constexpr uint32_t BINS = 1u << DIGIT, OWN = BINS / THREADS, TILE = THREADS * KEYS;
@@ -209,10 +218,12 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
   if (tid == 0 && pair % a.kv.kv_heads == 0) a.lens_out[row] = kept;
   // the tile's keys; 0, the last of all, behind the row's end
   uint32_t keys[KEYS];
+  bool window = false;  // recent slots alone are kept
   auto rate = [&]() {
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
-      const uint32_t key = keep_key(w[i / 4][i % 4], p[i / 4][i % 4], late);
+      const uint32_t pos = p[i / 4][i % 4];
+      const uint32_t key = MANY && window ? newest_key(pos, late) : keep_key(w[i / 4][i % 4], pos, late);
       keys[i] = beg + i < n ? key : 0u;
     }
   };
@@ -241,6 +252,17 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
     }
     if (tid == 0 && !a.at_once) a.count[pair] = 0;
     return;
+  }
+  if constexpr (MANY) {
+    uint32_t mine = 0, all;
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load(tile, n);
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) mine += beg + i < n && p[i / 4][i % 4] >= late;
+    }
+    block_prefix<WAVES>(mine, s_wave[1], &all);
+    window = all > budget;
   }
   if (tiles == 1) rate();
 
@@ -377,8 +399,18 @@ CATENA_DEV void evict_choose(const EvictArgs& a) {
 }  // namespace
 
 // One workgroup per (row, kv head)
-extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_choose_1k(EvictArgs a) { evict_choose<256, 4>(a); }
-extern "C" __global__ __launch_bounds__(1024) void catena_kv_evict_choose_8k(EvictArgs a) { evict_choose<1024, 8>(a); }
+extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_choose_1k(EvictArgs a) {
+  evict_choose<256, 4, false>(a);
+}
+extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_choose_1k_many_recent(EvictArgs a) {
+  evict_choose<256, 4, true>(a);
+}
+extern "C" __global__ __launch_bounds__(1024) void catena_kv_evict_choose_8k(EvictArgs a) {
+  evict_choose<1024, 8, false>(a);
+}
+extern "C" __global__ __launch_bounds__(1024) void catena_kv_evict_choose_8k_many_recent(EvictArgs a) {
+  evict_choose<1024, 8, true>(a);
+}
 
 // grid = (pairs, ceil(most / 64)); 64 moves a workgroup.  Bound: HBM, 8 D bytes a
 // move: the 32 x 8 rows' 1024 slots too many, heads of 128, 47.6 us at 4.5 TB/s, the

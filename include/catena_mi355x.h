@@ -384,8 +384,9 @@ int catena_mi355x_kv_evict_paged_plan(const catena_paged_kv_t *kv, uint32_t budg
 
 /* Bounds a cache in pages: per (row, kv head), of the lens[row] slots in use
  * min(lens[row], budget) are kept -- those of the last `recent` of the
- * seen[row] positions, then those of the largest accumulated weight, the lower
- * slot where two are equal, a NaN weight behind every number -- and become the
+ * seen[row] positions (the newest where they are more than the budget), then
+ * those of the largest accumulated weight, the lower slot where two are equal, a
+ * NaN weight behind every number -- and become the
  * first slots: the i-th slot given up below the budget takes K, V, weight and
  * position of the i-th slot kept from the budget on; the others stay where
  * they are.  (Attention does not depend on the order of slots; RoPE is applied

@@ -355,6 +355,35 @@ def test_reorder_captured_and_replayed():
         case.check()
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("page,pages,budget,recent,lens", [
+    (16, 8, 40, 300, [128, 100, 41, 40, 7]),       # in LDS; one slot too many; none
+    (16, 8, 1, 2000, [128, 2]),                    # the newest alone
+    (16, 100, 700, 1 << 31, [1600, 1500, 701]),    # every position there was
+    (16, 90, 400, 4000, [1440, 1200, 1100]),
+    (1024, 20, 5000, 50000, [20001, 15000, 5001]), # tiles of 8192
+])
+def test_evict_keeps_the_newest_of_many_recent_positions(page, pages, budget, recent, lens, in_place):
+    """More slots of the last positions than the budget: the newest are kept, whatever
+    slots they are in."""
+    say(f"evict window, budget {budget} recent {recent} in place {in_place}")
+    rng = np.random.default_rng(budget)
+    cache = Cache(rng, lens, 2, 64, page, pages)
+    shape = (len(lens), 2, cache.slots)
+    seen = 3 * cache.slots
+    pos = np.broadcast_to(rng.permutation(seen)[:cache.slots].astype(np.uint32), shape).copy()
+    acc = _weights(rng, "anything", shape, cache.slots)
+    for r, n in enumerate(lens):  # one row after the other: its window is its own
+        one = Cache(rng, [n], 2, 64, page, pages)
+        case = Evict(one, acc[r:r + 1], pos[r:r + 1], np.array([seen], np.uint32), budget, recent, in_place)
+        case()
+        late = np.sort(pos[r, 0, :n][pos[r, 0, :n].astype(np.int64) >= seen - recent])[::-1]
+        assert len(late) > budget or r > 0  # fewer in a shorter row: all are kept, then by weight
+        if len(late) > budget:
+            case.recent = seen - int(late[budget - 1])  # the same said with no more of them than the budget
+        case.check()
+
+
 # ---------------------------------------------------------------- reorder, pages that are not there
 
 def test_reorder_of_pages_that_are_not_there():
