@@ -437,10 +437,14 @@ int catena_mi355x_beam_select_plan(uint32_t groups, uint32_t beams, uint32_t voc
  * [groups][beams] f32 (log probabilities so far) the `beams` largest
  *   scores[w] + logits[w][v] - log sum_u exp(logits[w][u])
  * over a group's beams w and tokens v, larger first; equal scores (of two beams:
- * to 2^-42 of them): the lower beam, then the larger logit, then the lower token.  done[groups][beams] u32
- * (NULL: none): a beam that is not 0 there offers only token eos, at its own
- * score.  Writes per place tokens, parents (rows: group * beams + w), scores_out
- * (computed in f64, rounded to f32) and done_out (may be NULL): 1 where the
+ * to 2^-42 of them): the lower beam, then the larger logit, then the lower token.
+ * A beam's log sum is off by up to 3e-6: its exponentials and their sums by 16 are
+ * f32, all further sums f64.  So a beam's own tokens come in the order of their
+ * logits, but continuations of two beams that are less than 6e-6 apart may
+ * come in either order, and scores_out is off by as much and its rounding to f32.
+ * done[groups][beams] u32 (NULL: none): a beam that is not 0 there offers only
+ * token eos, at its own score.  Writes per place tokens, parents (rows:
+ * group * beams + w), scores_out and done_out (may be NULL): 1 where the
  * parent was done or the token is eos.  eos 0xFFFFFFFF: no token ends a beam
  * (done must then be NULL).  A continuation whose score is not finite is not
  * offered; NaN or +inf among a beam's logits take all of them.  A place that

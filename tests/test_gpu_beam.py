@@ -235,3 +235,45 @@ def test_in_place_and_replayed():
         other()
         case.check()
         other.check()
+
+
+@pytest.mark.parametrize("groups,vocab", [(1, 5000), (1, 128000), (40, 32000)])
+def test_beams_of_different_shape_close_together(groups, vocab):
+    """One logit far above many equal ones, all alike, and a spread: sums that are off
+    by different amounts.  An exponential is off by 2.3 u of |x - max| (the
+    difference, its product with log2 e, log2 e itself) and 2 u, a sum of 16 of them by 5
+    u; the mean of |x - max| under the row's probabilities is at most ln(vocab), 18: 3e-6
+    in all, and the result's rounding.  No continuation comes before one that is 6e-6
+    above it."""
+    say(f"beam_select shapes {groups} x {vocab}")
+    rng = np.random.default_rng(vocab)
+    beams, offset = 6, 0.3125
+    x = np.zeros((groups, beams, vocab), np.float32)
+    x[:, 0, 11] = 8.59
+    x[:, 1] = offset
+    x[:, 2] = 2.5 * rng.standard_normal((groups, vocab))
+    x[:, 3, :7] = 12.2
+    x[:, 4] = rng.random((groups, vocab))
+    x[:, 5, ::3] = -9.7
+    best = x.astype(np.float64).max(-1)
+    lse = best + np.log(np.exp(x - best[..., None].astype(np.float64)).sum(-1))
+    # the beams' best continuations 8e-6 apart, in any order, their scores as far as f32 has them
+    place = np.argsort(rng.random((groups, beams)), -1)
+    scores = (-1.0 - 8e-6 * place - (best - lse)).astype(np.float32)
+    exact = scores.astype(np.float64) + (best - lse)
+    case = Select(x, scores, np.zeros((groups, beams), np.uint32))
+    case()
+    tokens, parents, got, _ = case.read()
+    for g in range(groups):
+        order = np.sort(exact[g])[::-1]
+        assert abs(got[g, 0] - order[0]) <= 3e-6 + U * abs(order[0])
+        first = parents[g, 0] - g * beams
+        assert exact[g, first] >= order[0] - 6e-6
+    # every score is its continuation's
+    x64 = x.astype(np.float64)
+    for g in range(groups):
+        w = parents[g] - g * beams
+        want = scores[g, w].astype(np.float64) + x64[g, w, tokens[g]] - lse[g, w]
+        assert np.all(np.abs(got[g] - want) <= 3e-6 + U * np.abs(want))
+        # and what comes before another is not behind it by more than both are off
+        assert np.all(np.diff(want) <= 6e-6)
