@@ -12,8 +12,9 @@
 //   y1 = x1 c - x2 s, y2 = x2 c + x1 s  (each operation rounded)
 // q to q_out[rows * tq][heads * D], k and v to the slot's page, all bf16 RNE; a
 // tracked cache's weight of the slot starts at 0 and its position is noted.
-// A token whose slot or position does not exist writes q turned by tab[0] and
-// nothing else; one whose page does not exist writes q alone.
+// A token whose slot or position does not exist, or whose row has fewer of either than
+// tq, writes q turned by tab[0] and nothing else; one whose page does not exist writes
+// q alone.
 //
 // Bound: HBM for prompts (4 bytes in, 2 out per value), one launch's latency for
 // a decode step.  A thread takes four pairs (two 16-byte loads of x, two of the

@@ -369,7 +369,8 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q
  * [max_pages * page_size] f32 and u32, both or neither): the new slots' weight
  * 0 and their position.  A token whose slot lies outside the table or whose
  * position outside rope_tab writes q (rotated by rope_tab's first position)
- * and nothing else, one whose page does not exist q alone.  No two rows append
+ * and nothing else, and so do all tokens of a row whose lens or seen is below tq;
+ * one whose page does not exist writes q alone.  No two rows append
  * into the same page.  qkv, rope_tab and q 16-byte aligned.  No reference
  * counterpart. */
 int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t *kv, const float *qkv,

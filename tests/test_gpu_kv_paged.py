@@ -355,6 +355,42 @@ def test_reorder_captured_and_replayed():
         case.check()
 
 
+# ---------------------------------------------------------------- append, rows that share pages
+
+def test_append_of_rows_shorter_than_the_call():
+    """A row of fewer slots, or fewer positions, than the call has tokens a row takes
+    none of them, those that would have a slot included; its q is turned by the first
+    position.  (The tokens of prompts of different lengths are rows of one token.)"""
+    say("append to short rows")
+    rng = np.random.default_rng(5)
+    heads, kvh, dim, tq = 4, 2, 128, 5
+    cache = Cache(rng, [3, 9, 4, 5], kvh, dim, 16, 2)
+    seen = np.array([3, 4, 60, 7], np.uint32)  # too few slots; positions; slots again; good
+    tab = _table(80, dim)
+    qkv = rng.standard_normal((4, tq, heads + 2 * kvh, dim)).astype(np.float32)
+    acc = rng.random((4, kvh, 32)).astype(np.float32)
+    kv = cache.upload()
+    accb, posb, q = ca.Buffer.from_array(acc), ca.Buffer.from_array(np.full(acc.shape, 9, np.uint32)), ca.Buffer(4 * tq * heads * dim * 2)
+    ca.rope_qkv_paged_bf16(kv, ca.Buffer.from_array(qkv), ca.Buffer.from_array(tab), len(tab), cache.lb,
+                           ca.Buffer.from_array(seen), q, tq, heads, accb, posb)
+    got = f64(q.read(np.uint16, (4, tq, heads, dim)))
+    for r, pos in enumerate(([0] * 5, [0] * 5, [0] * 5, [2, 3, 4, 5, 6])):
+        y, tol = _rotated(qkv[r, :, :heads].astype(np.float64), tab[pos][:, None])
+        assert np.all(np.abs(got[r] - y) <= tol), r
+    k, v = cache.download()
+    slots = np.arange(5)
+    at = (cache.table[3, slots // 16], slice(None), slots % 16)
+    assert np.array_equal(v[at], bf16(qkv[3, :, heads + kvh:]))
+    for new, old in ((k, cache.k), (v, cache.v)):
+        new[at] = old[at]
+        assert np.array_equal(new, old)
+    acc[3, :, slots] = 0
+    assert np.array_equal(accb.read(np.float32, acc.shape), acc)
+    where = np.full(acc.shape, 9, np.uint32)
+    where[3, :, slots] = slots[:, None] + 2
+    assert np.array_equal(posb.read(np.uint32, acc.shape), where)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("page,pages,budget,recent,lens", [
     (16, 8, 40, 300, [128, 100, 41, 40, 7]),       # in LDS; one slot too many; none
