@@ -370,8 +370,10 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q
  * 0 and their position.  A token whose slot lies outside the table or whose
  * position outside rope_tab writes q (rotated by rope_tab's first position)
  * and nothing else, and so do all tokens of a row whose lens or seen is below tq;
- * one whose page does not exist writes q alone.  No two rows append
- * into the same page.  qkv, rope_tab and q 16-byte aligned.  No reference
+ * one whose page does not exist writes q alone.  No two tokens of a call go to
+ * the same slot of a page; rows may share pages, so that the tokens of prompts of
+ * different lengths are rows of one token each, whose tables are their prompt's
+ * (acc and slot_pos belong to a row: NULL there).  qkv, rope_tab and q 16-byte aligned.  No reference
  * counterpart. */
 int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t *kv, const float *qkv,
                                       const float *rope_tab, uint32_t table_positions,

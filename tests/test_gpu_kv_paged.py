@@ -391,6 +391,37 @@ def test_append_of_rows_shorter_than_the_call():
     assert np.array_equal(posb.read(np.uint32, acc.shape), where)
 
 
+def test_append_of_prompts_of_different_lengths():
+    """Their tokens as rows of one token, whose tables are their sequence's: rows
+    that write different slots of one page, the same as a call a prompt."""
+    say("append of ragged prompts")
+    rng = np.random.default_rng(6)
+    heads, kvh, dim, prompts = 6, 2, 64, [1, 37, 16, 50, 33]
+    whole = Cache(rng, [0] * len(prompts), kvh, dim, 16, 4)
+    tab = ca.Buffer.from_array(_table(64, dim))
+    qkv = rng.standard_normal((sum(prompts), heads + 2 * kvh, dim)).astype(np.float32)
+    kv = whole.upload()
+    begins = np.cumsum([0] + prompts)
+    want_q = []
+    for r, n in enumerate(prompts):
+        table, q = ca.Buffer.from_array(whole.table[r]), ca.Buffer(n * heads * dim * 2)
+        one = ca.PagedKV(kv.k, kv.v, table.ptr, kv.num_pages, 16, 1, 4, kvh, dim)
+        ca.rope_qkv_paged_bf16(one, ca.Buffer.from_array(qkv[begins[r]:begins[r + 1]]), tab, 64,
+                               ca.Buffer.from_array(np.array([n], np.uint32)), None, q, n, heads)
+        want_q.append(q.read(np.uint16, (n, heads, dim)))
+    want = whole.download()
+    kv = whole.upload()  # the pages as they were
+    rows = np.repeat(np.arange(len(prompts)), prompts)
+    table = ca.Buffer.from_array(whole.table[rows])
+    lens = np.concatenate([np.arange(1, n + 1) for n in prompts]).astype(np.uint32)
+    q = ca.Buffer(sum(prompts) * heads * dim * 2)
+    each = ca.PagedKV(kv.k, kv.v, table.ptr, kv.num_pages, 16, sum(prompts), 4, kvh, dim)
+    ca.rope_qkv_paged_bf16(each, ca.Buffer.from_array(qkv), tab, 64, ca.Buffer.from_array(lens), None, q, 1, heads)
+    assert np.array_equal(q.read(np.uint16, (sum(prompts), heads, dim)), np.concatenate(want_q))
+    for got, pool in zip(whole.download(), want):
+        assert np.array_equal(got, pool)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("page,pages,budget,recent,lens", [
     (16, 8, 40, 300, [128, 100, 41, 40, 7]),       # in LDS; one slot too many; none
