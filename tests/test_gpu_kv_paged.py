@@ -422,6 +422,24 @@ def test_append_of_prompts_of_different_lengths():
         assert np.array_equal(got, pool)
 
 
+# ---------------------------------------------------------------- eviction, ties in long rows, windows
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kind", ["equal", "few values", "anything"])
+@pytest.mark.parametrize("budget,recent", [(50000, 3000), (9000, 100), (65000, 0), (30000, 30000), (70000, 500)])
+def test_evict_equal_weights_in_long_rows(budget, recent, kind, in_place):
+    """The lower slot where weights are equal, where the last one that is kept lies in
+    any of a row's tiles of 8192."""
+    say(f"evict long row, {kind}, budget {budget} recent {recent} in place {in_place}")
+    rng = np.random.default_rng(budget + recent)
+    cache = Cache(rng, [70001, 69000], 1, 64, 1024, 69)
+    pos = np.stack([rng.permutation(2 * cache.slots)[:cache.slots] for _ in range(2)])[:, None].astype(np.uint32)
+    case = Evict(cache, _weights(rng, kind, (2, 1, cache.slots), cache.slots), pos, np.full(2, 2 * cache.slots, np.uint32),
+                 budget, recent, in_place)
+    case()
+    case.check()
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("page,pages,budget,recent,lens", [
     (16, 8, 40, 300, [128, 100, 41, 40, 7]),       # in LDS; one slot too many; none
