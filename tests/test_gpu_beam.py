@@ -237,6 +237,40 @@ def test_in_place_and_replayed():
         other.check()
 
 
+@pytest.mark.parametrize("groups,beams,vocab", [
+    (64, 2, 8191), (32, 4, 8192), (16, 4, 16385), (8, 32, 4097), (256, 1, 4096), (1, 16, 70001), (1, 32, 200001), (300, 1, 100),
+])
+def test_wide_runs(groups, beams, vocab):
+    """Batches large enough for runs of 4096 logits: their borders, what is left behind
+    the last whole one, and (32 beams) more lists than are joined at once."""
+    say(f"beam_select wide runs {groups} x {beams} x {vocab}")
+    assert groups * beams * -(-vocab // 4096) >= 256
+    case = _draw(beams + vocab, groups, beams, vocab)
+    case()
+    case.check()
+
+
+@pytest.mark.parametrize("groups,beams,vocab", [(64, 4, 5000), (1, 32, 200001)])
+def test_equal_logits_in_wide_runs(groups, beams, vocab):
+    """More equal logits than a run's list or the join's holds, chunk after chunk of
+    lists: the lower beam, then the larger logit, then the lower token."""
+    say(f"beam_select equal logits, wide runs {groups} x {beams} x {vocab}")
+    rng = np.random.default_rng(vocab)
+    logits = np.zeros((groups, 1, vocab), np.float32)
+    if groups > 1:
+        logits[1], logits[2, :, ::2] = rng.integers(0, 3, vocab), -0.0
+        logits[3] = np.where(rng.random(vocab) < 0.5, 7.0, -3.0)
+    # a group's beams alike, so that their sums are
+    case = Select(np.repeat(logits, beams, 1), np.zeros((groups, beams), np.float32), None, ca.BEAM_NO_EOS)
+    case()
+    case.check(tied=True)
+    late = np.zeros((1, beams, vocab), np.float32)
+    late[0, :, vocab - 40:] = 1  # the best in the last run of all
+    case = Select(late, np.zeros((1, beams), np.float32), None, ca.BEAM_NO_EOS)
+    case()
+    case.check(tied=True)
+
+
 @pytest.mark.parametrize("groups,vocab", [(1, 5000), (1, 128000), (40, 32000)])
 def test_beams_of_different_shape_close_together(groups, vocab):
     """One logit far above many equal ones, all alike, and a spread: sums that are off
