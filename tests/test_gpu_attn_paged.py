@@ -340,6 +340,44 @@ def test_values_near_the_largest_that_weigh(case, out_f32):
     check(cache, bf16(q), heads, 1.0, got, out_f32, call.acc.read(np.float32, acc.shape), acc)
 
 
+CUT = [  # full rows are longer than what is taken whole
+    # heads, kv heads, dim, page, max pages, lens
+    # more than 64 rows on one line, several without slots before longer ones
+    (8, 4, 128, 32, 50, [0, 0, 1600] + [(29 * i) % 180 for i in range(60)] + [0, 1600, 0, 0, 1590] + [0, 7] * 10 + [1600, 0, 64]),
+    # the join without pieces, by few long rows
+    (8, 8, 64, 64, 64, [4096] + [100, 0, 1, 33, 900] * 7 + [4096, 3000, 0, 2]),
+    # long parts: 16384 tiles, of few units (128 wide and 64), of more than there are CUs
+    (8, 8, 128, 1024, 64, [65536]),
+    (16, 8, 64, 1024, 65, [66560]),
+    (8, 8, 128, 64, 64, [1650] * 39 + [4096]),
+    # more rows than the join's grid: with a piece a head, without pieces
+    (128, 8, 128, 32, 65, [2080, 0, 31] + [97 * i for i in range(1, 16)]),
+    (16, 8, 64, 1024, 9, [9216] + [(7 * i) % 40 for i in range(298)] + [9000]),
+]
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("case", range(len(CUT)))
+def test_cut_rows(case, weights):
+    heads, kvh, dim, page, pages, lens = CUT[case]
+    say(f"attn_paged cut rows, case {case} heads {heads}/{kvh} dim {dim} rows {len(lens)} weights {weights}")
+    rng = np.random.default_rng(300 + case)
+    cache = Cache(rng, lens, kvh, dim, page, pages, lazy=True)
+    q = bf16(rng.standard_normal((len(lens), heads, dim)))
+    acc = rng.random((len(lens), kvh, cache.slots)).astype(np.float32) if weights else None
+    out_f32 = case % 2 == 0
+    call = Call(cache, q, heads, dim ** -0.5, out_f32, acc)
+    # a plan of parts for a table's full rows, and full rows: cut, whatever the others' lengths
+    units, tiles = len(lens) * kvh, kvh * sum(-(-n // 32) for n in lens)
+    parts = ca.attn_paged_plan(cache.kv, heads)[0]
+    assert parts > 0 and call.parts > 0 and max(lens) == cache.slots
+    assert [len(lens) > 64 and parts <= 2 * units, parts <= 2 * units and len(lens) <= 64, parts == 256 and tiles >= 16384,
+            parts == 256 and tiles >= 16384, parts > 256 and tiles >= 16384, 2 * units < parts <= 16 * units,
+            parts <= 2 * units and len(lens) > 256][case]
+    got, got_acc = call.run()
+    check(cache, q, heads, dim ** -0.5, got, out_f32, acc, got_acc)
+
+
 @pytest.mark.parametrize("size", [1e-33, 1e-25, 1e18, 1e35])
 @pytest.mark.parametrize("lens", [[80], [16384]])
 def test_values_of_any_size(lens, size):
