@@ -39,8 +39,9 @@
 // Rounding: scores and sums in f32.  p goes into the product as bf16 terms,
 // each the upper half of what the one before left over: three (all 24 bits) for
 // an f32 output, two (2^-16 relative) for a bf16 one; the further products hide
-// under the cache's stream.  A term that would be 0 behind another is 2^-30 of that
-// instead, so that an infinity in V gives infinity and not 0 * infinity.
+// under the cache's stream (1 to 3 % of a bf16 output's time).  A term that would be 0
+// behind another is 2^-30 p instead, so that an infinity in V gives infinity and not 0 *
+// infinity.
 //
 // The maximum is raised only where a score passes it by more than 8 in base 2,
 // for all lanes of a head at once: until then p stays below 2^8, which costs no
@@ -361,6 +362,9 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
     // p's bf16 terms
     constexpr int TERMS = F32 ? 3 : 2;
     bf16x8_t pt[TERMS];
+    float least[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) least[j] = p[j] * 0x1p-30f;
 #pragma unroll
     for (int y = 0; y < TERMS; ++y) {
       u32x4_t word;
@@ -370,8 +374,8 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
           const uint32_t b0 = __float_as_uint(p[2 * j]), b1 = __float_as_uint(p[2 * j + 1]);
           word[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
           const float hi0 = __uint_as_float(b0 & 0xFFFF0000u), hi1 = __uint_as_float(b1 & 0xFFFF0000u);
-          p[2 * j] = __builtin_fmaxf(p[2 * j] - hi0, hi0 * 0x1p-30f);
-          p[2 * j + 1] = __builtin_fmaxf(p[2 * j + 1] - hi1, hi1 * 0x1p-30f);
+          p[2 * j] = __builtin_fmaxf(p[2 * j] - hi0, least[2 * j]);
+          p[2 * j + 1] = __builtin_fmaxf(p[2 * j + 1] - hi1, least[2 * j + 1]);
         } else {
           word[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
         }

@@ -389,3 +389,22 @@ def test_values_of_any_size(lens, size):
     q = bf16(rng.standard_normal((1, 3, 64)))
     got, _ = Call(cache, q, 3, 0.125, True).run()
     check(cache, q, 3, 0.125, got, True)
+
+
+@pytest.mark.parametrize("out_f32", [True, False])
+@pytest.mark.parametrize("lens", [[80], [4096]])
+def test_infinite_values_of_little_weight(lens, out_f32):
+    """Slots of weight 2^-65, of whose bits nothing is left for a second term, with
+    infinite values: infinity, as in the formula, not the NaN of a term that is 0."""
+    say(f"attn_paged infinite value of little weight, {lens[0]} slots, f32 {out_f32}")
+    rng = np.random.default_rng(16)
+    cache = Cache(rng, lens, 1, 128, 16, lens[0] // 16)
+    q = np.zeros((1, 2, 128), np.float32)
+    q[..., 0] = 1
+    k = 0.5 * rng.standard_normal((1, lens[0], 128))
+    k[..., 0] = 0
+    k[:, [5, lens[0] - 2], 0] = -65
+    cache.put(cache.k, 0, np.arange(lens[0]), bf16(k))
+    cache.put(cache.v, 0, np.array([5, lens[0] - 2]), np.full((1, 2, 128), 0x7F80, np.uint16))
+    got, _ = Call(cache, bf16(q), 2, np.log(2.0), out_f32).run()  # scores in base 2 as they are
+    assert np.all(np.isposinf(got))
