@@ -83,7 +83,10 @@ int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPl
   // at one CU's 38 GB/s against a join and, the more units there are, their short
   // parts.  Units x slots of 128 (ragged from 256 on), a workgroup a unit / cut, us:
   // 16 x 384 6.7 / 8.0, x 512 7.9 / 8.0, x 2048 28.5 / 9.4; 64 x 512 10.1 / 9.0; 128 x
-  // 640 12.8 / 13.0; 256 x 1024 18.0 / 25.5, x 1536 25.9 / 32.9 (a unit for every CU);
+  // 640 12.8 / 13.0; 256 x 1024 18.0 / 25.5, x 1536 25.9 / 32.9 (a unit for every CU;
+  // the bound that this gives 129 to 256 units is too high for the fewer of them, and
+  // for few full rows among short ones: 136 units x 1952 32.7 / 28.1, of which one row's
+  // 8 are full and the others 64 slots 27.5 / 11.3; 192 35.1 / 36.3, 28.0 / 11.4);
   // 512 x 1024 32.6 / 37, x 1536 47.7 / 44.7, x 4096 119 / 89; 1024 x 2048 97 / 101, x
   // 4096 209 / 178; 2048 x 2048 191 / 214, x 4096 364 / 356.
   // Where a full table is that short, a workgroup per unit and no second kernel

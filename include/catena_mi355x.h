@@ -342,13 +342,15 @@ int catena_mi355x_attn_paged_plan(const catena_paged_kv_t *kv, uint32_t heads, i
  * [head_dim] f32 (out_f32 != 0) or bf16 RNE.  Query head h reads kv head
  * h / (heads / kv_heads); o = sum_j p_j v_j, p = softmax(scale * q . k_j) with
  * the exponential itself (not math.exp-approx), sums in f32 that finite values of
- * any size do not overflow.  A row of no slots gives 0, a row whose pages are all
- * unknown NaN.  What the cache holds past a
- * row's slots is never used.
+ * any size do not overflow (p to 24 bits for an f32 o, to 2^-16 for a bf16 one).
+ * A row of no slots gives 0, a row whose pages are all unknown NaN.  What the
+ * cache holds past a row's slots is never used.
  * acc_in / acc_out[rows][kv_heads][max_pages * page_size] f32 (both or
  * neither, may be the same): acc_out[j] = acc_in[j] + the sum of p_j over the
  * query heads of a kv head, for the slots in use; others are left as they are.
- * The result depends on the sizes and the inputs alone, bit by bit.
+ * The result depends on the sizes and the inputs alone, bit by bit; where the work
+ * is cut follows from the lengths of all rows, so a row's last bits may differ
+ * beside other rows.
  * workspace: 16-byte aligned, as many bytes as the plan says, used until the
  * call's work has run; calls that may overlap (two captured graphs) take one
  * each.  q and o 16-byte aligned.  Allocates nothing; may be captured. */
@@ -373,8 +375,8 @@ int catena_mi355x_attn_paged_bf16(const catena_paged_kv_t *kv, const uint16_t *q
  * one whose page does not exist writes q alone.  No two tokens of a call go to
  * the same slot of a page; rows may share pages, so that the tokens of prompts of
  * different lengths are rows of one token each, whose tables are their prompt's
- * (acc and slot_pos belong to a row: NULL there).  qkv, rope_tab and q 16-byte aligned.  No reference
- * counterpart. */
+ * (acc and slot_pos belong to a row: NULL there).  qkv, rope_tab and q 16-byte
+ * aligned.  No reference counterpart. */
 int catena_mi355x_rope_qkv_paged_bf16(const catena_paged_kv_t *kv, const float *qkv,
                                       const float *rope_tab, uint32_t table_positions,
                                       const uint32_t *lens, const uint32_t *seen, uint16_t *q,
