@@ -46,22 +46,6 @@ int paged_check(const catena_paged_kv_t* kv, bool pools, PagedKv* out) {
   return CATENA_OK;
 }
 
-// struct AttnPagedArgs of attn_paged.hip, field for field
-struct AttnPagedArgs {
-  PagedKv kv;
-  const uint16_t* q;
-  const uint32_t* lens;
-  void* o;
-  float* part_o;
-  float* part_ml;
-  float* whole_ml;
-  float* scores;
-  const float* acc_in;
-  float* acc_out;
-  uint32_t group, head_tiles, blocks, short_slots;
-  float scale_log2;
-};
-
 constexpr uint64_t kJoinBlocks = 2048;  // eight a CU; they take several rows each
 struct AttnPagedPlan {
   uint32_t group, head_tiles, blocks, short_slots, pieces;
@@ -133,37 +117,7 @@ int evict_plan(const PagedKv& kv, uint32_t budget, uint64_t* bytes) {
   return CATENA_OK;
 }
 
-// struct EvictArgs of kv_paged.hip, field for field
-struct EvictArgs {
-  PagedKv kv;
-  const uint32_t* lens;
-  const uint32_t* seen;
-  const float* acc_in;
-  const uint32_t* pos_in;
-  uint32_t* lens_out;
-  float* acc_out;
-  uint32_t* pos_out;
-  uint32_t* count;
-  uint32_t* holes;
-  uint32_t* sources;
-  uint32_t most, budget, recent, at_once;
-};
-
-// structs ReorderArgs and ReorderPools of kv_paged.hip, field for field
-struct ReorderArgs {
-  PagedKv kv;
-  const uint32_t* lens;
-  const uint32_t* parents;
-  const uint32_t* spare;
-  uint32_t* table_out;
-  uint32_t* lens_out;
-  uint32_t* spare_out;
-  uint32_t n_pools, tables;
-};
 constexpr uint32_t kReorderFew = 8, kReorderMost = 128;
-struct ReorderPools {
-  uint16_t* p[kReorderMost];
-};
 }  // namespace
 
 extern "C" {
@@ -344,7 +298,7 @@ int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t* kv, uint16_t*
   for (uint32_t first = 0; first == 0 || first < n_pools; first += kReorderMost) {
     ReorderArgs a{c, lens, parents, spare, table_out, lens_out, spare_out, std::min(n_pools - first, kReorderMost),
                   first == 0};
-    ReorderPools p;
+    ReorderPools<kReorderMost> p;
     const bool few = a.n_pools <= kReorderFew;
     for (uint32_t i = 0; i < (few ? kReorderFew : kReorderMost); ++i)
       p.p[i] = i < a.n_pools ? pools[first + i] : nullptr;

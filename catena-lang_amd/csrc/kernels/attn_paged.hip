@@ -87,23 +87,6 @@ CATENA_DEV float anchor(float m) { return m == kNegInf ? 0.0f : m; }
 // p's power of two in the products of a row of n > 0 slots: n of p < 2^8 stay below 1/2
 CATENA_DEV float ease_of(uint32_t n) { return __uint_as_float((uint32_t)(127 - 41 + __builtin_clz(n)) << 23); }
 
-struct AttnPagedArgs {
-  PagedKv kv;
-  const uint16_t* q;      // [rows][heads][D]
-  const uint32_t* lens;   // [rows]
-  void* o;                // [rows][heads][D]
-  float* part_o;          // [blocks][2][min(group, 16)][D]
-  float* part_ml;         // [blocks][2][min(group, 16)][2]: maximum (base 2), sum
-  float* whole_ml;        // [rows][heads][2]: of units that were not cut, with weights that the join adds
-  float* scores;          // [rows][heads][slots] base-2 scores, with weights only
-  const float* acc_in;    // [rows][kv_heads][slots]
-  float* acc_out;
-  uint32_t group, head_tiles;
-  uint32_t blocks;        // workgroups; 0: one a unit
-  uint32_t short_slots;   // whole units while no row is longer
-  float scale_log2;       // scale * log2(e)
-};
-
 // Four columns of o / l of a row of n slots, whose o is the eased sum; 0 where there are
 // none
 template <bool F32>

@@ -113,22 +113,6 @@ CATENA_DEV uint32_t block_prefix(uint32_t x, uint32_t* s_wave, uint32_t* total) 
   return before + in - x;
 }
 
-struct EvictArgs {
-  PagedKv kv;
-  const uint32_t* lens;
-  const uint32_t* seen;
-  const float* acc_in;
-  const uint32_t* pos_in;
-  uint32_t* lens_out;
-  float* acc_out;
-  uint32_t* pos_out;
-  uint32_t* count;    // [pairs]
-  uint32_t* holes;    // [pairs][most]
-  uint32_t* sources;  // [pairs][most]
-  uint32_t most, budget, recent;
-  uint32_t at_once;   // the choosing workgroup makes the moves itself
-};
-
 // Moves first, first + step, ... of a (row, kv head), four at a time: a row of K and
 // of V (16 bytes a lane), the slot's weight and position.  Sources lie from the
 // budget on and are never written, so the order does not matter.
@@ -441,20 +425,6 @@ extern "C" __global__ __launch_bounds__(256) void catena_kv_evict_move(EvictArgs
 // us, 5.5 TB/s; 4 rows 2.4 us.
 // grid = (rows, kv_heads, pools): one (row, head, pool)'s slots of the last page;
 // the workgroups of head 0 and pool 0 write the row's table.
-struct ReorderArgs {
-  PagedKv kv;
-  const uint32_t* lens;
-  const uint32_t* parents;
-  const uint32_t* spare;
-  uint32_t* table_out;
-  uint32_t* lens_out;
-  uint32_t* spare_out;
-  uint32_t n_pools, tables;
-};
-template <int MOST>
-struct ReorderPools {
-  uint16_t* p[MOST];
-};
 
 namespace {
 CATENA_DEV void kv_reorder(const ReorderArgs& a, uint16_t* const* pools) {

@@ -46,3 +46,55 @@ CATENA_HD bool paged_place(const PagedKv& kv, uint32_t row, uint32_t head, uint3
   *at = paged_offset(kv, page, head, slot & ((1u << kv.page_shift) - 1u));
   return true;
 }
+
+// The kernels' arguments, which the host fills.
+
+// attn_paged.hip
+struct AttnPagedArgs {
+  PagedKv kv;
+  const uint16_t* q;      // [rows][heads][D]
+  const uint32_t* lens;   // [rows]
+  void* o;                // [rows][heads][D]
+  float* part_o;          // [blocks][2][min(group, 16)][D]
+  float* part_ml;         // [blocks][2][min(group, 16)][2]: maximum (base 2), sum
+  float* whole_ml;        // [rows][heads][2]: of units that were not cut, with weights that the join adds
+  float* scores;          // [rows][heads][slots] base-2 scores, with weights only
+  const float* acc_in;    // [rows][kv_heads][slots]
+  float* acc_out;
+  uint32_t group, head_tiles;
+  uint32_t blocks;        // workgroups; 0: one a unit
+  uint32_t short_slots;   // whole units while no row is longer
+  float scale_log2;       // scale * log2(e)
+};
+
+// kv_paged.hip: eviction, reordering
+struct EvictArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* seen;
+  const float* acc_in;
+  const uint32_t* pos_in;
+  uint32_t* lens_out;
+  float* acc_out;
+  uint32_t* pos_out;
+  uint32_t* count;    // [pairs]
+  uint32_t* holes;    // [pairs][most]
+  uint32_t* sources;  // [pairs][most]
+  uint32_t most, budget, recent;
+  uint32_t at_once;   // the choosing workgroup makes the moves itself
+};
+
+struct ReorderArgs {
+  PagedKv kv;
+  const uint32_t* lens;
+  const uint32_t* parents;
+  const uint32_t* spare;
+  uint32_t* table_out;
+  uint32_t* lens_out;
+  uint32_t* spare_out;
+  uint32_t n_pools, tables;
+};
+template <int MOST>
+struct ReorderPools {
+  uint16_t* p[MOST];
+};
