@@ -50,8 +50,8 @@
 // Range: the sums of p v are divided by that of p at the end alone.  p enters the
 // products times a power of two below 2^-8 / n, so that no sum passes half the
 // largest |v| and any finite values give a finite mean; the division takes the
-// power back.  (What it costs lies at the other end: products below f32's smallest, of
-// values below some 2^-80.)
+// power back.  (It costs the other end: products of values below some 2^-80 are f32's
+// smallest numbers and lose their last bits.)
 #include "common.h"
 #include "paged.h"
 
