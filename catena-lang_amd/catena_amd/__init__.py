@@ -11,6 +11,8 @@ Layout mirrors the C header:
                    and the decoder-block pieces (rmsnorm, rope, silu_mul, argmax, ...)
   * paged cache:   PagedKV, attn_paged_bf16, rope_qkv_paged_bf16, kv_evict_paged_bf16,
                    beam_select_f32, beam_reorder_paged_bf16 and their plans
+  * requests:      kv_admit_paged, kv_release_paged, rope_packed_bf16, attn_prompt_bf16,
+                   attn_packed_bf16; in 4 bits PagedKV4, rope_packed_q4, attn_paged_q4
   * decoder:       Decoder (catena_mi355x_decoder_*)
   * program ABI:   program_* functions (fail-stop: they trap on bad input)
   * runtime:       Runtime (catena_runtime_*), mirrors Runtime::from_sources /
@@ -115,6 +117,19 @@ class PagedKV(ctypes.Structure):
         return self.max_pages * self.page_size
 
 
+class PagedKV4(ctypes.Structure):
+    """catena_paged_kv4_t: a cache in pages held in 4 bits."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("num_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("rows", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
+
+    @property
+    def slots(self) -> int:
+        return self.max_pages * self.page_size
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
@@ -171,6 +186,22 @@ SIGNATURES = {
     "catena_mi355x_kv_evict_paged_bf16": (_int, [ctypes.POINTER(PagedKV)] + [_vp] * 7 + [_u32, _u32, _vp, _u64]),
     "catena_mi355x_beam_reorder_paged_bf16": (_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(_vp), _u32]
                                               + [_vp] * 6),
+    "catena_mi355x_kv_admit_paged": (_int, [ctypes.POINTER(PagedKV)] + [_vp] * 12 + [_u32, _vp, _vp]),
+    "catena_mi355x_kv_release_paged": (_int, [ctypes.POINTER(PagedKV)] + [_vp] * 9),
+    "catena_mi355x_rope_inv_freq_scaled": (_int, [ctypes.POINTER(ctypes.c_double), _u32, ctypes.c_double, _u32]
+                                           + [ctypes.c_double] * 4),
+    "catena_mi355x_rope_table_scaled_f32": (_int, [_vp, _vp, _u32, _u32, _u32, ctypes.c_double]),
+    "catena_mi355x_rope_packed_bf16": (_int, [ctypes.POINTER(PagedKV), _vp, _int, _vp, _u32, _u32, _int, _vp,
+                                              _vp, _vp, _u64, _u32, _vp, _vp]),
+    "catena_mi355x_rope_packed_q4": (_int, [ctypes.POINTER(PagedKV4), _vp, _int, _vp, _u32, _u32, _int, _vp,
+                                            _vp, _vp, _u64, _u32, _vp, _vp]),
+    "catena_mi355x_attn_prompt_plan": (_int, [ctypes.POINTER(PagedKV), _u64, _u32, ctypes.POINTER(_u64)]),
+    "catena_mi355x_attn_prompt_bf16": (_int, [ctypes.POINTER(PagedKV)] + [_vp] * 4 + [_u64, _u32, _f32, _vp, _u64]),
+    "catena_mi355x_attn_packed_plan": (_int, [_u32, _u64, _u32, _u32, _u32, ctypes.POINTER(_u64)]),
+    "catena_mi355x_attn_packed_bf16": (_int, [_vp] * 5 + [_u32, _u64, _u32, _u32, _u32, _u64, _f32, _vp, _u64]),
+    "catena_mi355x_attn_paged_q4_plan": (_int, [ctypes.POINTER(PagedKV4), _u32, ctypes.POINTER(_u32),
+                                                ctypes.POINTER(_u64)]),
+    "catena_mi355x_attn_paged_q4": (_int, [ctypes.POINTER(PagedKV4), _vp, _vp, _vp, _u32, _f32, _vp, _u64]),
     "catena_mi355x_beam_select_plan": (_int, [_u32, _u32, _u32, ctypes.POINTER(_u64)]),
     "catena_mi355x_beam_select_f32": (_int, [_vp] * 7 + [_u32] * 4 + [_vp, _u64]),
     "catena_mi355x_argmax_f32": (_int, [_vp, _vp, _u64, _u64]),
@@ -544,6 +575,97 @@ def beam_reorder_paged_bf16(kv: PagedKV, pools, lens, parents, spare, table_out,
     check(lib().catena_mi355x_beam_reorder_paged_bf16(kv, arr, len(pools), lens, parents,
                                                       spare, table_out, lens_out,
                                                       spare_out))
+
+
+def kv_admit_paged(kv: PagedKV, table, lens, held, want, free_pages, free_count, lens_out, held_out, starts,
+                   free_count_out, token_pos, slot_map, max_tokens: int, seen=None, seen_out=None) -> None:
+    """Pages from the stack free_pages[0 .. free_count) for the want[r] tokens that every
+    row asks for: table, lengths, starts[rows + 1], and every token's position and slot."""
+    check(lib().catena_mi355x_kv_admit_paged(kv, table, lens, held, want, free_pages, free_count, lens_out,
+                                             held_out, starts, free_count_out, token_pos, slot_map,
+                                             max_tokens, seen, seen_out))
+
+
+def kv_release_paged(kv: PagedKV, table, lens, held, finished, free_pages, free_count, lens_out, held_out,
+                     free_count_out) -> None:
+    """The pages of rows that have ended, back onto the stack."""
+    check(lib().catena_mi355x_kv_release_paged(kv, table, lens, held, finished, free_pages, free_count,
+                                               lens_out, held_out, free_count_out))
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)  # catena_rope_scaling_t
+
+
+def rope_inv_freq_scaled(rotary_dim: int, base: float, kind: int = ROPE_PLAIN, factor: float = 1.0,
+                         trained: float = 0.0, low: float = 0.0, high: float = 0.0) -> np.ndarray:
+    """Frequencies of rotary positions in double, on the host."""
+    out = (ctypes.c_double * max(rotary_dim // 2, 1))()
+    check(lib().catena_mi355x_rope_inv_freq_scaled(out, rotary_dim, base, kind, factor, trained, low, high))
+    return np.array(out[:rotary_dim // 2], np.float64)
+
+
+def rope_table_scaled_f32(inv_freq, tab, first: int, positions: int, rotary_dim: int, mscale: float = 1.0) -> None:
+    """(cos, sin) of positions first .. first + positions - 1, angles in double."""
+    check(lib().catena_mi355x_rope_table_scaled_f32(inv_freq, tab, first, positions, rotary_dim, mscale))
+
+
+def rope_packed_bf16(kv: PagedKV, qkv, qkv_f32: bool, rope_tab, table_positions: int, rotary_dim: int,
+                     interleaved: bool, token_pos, slot_map, q, tokens: int, heads: int, k_out=None,
+                     v_out=None) -> None:
+    """Rotation of a list of tokens, and their keys and values into the slots of slot_map."""
+    check(lib().catena_mi355x_rope_packed_bf16(kv, qkv, 1 if qkv_f32 else 0, rope_tab, table_positions,
+                                               rotary_dim, 1 if interleaved else 0, token_pos, slot_map, q,
+                                               tokens, heads, k_out, v_out))
+
+
+def rope_packed_q4(kv: PagedKV4, qkv, qkv_f32: bool, rope_tab, table_positions: int, rotary_dim: int,
+                   interleaved: bool, token_pos, slot_map, q, tokens: int, heads: int, k_out=None,
+                   v_out=None) -> None:
+    """rope_packed_bf16 into a cache in 4 bits; k_out / v_out: the values that it then holds."""
+    check(lib().catena_mi355x_rope_packed_q4(kv, qkv, 1 if qkv_f32 else 0, rope_tab, table_positions,
+                                             rotary_dim, 1 if interleaved else 0, token_pos, slot_map, q,
+                                             tokens, heads, k_out, v_out))
+
+
+def attn_prompt_plan(kv: PagedKV, tokens: int, heads: int) -> int:
+    """Workspace bytes of attn_prompt_bf16; needs no device."""
+    nbytes = _u64()
+    check(lib().catena_mi355x_attn_prompt_plan(kv, tokens, heads, nbytes))
+    return nbytes.value
+
+
+def attn_prompt_bf16(kv: PagedKV, q, starts, lens, o, tokens: int, heads: int, scale: float,
+                     workspace=None) -> None:
+    """Causal attention of packed sequences over a cache in pages."""
+    check(lib().catena_mi355x_attn_prompt_bf16(kv, q, starts, lens, o, tokens, heads, scale,
+                                               *_workspace(workspace)))
+
+
+def attn_packed_plan(rows: int, tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace bytes of attn_packed_bf16; needs no device."""
+    nbytes = _u64()
+    check(lib().catena_mi355x_attn_packed_plan(rows, tokens, heads, kv_heads, head_dim, nbytes))
+    return nbytes.value
+
+
+def attn_packed_bf16(q, k, v, starts, o, rows: int, tokens: int, heads: int, kv_heads: int, head_dim: int,
+                     scale: float, workspace=None, kv_stride: int = 0) -> None:
+    """Causal attention of packed prompts over their own keys and values."""
+    check(lib().catena_mi355x_attn_packed_bf16(q, k, v, starts, o, rows, tokens, heads, kv_heads, head_dim,
+                                               kv_stride, scale, *_workspace(workspace)))
+
+
+def attn_paged_q4_plan(kv: PagedKV4, heads: int):
+    """(parts that all rows' slots are cut into or 0, workspace bytes) of
+    attn_paged_q4; needs no device."""
+    parts, nbytes = _u32(), _u64()
+    check(lib().catena_mi355x_attn_paged_q4_plan(kv, heads, parts, nbytes))
+    return parts.value, nbytes.value
+
+
+def attn_paged_q4(kv: PagedKV4, q, lens, o, heads: int, scale: float, workspace=None) -> None:
+    """One new token per row over a cache in 4 bits; o in bf16."""
+    check(lib().catena_mi355x_attn_paged_q4(kv, q, lens, o, heads, scale, *_workspace(workspace)))
 
 
 BEAM_NO_EOS = 0xFFFFFFFF  # no token ends a beam

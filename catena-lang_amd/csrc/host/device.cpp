@@ -132,6 +132,19 @@ const KernelSpec kKernels[] = {
     {KernelId::KvEvictMove, "kv_paged", "catena_kv_evict_move"},
     {KernelId::KvReorder8, "kv_paged", "catena_kv_reorder_8"},
     {KernelId::KvReorder128, "kv_paged", "catena_kv_reorder_128"},
+    {KernelId::KvAdmit, "kv_admit", "catena_kv_admit"},
+    {KernelId::KvRelease, "kv_admit", "catena_kv_release"},
+    {KernelId::RopeTableF64, "rope_packed", "catena_rope_table_f64"},
+    {KernelId::RopePackedF32, "rope_packed", "catena_rope_packed_f32in"},
+    {KernelId::RopePackedBf16, "rope_packed", "catena_rope_packed_bf16in"},
+    {KernelId::RopePackedQ4F32, "rope_packed", "catena_rope_packed_q4_f32in"},
+    {KernelId::RopePackedQ4Bf16, "rope_packed", "catena_rope_packed_q4_bf16in"},
+    {KernelId::AttnPromptD128, "attn_prompt", "catena_attn_prompt_d128"},
+    {KernelId::AttnPromptD64, "attn_prompt", "catena_attn_prompt_d64"},
+    {KernelId::AttnPackedD128, "attn_prompt", "catena_attn_packed_d128"},
+    {KernelId::AttnPackedD64, "attn_prompt", "catena_attn_packed_d64"},
+    {KernelId::AttnPagedQ4D128, "attn_paged_q4", "catena_attn_paged_q4_d128"},
+    {KernelId::AttnPagedQ4D64, "attn_paged_q4", "catena_attn_paged_q4_d64"},
     {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},
     {KernelId::BeamRuns16, "beam", "catena_beam_runs_16"},
     {KernelId::BeamJoin, "beam", "catena_beam_join"},

@@ -95,6 +95,19 @@ enum class KernelId : int {
   KvEvictMove,
   KvReorder8,
   KvReorder128,
+  KvAdmit,  // a step over requests of different lengths (kv_admit.hip)
+  KvRelease,
+  RopeTableF64,  // packed rotation (rope_packed.hip)
+  RopePackedF32,
+  RopePackedBf16,
+  RopePackedQ4F32,
+  RopePackedQ4Bf16,
+  AttnPromptD128,  // packed sequences (attn_prompt.hip)
+  AttnPromptD64,
+  AttnPackedD128,
+  AttnPackedD64,
+  AttnPagedQ4D128,  // a cache in 4 bits (attn_paged_q4.hip)
+  AttnPagedQ4D64,
   BeamRuns8,  // beam search's selection (beam.hip)
   BeamRuns16,
   BeamJoin,

@@ -1,0 +1,318 @@
+// Attention of one new token per row over a key-value cache held in 4 bits.
+//
+//   k_j = 2^(e - 127) c (a power of two for 32 values), v_j = s_j c (one scale a
+//   slot and head), c in e2m1; s_j = scale * q . k_j, o = softmax(s) . v
+//
+// as attn_paged.hip has it for bf16: the same line of tiles, parts and join.
+//
+// Bound: the cache is read once, D + D / 32 + 2 bytes per (slot, kv head), so HBM,
+// if the codes cost no more than about ten instructions of a wave for 256 of them.
+//
+// A wave takes 128 slots at a time, its lane group g (lanes 16 g ..) slots 32 g ..
+// 32 g + 31 of them.
+//   S^T = K Q^T (16 x 16 x 32 products): instruction set u of eight takes slots 32 (c
+//     / 4) + 8 (c % 4) + u as its 16 rows, so that the results leave lane (c, g) with
+//     head c's scores of its own group's slots 32 g + 8 j + u (j: the register).  The
+//     order of d in the sum is free: the lane loads a quarter of a slot's codes, D / 8
+//     bytes, which lie in one block of 32, and converts them with that block's scale
+//     (two values an instruction).
+//   O^T = V^T P^T: v lies by pairs of columns, so a lane's 32 slots of one pair are 32
+//     bytes in two runs of 16.  Halves of two dwords mixed give eight codes of one
+//     column, slots (0, 4, 1, 5, 2, 6, 3, 7), and P's terms are packed in that order.
+//     The slots' scales go into P.
+//
+// Codes are finite whatever their bits, so what lies behind a row's end is masked in
+// the scores and the scales alone.
+#include "attn_line.h"
+
+struct AttnQ4Pools {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* k_scale;
+  const uint16_t* v_scale;
+};
+
+namespace {
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+
+template <int D>
+struct Shared {
+  float m[kWaves][16], l[kWaves][16];
+  __attribute__((aligned(16))) float o[kWaves][16][D + 4];
+};
+
+// Eight codes times a power of two, in bf16 (exact)
+CATENA_DEV bf16x8_t widen8(uint32_t codes, float unit) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, 0);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, 1);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, 2);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, 3);
+  return __builtin_bit_cast(bf16x8_t, u32x4_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                              __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)});
+}
+
+template <int D>
+struct Tile {
+  u32x4_t k[8];         // D = 64: the first two dwords
+  u32x2_t ks;           // block scales of slots 8 (c % 4) .. + 7 of group c / 4
+  u32x4_t v[D / 32][2];  // pair of columns 16 i + c, slots 16 h .. + 15 of the lane's group
+  u32x4_t vs[2][2];     // their scales
+};
+
+template <int D>
+CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& pools) {
+  constexpr int KC = D / 32;  // products of S
+  constexpr int VG = D / 32;  // groups of 16 column pairs
+  __shared__ Shared<D> sh;
+  const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t heads = a.group * a.kv.kv_heads;
+  const uint32_t part_heads = a.group < 16 ? a.group : 16;
+  const uint32_t page_size = 1u << a.kv.page_shift, mask = page_size - 1u;
+  const uint32_t k_slot = 32 * (c >> 2) + 8 * (c & 3);  // the lane's slots of K, from the tile's first
+
+  // Pages of the runs of slots that a lane reads (its slots of K; two runs of V)
+  struct Pages {
+    uint32_t k, v[2];
+  };
+  auto look_up = [&](const Part& p, uint32_t t) {
+    Pages x{0xFFFFFFFFu, {0xFFFFFFFFu, 0xFFFFFFFFu}};
+    if (t >= p.end) return x;
+    const uint32_t end = 32 * p.end < p.len ? 32 * p.end : p.len;
+    const uint32_t* row = a.kv.table + (uint64_t)p.row * a.kv.max_pages;
+    const uint32_t s = 32 * t + k_slot, s0 = 32 * t + 32 * g;
+    if (s < end) x.k = row[s >> a.kv.page_shift];
+    if (s0 < end) x.v[0] = row[s0 >> a.kv.page_shift];
+    if (s0 + 16 < end) x.v[1] = row[(s0 + 16) >> a.kv.page_shift];
+    return x;
+  };
+  // (what is not there is read from the pool's first page and masked)
+  auto request = [&](Tile<D>& x, const Part& p, uint32_t t, const Pages& at) {
+    const uint32_t s = (32 * t + k_slot) & mask, s0 = (32 * t + 32 * g) & mask, s1 = (32 * t + 32 * g + 16) & mask;
+    const uint64_t kc = paged_cells(a.kv.kv_heads, a.kv.page_shift, at.k < a.kv.num_pages ? at.k : 0u, p.kvh);
+    const uint8_t* k = pools.k + (kc + s) * (D / 2) + g * (D / 8);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if constexpr (D == 128) {
+        x.k[u] = *reinterpret_cast<const u32x4_t*>(k + u * (D / 2));
+      } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(k + u * (D / 2));
+        x.k[u][0] = w[0];
+        x.k[u][1] = w[1];
+      }
+    }
+    x.ks = *reinterpret_cast<const u32x2_t*>(pools.k_scale + kc * (D / 32) + (uint64_t)(g * (D / 32) / 4) * page_size + s);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint64_t vc = paged_cells(a.kv.kv_heads, a.kv.page_shift, at.v[h] < a.kv.num_pages ? at.v[h] : 0u, p.kvh);
+      const uint32_t sh0 = h ? s1 : s0;
+#pragma unroll
+      for (int i = 0; i < VG; ++i)
+        x.v[i][h] = *reinterpret_cast<const u32x4_t*>(pools.v + vc * (D / 2) + (uint64_t)(16 * i + c) * page_size + sh0);
+      const u32x4_t* vs = reinterpret_cast<const u32x4_t*>(pools.v_scale + vc + sh0);
+      x.vs[h][0] = vs[0];
+      x.vs[h][1] = vs[1];
+    }
+  };
+
+  bf16x8_t qf[KC];
+  float m, l, ease;
+  f32x4_t acc[VG][2];
+  auto begin = [&](const Part& p) {
+    const uint16_t* q = a.q + ((uint64_t)p.row * heads + p.kvh * a.group + 16 * p.ht + (c < p.gn ? c : 0)) * D;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + (D / 4) * g + 8 * i);
+      if (c >= p.gn) w = u32x4_t{0, 0, 0, 0};
+      qf[i] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    m = kNegInf;
+    l = 0.0f;
+    ease = ease_of(p.len | 1u);
+#pragma unroll
+    for (int i = 0; i < VG; ++i) acc[i][0] = acc[i][1] = f32x4_t{0, 0, 0, 0};
+  };
+
+  auto take = [&](const Tile<D>& x, const Part& p, uint32_t t, const Pages& at) {
+    // scores in base 2: s[8 j + u] is slot 32 g + 8 j + u of head c
+    float s[32];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t byte = (x.ks[u / 4] >> (8 * (u % 4))) & 255u;
+      const float unit = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+      f32x4_t y = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(x.k[u][i], unit), qf[i], y, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[8 * j + u] = y[j] * a.scale_log2;
+    }
+    const uint32_t end = 32 * p.end < p.len ? 32 * p.end : p.len;
+    const bool here0 = at.v[0] < a.kv.num_pages, here1 = at.v[1] < a.kv.num_pages;
+    const bool full = __all(here0 && here1) && 32 * t + 128 <= end;
+    const uint32_t first = 32 * t + 32 * g;
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i] = first + i < end && (i < 16 ? here0 : here1) ? s[i] : kNegInf;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, s[i]);
+    if (__any(top > m + 8.0f)) {
+      top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float m2 = __builtin_fmaxf(m, top);
+      const float f = exp2_fast(m - anchor(m2));
+      m = m2;
+      l = l * f;
+#pragma unroll
+      for (int i = 0; i < VG; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i][0][j] = acc[i][0][j] * f;
+          acc[i][1][j] = acc[i][1][j] * f;
+        }
+    }
+    const float base = anchor(m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // eight slots: p to l, times ease and the slots' scales to two bf16 terms
+      float p8[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float e = exp2_fast(s[8 * j + u] - base);
+        l = l + e;
+        const uint32_t w = x.vs[j / 2][j % 2][u / 2];
+        const float sv = u % 2 ? bf16hi(w) : bf16lo(w);
+        p8[u] = e * ease * sv;
+        if (!full) p8[u] = s[8 * j + u] == kNegInf ? 0.0f : p8[u];  // a scale that is not the row's may be anything
+      }
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        hi[b] = pack_bf16x2(p8[b], p8[b + 4]);
+        lo[b] = pack_bf16x2(p8[b] - bf16lo(hi[b]), p8[b + 4] - bf16hi(hi[b]));
+      }
+      const bf16x8_t p0 = __builtin_bit_cast(bf16x8_t, hi), p1 = __builtin_bit_cast(bf16x8_t, lo);
+#pragma unroll
+      for (int i = 0; i < VG; ++i) {
+        const uint32_t w0 = x.v[i][j / 2][2 * (j % 2)], w1 = x.v[i][j / 2][2 * (j % 2) + 1];
+        const uint32_t even = (w0 & 0x0F0F0F0Fu) | (w1 << 4 & 0xF0F0F0F0u);
+        const uint32_t odd = (w0 >> 4 & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u);
+        const bf16x8_t v0 = widen8(even, 1.0f), v1 = widen8(odd, 1.0f);
+        acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p0, acc[i][0], 0, 0, 0);
+        acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p0, acc[i][1], 0, 0, 0);
+        acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p1, acc[i][0], 0, 0, 0);
+        acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p1, acc[i][1], 0, 0, 0);
+      }
+    }
+  };
+
+  bool whole = a.blocks == 0;  // units are not cut
+  auto finish = [&](const Part& p) {
+    l = l + __shfl_xor(l, 16);
+    l = l + __shfl_xor(l, 32);
+    __syncthreads();  // the last unit's values have been read
+    if (g == 0) {
+      sh.m[wave][c] = m;
+      sh.l[wave][c] = l;
+    }
+    if (c < p.gn) {
+      // lane (c, g), register j of acc[i][e]: column 2 (16 i + 4 g + j) + e of head c
+#pragma unroll
+      for (int i = 0; i < VG; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          *reinterpret_cast<f32x4_t*>(&sh.o[wave][c][2 * (16 * i + 4 * g + j)]) =
+              f32x4_t{acc[i][0][j], acc[i][1][j], acc[i][0][j + 1], acc[i][1][j + 1]};
+    }
+    __syncthreads();
+    for (uint32_t id = threadIdx.x; id < p.gn * (D / 4); id += 64 * kWaves) {
+      const uint32_t h = id / (D / 4), d = id % (D / 4) * 4;
+      float mm = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh.m[w][h]);
+      float ll = 0.0f;
+      f32x4_t o = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = exp2_fast(sh.m[w][h] - anchor(mm));
+        ll = ll + sh.l[w][h] * f;
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&sh.o[w][h][d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = o[i] + y[i] * f;
+      }
+      if (p.beg != 0 || p.end != p.tiles) {
+        // the first part of a unit in the workgroup's second place, else the first
+        const uint64_t at = ((uint64_t)blockIdx.x * 2 + (p.beg == 0)) * part_heads + h;
+        if (d == 0) {
+          a.part_ml[2 * at] = mm;
+          a.part_ml[2 * at + 1] = ll;
+        }
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = o;
+        continue;
+      }
+      store_o<false>(a, ((uint64_t)p.row * heads + p.kvh * a.group + 16 * p.ht + h) * D + d, o, ll, p.len);
+    }
+  };
+
+  // what is left behind `now`: places of the line, or whole units
+  const uint32_t units = a.kv.kv_heads * a.head_tiles;
+  uint32_t at, last;
+  Part now;
+  auto unit_from = [&](uint32_t u) {
+    const uint32_t row = u / units;
+    return part_from(a, row, paged_len(a.kv, scalar_word(a.lens, row)), u % units, 0, 0xFFFFFFFFu);
+  };
+  if (!whole) {
+    const FirstRows rows = first_rows(a);
+    const Line line = line_of(a, rows);
+    whole = line.whole;
+    if (!whole) {
+      at = blockIdx.x * line.per;
+      if (at >= line.tiles) return;
+      last = line.tiles - at < line.per ? line.tiles : at + line.per;
+      const RowOnLine r = row_at_place(a, rows, at);
+      now = part_from(a, r.row, r.len, (at - r.first) / r.tiles, (at - r.first) % r.tiles, last - at);
+      at += now.end - now.beg;
+    }
+  }
+  if (whole) {
+    at = blockIdx.x;
+    last = a.kv.rows * units;
+    if (at >= last) return;
+    now = unit_from(at);
+    at += gridDim.x;
+  }
+  for (;;) {
+    begin(now);
+    Tile<D> x;
+    for (uint32_t t = now.beg + 4 * wave; t < now.end; t += 4 * kWaves) {
+      const Pages pages = look_up(now, t);
+      request(x, now, t, pages);
+      take(x, now, t, pages);
+    }
+    finish(now);
+    if (at >= last) return;
+    if (whole) {
+      now = unit_from(at);
+      at += gridDim.x;
+    } else {
+      now = part_behind(a, now, last - at);
+      at += now.end - now.beg;
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_q4_d128(AttnPagedArgs a, AttnQ4Pools pools) {
+  attn_paged_q4_run<128>(a, pools);
+}
+extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_q4_d64(AttnPagedArgs a, AttnQ4Pools pools) {
+  attn_paged_q4_run<64>(a, pools);
+}

@@ -47,6 +47,25 @@ CATENA_HD bool paged_place(const PagedKv& kv, uint32_t row, uint32_t head, uint3
   return true;
 }
 
+// The same cache in 4 bits (e2m1, two values a byte, the first in the lower half):
+//   k [num_pages][kv_heads][page][head_dim / 2], k_scale [..][head_dim / 32][page]:
+//     32 values of a slot share the power of two 2^(byte - 127)
+//   v [num_pages][kv_heads][head_dim / 2][page], v_scale [..][page]: one bf16 scale
+//     a (slot, head)
+struct PagedKv4 {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint16_t* v_scale;
+  const uint32_t* table;
+  uint32_t num_pages, page_shift, rows, max_pages, kv_heads, head_dim;
+};
+
+// Slots in front of (page, head) in a pool, in 64 bits
+CATENA_HD uint64_t paged_cells(uint32_t kv_heads, uint32_t page_shift, uint32_t page, uint32_t head) {
+  return ((uint64_t)page * kv_heads + head) << page_shift;
+}
+
 // The kernels' arguments, which the host fills.
 
 // attn_paged.hip
@@ -97,4 +116,62 @@ struct ReorderArgs {
 template <int MOST>
 struct ReorderPools {
   uint16_t* p[MOST];
+};
+
+// kv_admit.hip
+struct AdmitArgs {
+  uint32_t rows, max_pages, page_shift, num_pages;
+  uint32_t* table;
+  const uint32_t* lens;
+  const uint32_t* held;
+  const uint32_t* want;
+  const uint32_t* seen;  // may be null, then seen_out is
+  const uint32_t* free_pages;
+  const uint32_t* free_count;
+  uint32_t* lens_out;
+  uint32_t* held_out;
+  uint32_t* seen_out;
+  uint32_t* starts;
+  uint32_t* free_count_out;
+  uint32_t* token_pos;
+  uint64_t* slot_map;
+  uint32_t max_tokens;
+};
+
+struct ReleaseArgs {
+  uint32_t rows, max_pages, num_pages;
+  uint32_t* table;
+  const uint32_t* lens;
+  const uint32_t* held;
+  const uint32_t* finished;
+  uint32_t* free_pages;
+  const uint32_t* free_count;
+  uint32_t* lens_out;
+  uint32_t* held_out;
+  uint32_t* free_count_out;
+};
+
+// rope_packed.hip
+struct RopePackedArgs {
+  const void* qkv;
+  const float* tab;         // [positions][rot / 2] (cos, sin)
+  const uint32_t* pos;      // [tokens]
+  const uint64_t* slots;    // [tokens] page * page_size + place; may be null
+  uint16_t* q;
+  uint16_t* k_out;          // [tokens][kv_heads][head_dim], may be null
+  uint16_t* v_out;
+  uint32_t positions, rot, interleaved, heads;
+};
+
+// attn_prompt.hip
+struct AttnPromptArgs {
+  PagedKv kv;               // table null: k, v [tokens][kv_heads][head_dim], stride apart
+  const uint16_t* q;        // [tokens][heads][D]
+  const uint32_t* starts;   // [rows + 1]
+  const uint32_t* lens;     // [rows]; null: as many as new tokens
+  uint16_t* o;              // [tokens][heads][D]
+  uint64_t stride;          // elements from a token's k to the next one's, without a table
+  uint32_t tokens, group;
+  float scale_log2;         // |scale| log2(e)
+  uint32_t flip;            // 0x80008000 where the scale is negative: q's signs
 };

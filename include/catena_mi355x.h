@@ -433,6 +433,184 @@ int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t *kv, uint16_t 
                                           uint32_t *table_out, uint32_t *lens_out,
                                           uint32_t *spare_out);
 
+/* -- a step over requests of different lengths -- */
+
+/* The step's tokens form one list, row after row (a row: a request's place in the
+ * table); row r's new ones are starts[r] .. starts[r + 1] - 1.  In order:
+ * catena_mi355x_kv_admit_paged finds their places, catena_mi355x_rope_packed_bf16
+ * (or _q4) writes them, catena_mi355x_attn_prompt_bf16 lets them attend; rows of
+ * one token each also catena_mi355x_attn_paged_bf16 or catena_mi355x_attn_paged_q4.
+ * All of it may be captured: lists have a length that the call names, and what lies
+ * behind the last token is marked as no token. */
+
+/* Pages for a step.  kv gives the sizes (k, v and table are not used); table[rows]
+ * [max_pages] is written in place: row r has lens[r] slots in the pages table[r]
+ * [0 .. held[r] - 1] and asks for want[r] more slots.  free_pages[0 .. *free_count - 1]
+ * (of num_pages entries at most) is a stack of free pages, its top the last one.
+ * A row asks for its tokens if lens[r] + want[r] slots fit the table (else for none),
+ * and for the pages that they need and it does not hold.  It is admitted where the
+ * tokens asked for by the rows up to it are at most max_tokens, and it needs no page
+ * or the pages asked for by the rows up to it are at most *free_count.  So the rows
+ * that are refused are behind the admitted ones (but for rows that ask for no page, or
+ * do not fit the table), and take nothing.  Admitted rows enter their pages into the table behind those that
+ * they hold, the lowest row from the top of the stack.
+ * Writes lens_out, held_out (both [rows]), starts[rows + 1], *free_count_out, and for
+ * each of the max_tokens places of the list its position token_pos and its slot
+ * slot_map = page * page_size + place in the page: token t of row r has position
+ * lens[r] + t (seen[r] + t where seen is given, which counts given-up positions too,
+ * as in catena_mi355x_rope_qkv_paged_bf16; seen_out[r] then counts the new ones) and
+ * goes to slot lens[r] + t.  Places behind the last token have position 0 and slot
+ * 0xFFFFFFFFFFFFFFFF, which names no place; so has a token whose page does not exist.
+ * The free pages themselves stay as they are.  No output is an input; table entries
+ * that are handed out are the only ones written.  No reference counterpart. */
+int catena_mi355x_kv_admit_paged(const catena_paged_kv_t *kv, uint32_t *table, const uint32_t *lens,
+                                 const uint32_t *held, const uint32_t *want,
+                                 const uint32_t *free_pages, const uint32_t *free_count,
+                                 uint32_t *lens_out, uint32_t *held_out, uint32_t *starts,
+                                 uint32_t *free_count_out, uint32_t *token_pos, uint64_t *slot_map,
+                                 uint32_t max_tokens, const uint32_t *seen, uint32_t *seen_out);
+
+/* Rows with finished[r] != 0 have ended: their pages table[r][0 .. held[r] - 1] go
+ * onto the stack, in the order of rows and entries, those entries become 0xFFFFFFFF,
+ * lens_out[r] and held_out[r] 0; other rows keep theirs.  free_pages is written in
+ * place behind *free_count (it has num_pages entries; what would not fit is dropped).
+ * The pages must be the row's own.  No output but free_pages and table is an input.
+ * No reference counterpart. */
+int catena_mi355x_kv_release_paged(const catena_paged_kv_t *kv, uint32_t *table,
+                                   const uint32_t *lens, const uint32_t *held,
+                                   const uint32_t *finished, uint32_t *free_pages,
+                                   const uint32_t *free_count, uint32_t *lens_out,
+                                   uint32_t *held_out, uint32_t *free_count_out);
+
+/* Frequencies of rotary positions on the host, in double: out_host[i], i <
+ * rotary_dim / 2, from f_i = base^(-2 i / rotary_dim):
+ *   PLAIN   f_i
+ *   LINEAR  f_i / factor (positions stretched)
+ *   BASE    f_i with base * factor^(rotary_dim / (rotary_dim - 2)): the lowest
+ *           frequency is divided by factor, the highest kept
+ *   PARTS   by the turns f_i makes in the trained length, trained * f_i / (2 pi):
+ *           kept from `high` turns on, divided by factor up to `low` turns, a linear
+ *           mix of both between
+ * No reference counterpart. */
+typedef enum catena_rope_scaling {
+  CATENA_ROPE_PLAIN = 0,
+  CATENA_ROPE_LINEAR = 1,
+  CATENA_ROPE_BASE = 2,
+  CATENA_ROPE_PARTS = 3
+} catena_rope_scaling_t;
+int catena_mi355x_rope_inv_freq_scaled(double *out_host, uint32_t rotary_dim, double base,
+                                       uint32_t kind, double factor, double trained, double low,
+                                       double high);
+
+/* tab[i][j] = mscale * (cos, sin) of (first + i) * inv_freq[j], i < positions, j <
+ * rotary_dim / 2, f32: angles, sines and the product in double (inv_freq too, on the
+ * device), so that far positions are as good as near ones.  (mscale: the factor that
+ * some scalings put on q and k.)  No reference counterpart;
+ * catena_mi355x_rope_table_f32 has the reference's sine. */
+int catena_mi355x_rope_table_scaled_f32(const double *inv_freq, float *tab, uint32_t first,
+                                        uint32_t positions, uint32_t rotary_dim, double mscale);
+
+/* Rotation of a list of tokens and their append: qkv[tokens][(heads + 2 kv_heads) *
+ * head_dim] (columns: q heads | k heads | v heads; f32 where qkv_f32 != 0, else bf16).
+ * Of each q and k head the first rotary_dim values (a multiple of 16) turn by
+ * rope_tab[token_pos][rotary_dim / 2] (cos, sin), in pairs (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) where interleaved != 0, each operation rounded to f32 and the results to
+ * bf16; the others are rounded alone.  Writes q[tokens][heads][head_dim], k and v into
+ * slot slot_map[token] of kv's pools (page * page_size + place; the table is not used),
+ * and k_out / v_out[tokens][kv_heads][head_dim] (both or neither).  slot_map may be NULL:
+ * no token has a slot.  A token whose slot names no place, or whose position is not
+ * below table_positions (it turns by rope_tab's first position), writes q and the
+ * copies alone.  No two tokens have the same slot.  qkv, rope_tab, q, k_out and v_out
+ * 16-byte aligned.  No reference counterpart. */
+int catena_mi355x_rope_packed_bf16(const catena_paged_kv_t *kv, const void *qkv, int qkv_f32,
+                                   const float *rope_tab, uint32_t table_positions,
+                                   uint32_t rotary_dim, int interleaved, const uint32_t *token_pos,
+                                   const uint64_t *slot_map, uint16_t *q, uint64_t tokens,
+                                   uint32_t heads, uint16_t *k_out, uint16_t *v_out);
+
+/* Causal attention of packed sequences over a cache in pages: q[tokens][heads]
+ * [head_dim] bf16, starts[rows + 1] (device u32), lens[rows] (device u32: a row's
+ * slots with the new tokens' among them; past the table: the table's).  Token t of row
+ * r's n = starts[r + 1] - starts[r] sees the row's first lens[r] - n + t + 1 slots, n
+ * = 1 alone all of them, so prompts, later parts of prompts and single tokens may stand
+ * beside each other.  Query head h reads kv head h / (heads / kv_heads).  o[tokens]
+ * [heads][head_dim] bf16 RNE: scores, sums and o in f32, p rounded to bf16 (2^-8 of
+ * it) where it meets v.  A token that sees no slot gives 0; slots without a page are
+ * not seen, and a token whose slots all have none gives NaN.  What lies in slots that
+ * a token does not see never reaches it, infinities and NaN included.  Sums of finite
+ * values do not overflow (a mean within 2^-8 of the type's largest may).  starts past `tokens` are cut there, rows that end before
+ * they begin have no tokens; places of q and o that belong to no row are not touched.
+ * No two rows' tokens overlap.  o is not q, k or v.
+ * workspace as for catena_mi355x_attn_paged_bf16, of attn_prompt_plan's size, which is
+ * a function of the sizes alone and needs no device.  q and o 16-byte aligned.
+ * Allocates nothing; may be captured.  No reference counterpart. */
+int catena_mi355x_attn_prompt_plan(const catena_paged_kv_t *kv, uint64_t tokens, uint32_t heads,
+                                   uint64_t *workspace_bytes);
+int catena_mi355x_attn_prompt_bf16(const catena_paged_kv_t *kv, const uint16_t *q,
+                                   const uint32_t *starts, const uint32_t *lens, uint16_t *o,
+                                   uint64_t tokens, uint32_t heads, float scale, void *workspace,
+                                   uint64_t workspace_bytes);
+
+/* The same over packed keys and values, of prompts with nothing before them: k, v
+ * [tokens][kv_heads][head_dim] bf16, token after token kv_stride elements apart (0:
+ * kv_heads * head_dim; a multiple of 8, up to 2^25), 16-byte aligned; token t of a row
+ * sees the row's tokens 0 .. t.  head_dim 64 or 128.  No reference counterpart
+ * (catena_mi355x_attn_causal_bf16 has the reference's exponential and equal lengths). */
+int catena_mi355x_attn_packed_plan(uint32_t rows, uint64_t tokens, uint32_t heads,
+                                   uint32_t kv_heads, uint32_t head_dim, uint64_t *workspace_bytes);
+int catena_mi355x_attn_packed_bf16(const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                   const uint32_t *starts, uint16_t *o, uint32_t rows,
+                                   uint64_t tokens, uint32_t heads, uint32_t kv_heads,
+                                   uint32_t head_dim, uint64_t kv_stride, float scale,
+                                   void *workspace, uint64_t workspace_bytes);
+
+/* A cache in pages held in 4 bits: e2m1 values (code 0 .. 7: 0, .5, 1, 1.5, 2, 3, 4, 6;
+ * 8 more: negative), two a byte, the first in the lower half.
+ *   k       [num_pages][kv_heads][page_size][head_dim / 2] bytes
+ *   k_scale [num_pages][kv_heads][head_dim / 32][page_size] bytes: 32 neighbouring
+ *           values of a slot count 2^(byte - 127) each, 255: NaN
+ *   v       [num_pages][kv_heads][head_dim / 2][page_size] bytes: byte (i, j) holds
+ *           values 2 i and 2 i + 1 of slot j
+ *   v_scale [num_pages][kv_heads][page_size] bf16: what a slot's values count
+ * Sizes and table as in catena_paged_kv_t; all pools 16-byte aligned.  A slot takes
+ * head_dim + head_dim / 32 + 2 bytes a head, 0.26 of bf16's (head_dim 128). */
+typedef struct catena_paged_kv4 {
+  uint8_t *k;
+  uint8_t *v;
+  uint8_t *k_scale;
+  uint16_t *v_scale;
+  const uint32_t *table;
+  uint32_t num_pages;
+  uint32_t page_size;
+  uint32_t rows;
+  uint32_t max_pages; /* table entries per row */
+  uint32_t kv_heads;
+  uint32_t head_dim;
+} catena_paged_kv4_t;
+
+/* catena_mi355x_rope_packed_bf16 into a cache in 4 bits.  The bf16 k and v are cut to
+ * codes: a block of keys counts the smallest power of two, 2^-127 at least, of which
+ * its largest |x| is at most 6; a head's values count a sixth of their largest |x|,
+ * rounded up to bf16; each code is the nearest, of two the even one.  A block with an
+ * infinity or NaN becomes NaN.  k_out and v_out are the values that the codes stand for
+ * (v's rounded to bf16), so that a prompt attends to what later steps will.
+ * kv_heads <= 128. */
+int catena_mi355x_rope_packed_q4(const catena_paged_kv4_t *kv, const void *qkv, int qkv_f32,
+                                 const float *rope_tab, uint32_t table_positions,
+                                 uint32_t rotary_dim, int interleaved, const uint32_t *token_pos,
+                                 const uint64_t *slot_map, uint16_t *q, uint64_t tokens,
+                                 uint32_t heads, uint16_t *k_out, uint16_t *v_out);
+
+/* Attention of one new token per row over a cache in 4 bits, as
+ * catena_mi355x_attn_paged_bf16 has it: lens, absent pages, rows of no slots, scores
+ * and sums in f32 (p to 2^-16), o[rows][heads][head_dim] bf16 RNE; workspace of
+ * attn_paged_q4_plan's size.  No reference counterpart. */
+int catena_mi355x_attn_paged_q4_plan(const catena_paged_kv4_t *kv, uint32_t heads, uint32_t *parts,
+                                     uint64_t *workspace_bytes);
+int catena_mi355x_attn_paged_q4(const catena_paged_kv4_t *kv, const uint16_t *q,
+                                const uint32_t *lens, uint16_t *o, uint32_t heads, float scale,
+                                void *workspace, uint64_t workspace_bytes);
+
 /* Bytes of workspace that catena_mi355x_beam_select_f32 takes.  A function of
  * the sizes alone; needs no device. */
 int catena_mi355x_beam_select_plan(uint32_t groups, uint32_t beams, uint32_t vocab,
