@@ -6,6 +6,7 @@
 // Arguments are checked before the device is looked for, so a refused call is
 // refused without one.
 #include <cmath>
+#include <cstdlib>
 
 #include "paged_host.h"
 
@@ -52,7 +53,8 @@ int rope_packed_check(uint32_t kv_heads, uint32_t dim, const void* qkv, const fl
 }
 
 struct PromptPlan {
-  uint64_t tiles;  // of 128 query rows, at most
+  uint32_t waves;  // of a workgroup, 32 query rows each
+  uint64_t tiles;   // workgroups' query rows of a kv head, at most
   uint64_t bytes;
 };
 int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_heads, PromptPlan* p) {
@@ -62,7 +64,9 @@ int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_head
   if (tokens > 0x7FFFFFFFull || rows > 0x7FFFFFFFu || kv_heads > 65535)
     return fail(CATENA_ERR_UNSUPPORTED, "too many tokens, rows or heads");
   if (tokens * group > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many tokens and heads");
-  p->tiles = tokens * group / 128 + std::min<uint64_t>(rows, tokens);
+  p->waves = tokens * group / 256 * kv_heads >= 128 ? 8 : 4;
+  if (const char* e = getenv("CATENA_W")) p->waves = atoi(e);
+  p->tiles = tokens * group / (32 * p->waves) + std::min<uint64_t>(rows, tokens);
   if (p->tiles * kv_heads > grid_most(256)) return fail(CATENA_ERR_UNSUPPORTED, "too many tokens, rows and heads");
   p->bytes = 0;
   return CATENA_OK;
@@ -70,9 +74,10 @@ int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_head
 int prompt_launch(const AttnPromptArgs& a, uint32_t head_dim, bool paged, const PromptPlan& p) {
   AttnPromptArgs args_value = a;
   void* args[] = {&args_value};
-  const KernelId id = paged ? (head_dim == 128 ? KernelId::AttnPromptD128 : KernelId::AttnPromptD64)
-                            : (head_dim == 128 ? KernelId::AttnPackedD128 : KernelId::AttnPackedD64);
-  return launch(id, dim3((unsigned)(p.tiles * a.kv.kv_heads)), dim3(256), 64 * head_dim * 8, args);
+  // kernels in the order of their ids: D128 and D64 by waves, in pages, then packed
+  const int id = static_cast<int>(KernelId::AttnPromptD128W4) + (paged ? 0 : 4) + (head_dim == 64 ? 2 : 0) + (p.waves == 8);
+  return launch(static_cast<KernelId>(id), dim3((unsigned)(p.tiles * a.kv.kv_heads)), dim3(64 * p.waves),
+                64 * head_dim * 2 * 6, args);
 }
 void prompt_scale(float scale, AttnPromptArgs* a) {
   // (0 would meet the -inf of what is not seen: the least normal number instead, which
