@@ -139,14 +139,14 @@ const KernelSpec kKernels[] = {
     {KernelId::RopePackedBf16, "rope_packed", "catena_rope_packed_bf16in"},
     {KernelId::RopePackedQ4F32, "rope_packed", "catena_rope_packed_q4_f32in"},
     {KernelId::RopePackedQ4Bf16, "rope_packed", "catena_rope_packed_q4_bf16in"},
-    {KernelId::AttnPromptD128W4, "attn_prompt", "catena_attn_prompt_d128_w4"},
-    {KernelId::AttnPromptD128W8, "attn_prompt", "catena_attn_prompt_d128_w8"},
-    {KernelId::AttnPromptD64W4, "attn_prompt", "catena_attn_prompt_d64_w4"},
-    {KernelId::AttnPromptD64W8, "attn_prompt", "catena_attn_prompt_d64_w8"},
-    {KernelId::AttnPackedD128W4, "attn_prompt", "catena_attn_packed_d128_w4"},
-    {KernelId::AttnPackedD128W8, "attn_prompt", "catena_attn_packed_d128_w8"},
-    {KernelId::AttnPackedD64W4, "attn_prompt", "catena_attn_packed_d64_w4"},
-    {KernelId::AttnPackedD64W8, "attn_prompt", "catena_attn_packed_d64_w8"},
+    {KernelId::AttnPromptD128, "attn_prompt", "catena_attn_prompt_d128"},
+    {KernelId::AttnPromptD64, "attn_prompt", "catena_attn_prompt_d64"},
+    {KernelId::AttnPackedD128, "attn_prompt", "catena_attn_packed_d128"},
+    {KernelId::AttnPackedD64, "attn_prompt", "catena_attn_packed_d64"},
+    {KernelId::AttnPromptList, "attn_prompt", "catena_attn_prompt_list"},
+    {KernelId::AttnPackedList, "attn_prompt", "catena_attn_packed_list"},
+    {KernelId::AttnPromptJoinD128, "attn_prompt", "catena_attn_prompt_join_d128"},
+    {KernelId::AttnPromptJoinD64, "attn_prompt", "catena_attn_prompt_join_d64"},
     {KernelId::AttnPagedQ4D128, "attn_paged_q4", "catena_attn_paged_q4_d128"},
     {KernelId::AttnPagedQ4D64, "attn_paged_q4", "catena_attn_paged_q4_d64"},
     {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},

@@ -102,14 +102,14 @@ enum class KernelId : int {
   RopePackedBf16,
   RopePackedQ4F32,
   RopePackedQ4Bf16,
-  AttnPromptD128W4,  // packed sequences (attn_prompt.hip), four or eight waves a workgroup
-  AttnPromptD128W8,
-  AttnPromptD64W4,
-  AttnPromptD64W8,
-  AttnPackedD128W4,
-  AttnPackedD128W8,
-  AttnPackedD64W4,
-  AttnPackedD64W8,
+  AttnPromptD128,  // packed sequences (attn_prompt.hip)
+  AttnPromptD64,
+  AttnPackedD128,
+  AttnPackedD64,
+  AttnPromptList,
+  AttnPackedList,
+  AttnPromptJoinD128,
+  AttnPromptJoinD64,
   AttnPagedQ4D128,  // a cache in 4 bits (attn_paged_q4.hip)
   AttnPagedQ4D64,
   BeamRuns8,  // beam search's selection (beam.hip)

@@ -6,7 +6,6 @@
 // Arguments are checked before the device is looked for, so a refused call is
 // refused without one.
 #include <cmath>
-#include <cstdlib>
 
 #include "paged_host.h"
 
@@ -53,31 +52,56 @@ int rope_packed_check(uint32_t kv_heads, uint32_t dim, const void* qkv, const fl
 }
 
 struct PromptPlan {
-  uint32_t waves;  // of a workgroup, 32 query rows each
-  uint64_t tiles;   // workgroups' query rows of a kv head, at most
-  uint64_t bytes;
+  uint32_t units;   // of 256 query rows of a row and kv head, at most
+  bool list;        // dealt out from a list, long ones first and cut
+  uint32_t items, splits, part_rows;
+  uint64_t splits_at, ml_at, o_at, bytes;  // in the workspace: counts, items, splits, part_ml, part_o
 };
-int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_heads, PromptPlan* p) {
+// slots: of a row, at most
+int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint64_t slots,
+                PromptPlan* p) {
   if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0)
     return fail(CATENA_ERR_INVALID_ARGUMENT, "%u query heads over %u kv heads", heads, kv_heads);
   const uint32_t group = heads / kv_heads;
   if (tokens > 0x7FFFFFFFull || rows > 0x7FFFFFFFu || kv_heads > 65535)
     return fail(CATENA_ERR_UNSUPPORTED, "too many tokens, rows or heads");
   if (tokens * group > 0x7FFFFFFFull) return fail(CATENA_ERR_UNSUPPORTED, "too many tokens and heads");
-  p->waves = tokens * group / 256 * kv_heads >= 128 ? 8 : 4;
-  if (const char* e = getenv("CATENA_W")) p->waves = atoi(e);
-  p->tiles = tokens * group / (32 * p->waves) + std::min<uint64_t>(rows, tokens);
-  if (p->tiles * kv_heads > grid_most(256)) return fail(CATENA_ERR_UNSUPPORTED, "too many tokens, rows and heads");
+  const uint64_t units = tokens * group / 256 + std::min<uint64_t>(rows, tokens);
+  if (units * kv_heads > grid_most(512)) return fail(CATENA_ERR_UNSUPPORTED, "too many tokens, rows and heads");
+  p->units = (uint32_t)units;
+  p->list = slots > 1024 && units <= 16384;
   p->bytes = 0;
+  if (!p->list) return CATENA_OK;
+  p->items = p->units + kPromptParts;
+  p->splits = (uint32_t)std::min<uint64_t>(units, std::max(1u, kPromptParts / 2 / kv_heads));
+  p->part_rows = (uint32_t)std::min<uint64_t>(256, tokens * group);
+  p->splits_at = 64 + (uint64_t)p->items * sizeof(PromptItem);
+  p->ml_at = p->splits_at + (uint64_t)p->splits * sizeof(PromptItem);
+  p->o_at = p->ml_at + (uint64_t)kPromptParts * p->part_rows * 8;
+  p->bytes = p->o_at + (uint64_t)kPromptParts * p->part_rows * head_dim * 4;
   return CATENA_OK;
 }
-int prompt_launch(const AttnPromptArgs& a, uint32_t head_dim, bool paged, const PromptPlan& p) {
-  AttnPromptArgs args_value = a;
-  void* args[] = {&args_value};
-  // kernels in the order of their ids: D128 and D64 by waves, in pages, then packed
-  const int id = static_cast<int>(KernelId::AttnPromptD128W4) + (paged ? 0 : 4) + (head_dim == 64 ? 2 : 0) + (p.waves == 8);
-  return launch(static_cast<KernelId>(id), dim3((unsigned)(p.tiles * a.kv.kv_heads)), dim3(64 * p.waves),
-                64 * head_dim * 2 * 6, args);
+int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* workspace) {
+  const bool d64 = a.kv.head_dim == 64;
+  const KernelId id = paged ? (d64 ? KernelId::AttnPromptD64 : KernelId::AttnPromptD128)
+                            : (d64 ? KernelId::AttnPackedD64 : KernelId::AttnPackedD128);
+  const size_t lds = 64 * a.kv.head_dim * 2 * 6;
+  void* args[] = {&a};
+  if (!p.list) return launch(id, dim3(p.units * a.kv.kv_heads), dim3(512), lds, args);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  a.counts = reinterpret_cast<uint32_t*>(ws);
+  a.items = reinterpret_cast<PromptItem*>(ws + 64);
+  a.splits = reinterpret_cast<PromptItem*>(ws + p.splits_at);
+  a.part_ml = reinterpret_cast<float*>(ws + p.ml_at);
+  a.part_o = reinterpret_cast<float*>(ws + p.o_at);
+  a.part_rows = p.part_rows;
+  a.first_tickets = kPromptCus / kPromptQueues;
+  a.max_items = p.items;
+  int st = launch(paged ? KernelId::AttnPromptList : KernelId::AttnPackedList, dim3(1), dim3(1024), 0, args);
+  if (!st) st = launch(id, dim3(kPromptCus), dim3(512), lds, args);
+  if (st) return st;
+  return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(p.splits, a.kv.kv_heads, 8),
+                dim3(256), 0, args);
 }
 void prompt_scale(float scale, AttnPromptArgs* a) {
   // (0 would meet the -inf of what is not seen: the least normal number instead, which
@@ -250,7 +274,7 @@ int catena_mi355x_attn_prompt_plan(const catena_paged_kv_t* kv, uint64_t tokens,
   PagedKv c;
   PromptPlan p;
   int st = paged_check(kv, false, &c);
-  if (!st) st = prompt_plan(c.rows, tokens, heads, c.kv_heads, &p);
+  if (!st) st = prompt_plan(c.rows, tokens, heads, c.kv_heads, c.head_dim, paged_slots(c), &p);
   if (!st) *workspace_bytes = p.bytes;
   return st;
 }
@@ -261,7 +285,7 @@ int catena_mi355x_attn_prompt_bf16(const catena_paged_kv_t* kv, const uint16_t* 
   AttnPromptArgs a{};
   PromptPlan p;
   int st = paged_check(kv, true, &a.kv);
-  if (!st) st = prompt_plan(a.kv.rows, tokens, heads, a.kv.kv_heads, &p);
+  if (!st) st = prompt_plan(a.kv.rows, tokens, heads, a.kv.kv_heads, a.kv.head_dim, paged_slots(a.kv), &p);
   if (st || a.kv.rows == 0 || tokens == 0) return st;
   if (!q || !starts || !lens || !o) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
   if (!aligned(q, 16) || !aligned(o, 16) || !aligned(starts, 4) || !aligned(lens, 4))
@@ -278,7 +302,7 @@ int catena_mi355x_attn_prompt_bf16(const catena_paged_kv_t* kv, const uint16_t* 
   a.tokens = (uint32_t)tokens;
   a.group = heads / a.kv.kv_heads;
   prompt_scale(scale, &a);
-  return prompt_launch(a, a.kv.head_dim, true, p);
+  return prompt_launch(a, true, p, workspace);
 }
 
 int catena_mi355x_attn_packed_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_heads,
@@ -287,7 +311,7 @@ int catena_mi355x_attn_packed_plan(uint32_t rows, uint64_t tokens, uint32_t head
   PromptPlan p;
   if (head_dim != 64 && head_dim != 128)
     return fail(CATENA_ERR_UNSUPPORTED, "packed attention head_dim %u unsupported (64 or 128)", head_dim);
-  const int st = prompt_plan(rows, tokens, heads, kv_heads, &p);
+  const int st = prompt_plan(rows, tokens, heads, kv_heads, head_dim, tokens, &p);
   if (!st) *workspace_bytes = p.bytes;
   return st;
 }
@@ -300,7 +324,7 @@ int catena_mi355x_attn_packed_bf16(const uint16_t* q, const uint16_t* k, const u
   PromptPlan p;
   if (head_dim != 64 && head_dim != 128)
     return fail(CATENA_ERR_UNSUPPORTED, "packed attention head_dim %u unsupported (64 or 128)", head_dim);
-  int st = prompt_plan(rows, tokens, heads, kv_heads, &p);
+  int st = prompt_plan(rows, tokens, heads, kv_heads, head_dim, tokens, &p);
   if (st) return st;
   if (kv_stride == 0) kv_stride = (uint64_t)kv_heads * head_dim;
   if (kv_stride < (uint64_t)kv_heads * head_dim || kv_stride % 8 != 0)
@@ -324,7 +348,7 @@ int catena_mi355x_attn_packed_bf16(const uint16_t* q, const uint16_t* k, const u
   a.tokens = (uint32_t)tokens;
   a.group = heads / kv_heads;
   prompt_scale(scale, &a);
-  return prompt_launch(a, head_dim, false, p);
+  return prompt_launch(a, false, p, workspace);
 }
 
 int catena_mi355x_attn_paged_q4_plan(const catena_paged_kv4_t* kv, uint32_t heads, uint32_t* parts,

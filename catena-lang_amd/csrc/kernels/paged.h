@@ -164,6 +164,18 @@ struct RopePackedArgs {
 };
 
 // attn_prompt.hip
+constexpr uint32_t kPromptWhole = 0xFFFFFFFFu;  // an item that is all of its unit
+constexpr uint32_t kPromptQueues = 8;           // one an XCD
+constexpr uint32_t kPromptCus = 256;
+constexpr uint32_t kPromptLeast = 16;           // tiles of 64 slots: shorter units are not cut
+constexpr uint32_t kPromptParts = 2 * kPromptCus;  // parts there may be, of all kv heads
+// 256 query rows (unit `unit`) of a row's n new tokens, `old` slots in front of them: tiles [beg, end) of what they
+// see.  In the list of cut units: beg is the number of parts, `part` the first one.
+struct PromptItem {
+  uint32_t row, unit, first, n;
+  int32_t old;
+  uint32_t beg, end, part;
+};
 struct AttnPromptArgs {
   PagedKv kv;               // table null: k, v [tokens][kv_heads][head_dim], stride apart
   const uint16_t* q;        // [tokens][heads][D]
@@ -171,6 +183,14 @@ struct AttnPromptArgs {
   const uint32_t* lens;     // [rows]; null: as many as new tokens
   uint16_t* o;              // [tokens][heads][D]
   uint64_t stride;          // elements from a token's k to the next one's, without a table
+  PromptItem* items;        // the list; null: a workgroup a unit
+  PromptItem* splits;       // units that were cut
+  uint32_t* counts;         // items, splits, tickets taken of each queue
+  float* part_o;            // [part][kv_heads][part_rows][D]
+  float* part_ml;           // [part][kv_heads][part_rows][2]: reference point (base 2), sum
+  uint32_t part_rows;       // query rows of a unit that there may be
+  uint32_t first_tickets;   // what a queue's tickets begin with
+  uint32_t max_items;
   uint32_t tokens, group;
   float scale_log2;         // |scale| log2(e)
   uint32_t flip;            // 0x80008000 where the scale is negative: q's signs
