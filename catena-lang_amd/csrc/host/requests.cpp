@@ -85,7 +85,7 @@ int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* works
   const bool d64 = a.kv.head_dim == 64;
   const KernelId id = paged ? (d64 ? KernelId::AttnPromptD64 : KernelId::AttnPromptD128)
                             : (d64 ? KernelId::AttnPackedD64 : KernelId::AttnPackedD128);
-  const size_t lds = 64 * a.kv.head_dim * 2 * 6;
+  const size_t lds = 8 * 32 * (a.kv.head_dim * 4 + 8);  // the waves' results; the tiles take less
   void* args[] = {&a};
   if (!p.list) return launch(id, dim3(p.units * a.kv.kv_heads), dim3(512), lds, args);
   unsigned char* ws = static_cast<unsigned char*>(workspace);

@@ -20,6 +20,11 @@
 // Blocks of 32 slots go through a pipeline of three phases (scores, exponentials, o), so
 // that the exponentials of one block run under the products of its neighbours.
 //
+// Units of up to 64 query rows (single tokens, short chunks) leave most waves without
+// rows and wait for memory instead: there each wave takes blocks of 32 slots of its own,
+// with its own loads and no barrier, for 32 rows, and the waves' results are joined at
+// the end.
+//
 // Units are dealt out in one of two ways.  Few short ones: a workgroup each, which finds
 // it from the rows' lengths.  Else a kernel before lists them by length, long ones first,
 // units above a CU's even share cut into equal parts, and a workgroup a CU takes them
@@ -46,6 +51,7 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kEase = 40.0f;
 constexpr int kWaves = 8;
 constexpr uint32_t kRows = 32 * kWaves;  // query rows of a unit
+constexpr uint32_t kNarrow = 64;         // of so many a narrow unit
 constexpr int kKeys = 64;                // slots of a tile
 constexpr int kStages = 3;               // tiles of K, and of V, in LDS
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -84,7 +90,7 @@ CATENA_DEV Tokens tokens_of(const AttnPromptArgs& a, uint32_t row) {
   return Tokens{beg, beg < end ? end - beg : 0u};
 }
 CATENA_DEV uint32_t units_of(const AttnPromptArgs& a, uint32_t n) {
-  return (uint32_t)(((uint64_t)n * a.group + kRows - 1) / kRows);
+  return (n * a.group + (kRows - 1)) / kRows;  // (the host sees to it that n * group < 2^31)
 }
 // Slots of a row in front of its n new tokens; below 0: the first of them see nothing
 template <bool PAGED>
@@ -94,7 +100,7 @@ CATENA_DEV int32_t old_of(const AttnPromptArgs& a, uint32_t row, uint32_t n) {
 }
 // Slots that the last token of a row's unit sees
 CATENA_DEV int32_t most_of(const AttnPromptArgs& a, uint32_t unit, uint32_t n, int32_t old) {
-  const uint32_t last = (uint32_t)(((uint64_t)unit * kRows + kRows - 1) / a.group);
+  const uint32_t last = (unit * kRows + (kRows - 1)) / a.group;  // (rows stay below 2^31)
   return old + (int32_t)(last < n ? last + 1 : n);
 }
 CATENA_DEV uint32_t tiles_of(int32_t slots) { return slots > 0 ? ((uint32_t)slots + kKeys - 1) / kKeys : 0u; }
@@ -146,8 +152,11 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   const uint32_t heads = a.group * a.kv.kv_heads;
   const uint32_t len = (uint32_t)(it.old + (int32_t)it.n);  // slots in use
 
-  // the lane's query row
-  const uint32_t w_row = it.unit * kRows + wave * 32, m_row = w_row + c, t_row = m_row / a.group;
+  // The lane's query row.  Up to 64 rows: one or two blocks of 32 (in turn over the waves, which share out the slots).
+  const uint32_t rows_left = it.n * a.group - it.unit * kRows, rows = rows_left < kRows ? rows_left : kRows;
+  const bool narrow = rows <= kNarrow;
+  const uint32_t blocks = rows <= 32 ? 1 : 2;
+  const uint32_t w_row = it.unit * kRows + 32 * (narrow ? wave % blocks : wave), m_row = w_row + c, t_row = m_row / a.group;
   const bool live = t_row < it.n;
   const uint64_t q_at =
       ((uint64_t)(it.first + (live ? t_row : 0u)) * heads + kvh * a.group + (live ? m_row % a.group : 0u)) * D;
@@ -162,7 +171,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   }
   // Of the item's tiles, the first `whole` are seen by all its rows (rows that are not live see none, and need
   // not) and have their pages
-  const int32_t least = it.old + (int32_t)((uint64_t)it.unit * kRows / a.group) + 1;
+  const int32_t least = it.old + (int32_t)(it.unit * kRows / a.group) + 1;
   uint32_t upto = least > 0 ? (uint32_t)least / kKeys : 0u;
   if constexpr (PAGED) {
     const uint32_t entries = (uint32_t)(((uint64_t)upto * kKeys + (1u << a.kv.page_shift) - 1) >> a.kv.page_shift);
@@ -186,25 +195,20 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   // Loads: run wave / kWavesARun of a tile, which lies inside one page
   const uint32_t row_bytes = PAGED ? D * 2 : (uint32_t)(a.stride * 2);
   const uint32_t run = wave / kWavesARun, first_block = wave % kWavesARun * kLoads;
-  uint32_t k_off[kLoads], v_off[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    k_off[i] = (lane & 15u) * row_bytes + 64 * (first_block + i) + 16 * (lane >> 4);
-    v_off[i] = (lane >> 2) * row_bytes + 64 * (first_block + i) + 16 * (lane & 3u);
-  }
+  // (a block's 64 bytes of a row by the scalar offset, which the range check leaves out: rows are inside or not)
+  const uint32_t k_off = (lane & 15u) * row_bytes + 16 * (lane >> 4), v_off = (lane >> 2) * row_bytes + 16 * (lane & 3u);
   auto page_of = [&](uint32_t slot) -> uint32_t {
     if constexpr (PAGED)
       return slot < len ? scalar_word(a.kv.table, (uint64_t)it.row * a.kv.max_pages + (slot >> a.kv.page_shift)) : 0xFFFFFFFFu;
     return 0;
   };
-  // The wave's slots of the item's tile i: where they are and how many.  Their page is looked up a tile before
-  // they are asked for, so that nothing waits for it.
+  // A run of 16 slots: where they are and how many.  Its page is looked up a tile before they are asked for, so that
+  // nothing waits for it.
   struct Slots {
     uint64_t at;
     uint32_t n;
   };
-  auto slots_of = [&](uint32_t i, uint32_t page) {
-    const uint32_t slot = (it.beg + i) * kKeys + 16 * run;
+  auto slots_at = [&](uint32_t slot, uint32_t page) {
     Slots r{0, slot < len ? (len - slot < 16 ? len - slot : 16u) : 0u};
     if constexpr (PAGED) {
       if (page < a.kv.num_pages)
@@ -216,16 +220,23 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     }
     return r;
   };
-  auto look_up = [&](uint32_t i) { return page_of((it.beg + i) * kKeys + 16 * run); };
-  // K (what 0) or V (1) of them to a place of the ring
-  auto issue = [&](uint32_t stage, const Slots& r, int what) {
+  // Blocks first .. first + N - 1 of their K (what 0) or V (1) to LDS
+  auto load = [&](const Slots& r, int what, uint32_t first, auto n_, uint16_t* dst) {
     const int bytes = r.n ? (int)((r.n - 1) * row_bytes + D * 2) : 0;
     const __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc((void*)((what ? pool_v : pool_k) + r.at), (short)0, bytes, 0x00020000);
-    uint16_t* dst = smem + ((what ? kStages : 0) + stage) * kTile + (run * kAcross + first_block) * 512;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 512 * i), 16, (int)(what ? v_off[i] : k_off[i]), 0, 0, 0);
+    for (int i = 0; i < n_.value; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 512 * i), 16, (int)(what ? v_off : k_off),
+                                               (int)(64 * (first + i)), 0, 0);
+  };
+  // The wave's run of the item's tile i
+  auto run_slot = [&](uint32_t i) { return (it.beg + i) * kKeys + 16 * run; };
+  auto look_up = [&](uint32_t i) { return page_of(run_slot(i)); };
+  auto slots_of = [&](uint32_t i, uint32_t page) { return slots_at(run_slot(i), page); };
+  auto issue = [&](uint32_t stage, const Slots& r, int what) {
+    load(r, what, first_block, std::integral_constant<int, kLoads>{},
+         smem + ((what ? kStages : 0) + stage) * kTile + (run * kAcross + first_block) * 512);
   };
   // All that this wave has asked for is in LDS, what it has read of LDS has arrived, and so for the others
   auto arrive = [&]() {
@@ -294,69 +305,67 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   };
   auto passes = [&]() { return __any(top > limit) != 0; };
 
-  // Tile i, which not all rows see
-  auto take_masked = [&](uint32_t i0) {
-    const uint16_t* v_rows = smem + (kStages + i0 % kStages) * kTile;
-    lds_char* k = k_tile(i0);
-    lds_char* v = v_tile(i0);
-    const uint32_t slot0 = (it.beg + i0) * kKeys;
-    uint32_t found = 0;
-#pragma unroll 4
-    for (uint32_t i = lane; i < kTile / 8; i += 64) {
-      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(v_rows + 8 * i);
+  // A block of 32 slots from `slot` on by itself, in two halves: its scores, and the rest.  check: some rows may not
+  // see all of it.
+  auto block_scores = [&](lds_char* k, int half) {
+    f32x16_t s;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) found |= ((w[j] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-    }
-    const bool odd = __any(found != 0) != 0;
-    uint32_t runs = 0xFu;  // runs of 16 slots whose page exists
-    if constexpr (PAGED) {
-      runs = 0;
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) runs |= (page_of(slot0 + 16 * r) < a.kv.num_pages ? 1u : 0u) << r;
-    }
-    f32x16_t s[2];
-    top = kNegInf;
+    for (int i = 0; i < KS; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(k, half, i), qf[i], s, 0, 0, 0);
+    return s;
+  };
+  auto block_rest = [&](f32x16_t s, lds_char* v, const uint16_t* v_rows, int half, uint32_t slot, bool check) {
+    bool odd = false;
+    if (check) {
+      uint32_t found = 0;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+      for (int i = 0; i < kTile / 16 / 64; ++i) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(v_rows + half * (kTile / 2) + 8 * (64 * i + lane));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[y][i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) s[y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(k, y, i), qf[i], s[y], 0, 0, 0);
-      const int32_t left = sees - (int32_t)slot0 - 4 * (int32_t)h;
+        for (int j = 0; j < 4; ++j) found |= ((w[j] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+      }
+      odd = __any(found != 0) != 0;
+      uint32_t runs = 3u;  // runs of 16 slots whose page exists
+      if constexpr (PAGED)
+        runs = (page_of(slot) < a.kv.num_pages ? 1u : 0u) | (page_of(slot + 16) < a.kv.num_pages ? 2u : 0u);
+      const int32_t left = sees - (int32_t)slot - 4 * (int32_t)h;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool seen = (32 * y + 8 * (i / 4) + i % 4 < left) & ((runs >> (2 * y + i / 8) & 1u) != 0);
-        s[y][i] = seen ? s[y][i] : kNegInf;
-        top = larger(top, s[y][i]);
+        const bool seen = (8 * (i / 4) + i % 4 < left) & ((runs >> (i / 8) & 1u) != 0);
+        s[i] = seen ? s[i] : kNegInf;
       }
     }
+    top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = larger(top, s[i]);
     if (passes()) raise(nullptr);
     const float base = anchor(m) + kEase;
-    bf16x8_t p[4];
+    bf16x8_t p[2];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < 2; ++y) {
       u32x4_t w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[y / 2][8 * (y % 2) + 2 * i], a.scale_log2, -base)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[y / 2][8 * (y % 2) + 2 * i + 1], a.scale_log2, -base)));
+        w[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i], a.scale_log2, -base)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i + 1], a.scale_log2, -base)));
         l = add_pair(w[i], l);
       }
       p[y] = __builtin_bit_cast(bf16x8_t, w);
     }
     // V's values of one kind: the finite ones as they are (0), ones for inf (1), -inf (2), NaN (3)
     auto only = [&](int kind, int d, int x) {
-      u32x4_t w = v_frag(v, d, x);
+      u32x4_t w = v_frag(v, d, 2 * half + x);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t half[2] = {w[j] & 0xFFFFu, w[j] >> 16};
+        uint32_t two[2] = {w[j] & 0xFFFFu, w[j] >> 16};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t y = half[e];
+          const uint32_t y = two[e];
           const int is = (y & 0x7F80u) != 0x7F80u ? 0 : y == 0x7F80u ? 1 : y == 0xFF80u ? 2 : 3;
-          half[e] = is != kind ? 0u : kind == 0 ? y : 0x3F80u;
+          two[e] = is != kind ? 0u : kind == 0 ? y : 0x3F80u;
         }
-        w[j] = half[0] | half[1] << 16;
+        w[j] = two[0] | two[1] << 16;
       }
       return __builtin_bit_cast(bf16x8_t, w);
     };
@@ -364,18 +373,18 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int d = 0; d < DB; ++d) {
       if (!odd) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v_frag(v, d, x)), p[x], acc[d], 0, 0, 0);
+        for (int x = 0; x < 2; ++x)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v_frag(v, d, 2 * half + x)), p[x], acc[d], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(only(0, d, x), p[x], acc[d], 0, 0, 0);
+        for (int x = 0; x < 2; ++x) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(only(0, d, x), p[x], acc[d], 0, 0, 0);
 #pragma unroll 1
         for (int kind = 1; kind < 4; ++kind) {
           f32x16_t r;
 #pragma unroll
           for (int i = 0; i < 16; ++i) r[i] = 0.0f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) r = __builtin_amdgcn_mfma_f32_32x32x16_bf16(only(kind, d, x), p[x], r, 0, 0, 0);
+          for (int x = 0; x < 2; ++x) r = __builtin_amdgcn_mfma_f32_32x32x16_bf16(only(kind, d, x), p[x], r, 0, 0, 0);
           const float what = kind == 1 ? -kNegInf : kind == 2 ? kNegInf : __builtin_nanf("");
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] + (r[i] > 0.0f ? what : 0.0f);
@@ -383,6 +392,105 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       }
     }
   };
+
+  if (narrow) {
+    // Wave w: blocks of 32 slots w / blocks, + 8 / blocks, ...; K and V of one at a time in its own part of LDS, each
+    // asked for as soon as its place has been read
+    constexpr int kBlock = 2 * kAcross;  // loads of a block's K, or V
+    const uint32_t step = kWaves / blocks, all = 2 * count;
+    uint16_t* mine = smem + wave * kTile;
+    lds_char *k = place(mine, k_lane), *v = place(mine + kTile / 2, v_lane);
+    auto slot_of = [&](uint32_t b) { return it.beg * kKeys + 32 * b; };
+    struct Pair {
+      Slots s[2];
+    };
+    auto pair_of = [&](uint32_t b, uint32_t p0, uint32_t p1) {
+      return Pair{{slots_at(slot_of(b), p0), slots_at(slot_of(b) + 16, p1)}};
+    };
+    auto bring = [&](const Pair& p, int what) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        load(p.s[r], what, 0, std::integral_constant<int, kAcross>{}, mine + what * (kTile / 2) + r * kAcross * 512);
+    };
+    auto fence = [] { asm volatile("" ::: "memory"); };
+    uint32_t b = wave / blocks;
+    Pair next = pair_of(b, page_of(slot_of(b)), page_of(slot_of(b) + 16));
+    uint32_t p0 = page_of(slot_of(b + step)), p1 = page_of(slot_of(b + step) + 16);
+    if (b < all) {
+      bring(next, 0);
+      bring(next, 1);
+    }
+#pragma clang loop unroll(disable)
+    for (; b < all; b += step) {
+      const bool more = b + step < all;
+      next = pair_of(b + step, p0, p1);
+      p0 = page_of(slot_of(b + 2 * step));
+      p1 = page_of(slot_of(b + 2 * step) + 16);
+      fence();
+      __builtin_amdgcn_s_waitcnt(0x0F70 | kBlock);  // vmcnt: all but V's loads
+      fence();
+      const f32x16_t s = block_scores(k, 0);
+      fence();
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): K has been read
+      if (more) bring(next, 0);
+      fence();
+      if (more)
+        __builtin_amdgcn_s_waitcnt(0x0F70 | kBlock);  // all but the next K's
+      else
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+      fence();
+      // (a block inside `upto` tiles is seen by all rows)
+      block_rest(s, v, mine + kTile / 2, 0, slot_of(b), slot_of(b) + 32 > upto * kKeys);
+      fence();
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      if (more) bring(next, 1);
+    }
+    l = l + __shfl_xor(l, 32);
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);
+    float* sml = so + kWaves * 32 * D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4_t*>(so + (wave * 32 + c) * D + 32 * d + 2 * i + 4 * h) =
+            f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+    if (h == 0) {
+      sml[2 * (wave * 32 + c)] = m;
+      sml[2 * (wave * 32 + c) + 1] = l;
+    }
+    __syncthreads();
+    for (uint32_t id = threadIdx.x; id < rows * (D / 4); id += 64 * kWaves) {
+      const uint32_t row = id / (D / 4), d = id % (D / 4) * 4;
+      float mm = kNegInf, ll = 0.0f;
+      f32x4_t oo = {0, 0, 0, 0};
+      for (uint32_t w = row / 32; w < kWaves; w += blocks) mm = __builtin_fmaxf(mm, sml[2 * (w * 32 + row % 32)]);
+      for (uint32_t w = row / 32; w < kWaves; w += blocks) {
+        const uint32_t at = w * 32 + row % 32;
+        const float f = __builtin_amdgcn_exp2f(sml[2 * at] - anchor(mm));
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(so + at * D + d);
+        ll = ll + sml[2 * at + 1] * f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) oo[i] = oo[i] + y[i] * f;
+      }
+      if (it.part != kPromptWhole) {
+        const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh) * a.part_rows + row;
+        if (d == 0) {
+          a.part_ml[2 * at] = mm;
+          a.part_ml[2 * at + 1] = ll;
+        }
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = oo;
+        continue;
+      }
+      const uint32_t r = it.unit * kRows + row, t = r / a.group;
+      const float by = it.old + (int32_t)t + 1 > 0 ? ll : 1.0f;
+      uint2 w;
+      w.x = pack_bf16x2(oo[0] / by, oo[1] / by);
+      w.y = pack_bf16x2(oo[2] / by, oo[3] / by);
+      *reinterpret_cast<uint2*>(a.o + ((uint64_t)(it.first + t) * heads + kvh * a.group + r % a.group) * D + d) = w;
+    }
+    return;
+  }
 
   // Whole tiles: blocks of 32 slots, whose softmax runs under the products of their neighbours.  Phase j, between
   // the products of the scores of block j + 1 and of o of block j - 1: the exponentials of block j, the maximum of
@@ -495,7 +603,12 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     }
     next = slots_of(i + 2, after);
     after = look_up(i + 3);
-    if ((int32_t)((it.beg + i) * kKeys) < w_most) take_masked(i);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t slot = (it.beg + i) * kKeys + 32 * half;
+      if ((int32_t)slot < w_most)
+        block_rest(block_scores(k_tile(i), half), v_tile(i), smem + (kStages + i % kStages) * kTile, half, slot, true);
+    }
     arrive();
   }
 
@@ -561,10 +674,12 @@ CATENA_DEV uint32_t last_at_most(const uint32_t* s, uint32_t n, uint32_t x) {
   return at;
 }
 
-// The list: one workgroup of 1024 threads.  A unit of more tiles than `most` (a CU's share of all the work) is cut
-// into equal parts.  Rows stand in the order of their last (longest) unit's length, in 64 classes, and a row's units
-// behind each other, the long ones first: so the short ones end the work, and the workgroups of an XCD read the
-// same K and V at a time (8 ragged prompts of up to 4096 tokens, units by length alone 645 us, by rows PLACEHOLDER).
+// The list: one workgroup of 1024 threads.  A unit costs its tiles, a narrow one, which waits for memory beside
+// the others' products, half of them; one of more than three quarters of a CU's share of all the work
+// is cut into equal parts.
+// Rows stand in the order of their dearest unit's cost, in 64 classes, and a row's units behind each other, the
+// last (longest) first: so the short ones end the work, and the workgroups of an XCD read the same K and V at a time
+// (8 ragged prompts of up to 4096 tokens: units by length alone 645 us, by rows 486).
 // Which of two rows of a class comes first, and which place a part gets, is left to the order of the threads: no
 // result depends on it.
 template <bool PAGED>
@@ -579,35 +694,44 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
     s_work = 0;
     s_parts = s_splits = 0;
   }
-  __syncthreads();
   struct Row {
-    uint32_t row, units;
+    uint32_t units;
     Tokens t;
     int32_t old;
   };
-  auto tiles_at = [&](uint32_t unit, uint32_t n, int32_t old) { return tiles_of(most_of(a, unit, n, old)); };
-  // Every row to a thread, 1024 at a time: of_row(row); then every unit of theirs to one: of_unit(place of the row
-  // among the 1024, unit)
+  struct Cost {
+    uint32_t tiles, cost;
+  };
+  auto cost_of = [&](uint32_t unit, uint32_t n, int32_t old) {
+    const uint32_t tiles = tiles_of(most_of(a, unit, n, old));
+    const bool narrow = n * a.group - unit * kRows <= kNarrow;
+    return Cost{tiles, narrow ? tiles : 2 * tiles};
+  };
+  // Every row to a thread, 1024 at a time: of_row(row); then every unit of theirs to one: of_unit(row, its place
+  // among the 1024, unit).  Where there are no more rows than that they are looked at once.
+  Row x;
+  uint32_t all = 0;
+  bool known = false;
   auto every = [&](auto of_row, auto of_unit) {
     for (uint32_t r0 = 0; r0 < a.kv.rows; r0 += kThreads) {
-      Row x;
-      x.row = r0 + tid < a.kv.rows ? r0 + tid : a.kv.rows - 1;
-      x.t = tokens_of(a, x.row);
-      x.t.n = r0 + tid < a.kv.rows ? x.t.n : 0u;
-      x.old = old_of<PAGED>(a, x.row, x.t.n);
-      x.units = units_of(a, x.t.n);
-      const uint32_t in = wave_prefix(x.units);
-      if (lane == 63) s_wave[wave] = in;
-      __syncthreads();
-      uint32_t before = in - x.units, all = 0;
-      for (uint32_t w = 0; w < 16; ++w) {
-        before += w < wave ? s_wave[w] : 0u;
-        all += s_wave[w];
+      if (!known || a.kv.rows > kThreads) {
+        known = true;
+        const uint32_t row = r0 + tid < a.kv.rows ? r0 + tid : a.kv.rows - 1;
+        x.t = tokens_of(a, row);
+        x.t.n = r0 + tid < a.kv.rows ? x.t.n : 0u;
+        x.old = old_of<PAGED>(a, row, x.t.n);
+        x.units = units_of(a, x.t.n);
+        const uint32_t in = wave_prefix(x.units);
+        if (lane == 63) s_wave[wave] = in;
+        __syncthreads();
+        const uint32_t sums = wave_prefix(lane < 16 ? s_wave[lane] : 0u);
+        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave);
+        all = lane_of(sums, 15);
+        s_start[tid] = (w ? lane_of(sums, w - 1) : 0u) + in - x.units;  // (rows without units are never the last one at most)
+        s_first[tid] = x.t.first;
+        s_n[tid] = x.t.n;
+        s_old[tid] = (uint32_t)x.old;
       }
-      s_start[tid] = before;  // (rows without units are never the last one at most)
-      s_first[tid] = x.t.first;
-      s_n[tid] = x.t.n;
-      s_old[tid] = (uint32_t)x.old;
       if (x.units > 0) s_at[tid] = of_row(x);
       __syncthreads();
       for (uint32_t k = tid; k < all; k += kThreads) {
@@ -617,54 +741,59 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       __syncthreads();
     }
   };
-  auto nothing = [](const Row&) { return 0u; };
-  auto no_unit = [](uint32_t, uint32_t, uint32_t) {};
-  every(nothing, [&](uint32_t, uint32_t at, uint32_t unit) {
-    atomicAdd(&s_work, (unsigned long long)tiles_at(unit, s_n[at], (int32_t)s_old[at]));
+  uint64_t mine = 0;
+  every([](const Row&) { return 0u; }, [&](uint32_t, uint32_t at, uint32_t unit) {
+    mine += cost_of(unit, s_n[at], (int32_t)s_old[at]).cost;
   });
-  // (a cut unit has more than `most` tiles, so the parts of all heads are fewer than 2 work / most <= kPromptParts)
-  const uint64_t work = s_work * a.kv.kv_heads, share = (work + kPromptCus - 1) / kPromptCus;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
+  if (lane == 0 && mine) atomicAdd(&s_work, (unsigned long long)mine);
+  __syncthreads();
+  // (a cut unit costs more than `most`, so the parts of all heads are fewer than 2 work / most < kPromptParts)
+  const uint64_t work = s_work * a.kv.kv_heads, share = 3 * work / (4 * kPromptCus) + 1;
   const uint32_t most = share < kPromptLeast ? kPromptLeast : share < 0x7FFFFFFFull ? (uint32_t)share : 0x7FFFFFFFu;
-  auto class_of = [&](uint32_t tiles) { return (uint32_t)((uint64_t)(most - (tiles < most ? tiles : most)) * (kClasses - 1) / most); };
-  auto parts_of = [&](uint32_t tiles) { return tiles <= most ? 1u : (tiles + most - 1) / most; };
-  // items of a row's units from `unit` on: only its last units are cut
+  auto parts_of = [&](uint32_t cost) { return cost <= most ? 1u : (cost + most - 1) / most; };
+  // items of a row's units from `unit` on: of the wide units only the last ones are cut
   auto items_from = [&](uint32_t unit, uint32_t units, uint32_t n, int32_t old) {
     uint32_t items = units - unit;
     for (uint32_t u = units; u > unit; --u) {
-      const uint32_t parts = parts_of(tiles_at(u - 1, n, old));
-      if (parts == 1) break;
+      const uint32_t parts = parts_of(cost_of(u - 1, n, old).cost);
+      if (parts == 1 && u < units) break;
       items += parts - 1;
     }
     return items;
   };
-  every([&](const Row& x) {
-    return atomicAdd(&s_class[class_of(tiles_at(x.units - 1, x.t.n, x.old))], items_from(0, x.units, x.t.n, x.old));
-  }, no_unit);
+  auto place_of = [&](const Row& r) {
+    uint32_t cost = cost_of(r.units - 1, r.t.n, r.old).cost;
+    if (r.units > 1) cost = max(cost, cost_of(r.units - 2, r.t.n, r.old).cost);
+    const uint32_t at = (uint32_t)((uint64_t)(most - (cost < most ? cost : most)) * (kClasses - 1) / most);
+    return atomicAdd(&s_class[at], items_from(0, r.units, r.t.n, r.old));
+  };
+  every(place_of, [](uint32_t, uint32_t, uint32_t) {});
   if (tid < 64) {
     const uint32_t n = s_class[tid], upto = wave_prefix(n);
     s_class[tid] = upto - n;
     if (tid == 63) a.counts[0] = upto < a.max_items ? upto : a.max_items;
   }
   __syncthreads();
-  every([&](const Row& x) {
-    return atomicAdd(&s_class[class_of(tiles_at(x.units - 1, x.t.n, x.old))], items_from(0, x.units, x.t.n, x.old));
-  }, [&](uint32_t row, uint32_t place, uint32_t unit) {
+  every(place_of, [&](uint32_t row, uint32_t place, uint32_t unit) {
     const uint32_t n = s_n[place];
     const int32_t old = (int32_t)s_old[place];
-    const uint32_t tiles = tiles_at(unit, n, old), parts = parts_of(tiles), each = (tiles + parts - 1) / parts;
+    const Cost cost = cost_of(unit, n, old);
+    const uint32_t tiles = cost.tiles, parts = parts_of(cost.cost), each = (tiles + parts - 1) / parts;
     const uint32_t at = s_at[place] + items_from(unit + 1, units_of(a, n), n, old);
-    PromptItem x{row, unit, s_first[place], n, old, 0, tiles, kPromptWhole};
+    PromptItem y{row, unit, s_first[place], n, old, 0, tiles, kPromptWhole};
     if (parts > 1) {
-      x.part = atomicAdd(&s_parts, parts);
-      PromptItem z = x;
+      y.part = atomicAdd(&s_parts, parts);
+      PromptItem z = y;
       z.beg = parts;
       a.splits[atomicAdd(&s_splits, 1u)] = z;
     }
     for (uint32_t p = 0; p < parts; ++p) {
-      x.beg = p * each < tiles ? p * each : tiles;
-      x.end = x.beg + each < tiles ? x.beg + each : tiles;
-      if (at + p < a.max_items) a.items[at + p] = x;  // (always, but for rows that overlap)
-      if (parts > 1) ++x.part;
+      y.beg = p * each < tiles ? p * each : tiles;
+      y.end = y.beg + each < tiles ? y.beg + each : tiles;
+      if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap)
+      if (parts > 1) ++y.part;
     }
   });
   if (tid == 0) a.counts[1] = s_splits;

@@ -167,8 +167,8 @@ struct RopePackedArgs {
 constexpr uint32_t kPromptWhole = 0xFFFFFFFFu;  // an item that is all of its unit
 constexpr uint32_t kPromptQueues = 8;           // one an XCD
 constexpr uint32_t kPromptCus = 256;
-constexpr uint32_t kPromptLeast = 16;           // tiles of 64 slots: shorter units are not cut
-constexpr uint32_t kPromptParts = 2 * kPromptCus;  // parts there may be, of all kv heads
+constexpr uint32_t kPromptLeast = 32;           // what a unit costs that is not cut (two a tile of 64 slots)
+constexpr uint32_t kPromptParts = 4 * kPromptCus;  // parts there may be, of all kv heads
 // 256 query rows (unit `unit`) of a row's n new tokens, `old` slots in front of them: tiles [beg, end) of what they
 // see.  In the list of cut units: beg is the number of parts, `part` the first one.
 struct PromptItem {
