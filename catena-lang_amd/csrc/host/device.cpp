@@ -149,6 +149,10 @@ const KernelSpec kKernels[] = {
     {KernelId::AttnPromptJoinD64, "attn_prompt", "catena_attn_prompt_join_d64"},
     {KernelId::AttnPagedQ4D128, "attn_paged_q4", "catena_attn_paged_q4_d128"},
     {KernelId::AttnPagedQ4D64, "attn_paged_q4", "catena_attn_paged_q4_d64"},
+    {KernelId::AttnPagedQ4D128Wide, "attn_paged_q4", "catena_attn_paged_q4_d128_wide"},
+    {KernelId::AttnPagedQ4D64Wide, "attn_paged_q4", "catena_attn_paged_q4_d64_wide"},
+    {KernelId::AttnPagedQ4JoinD128, "attn_paged_q4", "catena_attn_paged_q4_join_d128"},
+    {KernelId::AttnPagedQ4JoinD64, "attn_paged_q4", "catena_attn_paged_q4_join_d64"},
     {KernelId::BeamRuns8, "beam", "catena_beam_runs_8"},
     {KernelId::BeamRuns16, "beam", "catena_beam_runs_16"},
     {KernelId::BeamJoin, "beam", "catena_beam_join"},

@@ -112,6 +112,10 @@ enum class KernelId : int {
   AttnPromptJoinD64,
   AttnPagedQ4D128,  // a cache in 4 bits (attn_paged_q4.hip)
   AttnPagedQ4D64,
+  AttnPagedQ4D128Wide,  // more than 8 query heads a kv head
+  AttnPagedQ4D64Wide,
+  AttnPagedQ4JoinD128,
+  AttnPagedQ4JoinD64,
   BeamRuns8,  // beam search's selection (beam.hip)
   BeamRuns16,
   BeamJoin,

@@ -50,7 +50,8 @@ struct AttnPagedPlan {
   uint64_t part_ml, whole_ml, scores, bytes;  // offsets and the sum; part_o comes first
 };
 
-inline int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPlan* p) {
+inline int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, AttnPagedPlan* p,
+                           bool four_bits = false) {
   if (heads == 0 || heads % kv.kv_heads != 0)
     return fail(CATENA_ERR_INVALID_ARGUMENT, "%u query heads over %u kv heads", heads, kv.kv_heads);
   p->group = heads / kv.kv_heads;
@@ -83,6 +84,13 @@ inline int attn_paged_plan(const PagedKv& kv, uint32_t heads, bool weights, Attn
     p->blocks = 0;
   else
     p->blocks = (uint32_t)std::min<uint64_t>(tiles >= 16384 && units <= 256 ? 256 : 512, ceil_div(tiles, 4));
+  if (four_bits) {
+    // a table that never holds a row to cut: one row alone is the first
+    const uint64_t longest = ceil_div(slots, kAttnQ4Slots), all = units * longest;
+    const uint64_t alone = (uint64_t)kv.kv_heads * p->head_tiles * longest;
+    const bool whole = longest <= kAttnQ4WholeMost && longest * kAttnQ4WholeShare <= alone + 2 * kAttnQ4WholeShare;
+    p->blocks = whole ? 0 : (uint32_t)std::min<uint64_t>(kv.head_dim == 64 && all >= kAttnQ4TwoACu ? 768 : 512, all);
+  }
   // the join by a unit's number of parts: a thread takes all of them, or some, or
   // some of a quarter of the columns (1 part a unit 5.0 / 6.6 us, 5 parts 4.5 / 3.7 /
   // 4.6, 64 parts - / 26 / 5)

@@ -103,11 +103,21 @@ int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* works
   return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(p.splits, a.kv.kv_heads, 8),
                 dim3(256), 0, args);
 }
-void prompt_scale(float scale, AttnPromptArgs* a) {
+// The scale as the kernels take it: above 0, a negative one's sign to q
+struct Scale {
+  float log2;
+  uint32_t flip;
+};
+Scale scale_of(float scale) {
   // (0 would meet the -inf of what is not seen: the least normal number instead, which
   // leaves the scores of any values below 2^100 apart by nothing that f32 keeps)
-  a->scale_log2 = scale == 0 ? 0x1p-126f : (float)(std::fabs((double)scale) * 1.4426950408889634);
-  a->flip = scale < 0 ? 0x80008000u : 0u;
+  return Scale{scale == 0 ? 0x1p-126f : (float)(std::fabs((double)scale) * 1.4426950408889634),
+               scale < 0 ? 0x80008000u : 0u};
+}
+void prompt_scale(float scale, AttnPromptArgs* a) {
+  const Scale s = scale_of(scale);
+  a->scale_log2 = s.log2;
+  a->flip = s.flip;
 }
 }  // namespace
 
@@ -359,7 +369,7 @@ int catena_mi355x_attn_paged_q4_plan(const catena_paged_kv4_t* kv, uint32_t head
   int st = paged4_check(kv, false, &c);
   if (st) return st;
   const PagedKv sizes{nullptr, nullptr, c.table, c.num_pages, c.page_shift, c.rows, c.max_pages, c.kv_heads, c.head_dim};
-  st = attn_paged_plan(sizes, heads, false, &p);
+  st = attn_paged_plan(sizes, heads, false, &p, true);
   if (st) return st;
   *parts = p.blocks;
   *workspace_bytes = p.bytes;
@@ -374,7 +384,7 @@ int catena_mi355x_attn_paged_q4(const catena_paged_kv4_t* kv, const uint16_t* q,
   int st = paged4_check(kv, true, &c);
   if (st) return st;
   a.kv = PagedKv{nullptr, nullptr, c.table, c.num_pages, c.page_shift, c.rows, c.max_pages, c.kv_heads, c.head_dim};
-  st = attn_paged_plan(a.kv, heads, false, &p);
+  st = attn_paged_plan(a.kv, heads, false, &p, true);
   if (st || c.rows == 0) return st;
   if (!q || !lens || !o) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
   if (!aligned(q, 16) || !aligned(o, 16) || !aligned(lens, 4))
@@ -394,22 +404,22 @@ int catena_mi355x_attn_paged_q4(const catena_paged_kv4_t* kv, const uint16_t* q,
   a.head_tiles = p.head_tiles;
   a.blocks = p.blocks;
   a.short_slots = p.short_slots;
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  struct {
-    const uint8_t *k, *v, *k_scale;
-    const uint16_t* v_scale;
-  } pools{c.k, c.v, c.k_scale, c.v_scale};
-  const bool d64 = c.head_dim == 64;
+  const Scale s = scale_of(scale);
+  a.scale_log2 = s.log2;
+  AttnQ4Pools pools{c.k, c.v, c.k_scale, c.v_scale, s.flip};
   const uint64_t pairs = (uint64_t)c.rows * c.kv_heads;
   void* args[] = {&a, &pools};
-  st = launch(d64 ? KernelId::AttnPagedQ4D64 : KernelId::AttnPagedQ4D128,
-              dim3(p.blocks ? p.blocks : (unsigned)std::min(pairs * p.head_tiles, grid_most(256))), dim3(256), 0, args);
+  const KernelId id = c.head_dim == 64 ? (p.group <= 8 ? KernelId::AttnPagedQ4D64 : KernelId::AttnPagedQ4D64Wide)
+                                       : (p.group <= 8 ? KernelId::AttnPagedQ4D128 : KernelId::AttnPagedQ4D128Wide);
+  // (a workgroup a unit also where units may be cut: what there is not to do for one it leaves)
+  const uint64_t grid = std::min(std::max<uint64_t>(pairs * p.head_tiles, p.blocks), grid_most(256));
+  st = launch(id, dim3((unsigned)grid), dim3(256), 0, args);
   if (st || p.blocks == 0) return st;
   uint32_t pieces = p.pieces;
   const uint64_t joins = pieces ? (uint64_t)p.group * pieces : ceil_div((uint64_t)p.group * c.head_dim, 1024);
   const uint64_t rows = std::min<uint64_t>(c.rows, std::max<uint64_t>(1, kJoinBlocks / (joins * c.kv_heads)));
   void* jargs[] = {&a, &pieces};
-  return launch(d64 ? KernelId::AttnPagedJoinD64Bf16 : KernelId::AttnPagedJoinD128Bf16,
+  return launch(c.head_dim == 64 ? KernelId::AttnPagedQ4JoinD64 : KernelId::AttnPagedQ4JoinD128,
                 dim3(c.kv_heads, (unsigned)joins, (unsigned)rows), dim3(256), 0, jargs);
 }
 

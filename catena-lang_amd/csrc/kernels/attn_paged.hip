@@ -52,6 +52,15 @@
 // largest |v| and any finite values give a finite mean; the division takes the
 // power back.  (It costs the other end: products of values below some 2^-80 are f32's
 // smallest numbers and lose their last bits.)
+#include "common.h"
+#include "paged.h"
+
+namespace {
+// long parts go to one workgroup a CU (D = 128, 32768 tiles: 83.1 us against 85.3 with
+// two; D = 64, whose tiles are half as long, ragged rows: 59.6 against 57.3)
+constexpr uint32_t kTileSlots = 32, kOneACu = 16384, kTwoACu = 0, kWholeShare = 0, kWholeMost = 0;
+}  // namespace
+
 #include "attn_line.h"
 
 namespace {
@@ -383,46 +392,6 @@ CATENA_DEV void attn_paged_run(const AttnPagedArgs& a) {
   }
 }
 
-// Where the parts of a unit are: the workgroups that have one are numbered on
-struct Parts {
-  uint32_t first, n;  // n < 2: one workgroup had the unit
-};
-CATENA_DEV Parts parts_of(const Line& line, const RowOnLine& r, uint32_t unit) {
-  if (r.tiles == 0) return Parts{0, 0};
-  const uint32_t beg = r.first + unit * r.tiles, first = beg / line.per;
-  return Parts{first, (beg + r.tiles - 1) / line.per - first + 1};
-}
-
-// Place of a unit's part i for head h of its 16: the unit's first part lies in the
-// second of its workgroup's places
-CATENA_DEV uint64_t part_place(const AttnPagedArgs& a, const Parts& p, uint32_t i, uint32_t h) {
-  return ((uint64_t)(p.first + i) * 2 + (i == 0)) * (a.group < 16 ? a.group : 16) + h;
-}
-
-// One thread's parts i = first, first + step, ... of a unit's head, with a running
-// maximum: four columns of o from `col` on
-struct Joined {
-  f32x4_t o;
-  float m, l;
-};
-template <int D>
-CATENA_DEV Joined join_parts(const AttnPagedArgs& a, const Parts& p, uint32_t h, uint32_t col, uint32_t first,
-                             uint32_t step) {
-  Joined j{f32x4_t{0, 0, 0, 0}, kNegInf, 0.0f};
-#pragma unroll 4
-  for (uint32_t i = first; i < p.n; i += step) {
-    const uint64_t at = part_place(a, p, i, h);
-    const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
-    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + col);
-    const float m = __builtin_fmaxf(j.m, pm), f = exp2_fast(j.m - anchor(m)), e = exp2_fast(pm - anchor(m));
-    j.m = m;
-    j.l = j.l * f + pl * e;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) j.o[c] = j.o[c] * f + y[c] * e;
-  }
-  return j;
-}
-
 // Joins the units that were cut, writes 0 for rows without slots, and adds the
 // weights that the first kernel could not.  blockIdx.x: the kv head, blockIdx.z:
 // rows in turn; blockIdx.y < joins: the o of 1024 / D query heads, a thread four
@@ -430,53 +399,14 @@ CATENA_DEV Joined join_parts(const AttnPagedArgs& a, const Parts& p, uint32_t h,
 // thread some of the parts; else 1024 slots' weights.
 template <int D, bool F32>
 CATENA_DEV void attn_paged_join(const AttnPagedArgs& a, uint32_t pieces) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  __shared__ f32x2 s_ml[64];
-  __shared__ __attribute__((aligned(16))) float s_o[256 * 4];
   __shared__ float s_m[16], s_r[16];
   const uint32_t tid = threadIdx.x, heads = a.group * a.kv.kv_heads, kvh = blockIdx.x;
   const FirstRows rows = first_rows(a);
   const Line line = line_of(a, rows);
   if (line.whole && (!a.acc_out || a.head_tiles == 1)) return;
-  constexpr uint32_t LANES = D / 4;
-  const uint32_t joins = pieces ? a.group * pieces : (a.group * LANES + 255) / 256;
-  const uint32_t quarters = pieces == 4 ? 2 : 0;  // pieces: 0, 1 or 4
+  const uint32_t joins = joins_of<D>(a, pieces);
   if (blockIdx.y < joins) {
-    if (line.whole) return;
-    const uint32_t lanes = LANES >> quarters;  // of a head's columns, 16 bytes each
-    const uint32_t head = pieces ? blockIdx.y >> quarters : blockIdx.y * (256 / LANES) + tid / LANES;
-    const uint32_t col = (pieces == 4 ? blockIdx.y % 4 * lanes * 4 : 0u) + tid % lanes * 4;
-    const uint32_t mine = tid / lanes, step = 256 / lanes;
-    for (uint32_t row = blockIdx.z; row < a.kv.rows; row += gridDim.z) {
-      const RowOnLine r = row_on_line(a, rows, row);
-      const uint64_t at = ((uint64_t)row * heads + kvh * a.group + head) * D + col;
-      const Parts p = parts_of(line, r, kvh * a.head_tiles + head / 16);
-      if (!pieces) {
-        if (head >= a.group || p.n == 1) continue;
-        const Joined j = join_parts<D>(a, p, head % 16, col, 0, 1);
-        store_o<F32>(a, at, j.o, j.l, r.len);
-        continue;
-      }
-      if (p.n == 1) continue;
-      const Joined j = join_parts<D>(a, p, head % 16, col, mine, step);
-      __syncthreads();  // the last one's values have been read
-      *reinterpret_cast<f32x4_t*>(&s_o[4 * tid]) = j.o;
-      if (tid % lanes == 0) s_ml[mine] = f32x2{j.m, j.l};
-      __syncthreads();
-      if (tid < lanes) {
-        float m = kNegInf, l = 0.0f;
-        f32x4_t o = f32x4_t{0, 0, 0, 0};
-        for (uint32_t i = 0; i < step; ++i) m = __builtin_fmaxf(m, s_ml[i][0]);
-        for (uint32_t i = 0; i < step; ++i) {
-          const float f = exp2_fast(s_ml[i][0] - anchor(m));
-          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&s_o[4 * (i * lanes + tid)]);
-          l = l + s_ml[i][1] * f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[c] = o[c] + y[c] * f;
-        }
-        store_o<F32>(a, at, o, l, r.len);
-      }
-    }
+    join_o<D, F32>(a, rows, line, pieces);
     return;
   }
   const uint32_t slot0 = (blockIdx.y - joins) * 1024;

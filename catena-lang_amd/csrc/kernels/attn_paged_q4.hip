@@ -11,8 +11,8 @@
 // A wave takes 128 slots at a time, its lane group g (lanes 16 g ..) slots 32 g ..
 // 32 g + 31 of them.
 //   S^T = K Q^T (16 x 16 x 32 products): instruction set u of eight takes slots 32 (c
-//     / 4) + 8 (c % 4) + u as its 16 rows, so that the results leave lane (c, g) with
-//     head c's scores of its own group's slots 32 g + 8 j + u (j: the register).  The
+//     / 4) + 4 u + c % 4 as its 16 rows, so that the results leave lane (c, g) with
+//     head c's scores of its own group's slots 32 g + 4 u + j (j: the register).  The
 //     order of d in the sum is free: the lane loads a quarter of a slot's codes, D / 8
 //     bytes, which lie in one block of 32, and converts them with that block's scale
 //     (two values an instruction).
@@ -20,24 +20,30 @@
 //     bytes in two runs of 16.  Halves of two dwords mixed give eight codes of one
 //     column, slots (0, 4, 1, 5, 2, 6, 3, 7), and P's terms are packed in that order.
 //     The slots' scales go into P.
+// P enters as two bf16 terms, together exact to 2^-16.  Up to 8 heads stand in a product's
+// 16 columns twice, and the second ones take the second term; more heads need a second
+// product.
+// K of the next 128 slots is asked for as soon as the scores are there, V once it has been
+// read, so that a wave's loads are under way all the time.
 //
 // Codes are finite whatever their bits, so what lies behind a row's end is masked in
 // the scores and the scales alone.
-#include "attn_line.h"
+#include "common.h"
+#include "paged.h"
 
-struct AttnQ4Pools {
-  const uint8_t* k;
-  const uint8_t* v;
-  const uint8_t* k_scale;
-  const uint16_t* v_scale;
-};
+namespace {
+constexpr int kWaves = 4;
+constexpr uint32_t kTileSlots = kAttnQ4Slots, kOneACu = 0xFFFFFFFFu, kTwoACu = kAttnQ4TwoACu;
+constexpr uint32_t kWholeShare = kAttnQ4WholeShare, kWholeMost = kAttnQ4WholeMost;
+static_assert(kTileSlots == 128 * kWaves, "a turn of a workgroup");
+}  // namespace
+
+#include "attn_line.h"
 
 namespace {
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-
-constexpr int kWaves = 4;
 
 template <int D>
 struct Shared {
@@ -57,13 +63,14 @@ CATENA_DEV bf16x8_t widen8(uint32_t codes, float unit) {
 
 template <int D>
 struct Tile {
-  u32x4_t k[8];         // D = 64: the first two dwords
-  u32x2_t ks;           // block scales of slots 8 (c % 4) .. + 7 of group c / 4
+  u32x4_t k[8];          // D = 64: the first two dwords
+  u32x4_t ks[2];         // block scales of the 32 slots of group c / 4
   u32x4_t v[D / 32][2];  // pair of columns 16 i + c, slots 16 h .. + 15 of the lane's group
-  u32x4_t vs[2][2];     // their scales
+  u32x4_t vs[2][2];      // their scales
 };
 
-template <int D>
+// TWICE: groups of up to 8 heads, which stand in columns c and c + 8
+template <int D, bool TWICE>
 CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& pools) {
   constexpr int KC = D / 32;  // products of S
   constexpr int VG = D / 32;  // groups of 16 column pairs
@@ -72,102 +79,131 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t heads = a.group * a.kv.kv_heads;
   const uint32_t part_heads = a.group < 16 ? a.group : 16;
+  const uint32_t head = TWICE ? c & 7u : c;
   const uint32_t page_size = 1u << a.kv.page_shift, mask = page_size - 1u;
-  const uint32_t k_slot = 32 * (c >> 2) + 8 * (c & 3);  // the lane's slots of K, from the tile's first
 
-  // Pages of the runs of slots that a lane reads (its slots of K; two runs of V)
-  struct Pages {
-    uint32_t k, v[2];
+  // (the lane's number by a register of its own, so that no address parts are kept through the loop: there is no
+  // room)
+  auto own_lane = [&] {
+    uint32_t x = lane;
+    asm("" : "+v"(x));
+    return x;
   };
-  auto look_up = [&](const Part& p, uint32_t t) {
-    Pages x{0xFFFFFFFFu, {0xFFFFFFFFu, 0xFFFFFFFFu}};
-    if (t >= p.end) return x;
-    const uint32_t end = 32 * p.end < p.len ? 32 * p.end : p.len;
-    const uint32_t* row = a.kv.table + (uint64_t)p.row * a.kv.max_pages;
-    const uint32_t s = 32 * t + k_slot, s0 = 32 * t + 32 * g;
-    if (s < end) x.k = row[s >> a.kv.page_shift];
-    if (s0 < end) x.v[0] = row[s0 >> a.kv.page_shift];
-    if (s0 + 16 < end) x.v[1] = row[(s0 + 16) >> a.kv.page_shift];
+  // Pages of the tile's eight runs of 16 slots.  Looked up by lanes, run lane % 8, a turn before the loads that they
+  // say where to find: so nothing waits for them that does not wait for older loads too.
+  struct Pages {
+    uint32_t n[8];
+    CATENA_DEV uint32_t of(uint32_t group, int run) const {
+      const uint32_t low = group & 1u ? n[2 + run] : n[run], high = group & 1u ? n[6 + run] : n[4 + run];
+      return group & 2u ? high : low;
+    }
+  };
+  auto look_up = [&](const Part& p, uint32_t slot, uint32_t end) {
+    const uint32_t s = slot + 16 * (own_lane() & 7u);
+    const uint32_t page = (a.kv.table + (uint64_t)p.row * a.kv.max_pages)[(s < end ? s : 0u) >> a.kv.page_shift];
+    return s < end ? page : 0xFFFFFFFFu;
+  };
+  auto spread = [&](uint32_t pages) {
+    Pages x;
+#pragma unroll
+    for (uint32_t r = 0; r < 8; ++r) x.n[r] = lane_of(pages, r);
     return x;
   };
   // (what is not there is read from the pool's first page and masked)
-  auto request = [&](Tile<D>& x, const Part& p, uint32_t t, const Pages& at) {
-    const uint32_t s = (32 * t + k_slot) & mask, s0 = (32 * t + 32 * g) & mask, s1 = (32 * t + 32 * g + 16) & mask;
-    const uint64_t kc = paged_cells(a.kv.kv_heads, a.kv.page_shift, at.k < a.kv.num_pages ? at.k : 0u, p.kvh);
-    const uint8_t* k = pools.k + (kc + s) * (D / 2) + g * (D / 8);
+  auto request_k = [&](Tile<D>& x, const Part& p, uint32_t slot, const Pages& at) {
+    const uint32_t me = own_lane(), c = me & 15u, g = me >> 4;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if constexpr (D == 128) {
-        x.k[u] = *reinterpret_cast<const u32x4_t*>(k + u * (D / 2));
-      } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(k + u * (D / 2));
-        x.k[u][0] = w[0];
-        x.k[u][1] = w[1];
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t s = (slot + 32 * (c >> 2) + 16 * r) & mask;
+      const uint32_t page = at.of(c >> 2, r);
+      const uint64_t kc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, p.kvh);
+      const uint8_t* k = pools.k + (kc + s + (c & 3u)) * (D / 2) + g * (D / 8);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (D == 128) {
+          x.k[4 * r + u] = *reinterpret_cast<const u32x4_t*>(k + 4 * u * (D / 2));
+        } else {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(k + 4 * u * (D / 2));
+          x.k[4 * r + u][0] = w[0];
+          x.k[4 * r + u][1] = w[1];
+        }
       }
+      x.ks[r] = *reinterpret_cast<const u32x4_t*>(pools.k_scale + kc * (D / 32) + (uint64_t)(g * (D / 32) / 4) * page_size + s);
     }
-    x.ks = *reinterpret_cast<const u32x2_t*>(pools.k_scale + kc * (D / 32) + (uint64_t)(g * (D / 32) / 4) * page_size + s);
+  };
+  auto request_v = [&](Tile<D>& x, const Part& p, uint32_t slot, const Pages& at) {
+    const uint32_t me = own_lane(), c = me & 15u, g = me >> 4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint64_t vc = paged_cells(a.kv.kv_heads, a.kv.page_shift, at.v[h] < a.kv.num_pages ? at.v[h] : 0u, p.kvh);
-      const uint32_t sh0 = h ? s1 : s0;
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t s = (slot + 32 * g + 16 * r) & mask;
+      const uint32_t page = at.of(g, r);
+      const uint64_t vc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, p.kvh);
+      const uint8_t* v = pools.v + vc * (D / 2) + (uint64_t)c * page_size + s;
 #pragma unroll
-      for (int i = 0; i < VG; ++i)
-        x.v[i][h] = *reinterpret_cast<const u32x4_t*>(pools.v + vc * (D / 2) + (uint64_t)(16 * i + c) * page_size + sh0);
-      const u32x4_t* vs = reinterpret_cast<const u32x4_t*>(pools.v_scale + vc + sh0);
-      x.vs[h][0] = vs[0];
-      x.vs[h][1] = vs[1];
+      for (int i = 0; i < VG; ++i) x.v[i][r] = *reinterpret_cast<const u32x4_t*>(v + (uint64_t)(16 * i) * page_size);
+      const u32x4_t* vs = reinterpret_cast<const u32x4_t*>(pools.v_scale + vc + s);
+      x.vs[r][0] = vs[0];
+      x.vs[r][1] = vs[1];
     }
   };
 
+  // m: the head's reference point (base 2); p and l are kept times ease
   bf16x8_t qf[KC];
-  float m, l, ease;
+  float m, limit, l, ease_log2;
   f32x4_t acc[VG][2];
   auto begin = [&](const Part& p) {
-    const uint16_t* q = a.q + ((uint64_t)p.row * heads + p.kvh * a.group + 16 * p.ht + (c < p.gn ? c : 0)) * D;
+    const uint16_t* q = a.q + ((uint64_t)p.row * heads + p.kvh * a.group + 16 * p.ht + (head < p.gn ? head : 0)) * D;
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + (D / 4) * g + 8 * i);
-      if (c >= p.gn) w = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = head < p.gn ? w[j] ^ pools.flip : 0u;
       qf[i] = __builtin_bit_cast(bf16x8_t, w);
     }
-    m = kNegInf;
+    m = limit = kNegInf;
     l = 0.0f;
-    ease = ease_of(p.len | 1u);
+    ease_log2 = (float)(__builtin_clz(p.len | 1u) - 41);  // of ease_of
 #pragma unroll
     for (int i = 0; i < VG; ++i) acc[i][0] = acc[i][1] = f32x4_t{0, 0, 0, 0};
   };
 
-  auto take = [&](const Tile<D>& x, const Part& p, uint32_t t, const Pages& at) {
-    // scores in base 2: s[8 j + u] is slot 32 g + 8 j + u of head c
-    float s[32];
+  // s[4 u + j]: slot 32 g + 4 u + j of the head, in units of the products
+  auto scores = [&](const Tile<D>& x, float (&s)[32]) {
+    const uint32_t c = own_lane() & 15u;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const uint32_t byte = (x.ks[u / 4] >> (8 * (u % 4))) & 255u;
+      const uint32_t byte = x.ks[u / 4][u % 4] >> (8 * (c & 3u)) & 255u;
       const float unit = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
       f32x4_t y = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KC; ++i)
         y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(x.k[u][i], unit), qf[i], y, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[8 * j + u] = y[j] * a.scale_log2;
+      for (int j = 0; j < 4; ++j) s[4 * u + j] = y[j];
+      if (u % 2) __builtin_amdgcn_sched_barrier(0);  // (few registers over those of the loads)
     }
-    const uint32_t end = 32 * p.end < p.len ? 32 * p.end : p.len;
-    const bool here0 = at.v[0] < a.kv.num_pages, here1 = at.v[1] < a.kv.num_pages;
-    const bool full = __all(here0 && here1) && 32 * t + 128 <= end;
-    const uint32_t first = 32 * t + 32 * g;
-    if (!full) {
+  };
+  auto take = [&](const Tile<D>& x, float (&s)[32], const Part& p, uint32_t slot, const Pages& at) {
+    bool full = slot + 128 <= p.len;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i] = first + i < end && (i < 16 ? here0 : here1) ? s[i] : kNegInf;
+    for (int r = 0; r < 8; ++r) full = full & (at.n[r] < a.kv.num_pages);
+    if (!full) {
+      const uint32_t g = own_lane() >> 4;
+      const uint32_t first = slot + 32 * g;
+      const bool here0 = at.of(g, 0) < a.kv.num_pages, here1 = at.of(g, 1) < a.kv.num_pages;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i] = first + i < p.len && (i < 16 ? here0 : here1) ? s[i] : kNegInf;
     }
     float top = s[0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, s[i]);
-    if (__any(top > m + 8.0f)) {
+    for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[i]);
+    if (__any(top > limit)) {
       top = __builtin_fmaxf(top, __shfl_xor(top, 16));
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float m2 = __builtin_fmaxf(m, top);
+      const float m2 = __builtin_fmaxf(m, top * a.scale_log2);
       const float f = exp2_fast(m - anchor(m2));
       m = m2;
+      limit = (m2 + 8.0f) / a.scale_log2;
       l = l * f;
 #pragma unroll
       for (int i = 0; i < VG; ++i)
@@ -177,18 +213,17 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
           acc[i][1][j] = acc[i][1][j] * f;
         }
     }
-    const float base = anchor(m);
+    const float base = ease_log2 - anchor(m);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // eight slots: p to l, times ease and the slots' scales to two bf16 terms
+      // eight slots: p to l, times the slots' scales to two bf16 terms
       float p8[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float e = exp2_fast(s[8 * j + u] - base);
+        const float e = exp2_fast(__builtin_fmaf(s[8 * j + u], a.scale_log2, base));
         l = l + e;
         const uint32_t w = x.vs[j / 2][j % 2][u / 2];
-        const float sv = u % 2 ? bf16hi(w) : bf16lo(w);
-        p8[u] = e * ease * sv;
+        p8[u] = e * (u % 2 ? bf16hi(w) : bf16lo(w));
         if (!full) p8[u] = s[8 * j + u] == kNegInf ? 0.0f : p8[u];  // a scale that is not the row's may be anything
       }
       u32x4_t hi, lo;
@@ -196,6 +231,7 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
       for (int b = 0; b < 4; ++b) {
         hi[b] = pack_bf16x2(p8[b], p8[b + 4]);
         lo[b] = pack_bf16x2(p8[b] - bf16lo(hi[b]), p8[b + 4] - bf16hi(hi[b]));
+        if (TWICE) hi[b] = c >= 8 ? lo[b] : hi[b];
       }
       const bf16x8_t p0 = __builtin_bit_cast(bf16x8_t, hi), p1 = __builtin_bit_cast(bf16x8_t, lo);
 #pragma unroll
@@ -206,9 +242,12 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
         const bf16x8_t v0 = widen8(even, 1.0f), v1 = widen8(odd, 1.0f);
         acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p0, acc[i][0], 0, 0, 0);
         acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p0, acc[i][1], 0, 0, 0);
-        acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p1, acc[i][0], 0, 0, 0);
-        acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p1, acc[i][1], 0, 0, 0);
+        if (!TWICE) {
+          acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p1, acc[i][0], 0, 0, 0);
+          acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p1, acc[i][1], 0, 0, 0);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -216,6 +255,16 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
   auto finish = [&](const Part& p) {
     l = l + __shfl_xor(l, 16);
     l = l + __shfl_xor(l, 32);
+    l = l * __uint_as_float((uint32_t)(127 - (int)ease_log2) << 23);
+    if constexpr (TWICE) {
+#pragma unroll
+      for (int i = 0; i < VG; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i][0][j] = acc[i][0][j] + __shfl_xor(acc[i][0][j], 8);
+          acc[i][1][j] = acc[i][1][j] + __shfl_xor(acc[i][1][j], 8);
+        }
+    }
     __syncthreads();  // the last unit's values have been read
     if (g == 0) {
       sh.m[wave][c] = m;
@@ -291,10 +340,26 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
   for (;;) {
     begin(now);
     Tile<D> x;
-    for (uint32_t t = now.beg + 4 * wave; t < now.end; t += 4 * kWaves) {
-      const Pages pages = look_up(now, t);
-      request(x, now, t, pages);
-      take(x, now, t, pages);
+    // a tile a turn, 128 slots a wave; the last tile of a row may leave a wave without any
+    uint32_t slot = now.beg * kTileSlots + 128 * wave;
+    const uint32_t end = now.end * kTileSlots < now.len ? now.end * kTileSlots : now.len;
+    Pages pages = spread(look_up(now, slot, end));
+    uint32_t ahead = look_up(now, slot + kTileSlots, end);
+    if (slot < end) {
+      request_k(x, now, slot, pages);
+      request_v(x, now, slot, pages);
+    }
+#pragma clang loop unroll(disable)
+    for (; slot < end; slot += kTileSlots) {
+      float s[32];
+      scores(x, s);
+      const Pages next = spread(ahead);
+      ahead = look_up(now, slot + 2 * kTileSlots, end);
+      request_k(x, now, slot + kTileSlots, next);
+      __builtin_amdgcn_sched_barrier(0);
+      take(x, s, now, slot, pages);
+      request_v(x, now, slot + kTileSlots, next);
+      pages = next;
     }
     finish(now);
     if (at >= last) return;
@@ -310,9 +375,21 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_q4_d128(AttnPagedArgs a, AttnQ4Pools pools) {
-  attn_paged_q4_run<128>(a, pools);
+#define CATENA_ATTN_Q4(D, NAME, TWICE)                                                                          \
+  extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_q4_##NAME(AttnPagedArgs a, AttnQ4Pools pools) { \
+    attn_paged_q4_run<D, TWICE>(a, pools);                                                                      \
+  }
+CATENA_ATTN_Q4(128, d128, true)
+CATENA_ATTN_Q4(64, d64, true)
+CATENA_ATTN_Q4(128, d128_wide, false)
+CATENA_ATTN_Q4(64, d64_wide, false)
+
+// (grid as the other join's)
+extern "C" __global__ __launch_bounds__(256) void catena_attn_paged_q4_join_d128(AttnPagedArgs a, uint32_t pieces) {
+  const FirstRows rows = first_rows(a);
+  join_o<128, false>(a, rows, line_of(a, rows), pieces);
 }
-extern "C" __global__ __launch_bounds__(256, 2) void catena_attn_paged_q4_d64(AttnPagedArgs a, AttnQ4Pools pools) {
-  attn_paged_q4_run<64>(a, pools);
+extern "C" __global__ __launch_bounds__(256) void catena_attn_paged_q4_join_d64(AttnPagedArgs a, uint32_t pieces) {
+  const FirstRows rows = first_rows(a);
+  join_o<64, false>(a, rows, line_of(a, rows), pieces);
 }

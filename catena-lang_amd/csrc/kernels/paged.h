@@ -86,6 +86,26 @@ struct AttnPagedArgs {
   float scale_log2;       // scale * log2(e)
 };
 
+// attn_paged_q4.hip.  Units (a row, kv head and up to 16 query heads) are cut into tiles of
+// kAttnQ4Slots slots for two workgroups a CU, or three where these hold them (64 columns) and there are kAttnQ4TwoACu
+// tiles (64 ragged rows up to 8192 slots 46 us against 52, up to 16384 76 / 83; 4 x 32768, 2048 tiles, 30.5 / 22.8).  Not where the longest row, which one workgroup
+// reads at about 2.2 us a tile, ends with the others: all of them take 7.1 us for 512 tiles
+// of 128 columns, cutting about 6; nor is it long beside the others, which would leave CUs
+// idle at the end.  Rows x slots of 8 kv heads, whole / cut, us: 2 x 1024 9.2 / 11.0, x 2048
+// 13.5 / 11.1, x 4096 22.4 / 11.6; 8 x 1024 9.3 / 11.5, x 2048 14.5 / 12.8, x 4096 23.2 /
+// 16.5; 16 x 2048 14.9 / 16.6, x 4096 23.6 / 21.1; 32 x 2048 17.3 / 21, x 4096 31 / 34.5;
+// 64 x 4096 55 / 57; ragged 32 up to 4096 25 / 29, 64 up to 2048 24 / 29, up to 8192 76 / 74,
+// up to 16384 147 / 128, 256 up to 4096 128 / 144.
+constexpr uint32_t kAttnQ4Slots = 512, kAttnQ4WholeShare = 200, kAttnQ4WholeMost = 12, kAttnQ4TwoACu = 4096;
+// The pools, in place of AttnPagedArgs' own
+struct AttnQ4Pools {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* k_scale;
+  const uint16_t* v_scale;
+  uint32_t flip;  // the signs of q, so that scale_log2 > 0
+};
+
 // kv_paged.hip: eviction, reordering
 struct EvictArgs {
   PagedKv kv;

@@ -60,7 +60,8 @@ SHAPES = [
     ([1], 1, 1, 64, 16, 1), ([1, 0, 15, 16, 17], 8, 2, 128, 16, 2), ([31, 32, 33, 64, 127, 128, 129], 4, 4, 64, 32, 5),
     ([500, 3, 640, 511], 16, 16, 128, 16, 40), ([1000, 1, 77], 40, 1, 128, 64, 16), ([2048], 24, 1, 64, 1024, 2),
     ([5000, 4999, 0, 130], 8, 8, 128, 128, 40), ([700] * 9, 35, 5, 64, 16, 44), ([300, 40000], 4, 1, 128, 16, 2500),
-    ([9000, 12], 32, 8, 64, 32, 300),
+    ([9000, 12], 32, 8, 64, 32, 300), ([3000, 600, 513], 12, 1, 128, 32, 100), ([4096, 1537], 34, 2, 64, 64, 100),
+    ([7000] + [1, 20, 37] * 170, 8, 8, 64, 128, 55),
 ]
 
 
