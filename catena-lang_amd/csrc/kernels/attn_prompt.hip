@@ -63,6 +63,10 @@ typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
 
 CATENA_DEV uint32_t lane_of(uint32_t x, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane); }
 CATENA_DEV float anchor(float m) { return m == kNegInf ? 0.0f : m; }
+// Of sums with the reference point m beside others with m2 >= m: never 0, so that an infinity stays one
+CATENA_DEV float weight(float m, float m2) {
+  return __builtin_fmaxf(__builtin_amdgcn_exp2f(m - anchor(m2)), 0x1p-126f);
+}
 CATENA_DEV float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }  // NaN where one is
 
 // Uniform words that this kernel does not write, by scalar loads
@@ -467,7 +471,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       for (uint32_t w = row / 32; w < kWaves; w += blocks) mm = __builtin_fmaxf(mm, sml[2 * (w * 32 + row % 32)]);
       for (uint32_t w = row / 32; w < kWaves; w += blocks) {
         const uint32_t at = w * 32 + row % 32;
-        const float f = __builtin_amdgcn_exp2f(sml[2 * at] - anchor(mm));
+        const float f = weight(sml[2 * at], mm);
         const f32x4_t y = *reinterpret_cast<const f32x4_t*>(so + at * D + d);
         ll = ll + sml[2 * at + 1] * f;
 #pragma unroll
@@ -819,7 +823,7 @@ CATENA_DEV void attn_prompt_join(const AttnPromptArgs& a) {
       const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
       const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
       const float m2 = __builtin_fmaxf(m, pm);
-      const float f = __builtin_amdgcn_exp2f(m - anchor(m2)), e = __builtin_amdgcn_exp2f(pm - anchor(m2));
+      const float f = weight(m, m2), e = weight(pm, m2);
       m = m2;
       l = l * f + pl * e;
 #pragma unroll
