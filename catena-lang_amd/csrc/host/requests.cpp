@@ -97,6 +97,7 @@ int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* works
   a.part_rows = p.part_rows;
   a.first_tickets = kPromptCus / kPromptQueues;
   a.max_items = p.items;
+  a.max_splits = p.splits;
   int st = launch(paged ? KernelId::AttnPromptList : KernelId::AttnPackedList, dim3(1), dim3(1024), 0, args);
   if (!st) st = launch(id, dim3(kPromptCus), dim3(512), lds, args);
   if (st) return st;

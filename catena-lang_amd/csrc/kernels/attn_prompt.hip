@@ -791,16 +791,17 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       y.part = atomicAdd(&s_parts, parts);
       PromptItem z = y;
       z.beg = parts;
-      a.splits[atomicAdd(&s_splits, 1u)] = z;
+      const uint32_t split = atomicAdd(&s_splits, 1u);
+      if (split < a.max_splits) a.splits[split] = z;
     }
     for (uint32_t p = 0; p < parts; ++p) {
       y.beg = p * each < tiles ? p * each : tiles;
       y.end = y.beg + each < tiles ? y.beg + each : tiles;
-      if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap)
+      if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap; so above)
       if (parts > 1) ++y.part;
     }
   });
-  if (tid == 0) a.counts[1] = s_splits;
+  if (tid == 0) a.counts[1] = s_splits < a.max_splits ? s_splits : a.max_splits;
   if (tid < kPromptQueues) a.counts[2 + tid] = a.first_tickets;
 }
 

@@ -210,7 +210,7 @@ struct AttnPromptArgs {
   float* part_ml;           // [part][kv_heads][part_rows][2]: reference point (base 2), sum
   uint32_t part_rows;       // query rows of a unit that there may be
   uint32_t first_tickets;   // what a queue's tickets begin with
-  uint32_t max_items;
+  uint32_t max_items, max_splits;
   uint32_t tokens, group;
   float scale_log2;         // |scale| log2(e)
   uint32_t flip;            // 0x80008000 where the scale is negative: q's signs

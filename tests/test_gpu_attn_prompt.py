@@ -375,3 +375,19 @@ def test_list_captured():
             results.append(p.read())
         assert all(np.array_equal(results[0], x) for x in results[1:])
         p.check(results[0], [0, 8, 59, 64, 130, -1])
+
+
+def test_list_overlapping_rows():
+    """Which is not allowed: what comes out is anything, and places of no row stay."""
+    say("list, rows that overlap")
+    rng = np.random.default_rng(20)
+    p = Prompt(rng, [2] + [0] * 39, [6400] + [3000] * 39, 2, 2, 64, 16, pad=1)
+    p.starts = np.array([0, 2] * 20 + [0], np.uint32)
+    p.lens[:] = 3000
+    p.lens[0] = 6402
+    up = ca.Buffer.from_array
+    o = up(np.full((4, 2, 64), MARK, np.uint16))
+    kv = p.cache.upload()
+    keep = [up(p.q), up(p.starts), up(p.lens.astype(np.uint32)), ca.Buffer(ca.attn_prompt_plan(kv, 3, 2))]
+    ca.attn_prompt_bf16(kv, keep[0], keep[1], keep[2], o, 3, 2, p.scale, keep[3])
+    assert np.all(o.read(np.uint16, (4, 2, 64))[2:] == MARK)
