@@ -74,8 +74,8 @@ int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_head
   if (!p->list) return CATENA_OK;
   p->items = p->units + kPromptParts;
   p->splits = (uint32_t)std::min<uint64_t>(units, std::max(1u, kPromptParts / 2 / kv_heads));
-  p->part_rows = (uint32_t)std::min<uint64_t>(256, tokens * group);
-  p->splits_at = 64 + (uint64_t)p->items * sizeof(PromptItem);
+  p->part_rows = (uint32_t)std::min<uint64_t>(kPromptNarrow, tokens * group);
+  p->splits_at = kPromptCountBytes + (uint64_t)p->items * sizeof(PromptItem);
   p->ml_at = p->splits_at + (uint64_t)p->splits * sizeof(PromptItem);
   p->o_at = p->ml_at + (uint64_t)kPromptParts * p->part_rows * 8;
   p->bytes = p->o_at + (uint64_t)kPromptParts * p->part_rows * head_dim * 4;
@@ -89,19 +89,19 @@ int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* works
   void* args[] = {&a};
   if (!p.list) return launch(id, dim3(p.units * a.kv.kv_heads), dim3(512), lds, args);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  a.counts = reinterpret_cast<uint32_t*>(ws);
-  a.items = reinterpret_cast<PromptItem*>(ws + 64);
+  static_assert(sizeof(PromptCounts) <= kPromptCountBytes, "the list's place");
+  a.counts = reinterpret_cast<PromptCounts*>(ws);
+  a.items = reinterpret_cast<PromptItem*>(ws + kPromptCountBytes);
   a.splits = reinterpret_cast<PromptItem*>(ws + p.splits_at);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml_at);
   a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   a.part_rows = p.part_rows;
-  a.first_tickets = kPromptCus / kPromptQueues;
   a.max_items = p.items;
   a.max_splits = p.splits;
   int st = launch(paged ? KernelId::AttnPromptList : KernelId::AttnPackedList, dim3(1), dim3(1024), 0, args);
   if (!st) st = launch(id, dim3(kPromptCus), dim3(512), lds, args);
   if (st) return st;
-  return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(p.splits, a.kv.kv_heads, 8),
+  return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(std::min(p.splits, std::max(1u, 256 / a.kv.kv_heads)), a.kv.kv_heads, 8),
                 dim3(256), 0, args);
 }
 // The scale as the kernels take it: above 0, a negative one's sign to q

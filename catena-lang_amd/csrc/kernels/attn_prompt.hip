@@ -50,8 +50,8 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kEase = 40.0f;
 constexpr int kWaves = 8;
-constexpr uint32_t kRows = 32 * kWaves;  // query rows of a unit
-constexpr uint32_t kNarrow = 64;         // of so many a narrow unit
+constexpr uint32_t kRows = kPromptRows, kNarrow = kPromptNarrow, kWidePlaces = kRows / kNarrow;
+static_assert(kRows == 32 * kWaves, "a wave's query rows");
 constexpr int kKeys = 64;                // slots of a tile
 constexpr int kStages = 3;               // tiles of K, and of V, in LDS
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -478,7 +478,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         for (int i = 0; i < 4; ++i) oo[i] = oo[i] + y[i] * f;
       }
       if (it.part != kPromptWhole) {
-        const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh) * a.part_rows + row;
+        const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh) * a.part_rows + row;  // (places of one head's)
         if (d == 0) {
           a.part_ml[2 * at] = mm;
           a.part_ml[2 * at + 1] = ll;
@@ -619,7 +619,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   l = l + __shfl_xor(l, 32);
   if (!live) return;
   if (it.part != kPromptWhole) {
-    const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh) * a.part_rows + wave * 32 + c;
+    const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh * kWidePlaces) * a.part_rows + wave * 32 + c;
     if (h == 0) {
       a.part_ml[2 * at] = m;
       a.part_ml[2 * at + 1] = l;
@@ -652,21 +652,41 @@ CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
     if (it.row != 0xFFFFFFFFu) attn_prompt_item<D, PAGED>(a, it, blockIdx.x % a.kv.kv_heads, a.kv.k, a.kv.v);
     return;
   }
-  // Work n of the list is kv head n % kv_heads of item n / kv_heads.  A workgroup's first is its own number; then it
-  // takes tickets of the eight queues' one that its number falls to: workgroups of one queue run on one XCD, whose
-  // L2 then holds the K and V of few heads.  (Each queue has every eighth work, so they end alike.)
+  // The list is two, of the rows with wide units and of the narrow ones, which some of the workgroups begin with; who
+  // finds no more of one kind goes on with the other.  Work n of a kind is kv head n % kv_heads of its item n /
+  // kv_heads, by tickets of eight queues: workgroups of one queue run on one XCD, whose L2 then holds the K and V of
+  // few heads.  (Each queue has every eighth work, so they end alike.)
   __shared__ uint32_t s_ticket;
-  const uint32_t all = a.counts[0] * a.kv.kv_heads, queue = blockIdx.x % kPromptQueues;
-  for (uint32_t n = blockIdx.x; n < all;) {
-    uint32_t ticket = 0;
-    if (threadIdx.x == 0) ticket = atomicAdd(a.counts + 2 + queue, 1u);
-    const u32x4_t x = scalar_four(a.items, 2 * (uint64_t)(n / a.kv.kv_heads)), y = scalar_four(a.items, 2 * (uint64_t)(n / a.kv.kv_heads) + 1);
+  const uint32_t queue = blockIdx.x % kPromptQueues, place = blockIdx.x / kPromptQueues;
+  const uint32_t items = scalar_word(&a.counts->items, 0), wide = scalar_word(&a.counts->wide, 0);
+  const uint32_t first = kPromptCus / kPromptQueues - scalar_word(&a.counts->narrow_first, 0);  // narrow from this place on
+  uint32_t kind = place >= first, ticket = kind ? place - first : place;
+  auto next = [&](uint32_t t) {  // a ticket's work, its item; false: no more of the kind
+    const uint32_t n = t * kPromptQueues + queue;
+    return n < (kind ? items - wide : wide) * a.kv.kv_heads ? n : 0xFFFFFFFFu;
+  };
+  auto draw = [&] { return threadIdx.x == 0 ? atomicAdd(&a.counts->tickets[kind][queue], 1u) : 0u; };
+  auto share = [&](uint32_t t) {
+    __syncthreads();  // the last ticket has been read
+    if (threadIdx.x == 0) s_ticket = t;
+    __syncthreads();
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)s_ticket);
+  };
+  uint32_t n = next(ticket);
+  for (bool other = false;;) {
+    if (n == 0xFFFFFFFFu) {
+      if (other) return;
+      other = true;
+      kind ^= 1u;
+      n = next(share(draw()));
+      continue;
+    }
+    const uint32_t t = draw();
+    const uint64_t at = 2 * ((uint64_t)(kind ? wide : 0u) + n / a.kv.kv_heads);
+    const u32x4_t x = scalar_four(a.items, at), y = scalar_four(a.items, at + 1);
     const PromptItem it{x[0], x[1], x[2], x[3], (int32_t)y[0], y[1], y[2], y[3]};
     attn_prompt_item<D, PAGED>(a, it, n % a.kv.kv_heads, a.kv.k, a.kv.v);
-    __syncthreads();  // the last ticket has been read
-    if (threadIdx.x == 0) s_ticket = ticket;
-    __syncthreads();
-    n = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_ticket) * kPromptQueues + queue;
+    n = next(share(t));
   }
 }
 
@@ -681,9 +701,11 @@ CATENA_DEV uint32_t last_at_most(const uint32_t* s, uint32_t n, uint32_t x) {
 // The list: one workgroup of 1024 threads.  A unit costs its tiles, a narrow one, which waits for memory beside
 // the others' products, half of them; one of more than three quarters of a CU's share of all the work
 // is cut into equal parts.
-// Rows stand in the order of their dearest unit's cost, in 64 classes, and a row's units behind each other, the
+// Rows stand in the order of their dearest unit's cost, in 32 classes, and a row's units behind each other, the
 // last (longest) first: so the short ones end the work, and the workgroups of an XCD read the same K and V at a time
-// (8 ragged prompts of up to 4096 tokens: units by length alone 645 us, by rows 486).
+// (8 ragged prompts of up to 4096 tokens: units by length alone 645 us, by rows 486).  Rows of one narrow unit stand
+// behind the others, in classes of their own: they wait for memory, the others for the matrix cores, so that both are
+// worked on at a time.
 // Which of two rows of a class comes first, and which place a part gets, is left to the order of the threads: no
 // result depends on it.
 template <bool PAGED>
@@ -691,11 +713,11 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
   constexpr uint32_t kThreads = 1024, kClasses = 64;
   __shared__ uint32_t s_start[kThreads], s_first[kThreads], s_n[kThreads], s_old[kThreads], s_at[kThreads], s_wave[16];
   __shared__ uint32_t s_class[kClasses], s_parts, s_splits;
-  __shared__ unsigned long long s_work;
+  __shared__ unsigned long long s_work, s_narrow;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   if (tid < kClasses) s_class[tid] = 0;
   if (tid == 0) {
-    s_work = 0;
+    s_work = s_narrow = 0;
     s_parts = s_splits = 0;
   }
   struct Row {
@@ -705,11 +727,12 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
   };
   struct Cost {
     uint32_t tiles, cost;
+    bool narrow;
   };
   auto cost_of = [&](uint32_t unit, uint32_t n, int32_t old) {
     const uint32_t tiles = tiles_of(most_of(a, unit, n, old));
     const bool narrow = n * a.group - unit * kRows <= kNarrow;
-    return Cost{tiles, narrow ? tiles : 2 * tiles};
+    return Cost{tiles, narrow ? tiles : 2 * tiles, narrow};
   };
   // Every row to a thread, 1024 at a time: of_row(row); then every unit of theirs to one: of_unit(row, its place
   // among the 1024, unit).  Where there are no more rows than that they are looked at once.
@@ -745,50 +768,65 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       __syncthreads();
     }
   };
-  uint64_t mine = 0;
+  auto alone = [&](uint32_t n) { return n * a.group <= kNarrow; };  // a row of one narrow unit
+  uint64_t mine = 0, narrow = 0;
   every([](const Row&) { return 0u; }, [&](uint32_t, uint32_t at, uint32_t unit) {
-    mine += cost_of(unit, s_n[at], (int32_t)s_old[at]).cost;
+    const uint32_t cost = cost_of(unit, s_n[at], (int32_t)s_old[at]).cost;
+    mine += cost;
+    narrow += alone(s_n[at]) ? cost : 0u;
   });
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
+  for (int d = 1; d < 64; d *= 2) {
+    mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
+    narrow += (uint64_t)__shfl_xor((unsigned long long)narrow, d);
+  }
   if (lane == 0 && mine) atomicAdd(&s_work, (unsigned long long)mine);
+  if (lane == 0 && narrow) atomicAdd(&s_narrow, (unsigned long long)narrow);
   __syncthreads();
-  // (a cut unit costs more than `most`, so the parts of all heads are fewer than 2 work / most < kPromptParts)
+  // (a cut unit costs more than the most of its kind, so the parts of all heads are fewer than 2 wide / most + 2 narrow /
+  // most_narrow; that is 8 / 3 CUs' places for the wide ones' work, and with most_narrow >= 0.9 most / 4 no more than 12
+  // for the narrow ones': fewer than kPromptParts)
   const uint64_t work = s_work * a.kv.kv_heads, share = 3 * work / (4 * kPromptCus) + 1;
   const uint32_t most = share < kPromptLeast ? kPromptLeast : share < 0x7FFFFFFFull ? (uint32_t)share : 0x7FFFFFFFu;
-  auto parts_of = [&](uint32_t cost) { return cost <= most ? 1u : (cost + most - 1) / most; };
+  // A narrow unit's parts have next to nothing to join, and the work ends more evenly with small ones behind the others
+  const uint32_t most_narrow = most / 4 < kPromptLeast / 2 ? kPromptLeast / 2 : most / 4;
+  auto most_for = [&](const Cost& x) { return x.narrow ? most_narrow : most; };
+  auto parts_of = [&](const Cost& x) { return x.cost <= most_for(x) ? 1u : (x.cost + most_for(x) - 1) / most_for(x); };
   // items of a row's units from `unit` on: of the wide units only the last ones are cut
   auto items_from = [&](uint32_t unit, uint32_t units, uint32_t n, int32_t old) {
     uint32_t items = units - unit;
     for (uint32_t u = units; u > unit; --u) {
-      const uint32_t parts = parts_of(cost_of(u - 1, n, old).cost);
+      const uint32_t parts = parts_of(cost_of(u - 1, n, old));
       if (parts == 1 && u < units) break;
       items += parts - 1;
     }
     return items;
   };
   auto place_of = [&](const Row& r) {
-    uint32_t cost = cost_of(r.units - 1, r.t.n, r.old).cost;
-    if (r.units > 1) cost = max(cost, cost_of(r.units - 2, r.t.n, r.old).cost);
-    const uint32_t at = (uint32_t)((uint64_t)(most - (cost < most ? cost : most)) * (kClasses - 1) / most);
+    const Cost last = cost_of(r.units - 1, r.t.n, r.old);
+    uint32_t cost = min(last.cost, most_for(last));
+    if (r.units > 1) cost = max(cost, min(cost_of(r.units - 2, r.t.n, r.old).cost, most));
+    const uint32_t at = (uint32_t)((uint64_t)(most - cost) * (kClasses / 2 - 1) / most) + (alone(r.t.n) ? kClasses / 2 : 0u);
     return atomicAdd(&s_class[at], items_from(0, r.units, r.t.n, r.old));
   };
   every(place_of, [](uint32_t, uint32_t, uint32_t) {});
   if (tid < 64) {
     const uint32_t n = s_class[tid], upto = wave_prefix(n);
     s_class[tid] = upto - n;
-    if (tid == 63) a.counts[0] = upto < a.max_items ? upto : a.max_items;
+    if (tid == kClasses / 2 - 1) a.counts->wide = upto < a.max_items ? upto : a.max_items;
+    if (tid == kClasses - 1) a.counts->items = upto < a.max_items ? upto : a.max_items;
   }
   __syncthreads();
   every(place_of, [&](uint32_t row, uint32_t place, uint32_t unit) {
     const uint32_t n = s_n[place];
     const int32_t old = (int32_t)s_old[place];
     const Cost cost = cost_of(unit, n, old);
-    const uint32_t tiles = cost.tiles, parts = parts_of(cost.cost), each = (tiles + parts - 1) / parts;
+    const uint32_t tiles = cost.tiles, parts = parts_of(cost), each = (tiles + parts - 1) / parts;
     const uint32_t at = s_at[place] + items_from(unit + 1, units_of(a, n), n, old);
     PromptItem y{row, unit, s_first[place], n, old, 0, tiles, kPromptWhole};
     if (parts > 1) {
-      y.part = atomicAdd(&s_parts, parts);
+      const uint32_t places = cost.narrow ? 1u : kWidePlaces;
+      y.part = atomicAdd(&s_parts, parts * places);
       PromptItem z = y;
       z.beg = parts;
       const uint32_t split = atomicAdd(&s_splits, 1u);
@@ -798,43 +836,54 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       y.beg = p * each < tiles ? p * each : tiles;
       y.end = y.beg + each < tiles ? y.beg + each : tiles;
       if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap; so above)
-      if (parts > 1) ++y.part;
+      if (parts > 1) y.part += cost.narrow ? 1u : kWidePlaces;
     }
   });
-  if (tid == 0) a.counts[1] = s_splits < a.max_splits ? s_splits : a.max_splits;
-  if (tid < kPromptQueues) a.counts[2 + tid] = a.first_tickets;
+  // Of a queue's workgroups three quarters of the narrow rows' share begin with them, so that wide units, of which
+  // the parts are larger, do not end the work
+  constexpr uint32_t kPlaces = kPromptCus / kPromptQueues;
+  const uint32_t some = s_work ? (uint32_t)(3 * s_narrow * kPlaces / (4 * s_work)) : 0u;
+  const uint32_t first = s_narrow == 0 ? 0u : s_narrow == s_work ? kPlaces : some < 1 ? 1u : some;
+  if (tid == 0) {
+    a.counts->splits = s_splits < a.max_splits ? s_splits : a.max_splits;
+    a.counts->narrow_first = first;
+  }
+  if (tid < 2 * kPromptQueues) a.counts->tickets[tid / kPromptQueues][tid % kPromptQueues] = tid / kPromptQueues ? first : kPlaces - first;
 }
 
-// A unit's parts to o: blockIdx.x the split, blockIdx.y the kv head, blockIdx.z in turns of 256 / (D / 4) query rows;
-// a thread four columns
+// The parts of cut units to o: blockIdx.x, in turn, the units, blockIdx.y the kv head, blockIdx.z in turns of 256 / (D /
+// 4) query rows; a thread four columns
 template <int D>
 CATENA_DEV void attn_prompt_join(const AttnPromptArgs& a) {
-  if (blockIdx.x >= a.counts[1]) return;
-  const PromptItem x = a.splits[blockIdx.x];
-  constexpr uint32_t kLanes = D / 4, kAtOnce = 256 / kLanes;
-  const uint32_t kvh = blockIdx.y, heads = a.group * a.kv.kv_heads, d = threadIdx.x % kLanes * 4;
-  for (uint32_t row = blockIdx.z * kAtOnce + threadIdx.x / kLanes; row < kRows; row += gridDim.z * kAtOnce) {
-    const uint32_t m_row = x.unit * kRows + row, t = m_row / a.group;
-    if (t >= x.n) return;
-    float m = kNegInf, l = 0.0f;
-    f32x4_t o = {0, 0, 0, 0};
+  const uint32_t splits = a.counts->splits;
+  for (uint32_t split = blockIdx.x; split < splits; split += gridDim.x) {
+    const PromptItem x = a.splits[split];
+    constexpr uint32_t kLanes = D / 4, kAtOnce = 256 / kLanes;
+    const uint32_t kvh = blockIdx.y, heads = a.group * a.kv.kv_heads, d = threadIdx.x % kLanes * 4;
+    const uint32_t places = x.n * a.group - x.unit * kRows <= kNarrow ? 1u : kWidePlaces;
+    for (uint32_t row = blockIdx.z * kAtOnce + threadIdx.x / kLanes; row < kRows; row += gridDim.z * kAtOnce) {
+      const uint32_t m_row = x.unit * kRows + row, t = m_row / a.group;
+      if (t >= x.n) break;
+      float m = kNegInf, l = 0.0f;
+      f32x4_t o = {0, 0, 0, 0};
 #pragma unroll 4
-    for (uint32_t p = 0; p < x.beg; ++p) {
-      const uint64_t at = ((uint64_t)(x.part + p) * a.kv.kv_heads + kvh) * a.part_rows + row;
-      const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
-      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
-      const float m2 = __builtin_fmaxf(m, pm);
-      const float f = weight(m, m2), e = weight(pm, m2);
-      m = m2;
-      l = l * f + pl * e;
+      for (uint32_t p = 0; p < x.beg; ++p) {
+        const uint64_t at = ((uint64_t)(x.part + p * places) * a.kv.kv_heads + kvh * places) * a.part_rows + row;
+        const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
+        const float m2 = __builtin_fmaxf(m, pm);
+        const float f = weight(m, m2), e = weight(pm, m2);
+        m = m2;
+        l = l * f + pl * e;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * f + y[i] * e;
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * f + y[i] * e;
+      }
+      const float by = x.old + (int32_t)t + 1 > 0 ? l : 1.0f;
+      uint2 w;
+      w.x = pack_bf16x2(o[0] / by, o[1] / by);
+      w.y = pack_bf16x2(o[2] / by, o[3] / by);
+      *reinterpret_cast<uint2*>(a.o + ((uint64_t)(x.first + t) * heads + kvh * a.group + m_row % a.group) * D + d) = w;
     }
-    const float by = x.old + (int32_t)t + 1 > 0 ? l : 1.0f;
-    uint2 w;
-    w.x = pack_bf16x2(o[0] / by, o[1] / by);
-    w.y = pack_bf16x2(o[2] / by, o[3] / by);
-    *reinterpret_cast<uint2*>(a.o + ((uint64_t)(x.first + t) * heads + kvh * a.group + m_row % a.group) * D + d) = w;
   }
 }
 

@@ -187,8 +187,9 @@ struct RopePackedArgs {
 constexpr uint32_t kPromptWhole = 0xFFFFFFFFu;  // an item that is all of its unit
 constexpr uint32_t kPromptQueues = 8;           // one an XCD
 constexpr uint32_t kPromptCus = 256;
-constexpr uint32_t kPromptLeast = 32;           // what a unit costs that is not cut (two a tile of 64 slots)
-constexpr uint32_t kPromptParts = 4 * kPromptCus;  // parts there may be, of all kv heads
+constexpr uint32_t kPromptRows = 256, kPromptNarrow = 64;  // query rows of a unit; of so many a narrow one
+constexpr uint32_t kPromptLeast = 32;              // what a unit costs that is not cut (two a tile of 64 slots)
+constexpr uint32_t kPromptParts = 16 * kPromptCus;  // places of kPromptNarrow query rows for the parts of all kv heads
 // 256 query rows (unit `unit`) of a row's n new tokens, `old` slots in front of them: tiles [beg, end) of what they
 // see.  In the list of cut units: beg is the number of parts, `part` the first one.
 struct PromptItem {
@@ -196,6 +197,13 @@ struct PromptItem {
   int32_t old;
   uint32_t beg, end, part;
 };
+struct PromptCounts {
+  uint32_t items, wide;   // of the list; of them, in front, those of rows with wide units
+  uint32_t splits;
+  uint32_t narrow_first;  // of a queue's workgroups so many begin with the others
+  uint32_t tickets[2][kPromptQueues];  // taken of each kind
+};
+constexpr uint32_t kPromptCountBytes = 128;  // in the workspace, in front of the list
 struct AttnPromptArgs {
   PagedKv kv;               // table null: k, v [tokens][kv_heads][head_dim], stride apart
   const uint16_t* q;        // [tokens][heads][D]
@@ -205,11 +213,12 @@ struct AttnPromptArgs {
   uint64_t stride;          // elements from a token's k to the next one's, without a table
   PromptItem* items;        // the list; null: a workgroup a unit
   PromptItem* splits;       // units that were cut
-  uint32_t* counts;         // items, splits, tickets taken of each queue
-  float* part_o;            // [part][kv_heads][part_rows][D]
-  float* part_ml;           // [part][kv_heads][part_rows][2]: reference point (base 2), sum
-  uint32_t part_rows;       // query rows of a unit that there may be
-  uint32_t first_tickets;   // what a queue's tickets begin with
+  PromptCounts* counts;
+  // part_rows query rows a place, as many as there may be up to kPromptNarrow; a part has one for each kv head, or, of
+  // a wide unit, kPromptRows / kPromptNarrow
+  float* part_o;            // [place][part_rows][D]
+  float* part_ml;           // [place][part_rows][2]: reference point (base 2), sum
+  uint32_t part_rows;
   uint32_t max_items, max_splits;
   uint32_t tokens, group;
   float scale_log2;         // |scale| log2(e)
