@@ -101,7 +101,7 @@ int prompt_launch(AttnPromptArgs a, bool paged, const PromptPlan& p, void* works
   int st = launch(paged ? KernelId::AttnPromptList : KernelId::AttnPackedList, dim3(1), dim3(1024), 0, args);
   if (!st) st = launch(id, dim3(kPromptCus), dim3(512), lds, args);
   if (st) return st;
-  return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(std::min(p.splits, std::max(1u, 256 / a.kv.kv_heads)), a.kv.kv_heads, 8),
+  return launch(d64 ? KernelId::AttnPromptJoinD64 : KernelId::AttnPromptJoinD128, dim3(std::min(p.splits, std::max(1u, 256 / a.kv.kv_heads)), a.kv.kv_heads, 16),
                 dim3(256), 0, args);
 }
 // The scale as the kernels take it: above 0, a negative one's sign to q

@@ -734,64 +734,15 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
     const bool narrow = n * a.group - unit * kRows <= kNarrow;
     return Cost{tiles, narrow ? tiles : 2 * tiles, narrow};
   };
-  // Every row to a thread, 1024 at a time: of_row(row); then every unit of theirs to one: of_unit(row, its place
-  // among the 1024, unit).  Where there are no more rows than that they are looked at once.
-  Row x;
-  uint32_t all = 0;
-  bool known = false;
-  auto every = [&](auto of_row, auto of_unit) {
-    for (uint32_t r0 = 0; r0 < a.kv.rows; r0 += kThreads) {
-      if (!known || a.kv.rows > kThreads) {
-        known = true;
-        const uint32_t row = r0 + tid < a.kv.rows ? r0 + tid : a.kv.rows - 1;
-        x.t = tokens_of(a, row);
-        x.t.n = r0 + tid < a.kv.rows ? x.t.n : 0u;
-        x.old = old_of<PAGED>(a, row, x.t.n);
-        x.units = units_of(a, x.t.n);
-        const uint32_t in = wave_prefix(x.units);
-        if (lane == 63) s_wave[wave] = in;
-        __syncthreads();
-        const uint32_t sums = wave_prefix(lane < 16 ? s_wave[lane] : 0u);
-        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave);
-        all = lane_of(sums, 15);
-        s_start[tid] = (w ? lane_of(sums, w - 1) : 0u) + in - x.units;  // (rows without units are never the last one at most)
-        s_first[tid] = x.t.first;
-        s_n[tid] = x.t.n;
-        s_old[tid] = (uint32_t)x.old;
-      }
-      if (x.units > 0) s_at[tid] = of_row(x);
-      __syncthreads();
-      for (uint32_t k = tid; k < all; k += kThreads) {
-        const uint32_t at = last_at_most(s_start, kThreads, k);
-        of_unit(r0 + at, at, k - s_start[at]);
-      }
-      __syncthreads();
-    }
-  };
   auto alone = [&](uint32_t n) { return n * a.group <= kNarrow; };  // a row of one narrow unit
-  uint64_t mine = 0, narrow = 0;
-  every([](const Row&) { return 0u; }, [&](uint32_t, uint32_t at, uint32_t unit) {
-    const uint32_t cost = cost_of(unit, s_n[at], (int32_t)s_old[at]).cost;
-    mine += cost;
-    narrow += alone(s_n[at]) ? cost : 0u;
-  });
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
-    narrow += (uint64_t)__shfl_xor((unsigned long long)narrow, d);
-  }
-  if (lane == 0 && mine) atomicAdd(&s_work, (unsigned long long)mine);
-  if (lane == 0 && narrow) atomicAdd(&s_narrow, (unsigned long long)narrow);
-  __syncthreads();
-  // (a cut unit costs more than the most of its kind, so the parts of all heads are fewer than 2 wide / most + 2 narrow /
-  // most_narrow; that is 8 / 3 CUs' places for the wide ones' work, and with most_narrow >= 0.9 most / 4 no more than 12
-  // for the narrow ones': fewer than kPromptParts)
-  const uint64_t work = s_work * a.kv.kv_heads, share = 3 * work / (4 * kPromptCus) + 1;
-  const uint32_t most = share < kPromptLeast ? kPromptLeast : share < 0x7FFFFFFFull ? (uint32_t)share : 0x7FFFFFFFu;
-  // A narrow unit's parts have next to nothing to join, and the work ends more evenly with small ones behind the others
-  const uint32_t most_narrow = most / 4 < kPromptLeast / 2 ? kPromptLeast / 2 : most / 4;
+  // What a unit costs that is not cut.  A narrow unit's parts have next to nothing to join, and the work ends more
+  // evenly with small ones behind the others.
+  uint32_t most = 0, most_narrow = 0;
+  float share = 0.0f, share_narrow = 0.0f;  // 1 / most
   auto most_for = [&](const Cost& x) { return x.narrow ? most_narrow : most; };
-  auto parts_of = [&](const Cost& x) { return x.cost <= most_for(x) ? 1u : (x.cost + most_for(x) - 1) / most_for(x); };
+  auto parts_of = [&](const Cost& x) {  // (a rounding may make a part a little larger or smaller, the same for all who ask)
+    return x.cost <= most_for(x) ? 1u : (uint32_t)((float)(x.cost - 1) * (x.narrow ? share_narrow : share)) + 1;
+  };
   // items of a row's units from `unit` on: of the wide units only the last ones are cut
   auto items_from = [&](uint32_t unit, uint32_t units, uint32_t n, int32_t old) {
     uint32_t items = units - unit;
@@ -806,22 +757,13 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
     const Cost last = cost_of(r.units - 1, r.t.n, r.old);
     uint32_t cost = min(last.cost, most_for(last));
     if (r.units > 1) cost = max(cost, min(cost_of(r.units - 2, r.t.n, r.old).cost, most));
-    const uint32_t at = (uint32_t)((uint64_t)(most - cost) * (kClasses / 2 - 1) / most) + (alone(r.t.n) ? kClasses / 2 : 0u);
-    return atomicAdd(&s_class[at], items_from(0, r.units, r.t.n, r.old));
+    const uint32_t from = (uint32_t)((float)(most - cost) * share * (kClasses / 2 - 1));
+    return atomicAdd(&s_class[from + (alone(r.t.n) ? kClasses / 2 : 0u)], items_from(0, r.units, r.t.n, r.old));
   };
-  every(place_of, [](uint32_t, uint32_t, uint32_t) {});
-  if (tid < 64) {
-    const uint32_t n = s_class[tid], upto = wave_prefix(n);
-    s_class[tid] = upto - n;
-    if (tid == kClasses / 2 - 1) a.counts->wide = upto < a.max_items ? upto : a.max_items;
-    if (tid == kClasses - 1) a.counts->items = upto < a.max_items ? upto : a.max_items;
-  }
-  __syncthreads();
-  every(place_of, [&](uint32_t row, uint32_t place, uint32_t unit) {
+  auto put = [&](uint32_t row, uint32_t place, uint32_t unit, const Cost& cost) {
     const uint32_t n = s_n[place];
     const int32_t old = (int32_t)s_old[place];
-    const Cost cost = cost_of(unit, n, old);
-    const uint32_t tiles = cost.tiles, parts = parts_of(cost), each = (tiles + parts - 1) / parts;
+    const uint32_t tiles = cost.tiles, parts = parts_of(cost), each = parts > 1 ? (tiles + parts - 1) / parts : tiles;
     const uint32_t at = s_at[place] + items_from(unit + 1, units_of(a, n), n, old);
     PromptItem y{row, unit, s_first[place], n, old, 0, tiles, kPromptWhole};
     if (parts > 1) {
@@ -838,11 +780,78 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap; so above)
       if (parts > 1) y.part += cost.narrow ? 1u : kWidePlaces;
     }
-  });
+  };
+  // Three times (pass: the costs' sum, the classes' sizes, the list) every row to a thread, 1024 at a time, and every
+  // unit of theirs to one.  Where there are no more rows than that they are looked at once.  (A loop, since code that
+  // runs once waits for its instructions.)
+  Row x;
+  uint32_t all = 0;
+  uint64_t mine = 0, narrow = 0;
+#pragma clang loop unroll(disable)
+  for (uint32_t pass = 0; pass < 3; ++pass) {
+    for (uint32_t r0 = 0; r0 < a.kv.rows; r0 += kThreads) {
+      if (pass == 0 || a.kv.rows > kThreads) {
+        const uint32_t row = r0 + tid < a.kv.rows ? r0 + tid : a.kv.rows - 1;
+        x.t = tokens_of(a, row);
+        x.t.n = r0 + tid < a.kv.rows ? x.t.n : 0u;
+        x.old = old_of<PAGED>(a, row, x.t.n);
+        x.units = units_of(a, x.t.n);
+        const uint32_t in = wave_prefix(x.units);
+        if (lane == 63) s_wave[wave] = in;
+        __syncthreads();
+        const uint32_t sums = wave_prefix(lane < 16 ? s_wave[lane] : 0u);
+        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave);
+        all = lane_of(sums, 15);
+        s_start[tid] = (w ? lane_of(sums, w - 1) : 0u) + in - x.units;  // (rows without units are never the last one at most)
+        s_first[tid] = x.t.first;
+        s_n[tid] = x.t.n;
+        s_old[tid] = (uint32_t)x.old;
+      }
+      if (pass > 0 && x.units > 0) s_at[tid] = place_of(x);
+      __syncthreads();
+      for (uint32_t k = pass == 1 ? all : tid; k < all; k += kThreads) {
+        const uint32_t at = last_at_most(s_start, kThreads, k), unit = k - s_start[at];
+        const Cost cost = cost_of(unit, s_n[at], (int32_t)s_old[at]);
+        if (pass == 0) {
+          mine += cost.cost;
+          narrow += alone(s_n[at]) ? cost.cost : 0u;
+        } else {
+          put(r0 + at, at, unit, cost);
+        }
+      }
+      __syncthreads();
+    }
+    if (pass == 0) {
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
+        narrow += (uint64_t)__shfl_xor((unsigned long long)narrow, d);
+      }
+      if (lane == 0 && mine) atomicAdd(&s_work, (unsigned long long)mine);
+      if (lane == 0 && narrow) atomicAdd(&s_narrow, (unsigned long long)narrow);
+      __syncthreads();
+      // (a cut unit costs more than the most of its kind, so the parts of all heads are fewer than 2 wide / most + 2
+      // narrow / most_narrow; that is 8 / 3 CUs' places for the wide ones' work, and with most_narrow >= 0.9 most / 4 no
+      // more than 12 for the narrow ones': fewer than kPromptParts)
+      const uint64_t work = s_work * a.kv.kv_heads, even = 3 * work / (4 * kPromptCus) + 1;
+      most = even < kPromptLeast ? kPromptLeast : even < 0x7FFFFFFFull ? (uint32_t)even : 0x7FFFFFFFu;
+      most_narrow = most / 4 < kPromptLeast / 2 ? kPromptLeast / 2 : most / 4;
+      share = 1.0f / (float)most;
+      share_narrow = 1.0f / (float)most_narrow;
+    } else if (pass == 1) {
+      if (tid < 64) {
+        const uint32_t n = s_class[tid], upto = wave_prefix(n);
+        s_class[tid] = upto - n;
+        if (tid == kClasses / 2 - 1) a.counts->wide = upto < a.max_items ? upto : a.max_items;
+        if (tid == kClasses - 1) a.counts->items = upto < a.max_items ? upto : a.max_items;
+      }
+      __syncthreads();
+    }
+  }
   // Of a queue's workgroups three quarters of the narrow rows' share begin with them, so that wide units, of which
   // the parts are larger, do not end the work
   constexpr uint32_t kPlaces = kPromptCus / kPromptQueues;
-  const uint32_t some = s_work ? (uint32_t)(3 * s_narrow * kPlaces / (4 * s_work)) : 0u;
+  const uint32_t some = s_work ? (uint32_t)(0.75f * kPlaces * (float)s_narrow / (float)s_work) : 0u;
   const uint32_t first = s_narrow == 0 ? 0u : s_narrow == s_work ? kPlaces : some < 1 ? 1u : some;
   if (tid == 0) {
     a.counts->splits = s_splits < a.max_splits ? s_splits : a.max_splits;
