@@ -138,9 +138,11 @@ CATENA_DEV PromptItem item_at(const AttnPromptArgs& a, uint32_t index) {
 
 // (the pools as arguments that nothing else points into: the compiler then does not make reads of LDS wait for
 // the loads into it, whose order the barriers below give)
-template <int D, bool PAGED>
+// put, get: called by all threads with a barrier between, get in front of the last stores, to look ahead
+template <int D, bool PAGED, class Put, class Get>
 CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, uint32_t kvh,
-                                 const uint16_t* __restrict__ pool_k, const uint16_t* __restrict__ pool_v) {
+                                 const uint16_t* __restrict__ pool_k, const uint16_t* __restrict__ pool_v,
+                                 const Put& put, const Get& get) {
   constexpr int KS = D / 16;        // steps of a score's sum
   constexpr int DB = D / 32;        // blocks of o's columns
   constexpr int kTile = kKeys * D;  // elements of K or V of a tile
@@ -165,32 +167,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   const uint64_t q_at =
       ((uint64_t)(it.first + (live ? t_row : 0u)) * heads + kvh * a.group + (live ? m_row % a.group : 0u)) * D;
   const int32_t sees = live ? it.old + (int32_t)t_row + 1 : 0;  // slots
-  bf16x8_t qf[KS];
-#pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    u32x4_t w = *reinterpret_cast<const u32x4_t*>(a.q + q_at + 16 * i + 8 * h);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] ^= a.flip;
-    qf[i] = __builtin_bit_cast(bf16x8_t, w);
-  }
-  // Of the item's tiles, the first `whole` are seen by all its rows (rows that are not live see none, and need
-  // not) and have their pages
-  const int32_t least = it.old + (int32_t)(it.unit * kRows / a.group) + 1;
-  uint32_t upto = least > 0 ? (uint32_t)least / kKeys : 0u;
-  if constexpr (PAGED) {
-    const uint32_t entries = (uint32_t)(((uint64_t)upto * kKeys + (1u << a.kv.page_shift) - 1) >> a.kv.page_shift);
-    const uint32_t* row = a.kv.table + (uint64_t)it.row * a.kv.max_pages;
-    for (uint32_t e = (it.beg * kKeys) >> a.kv.page_shift; e < entries; e += 64) {
-      const uint64_t gone = __ballot(e + lane < entries && row[e + lane < entries ? e + lane : e] >= a.kv.num_pages);
-      if (gone) {
-        const uint32_t first = e + (uint32_t)__ffsll((unsigned long long)gone) - 1;
-        upto = (first << a.kv.page_shift) / kKeys;
-        break;
-      }
-    }
-  }
   const uint32_t count = it.end - it.beg;
-  const uint32_t whole = upto <= it.beg ? 0u : upto < it.end ? upto - it.beg : count;
   // whether any of the wave's rows is live, and the slots that any of them sees
   const bool awake = w_row / a.group < it.n;
   const uint32_t w_last = (w_row + 31) / a.group;
@@ -249,6 +226,64 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+
+  // The last item's reads of LDS are done with, for all waves
+  auto begin = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // The first loads, before anything waits: a wide unit's first tiles, q
+  uint32_t after = 0;
+  Slots next{0, 0};  // of the tile behind the one worked on
+  if (!narrow) {
+    const uint32_t p0 = look_up(0), p1 = look_up(1);
+    after = look_up(2);
+    next = slots_of(0, p0);
+    begin();
+    if (count > 0) {
+      issue(0, next, 0);
+      issue(0, next, 1);
+    }
+    next = slots_of(1, p1);
+    if (count > 1) issue(1, next, 0);
+  } else {
+    begin();
+  }
+  bf16x8_t qf[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    u32x4_t w = *reinterpret_cast<const u32x4_t*>(a.q + q_at + 16 * i + 8 * h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] ^= a.flip;
+    qf[i] = __builtin_bit_cast(bf16x8_t, w);
+  }
+  // Of the item's tiles, the first `whole` are seen by all its rows (rows that are not live see none, and need
+  // not) and have their pages
+  const int32_t least = it.old + (int32_t)(it.unit * kRows / a.group) + 1;
+  uint32_t upto = least > 0 ? (uint32_t)least / kKeys : 0u;
+  if constexpr (PAGED) {
+    const uint32_t last = upto < it.end ? upto : it.end;
+    const uint32_t entries = (uint32_t)(((uint64_t)last * kKeys + (1u << a.kv.page_shift) - 1) >> a.kv.page_shift);
+    const uint32_t* row = a.kv.table + (uint64_t)it.row * a.kv.max_pages;
+    uint32_t gone = 0xFFFFFFFFu;  // the first one without a page, of the lane's
+    for (uint32_t e = ((it.beg * kKeys) >> a.kv.page_shift) + lane; e < entries; e += 4 * 64) {
+      uint32_t page[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) page[i] = row[e + 64 * i < entries ? e + 64 * i : e];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (page[i] >= a.kv.num_pages) gone = min(gone, e + 64 * i < entries ? e + 64 * i : e);
+    }
+    if (__any(gone != 0xFFFFFFFFu)) {
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) gone = min(gone, (uint32_t)__shfl_xor((int)gone, d));
+      gone = (uint32_t)__builtin_amdgcn_readfirstlane((int)gone);
+      upto = (uint32_t)(((uint64_t)gone << a.kv.page_shift) / kKeys);
+    }
+  }
+  const uint32_t whole = upto <= it.beg ? 0u : upto < it.end ? upto - it.beg : count;
 
   // The query row's exponents' reference point, a whole number (base 2), and from where on a score (in units of the
   // products) raises it; l of the lane's half of the slots
@@ -418,16 +453,16 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     };
     auto fence = [] { asm volatile("" ::: "memory"); };
     uint32_t b = wave / blocks;
-    Pair next = pair_of(b, page_of(slot_of(b)), page_of(slot_of(b) + 16));
+    Pair pair = pair_of(b, page_of(slot_of(b)), page_of(slot_of(b) + 16));
     uint32_t p0 = page_of(slot_of(b + step)), p1 = page_of(slot_of(b + step) + 16);
     if (b < all) {
-      bring(next, 0);
-      bring(next, 1);
+      bring(pair, 0);
+      bring(pair, 1);
     }
 #pragma clang loop unroll(disable)
     for (; b < all; b += step) {
       const bool more = b + step < all;
-      next = pair_of(b + step, p0, p1);
+      pair = pair_of(b + step, p0, p1);
       p0 = page_of(slot_of(b + 2 * step));
       p1 = page_of(slot_of(b + 2 * step) + 16);
       fence();
@@ -436,7 +471,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       const f32x16_t s = block_scores(k, 0);
       fence();
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): K has been read
-      if (more) bring(next, 0);
+      if (more) bring(pair, 0);
       fence();
       if (more)
         __builtin_amdgcn_s_waitcnt(0x0F70 | kBlock);  // all but the next K's
@@ -447,9 +482,10 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       block_rest(s, v, mine + kTile / 2, 0, slot_of(b), slot_of(b) + 32 > upto * kKeys);
       fence();
       __builtin_amdgcn_s_waitcnt(0xC07F);
-      if (more) bring(next, 1);
+      if (more) bring(pair, 1);
     }
     l = l + __shfl_xor(l, 32);
+    put();
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem);
     float* sml = so + kWaves * 32 * D;
@@ -463,6 +499,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       sml[2 * (wave * 32 + c)] = m;
       sml[2 * (wave * 32 + c) + 1] = l;
     }
+    get();
     __syncthreads();
     for (uint32_t id = threadIdx.x; id < rows * (D / 4); id += 64 * kWaves) {
       const uint32_t row = id / (D / 4), d = id % (D / 4) * 4;
@@ -487,10 +524,10 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         continue;
       }
       const uint32_t r = it.unit * kRows + row, t = r / a.group;
-      const float by = it.old + (int32_t)t + 1 > 0 ? ll : 1.0f;
+      const float by = 1.0f / (it.old + (int32_t)t + 1 > 0 ? ll : 1.0f);
       uint2 w;
-      w.x = pack_bf16x2(oo[0] / by, oo[1] / by);
-      w.y = pack_bf16x2(oo[2] / by, oo[3] / by);
+      w.x = pack_bf16x2(oo[0] * by, oo[1] * by);
+      w.y = pack_bf16x2(oo[2] * by, oo[3] * by);
       *reinterpret_cast<uint2*>(a.o + ((uint64_t)(it.first + t) * heads + kvh * a.group + r % a.group) * D + d) = w;
     }
     return;
@@ -547,15 +584,9 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int x = 0; x < 2; ++x) pr[cur][x] = __builtin_bit_cast(bf16x8_t, w[x]);
   };
 
-  Slots next = slots_of(0, look_up(0));  // of the tile behind the one worked on
-  if (count > 0) {
-    issue(0, next, 0);
-    issue(0, next, 1);
-  }
-  next = slots_of(1, look_up(1));
-  if (count > 1) issue(1, next, 0);
-  uint32_t after = look_up(2);
   arrive();
+  put();
+  if (count == 0) __syncthreads();
   if (whole > 0) {
     // (there is no block -1: its p is 0, and V at its place too)
     const u32x4_t none = {0, 0, 0, 0};
@@ -616,6 +647,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     arrive();
   }
 
+  get();
   l = l + __shfl_xor(l, 32);
   if (!live) return;
   if (it.part != kPromptWhole) {
@@ -632,15 +664,15 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         *reinterpret_cast<f32x4_t*>(o + 32 * d + 2 * i) = f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
     return;
   }
-  const float by = sees > 0 ? l : 1.0f;
+  const float by = 1.0f / (sees > 0 ? l : 1.0f);  // (l: p's sum times 2^-40, from 2^-48 on)
   uint16_t* o = a.o + q_at + 4 * h;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       uint2 w;
-      w.x = pack_bf16x2(acc[d][i] / by, acc[d][i + 1] / by);
-      w.y = pack_bf16x2(acc[d][i + 2] / by, acc[d][i + 3] / by);
+      w.x = pack_bf16x2(acc[d][i] * by, acc[d][i + 1] * by);
+      w.y = pack_bf16x2(acc[d][i + 2] * by, acc[d][i + 3] * by);
       *reinterpret_cast<uint2*>(o + 32 * d + 2 * i) = w;
     }
 }
@@ -649,7 +681,8 @@ template <int D, bool PAGED>
 CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
   if (!a.items) {
     const PromptItem it = item_at<PAGED>(a, blockIdx.x / a.kv.kv_heads);
-    if (it.row != 0xFFFFFFFFu) attn_prompt_item<D, PAGED>(a, it, blockIdx.x % a.kv.kv_heads, a.kv.k, a.kv.v);
+    auto nothing = [] {};
+    if (it.row != 0xFFFFFFFFu) attn_prompt_item<D, PAGED>(a, it, blockIdx.x % a.kv.kv_heads, a.kv.k, a.kv.v, nothing, nothing);
     return;
   }
   // The list is two, of the rows with wide units and of the narrow ones, which some of the workgroups begin with; who
@@ -657,36 +690,51 @@ CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
   // kv_heads, by tickets of eight queues: workgroups of one queue run on one XCD, whose L2 then holds the K and V of
   // few heads.  (Each queue has every eighth work, so they end alike.)
   __shared__ uint32_t s_ticket;
+  constexpr uint32_t kNone = 0xFFFFFFFFu;
   const uint32_t queue = blockIdx.x % kPromptQueues, place = blockIdx.x / kPromptQueues;
   const uint32_t items = scalar_word(&a.counts->items, 0), wide = scalar_word(&a.counts->wide, 0);
   const uint32_t first = kPromptCus / kPromptQueues - scalar_word(&a.counts->narrow_first, 0);  // narrow from this place on
   uint32_t kind = place >= first, ticket = kind ? place - first : place;
   auto next = [&](uint32_t t) {  // a ticket's work, its item; false: no more of the kind
     const uint32_t n = t * kPromptQueues + queue;
-    return n < (kind ? items - wide : wide) * a.kv.kv_heads ? n : 0xFFFFFFFFu;
+    return n < (kind ? items - wide : wide) * a.kv.kv_heads ? n : kNone;
   };
   auto draw = [&] { return threadIdx.x == 0 ? atomicAdd(&a.counts->tickets[kind][queue], 1u) : 0u; };
-  auto share = [&](uint32_t t) {
-    __syncthreads();  // the last ticket has been read
-    if (threadIdx.x == 0) s_ticket = t;
-    __syncthreads();
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)s_ticket);
+  auto shared = [&] { return (uint32_t)__builtin_amdgcn_readfirstlane((int)s_ticket); };
+  u32x4_t x, y;
+  auto read = [&](uint32_t n) {
+    const uint64_t at = 2 * ((uint64_t)(kind ? wide : 0u) + n / a.kv.kv_heads);
+    x = scalar_four(a.items, at);
+    y = scalar_four(a.items, at + 1);
   };
   uint32_t n = next(ticket);
+  if (n != kNone) read(n);
   for (bool other = false;;) {
-    if (n == 0xFFFFFFFFu) {
+    if (n == kNone) {
       if (other) return;
       other = true;
       kind ^= 1u;
-      n = next(share(draw()));
+      ticket = draw();
+      __syncthreads();  // the last one has been read
+      if (threadIdx.x == 0) s_ticket = ticket;
+      __syncthreads();
+      n = next(shared());
+      if (n != kNone) read(n);
       continue;
     }
-    const uint32_t t = draw();
-    const uint64_t at = 2 * ((uint64_t)(kind ? wide : 0u) + n / a.kv.kv_heads);
-    const u32x4_t x = scalar_four(a.items, at), y = scalar_four(a.items, at + 1);
+    // The next ticket is drawn before the item is worked on, and its item read before its last stores.
+    ticket = draw();
     const PromptItem it{x[0], x[1], x[2], x[3], (int32_t)y[0], y[1], y[2], y[3]};
-    attn_prompt_item<D, PAGED>(a, it, n % a.kv.kv_heads, a.kv.k, a.kv.v);
-    n = next(share(t));
+    const uint32_t kvh = n % a.kv.kv_heads;
+    attn_prompt_item<D, PAGED>(
+        a, it, kvh, a.kv.k, a.kv.v,
+        [&] {
+          if (threadIdx.x == 0) s_ticket = ticket;
+        },
+        [&] {
+          n = next(shared());
+          if (n != kNone) read(n);
+        });
   }
 }
 
@@ -887,10 +935,10 @@ CATENA_DEV void attn_prompt_join(const AttnPromptArgs& a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = o[i] * f + y[i] * e;
       }
-      const float by = x.old + (int32_t)t + 1 > 0 ? l : 1.0f;
+      const float by = 1.0f / (x.old + (int32_t)t + 1 > 0 ? l : 1.0f);
       uint2 w;
-      w.x = pack_bf16x2(o[0] / by, o[1] / by);
-      w.y = pack_bf16x2(o[2] / by, o[3] / by);
+      w.x = pack_bf16x2(o[0] * by, o[1] * by);
+      w.y = pack_bf16x2(o[2] * by, o[3] * by);
       *reinterpret_cast<uint2*>(a.o + ((uint64_t)(x.first + t) * heads + kvh * a.group + m_row % a.group) * D + d) = w;
     }
   }
