@@ -391,3 +391,14 @@ def test_list_overlapping_rows():
     keep = [up(p.q), up(p.starts), up(p.lens.astype(np.uint32)), ca.Buffer(ca.attn_prompt_plan(kv, 3, 2))]
     ca.attn_prompt_bf16(kv, keep[0], keep[1], keep[2], o, 3, 2, p.scale, keep[3])
     assert np.all(o.read(np.uint16, (4, 2, 64))[2:] == MARK)
+
+
+def test_most_rows_and_heads():
+    say("most rows and heads")
+    rng = np.random.default_rng(21)
+    p = Prompt(rng, [1] * 5000, rng.integers(0, 5, 5000), 2, 1, 64, 16)
+    p.check(p.run())
+    p = Prompt(rng, [1] * 8, [0] * 8, 131072, 1, 64, 0)  # 512 units a row
+    got = p.run()
+    for t in range(8):  # one slot: its value
+        assert np.array_equal(got[t], np.broadcast_to(p.v[t], got[t].shape))
