@@ -23,7 +23,11 @@
 // Units of up to 64 query rows (single tokens, short chunks) leave most waves without
 // rows and wait for memory instead: there each wave takes blocks of 32 slots of its own,
 // with its own loads and no barrier, for 32 rows, and the waves' results are joined at
-// the end.
+// the end.  Eight waves share a unit; of many such units (2048) two do, and a workgroup
+// takes four kv heads' at a time, since what a unit costs besides its loads is latency
+// (8 kv heads, 256 single tokens behind up to 400 slots 106 us with eight waves, 68 with
+// two, behind up to 4000 407 / 400; of fewer units the larger items end unevenly: 130
+// tokens behind up to 4000 251 us with eight waves, 281 with four).
 //
 // Units are dealt out in one of two ways.  Few short ones: a workgroup each, which finds
 // it from the rows' lengths.  Else a kernel before lists them by length, long ones first,
@@ -138,9 +142,9 @@ CATENA_DEV PromptItem item_at(const AttnPromptArgs& a, uint32_t index) {
 
 // (the pools as arguments that nothing else points into: the compiler then does not make reads of LDS wait for
 // the loads into it, whose order the barriers below give)
-// put, get: called by all threads with a barrier between, get in front of the last stores, to look ahead
+// kvh0: the kv head, or the first of 8 / unit_waves of a narrow unit's.  put, get: called by all threads with a barrier between, get in front of the last stores, to look ahead
 template <int D, bool PAGED, class Put, class Get>
-CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, uint32_t kvh,
+CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, uint32_t kvh0, uint32_t unit_waves,
                                  const uint16_t* __restrict__ pool_k, const uint16_t* __restrict__ pool_v,
                                  const Put& put, const Get& get) {
   constexpr int KS = D / 16;        // steps of a score's sum
@@ -162,6 +166,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   const uint32_t rows_left = it.n * a.group - it.unit * kRows, rows = rows_left < kRows ? rows_left : kRows;
   const bool narrow = rows <= kNarrow;
   const uint32_t blocks = rows <= 32 ? 1 : 2;
+  const uint32_t kvh_w = kvh0 + (narrow ? wave / unit_waves : 0u), kvh = min(kvh_w, a.kv.kv_heads - 1);
   const uint32_t w_row = it.unit * kRows + 32 * (narrow ? wave % blocks : wave), m_row = w_row + c, t_row = m_row / a.group;
   const bool live = t_row < it.n;
   const uint64_t q_at =
@@ -433,10 +438,10 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   };
 
   if (narrow) {
-    // Wave w: blocks of 32 slots w / blocks, + 8 / blocks, ...; K and V of one at a time in its own part of LDS, each
+    // Wave w of a unit: blocks of 32 slots w / blocks, + unit_waves / blocks, ...; K and V of one at a time in its own part of LDS, each
     // asked for as soon as its place has been read
     constexpr int kBlock = 2 * kAcross;  // loads of a block's K, or V
-    const uint32_t step = kWaves / blocks, all = 2 * count;
+    const uint32_t step = unit_waves / blocks, all = kvh == kvh_w ? 2 * count : 0u;
     uint16_t* mine = smem + wave * kTile;
     lds_char *k = place(mine, k_lane), *v = place(mine + kTile / 2, v_lane);
     auto slot_of = [&](uint32_t b) { return it.beg * kKeys + 32 * b; };
@@ -452,7 +457,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         load(p.s[r], what, 0, std::integral_constant<int, kAcross>{}, mine + what * (kTile / 2) + r * kAcross * 512);
     };
     auto fence = [] { asm volatile("" ::: "memory"); };
-    uint32_t b = wave / blocks;
+    uint32_t b = wave % unit_waves / blocks;
     Pair pair = pair_of(b, page_of(slot_of(b)), page_of(slot_of(b) + 16));
     uint32_t p0 = page_of(slot_of(b + step)), p1 = page_of(slot_of(b + step) + 16);
     if (b < all) {
@@ -501,12 +506,14 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     }
     get();
     __syncthreads();
-    for (uint32_t id = threadIdx.x; id < rows * (D / 4); id += 64 * kWaves) {
-      const uint32_t row = id / (D / 4), d = id % (D / 4) * 4;
+    const uint32_t units = min(kWaves / unit_waves, a.kv.kv_heads - kvh0);
+    for (uint32_t id = threadIdx.x; id < units * rows * (D / 4); id += 64 * kWaves) {
+      const uint32_t u = id / (D / 4) / rows, row = id / (D / 4) % rows, d = id % (D / 4) * 4;
+      const uint32_t mine = u * unit_waves + row / 32, end = (u + 1) * unit_waves;
       float mm = kNegInf, ll = 0.0f;
       f32x4_t oo = {0, 0, 0, 0};
-      for (uint32_t w = row / 32; w < kWaves; w += blocks) mm = __builtin_fmaxf(mm, sml[2 * (w * 32 + row % 32)]);
-      for (uint32_t w = row / 32; w < kWaves; w += blocks) {
+      for (uint32_t w = mine; w < end; w += blocks) mm = __builtin_fmaxf(mm, sml[2 * (w * 32 + row % 32)]);
+      for (uint32_t w = mine; w < end; w += blocks) {
         const uint32_t at = w * 32 + row % 32;
         const float f = weight(sml[2 * at], mm);
         const f32x4_t y = *reinterpret_cast<const f32x4_t*>(so + at * D + d);
@@ -515,7 +522,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         for (int i = 0; i < 4; ++i) oo[i] = oo[i] + y[i] * f;
       }
       if (it.part != kPromptWhole) {
-        const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh) * a.part_rows + row;  // (places of one head's)
+        const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh0 + u) * a.part_rows + row;
         if (d == 0) {
           a.part_ml[2 * at] = mm;
           a.part_ml[2 * at + 1] = ll;
@@ -528,7 +535,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
       uint2 w;
       w.x = pack_bf16x2(oo[0] * by, oo[1] * by);
       w.y = pack_bf16x2(oo[2] * by, oo[3] * by);
-      *reinterpret_cast<uint2*>(a.o + ((uint64_t)(it.first + t) * heads + kvh * a.group + r % a.group) * D + d) = w;
+      *reinterpret_cast<uint2*>(a.o + ((uint64_t)(it.first + t) * heads + (kvh0 + u) * a.group + r % a.group) * D + d) = w;
     }
     return;
   }
@@ -682,28 +689,30 @@ CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
   if (!a.items) {
     const PromptItem it = item_at<PAGED>(a, blockIdx.x / a.kv.kv_heads);
     auto nothing = [] {};
-    if (it.row != 0xFFFFFFFFu) attn_prompt_item<D, PAGED>(a, it, blockIdx.x % a.kv.kv_heads, a.kv.k, a.kv.v, nothing, nothing);
+    if (it.row != 0xFFFFFFFFu) attn_prompt_item<D, PAGED>(a, it, blockIdx.x % a.kv.kv_heads, kWaves, a.kv.k, a.kv.v, nothing, nothing);
     return;
   }
   // The list is two, of the rows with wide units and of the narrow ones, which some of the workgroups begin with; who
-  // finds no more of one kind goes on with the other.  Work n of a kind is kv head n % kv_heads of its item n /
-  // kv_heads, by tickets of eight queues: workgroups of one queue run on one XCD, whose L2 then holds the K and V of
+  // finds no more of one kind goes on with the other.  Work n of a kind is kv head (or heads) n % groups of its item n /
+  // groups, by tickets of eight queues: workgroups of one queue run on one XCD, whose L2 then holds the K and V of
   // few heads.  (Each queue has every eighth work, so they end alike.)
   __shared__ uint32_t s_ticket;
   constexpr uint32_t kNone = 0xFFFFFFFFu;
   const uint32_t queue = blockIdx.x % kPromptQueues, place = blockIdx.x / kPromptQueues;
   const uint32_t items = scalar_word(&a.counts->items, 0), wide = scalar_word(&a.counts->wide, 0);
   const uint32_t first = kPromptCus / kPromptQueues - scalar_word(&a.counts->narrow_first, 0);  // narrow from this place on
+  const uint32_t narrow_waves = scalar_word(&a.counts->narrow_waves, 0), narrow_heads = kWaves / narrow_waves;
+  const uint32_t narrow_groups = (a.kv.kv_heads + narrow_heads - 1) / narrow_heads;
   uint32_t kind = place >= first, ticket = kind ? place - first : place;
   auto next = [&](uint32_t t) {  // a ticket's work, its item; false: no more of the kind
     const uint32_t n = t * kPromptQueues + queue;
-    return n < (kind ? items - wide : wide) * a.kv.kv_heads ? n : kNone;
+    return n < (kind ? (items - wide) * narrow_groups : wide * a.kv.kv_heads) ? n : kNone;
   };
   auto draw = [&] { return threadIdx.x == 0 ? atomicAdd(&a.counts->tickets[kind][queue], 1u) : 0u; };
   auto shared = [&] { return (uint32_t)__builtin_amdgcn_readfirstlane((int)s_ticket); };
   u32x4_t x, y;
   auto read = [&](uint32_t n) {
-    const uint64_t at = 2 * ((uint64_t)(kind ? wide : 0u) + n / a.kv.kv_heads);
+    const uint64_t at = 2 * (kind ? (uint64_t)wide + n / narrow_groups : n / a.kv.kv_heads);
     x = scalar_four(a.items, at);
     y = scalar_four(a.items, at + 1);
   };
@@ -725,9 +734,9 @@ CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
     // The next ticket is drawn before the item is worked on, and its item read before its last stores.
     ticket = draw();
     const PromptItem it{x[0], x[1], x[2], x[3], (int32_t)y[0], y[1], y[2], y[3]};
-    const uint32_t kvh = n % a.kv.kv_heads;
+    const uint32_t kvh = kind ? n % narrow_groups * narrow_heads : n % a.kv.kv_heads;
     attn_prompt_item<D, PAGED>(
-        a, it, kvh, a.kv.k, a.kv.v,
+        a, it, kvh, kind ? narrow_waves : kWaves, a.kv.k, a.kv.v,
         [&] {
           if (threadIdx.x == 0) s_ticket = ticket;
         },
@@ -762,11 +771,12 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
   __shared__ uint32_t s_start[kThreads], s_first[kThreads], s_n[kThreads], s_old[kThreads], s_at[kThreads], s_wave[16];
   __shared__ uint32_t s_class[kClasses], s_parts, s_splits;
   __shared__ unsigned long long s_work, s_narrow;
+  __shared__ uint32_t s_alone;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   if (tid < kClasses) s_class[tid] = 0;
   if (tid == 0) {
     s_work = s_narrow = 0;
-    s_parts = s_splits = 0;
+    s_parts = s_splits = s_alone = 0;
   }
   struct Row {
     uint32_t units;
@@ -856,6 +866,10 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
         s_old[tid] = (uint32_t)x.old;
       }
       if (pass > 0 && x.units > 0) s_at[tid] = place_of(x);
+      if (pass == 1) {
+        const uint64_t some = __ballot(x.units > 0 && alone(x.t.n));
+        if (lane == 0 && some) atomicAdd(&s_alone, (uint32_t)__popcll((unsigned long long)some));
+      }
       __syncthreads();
       for (uint32_t k = pass == 1 ? all : tid; k < all; k += kThreads) {
         const uint32_t at = last_at_most(s_start, kThreads, k), unit = k - s_start[at];
@@ -904,6 +918,8 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
   if (tid == 0) {
     a.counts->splits = s_splits < a.max_splits ? s_splits : a.max_splits;
     a.counts->narrow_first = first;
+    const uint64_t narrow_units = (uint64_t)s_alone * a.kv.kv_heads;
+    a.counts->narrow_waves = narrow_units >= 8 * kPromptCus ? 2u : (uint32_t)kWaves;
   }
   if (tid < 2 * kPromptQueues) a.counts->tickets[tid / kPromptQueues][tid % kPromptQueues] = tid / kPromptQueues ? first : kPlaces - first;
 }

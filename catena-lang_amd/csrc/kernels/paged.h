@@ -201,6 +201,7 @@ struct PromptCounts {
   uint32_t items, wide;   // of the list; of them, in front, those of rows with wide units
   uint32_t splits;
   uint32_t narrow_first;  // of a queue's workgroups so many begin with the others
+  uint32_t narrow_waves;  // so many waves to one of their units
   uint32_t tickets[2][kPromptQueues];  // taken of each kind
 };
 constexpr uint32_t kPromptCountBytes = 128;  // in the workspace, in front of the list

@@ -402,3 +402,24 @@ def test_most_rows_and_heads():
     got = p.run()
     for t in range(8):  # one slot: its value
         assert np.array_equal(got[t], np.broadcast_to(p.v[t], got[t].shape))
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(16, 8, 64), (6, 3, 128), (80, 5, 64)])
+def test_many_narrow_units(heads, kvh, dim):
+    """So many that a workgroup takes several kv heads' of them: also where these do not come out even, units of one
+    and two blocks of 32 query rows, parts, rows that see nothing, wide units beside them."""
+    say(f"many narrow units {heads} {kvh} {dim}")
+    rng = np.random.default_rng(22)
+    rows = 2100 // kvh + 1
+    n, ctx = rng.integers(0, 3, rows) + 1, rng.integers(0, 70, rows)
+    n[:4], ctx[:4] = [200, 1, 4, 2], [100, 2300, 1500, 1100]
+    p = Prompt(rng, n, ctx, heads, kvh, dim, 16, gap=1, pad=2)
+    p.lens[5] = 1  # of n tokens: the last sees the slot
+    n5, p.ctx[5] = p.n[5], 1 - p.n[5]
+    got = p.run()
+    at = int(p.starts[5])
+    assert np.all(f64(got[at:at + n5 - 1]) == 0)
+    p.n[5] = 0
+    p.check(got, [0, 1, 2, 3, 100, 199])
+    p.n[5] = n5
+    assert np.array_equal(p.run(again=2), got)
