@@ -12,8 +12,9 @@
 // workgroup takes the sums itself, from the rows' words in L2, and then its share
 // of the tokens; one launch.
 //
-// Bound: latency.  A workgroup of 256 threads sums 1024 rows at a time, then
-// finds a token's row by halving.
+// Bound: latency: the rows' words, two sums over a workgroup's 1024 rows, a token's row
+// by halving, its page, one after the other.  A step of 64 rows 4.7 us (4.0 on the
+// device), 8192 tokens of 12 prompts 5.7 (5.6); as tensor operations 420.
 #include "common.h"
 #include "paged.h"
 

@@ -17,7 +17,12 @@
 // NaN.
 //
 // Bound: HBM for prompts, one launch's latency for a decode step.  A workgroup
-// serves one token, a thread 16 values of a head: 8 pairs, or 16 that do not turn.
+// serves one token, a thread 16 values of a head: 8 pairs, or 16 that do not turn, so
+// that a pair meets in one thread and both its halves are loads of 16 bytes.  Into 4 bits
+// a thread then takes 8 values from LDS (16, with half of the threads idle: 62 us).
+// 32 + 2 x 8 heads of 128, 8192 tokens: f32 in, bf16 pages 55 us (303 MB, 5.5 TB/s; 60
+// without the loads ahead), bf16 in, 4-bit pages and copies 56 us (211 MB, 3.8 TB/s: v's
+// bytes go out one by one); 56 tokens 4.7 us, of which 3.7 on the device.
 #include "common.h"
 #include "paged.h"
 
@@ -37,22 +42,30 @@ CATENA_DEV Place place_of(const RopePackedArgs& a, uint32_t num_pages, uint32_t 
   return Place{(uint32_t)page, (uint32_t)slot & ((1u << shift) - 1u), known ? pos : 0u, known && page < num_pages};
 }
 
+// Eight values as they lie, and as floats
 template <bool WIDE>
-CATENA_DEV void load8(const void* base, uint64_t at, float* x) {
-  if constexpr (WIDE) {
-    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(base) + at);
-    const f32x4_t u = p[0], v = p[1];
+struct Eight {
+  u32x4_t w[WIDE ? 2 : 1];
+};
+template <bool WIDE>
+CATENA_DEV Eight<WIDE> load8(const void* base, uint64_t at) {
+  Eight<WIDE> r;
+  const u32x4_t* p = WIDE ? reinterpret_cast<const u32x4_t*>(static_cast<const float*>(base) + at)
+                          : reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(base) + at);
+  r.w[0] = p[0];
+  if constexpr (WIDE) r.w[1] = p[1];
+  return r;
+}
+template <bool WIDE>
+CATENA_DEV void floats8(const Eight<WIDE>& r, float* x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = u[i];
-      x[4 + i] = v[i];
-    }
-  } else {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(base) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = bf16lo(w[i]);
-      x[2 * i + 1] = bf16hi(w[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (WIDE) {
+      x[i] = __uint_as_float(r.w[0][i]);
+      x[4 + i] = __uint_as_float(r.w[1][i]);
+    } else {
+      x[2 * i] = bf16lo(r.w[0][i]);
+      x[2 * i + 1] = bf16hi(r.w[0][i]);
     }
   }
 }
@@ -61,21 +74,34 @@ CATENA_DEV u32x4_t pack8(const float* y) {
 }
 
 // A thread's 16 values of a head: eight from `first`, eight from `second`
+template <bool WIDE>
+struct Taken {
+  Eight<WIDE> lo, hi;
+};
 struct Sixteen {
   uint32_t first, second;
   u32x4_t lo, hi;  // rounded
 };
 // unit: which 16 of the head's D; turns: the head is one of q or k
-template <bool WIDE>
-CATENA_DEV Sixteen turned(const RopePackedArgs& a, uint64_t head_at, uint32_t unit, bool turns, uint32_t pos) {
+CATENA_DEV Sixteen places_of(const RopePackedArgs& a, uint32_t unit, bool turns) {
   Sixteen r;
-  const bool pairs = turns && 16 * unit < a.rot;
-  const bool apart = pairs && !a.interleaved;
+  const bool apart = turns && 16 * unit < a.rot && !a.interleaved;
   r.first = apart ? 8 * unit : 16 * unit;
   r.second = apart ? 8 * unit + a.rot / 2 : 16 * unit + 8;
+  return r;
+}
+template <bool WIDE>
+CATENA_DEV Taken<WIDE> take(const RopePackedArgs& a, uint64_t head_at, uint32_t unit, bool turns) {
+  const Sixteen r = places_of(a, unit, turns);
+  return Taken<WIDE>{load8<WIDE>(a.qkv, head_at + r.first), load8<WIDE>(a.qkv, head_at + r.second)};
+}
+template <bool WIDE>
+CATENA_DEV Sixteen turned(const RopePackedArgs& a, const Taken<WIDE>& t, uint32_t unit, bool turns, uint32_t pos) {
+  Sixteen r = places_of(a, unit, turns);
+  const bool pairs = turns && 16 * unit < a.rot, apart = pairs && !a.interleaved;
   float x[16], y[16];
-  load8<WIDE>(a.qkv, head_at + r.first, x);
-  load8<WIDE>(a.qkv, head_at + r.second, x + 8);
+  floats8<WIDE>(t.lo, x);
+  floats8<WIDE>(t.hi, x + 8);
   if (pairs) {
     const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(a.tab + ((uint64_t)pos * (a.rot / 2) + 8 * unit) * 2);
     float c[8], s[8];
@@ -118,41 +144,57 @@ CATENA_DEV void store16(uint16_t* head, const Sixteen& x) {
   *reinterpret_cast<u32x4_t*>(head + x.second) = x.hi;
 }
 
+// Every 16 values of a token's heads to a thread in turn: each(head, the token's place, they).  A turn's values are
+// asked for before the token's position, or the last turn, is worked on.
+template <bool WIDE, class KV, class Each>
+CATENA_DEV Place each_unit(const RopePackedArgs& a, const KV& kv, uint32_t token, uint32_t all, const Each& each) {
+  const uint32_t D = kv.head_dim, units = D / 16, most = all * units;
+  auto ask = [&](uint32_t id) {
+    const uint32_t head = id / units;
+    return take<WIDE>(a, ((uint64_t)token * all + head) * D, id % units, head < a.heads + kv.kv_heads);
+  };
+  uint32_t id = threadIdx.x;
+  Taken<WIDE> next;
+  if (id < most) next = ask(id);
+  const Place at = place_of(a, kv.num_pages, kv.page_shift, token);
+  while (id < most) {
+    const Taken<WIDE> now = next;
+    const uint32_t head = id / units, unit = id % units;
+    id += kThreads;
+    if (id < most) next = ask(id);
+    each(head, at, turned<WIDE>(a, now, unit, head < a.heads + kv.kv_heads, at.pos));
+  }
+  return at;
+}
+
 // grid = tokens
 template <bool WIDE>
 CATENA_DEV void rope_packed(const PagedKv& kv, const RopePackedArgs& a) {
-  const uint32_t token = blockIdx.x, D = kv.head_dim, units = D / 16, all = a.heads + 2 * kv.kv_heads;
-  const Place at = place_of(a, kv.num_pages, kv.page_shift, token);
-  for (uint32_t id = threadIdx.x; id < all * units; id += kThreads) {
-    const uint32_t head = id / units, unit = id % units;
+  const uint32_t token = blockIdx.x, D = kv.head_dim, all = a.heads + 2 * kv.kv_heads;
+  each_unit<WIDE>(a, kv, token, all, [&](uint32_t head, const Place& at, const Sixteen& x) {
     const bool is_k = head < a.heads + kv.kv_heads;
-    const Sixteen x = turned<WIDE>(a, ((uint64_t)token * all + head) * D, unit, is_k, at.pos);
     if (head < a.heads) {
       store16(a.q + ((uint64_t)token * a.heads + head) * D, x);
-      continue;
+      return;
     }
     const uint32_t h = (head - a.heads) % kv.kv_heads;
     if (a.k_out) store16((is_k ? a.k_out : a.v_out) + ((uint64_t)token * kv.kv_heads + h) * D, x);
     if (at.there) store16((is_k ? kv.k : kv.v) + paged_offset(kv, at.page, h, at.place), x);
-  }
+  });
 }
 
 CATENA_DEV uint32_t larger(uint32_t x, uint32_t y) { return x > y ? x : y; }
 
-// 16 bf16 values over `by` and the power of two `unit` as codes (two dwords)
-CATENA_DEV void codes16(const u32x4_t& lo, const u32x4_t& hi, float by, float unit, uint32_t* code) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t w = 0;
-    const u32x4_t x = i ? hi : lo;
+// Eight bf16 values over `by` and the power of two `unit` as codes
+CATENA_DEV uint32_t codes8(const u32x4_t& x, float by, float unit) {
+  uint32_t w = 0;
 #define CATENA_CODES(j) w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, bf16lo(x[j]) / by, bf16hi(x[j]) / by, unit, j);
-    CATENA_CODES(0)
-    CATENA_CODES(1)
-    CATENA_CODES(2)
-    CATENA_CODES(3)
+  CATENA_CODES(0)
+  CATENA_CODES(1)
+  CATENA_CODES(2)
+  CATENA_CODES(3)
 #undef CATENA_CODES
-    code[i] = w;
-  }
+  return w;
 }
 // The values of four codes' pairs, times unit, rounded to bf16
 CATENA_DEV u32x4_t values8(uint32_t code, float unit) {
@@ -170,14 +212,11 @@ CATENA_DEV u32x4_t values8(uint32_t code, float unit) {
 #undef CATENA_VALUES
   return r;
 }
-// The largest |x| of 16 bf16 values, as bits (an infinity or NaN is above all others)
-CATENA_DEV uint32_t top16(const u32x4_t& lo, const u32x4_t& hi) {
+// The largest |x| of eight bf16 values, as bits (an infinity or NaN is above all others)
+CATENA_DEV uint32_t top8(const u32x4_t& x) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    top = larger(top, larger(lo[i] << 16 & 0x7FFF0000u, lo[i] & 0x7FFF0000u));
-    top = larger(top, larger(hi[i] << 16 & 0x7FFF0000u, hi[i] & 0x7FFF0000u));
-  }
+  for (int i = 0; i < 4; ++i) top = larger(top, larger(x[i] << 16 & 0x7FFF0000u, x[i] & 0x7FFF0000u));
   return top;
 }
 
@@ -185,27 +224,24 @@ CATENA_DEV uint32_t top16(const u32x4_t& lo, const u32x4_t& hi) {
 template <bool WIDE>
 CATENA_DEV void rope_packed_q4(const PagedKv4& kv, const RopePackedArgs& a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t s_kv[];
-  const uint32_t token = blockIdx.x, D = kv.head_dim, units = D / 16, all = a.heads + 2 * kv.kv_heads;
-  const Place at = place_of(a, kv.num_pages, kv.page_shift, token);
-  for (uint32_t id = threadIdx.x; id < all * units; id += kThreads) {
-    const uint32_t head = id / units, unit = id % units;
-    const Sixteen x = turned<WIDE>(a, ((uint64_t)token * all + head) * D, unit, head < a.heads + kv.kv_heads, at.pos);
+  const uint32_t token = blockIdx.x, D = kv.head_dim, all = a.heads + 2 * kv.kv_heads;
+  const Place at = each_unit<WIDE>(a, kv, token, all, [&](uint32_t head, const Place&, const Sixteen& x) {
     store16(head < a.heads ? a.q + ((uint64_t)token * a.heads + head) * D : s_kv + (uint64_t)(head - a.heads) * D, x);
-  }
+  });
   __syncthreads();
   const uint32_t page = 1u << kv.page_shift;
-  // whole waves: a head's threads are neighbours in one
-  const uint32_t items = 2 * kv.kv_heads * units;
+  // Eight values to a thread; whole waves: a head's threads are neighbours in one
+  const uint32_t units = D / 8, items = 2 * kv.kv_heads * units;
   for (uint32_t id = threadIdx.x; id < (items + 63) / 64 * 64; id += kThreads) {
     const bool in = id < items;
     const uint32_t vec = in ? id / units : 0u, unit = id % units, h = vec % kv.kv_heads;
     const bool is_k = vec < kv.kv_heads;
-    const u32x4_t* src = reinterpret_cast<const u32x4_t*>(s_kv + (uint64_t)vec * D + 16 * unit);
-    const u32x4_t lo = src[0], hi = src[1];
-    uint32_t top = top16(lo, hi);
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(s_kv + (uint64_t)vec * D + 8 * unit);
+    uint32_t top = top8(x);
     top = larger(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = larger(top, (uint32_t)__shfl_xor((int)top, 2));
     if (!is_k)
-      for (uint32_t step = 2; step < units; step *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, (int)step));
+      for (uint32_t step = 4; step < units; step *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, (int)step));
     const bool odd = top >= 0x7F800000u;  // an infinity or NaN
     float scale;
     uint32_t byte = 0;
@@ -218,27 +254,22 @@ CATENA_DEV void rope_packed_q4(const PagedKv4& kv, const RopePackedArgs& a) {
       const float s = __uint_as_float(top) / 6.0f;
       scale = __uint_as_float(odd ? 0x7FC00000u : (__float_as_uint(s) + 0xFFFFu) & 0xFFFF0000u);
     }
-    uint32_t code[2];
-    codes16(lo, hi, is_k ? 1.0f : scale, is_k ? scale : 1.0f, code);
     const uint32_t some = 0u - (uint32_t)(!odd & (scale > 0.0f));
-    code[0] &= some;
-    code[1] &= some;
+    const uint32_t code = codes8(x, is_k ? 1.0f : scale, is_k ? scale : 1.0f) & some;
     if (!in) continue;
     if (a.k_out) {
-      uint16_t* out = (is_k ? a.k_out : a.v_out) + ((uint64_t)token * kv.kv_heads + h) * D + 16 * unit;
-      const float worth = odd ? __uint_as_float(0x7FC00000u) : scale;
-      *reinterpret_cast<u32x4_t*>(out) = values8(code[0], worth);
-      *reinterpret_cast<u32x4_t*>(out + 8) = values8(code[1], worth);
+      uint16_t* out = (is_k ? a.k_out : a.v_out) + ((uint64_t)token * kv.kv_heads + h) * D + 8 * unit;
+      *reinterpret_cast<u32x4_t*>(out) = values8(code, odd ? __uint_as_float(0x7FC00000u) : scale);
     }
     if (!at.there) continue;
     const uint64_t cells = paged_cells(kv.kv_heads, kv.page_shift, at.page, h);
     if (is_k) {
-      *reinterpret_cast<uint2*>(kv.k + (cells + at.place) * (D / 2) + 8 * unit) = uint2{code[0], code[1]};
-      if (unit % 2 == 0) kv.k_scale[cells * (D / 32) + (unit / 2) * page + at.place] = (uint8_t)byte;
+      *reinterpret_cast<uint32_t*>(kv.k + (cells + at.place) * (D / 2) + 4 * unit) = code;
+      if (unit % 4 == 0) kv.k_scale[cells * (D / 32) + (unit / 4) * page + at.place] = (uint8_t)byte;
     } else {
-      uint8_t* dst = kv.v + cells * (D / 2) + (uint64_t)(8 * unit) * page + at.place;
+      uint8_t* dst = kv.v + cells * (D / 2) + (uint64_t)(4 * unit) * page + at.place;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dst[i * page] = (uint8_t)(code[i / 4] >> (8 * (i % 4)));
+      for (int i = 0; i < 4; ++i) dst[i * page] = (uint8_t)(code >> (8 * i));
       if (unit == 0) kv.v_scale[cells + at.place] = (uint16_t)(__float_as_uint(scale) >> 16);
     }
   }
