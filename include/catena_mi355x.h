@@ -535,11 +535,13 @@ int catena_mi355x_rope_packed_bf16(const catena_paged_kv_t *kv, const void *qkv,
  * = 1 alone all of them, so prompts, later parts of prompts and single tokens may stand
  * beside each other.  Query head h reads kv head h / (heads / kv_heads).  o[tokens]
  * [heads][head_dim] bf16 RNE: scores, sums and o in f32, p rounded to bf16 (2^-8 of
- * it) where it meets v.  A token that sees no slot gives 0; slots without a page are
- * not seen, and a token whose slots all have none gives NaN.  What lies in slots that
- * a token does not see never reaches it, infinities and NaN included.  Sums of finite
- * values do not overflow (a mean within 2^-8 of the type's largest may).  starts past `tokens` are cut there, rows that end before
- * they begin have no tokens; places of q and o that belong to no row are not touched.
+ * it) in the sum over v and in its own.  The same call gives the same bits; where long
+ * rows are cut, a row's last bits depend on the rows beside it.  A token that sees no
+ * slot gives 0; slots without a page are not seen, and a token whose slots all have none
+ * gives NaN.  What lies in slots that a token does not see never reaches it, infinities
+ * and NaN included.  Sums of finite values do not overflow (a mean within 2^-8 of the
+ * type's largest may).  starts past `tokens` are cut there, rows that end before they
+ * begin have no tokens; places of q and o that belong to no row are not touched.
  * No two rows' tokens overlap.  o is not q, k or v.
  * workspace as for catena_mi355x_attn_paged_bf16, of attn_prompt_plan's size, which is
  * a function of the sizes alone and needs no device.  q and o 16-byte aligned.
