@@ -8,8 +8,8 @@
 // Bound: the cache is read once, D + D / 32 + 2 bytes per (slot, kv head), so HBM, beside
 // about 1000 vector instructions of a wave for 128 slots of 128 columns, which keep the
 // SIMDs busy 40 % of the time.  64 rows x 4096 slots x 8 kv heads of 128 take 57 us (281
-// MB, 4.9 TB/s), 64 of 1 .. 8192 75 (as bf16 pages 88 for half the slots), one row of
-// 131072 of 64 columns 25 (6 the join), one of 640 and 16 heads 8.9.
+// MB, 4.9 TB/s), 64 of 1 .. 8192 70 to 75 (as bf16 pages 88 for half the slots), one row of
+// 131072 of 64 columns 25 (6 the join), one of 640 and 16 heads 9.
 //
 // A wave takes 128 slots at a time, its lane group g (lanes 16 g ..) slots 32 g ..
 // 32 g + 31 of them.
@@ -27,7 +27,8 @@
 // 16 columns twice, and the second ones take the second term; more heads need a second
 // product.
 // K of the next 128 slots is asked for as soon as the scores are there, V once it has been
-// read, so that a wave's loads are under way all the time.
+// read, or of the workgroup's next unit or part of one, so that a wave's loads are under way
+// all the time (64 rows of 1 .. 8192 slots: 74.7 us without the next part's, 70.4 with).
 //
 // Codes are finite whatever their bits, so what lies behind a row's end is masked in
 // the scores and the scales alone.
@@ -113,13 +114,13 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
     return x;
   };
   // (what is not there is read from the pool's first page and masked)
-  auto request_k = [&](Tile<D>& x, const Part& p, uint32_t slot, const Pages& at) {
+  auto request_k = [&](Tile<D>& x, uint32_t kvh, uint32_t slot, const Pages& at) {
     const uint32_t me = own_lane(), c = me & 15u, g = me >> 4;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint32_t s = (slot + 32 * (c >> 2) + 16 * r) & mask;
       const uint32_t page = at.of(c >> 2, r);
-      const uint64_t kc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, p.kvh);
+      const uint64_t kc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, kvh);
       const uint8_t* k = pools.k + (kc + s + (c & 3u)) * (D / 2) + g * (D / 8);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -134,13 +135,13 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
       x.ks[r] = *reinterpret_cast<const u32x4_t*>(pools.k_scale + kc * (D / 32) + (uint64_t)(g * (D / 32) / 4) * page_size + s);
     }
   };
-  auto request_v = [&](Tile<D>& x, const Part& p, uint32_t slot, const Pages& at) {
+  auto request_v = [&](Tile<D>& x, uint32_t kvh, uint32_t slot, const Pages& at) {
     const uint32_t me = own_lane(), c = me & 15u, g = me >> 4;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint32_t s = (slot + 32 * g + 16 * r) & mask;
       const uint32_t page = at.of(g, r);
-      const uint64_t vc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, p.kvh);
+      const uint64_t vc = paged_cells(a.kv.kv_heads, a.kv.page_shift, page < a.kv.num_pages ? page : 0u, kvh);
       const uint8_t* v = pools.v + vc * (D / 2) + (uint64_t)c * page_size + s;
 #pragma unroll
       for (int i = 0; i < VG; ++i) x.v[i][r] = *reinterpret_cast<const u32x4_t*>(v + (uint64_t)(16 * i) * page_size);
@@ -340,39 +341,56 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
     now = unit_from(at);
     at += gridDim.x;
   }
+  // A tile a turn, 128 slots a wave; a row's last tile may leave a wave without any.  A turn's loads, of the next turn or
+  // of the next part's first one, are under way while the one before is worked on.
+  auto first_of = [&](const Part& p) { return p.beg * kTileSlots + 128 * wave; };
+  auto end_of = [&](const Part& p) { return p.end * kTileSlots < p.len ? p.end * kTileSlots : p.len; };
+  Tile<D> x;
+  uint32_t slot = first_of(now), end = end_of(now);
+  begin(now);
+  Pages pages = spread(look_up(now, slot, end));
+  if (slot < end) {
+    request_k(x, now.kvh, slot, pages);
+    request_v(x, now.kvh, slot, pages);
+  }
+  uint32_t ahead = look_up(now, slot + kTileSlots, end);
   for (;;) {
-    begin(now);
-    Tile<D> x;
-    // a tile a turn, 128 slots a wave; the last tile of a row may leave a wave without any
-    uint32_t slot = now.beg * kTileSlots + 128 * wave;
-    const uint32_t end = now.end * kTileSlots < now.len ? now.end * kTileSlots : now.len;
-    Pages pages = spread(look_up(now, slot, end));
-    uint32_t ahead = look_up(now, slot + kTileSlots, end);
-    if (slot < end) {
-      request_k(x, now, slot, pages);
-      request_v(x, now, slot, pages);
+    const bool more = at < last;
+    Part then = now;
+    uint32_t then_slot = 0, then_end = 0, behind = 0xFFFFFFFFu;
+    if (more) {
+      then = whole ? unit_from(at) : part_behind(a, now, last - at);
+      at += whole ? gridDim.x : then.end - then.beg;
+      then_slot = first_of(then);
+      then_end = end_of(then);
+      behind = look_up(then, then_slot, then_end);
+    }
+    if (slot >= end && then_slot < then_end) {
+      pages = spread(behind);
+      request_k(x, then.kvh, then_slot, pages);
+      request_v(x, then.kvh, then_slot, pages);
     }
 #pragma clang loop unroll(disable)
     for (; slot < end; slot += kTileSlots) {
+      const bool here = !more || slot + kTileSlots < end;
+      const uint32_t kvh = here ? now.kvh : then.kvh, s2 = here ? slot + kTileSlots : then_slot;
       float s[32];
       scores(x, s);
-      const Pages next = spread(ahead);
+      const Pages next = spread(here ? ahead : behind);
       ahead = look_up(now, slot + 2 * kTileSlots, end);
-      request_k(x, now, slot + kTileSlots, next);
+      request_k(x, kvh, s2, next);
       __builtin_amdgcn_sched_barrier(0);
       take(x, s, now, slot, pages);
-      request_v(x, now, slot + kTileSlots, next);
+      request_v(x, kvh, s2, next);
       pages = next;
     }
     finish(now);
-    if (at >= last) return;
-    if (whole) {
-      now = unit_from(at);
-      at += gridDim.x;
-    } else {
-      now = part_behind(a, now, last - at);
-      at += now.end - now.beg;
-    }
+    if (!more) return;
+    now = then;
+    slot = then_slot;
+    end = then_end;
+    begin(now);
+    ahead = look_up(now, slot + kTileSlots, end);
   }
 }
 

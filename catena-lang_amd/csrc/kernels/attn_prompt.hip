@@ -8,7 +8,7 @@
 // bytes a slot and kv head that 256 query rows share.  They run at the chip's power limit:
 // 12000 tokens x 32 heads of 128 1000 to 1060 us (1.04 to 1.10 PFLOP/s; a large matrix
 // product of random values 1.2 to 1.36 on the same cards), 8 ragged prompts of up to
-// 4096 tokens 520 for 4.9e11 flop; 4 chunks of 500 tokens and 28 single ones over 8000
+// 4096 tokens 597 for 5.5e11 flop; 4 chunks of 500 tokens and 28 single ones over 8000
 // slots or fewer 230 (0.56 GB and 1.4e11 flop); 5 prompts of up to 130 tokens 7.7.
 //
 // A workgroup takes 256 query rows of one row and kv head (a unit): query row m is token

@@ -94,8 +94,8 @@ struct AttnPagedArgs {
 // idle at the end.  Rows x slots of 8 kv heads, whole / cut, us: 2 x 1024 9.2 / 11.0, x 2048
 // 13.5 / 11.1, x 4096 22.4 / 11.6; 8 x 1024 9.3 / 11.5, x 2048 14.5 / 12.8, x 4096 23.2 /
 // 16.5; 16 x 2048 14.9 / 16.6, x 4096 23.6 / 21.1; 32 x 2048 17.3 / 21, x 4096 31 / 34.5;
-// 64 x 4096 55 / 57; ragged 32 up to 4096 25 / 29, 64 up to 2048 24 / 29, up to 8192 76 / 74,
-// up to 16384 147 / 128, 256 up to 4096 128 / 144.
+// 64 x 4096 55 / 57; ragged 32 up to 4096 25 / 29, 64 up to 2048 24 / 29, up to 8192 76 / 70,
+// up to 16384 147 / 122, 256 up to 4096 128 / 144.
 constexpr uint32_t kAttnQ4Slots = 512, kAttnQ4WholeShare = 200, kAttnQ4WholeMost = 12, kAttnQ4TwoACu = 4096;
 // The pools, in place of AttnPagedArgs' own
 struct AttnQ4Pools {
