@@ -146,7 +146,8 @@ CATENA_DEV PromptItem item_at(const AttnPromptArgs& a, uint32_t index) {
 
 // (the pools as arguments that nothing else points into: the compiler then does not make reads of LDS wait for
 // the loads into it, whose order the barriers below give)
-// kvh0: the kv head, or the first of 8 / unit_waves of a narrow unit's.  put, get: called by all threads with a barrier between, get in front of the last stores, to look ahead
+// kvh0: the kv head, or the first of 8 / unit_waves of a narrow unit's.  put, get: called by all threads with a barrier
+// between, get in front of the last stores, to look ahead
 template <int D, bool PAGED, class Put, class Get>
 CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, uint32_t kvh0, uint32_t unit_waves,
                                  const uint16_t* __restrict__ pool_k, const uint16_t* __restrict__ pool_v,
@@ -442,8 +443,8 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   };
 
   if (narrow) {
-    // Wave w of a unit: blocks of 32 slots w / blocks, + unit_waves / blocks, ...; K and V of one at a time in its own part of LDS, each
-    // asked for as soon as its place has been read
+    // Wave w of a unit: blocks of 32 slots w / blocks, + unit_waves / blocks, ...; K and V of one at a time in its own
+    // part of LDS, each asked for as soon as its place has been read
     constexpr int kBlock = 2 * kAcross;  // loads of a block's K, or V
     const uint32_t step = unit_waves / blocks, all = kvh == kvh_w ? 2 * count : 0u;
     uint16_t* mine = smem + wave * kTile;
