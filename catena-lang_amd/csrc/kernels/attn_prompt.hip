@@ -709,7 +709,7 @@ CATENA_DEV void attn_prompt_run(const AttnPromptArgs& a) {
   const uint32_t narrow_waves = scalar_word(&a.counts->narrow_waves, 0), narrow_heads = kWaves / narrow_waves;
   const uint32_t narrow_groups = (a.kv.kv_heads + narrow_heads - 1) / narrow_heads;
   uint32_t kind = place >= first, ticket = kind ? place - first : place;
-  auto next = [&](uint32_t t) {  // a ticket's work, its item; false: no more of the kind
+  auto next = [&](uint32_t t) {  // a ticket's work; kNone: no more of the kind
     const uint32_t n = t * kPromptQueues + queue;
     return n < (kind ? (items - wide) * narrow_groups : wide * a.kv.kv_heads) ? n : kNone;
   };

@@ -14,7 +14,7 @@
 //
 // Bound: latency: the rows' words, two sums over a workgroup's 1024 rows, a token's row
 // by halving, its page, one after the other.  A step of 64 rows 4.7 us (4.0 on the
-// device), 8192 tokens of 12 prompts 5.7 (5.6); as tensor operations 420.
+// device), 64 prompts among 1024 rows, 131072 places 5.7 (5.6); as tensor operations 420.
 #include "common.h"
 #include "paged.h"
 
