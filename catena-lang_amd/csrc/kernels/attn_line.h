@@ -32,9 +32,10 @@ CATENA_DEV uint32_t tiles_of(uint32_t len) { return (len + (kTileSlots - 1)) / k
 // The work in one line: rows one after the other, a row's units (kv head and 16
 // query heads) one after the other, a unit's tiles in order.
 struct Line {
-  uint32_t tiles;  // in all
-  uint32_t per;    // a workgroup's
-  bool whole;      // not cut: a workgroup takes whole units in turn
+  uint32_t tiles;   // in all
+  uint32_t per;     // a workgroup's
+  uint32_t blocks;  // workgroups that share them out
+  bool whole;       // not cut: a workgroup takes whole units in turn
 };
 // A row on it
 struct RowOnLine {
@@ -96,7 +97,7 @@ CATENA_DEV Line line_of(const AttnPagedArgs& a, const FirstRows& f) {
   }
   uint32_t blocks = all >= kOneACu && a.blocks > 256 && a.kv.head_dim == 128 ? 256 : a.blocks;
   if constexpr (kTwoACu > 0) blocks = all < kTwoACu && blocks > 512 ? 512 : blocks;
-  return Line{all, (all + blocks - 1) / blocks, __all(whole) != 0};
+  return Line{all, (all + blocks - 1) / blocks, blocks, __all(whole) != 0};
 }
 // The row that place `at` of the line (below its end) belongs to
 CATENA_DEV RowOnLine row_at_place(const AttnPagedArgs& a, const FirstRows& f, uint32_t at) {

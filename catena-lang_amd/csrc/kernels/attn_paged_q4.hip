@@ -326,9 +326,10 @@ CATENA_DEV void attn_paged_q4_run(const AttnPagedArgs& a, const AttnQ4Pools& poo
     const Line line = line_of(a, rows);
     whole = line.whole;
     if (!whole) {
-      at = blockIdx.x * line.per;
-      if (at >= line.tiles) return;
-      last = line.tiles - at < line.per ? line.tiles : at + line.per;
+      const Stretch mine = stretch_of(line.tiles, line.per, line.blocks, blockIdx.x);
+      if (mine.beg == mine.end) return;
+      at = mine.beg;
+      last = mine.end;
       const RowOnLine r = row_at_place(a, rows, at);
       now = part_from(a, r.row, r.len, (at - r.first) / r.tiles, (at - r.first) % r.tiles, last - at);
       at += now.end - now.beg;

@@ -106,6 +106,17 @@ struct AttnQ4Pools {
   uint32_t flip;  // the signs of q, so that scale_log2 > 0
 };
 
+// Workgroup `block`'s stretch [beg, end) of a line of tiles (below 2^31), `per` to each of its `blocks` workgroups.  A
+// grid may have more, whose place would pass 32 bits: they have none, beg = end.
+struct Stretch {
+  uint32_t beg, end;
+};
+CATENA_HD Stretch stretch_of(uint32_t tiles, uint32_t per, uint32_t blocks, uint32_t block) {
+  const uint32_t beg = block < blocks ? block * per : tiles;
+  if (beg >= tiles) return Stretch{tiles, tiles};
+  return Stretch{beg, tiles - beg < per ? tiles : beg + per};
+}
+
 // kv_paged.hip: eviction, reordering
 struct EvictArgs {
   PagedKv kv;
