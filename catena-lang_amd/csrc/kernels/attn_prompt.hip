@@ -58,7 +58,7 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kEase = 40.0f;
 constexpr int kWaves = 8;
-constexpr uint32_t kRows = kPromptRows, kNarrow = kPromptNarrow, kWidePlaces = kRows / kNarrow;
+constexpr uint32_t kRows = kPromptRows, kNarrow = kPromptNarrow;
 static_assert(kRows == 32 * kWaves, "a wave's query rows");
 constexpr int kKeys = 64;                // slots of a tile
 constexpr int kStages = 3;               // tiles of K, and of V, in LDS
@@ -663,7 +663,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   l = l + __shfl_xor(l, 32);
   if (!live) return;
   if (it.part != kPromptWhole) {
-    const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh * kWidePlaces) * a.part_rows + wave * 32 + c;
+    const uint64_t at = ((uint64_t)it.part * a.kv.kv_heads + kvh * prompt_places(false)) * a.part_rows + wave * 32 + c;
     if (h == 0) {
       a.part_ml[2 * at] = m;
       a.part_ml[2 * at + 1] = l;
@@ -798,14 +798,9 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
     return Cost{tiles, narrow ? tiles : 2 * tiles, narrow};
   };
   auto alone = [&](uint32_t n) { return n * a.group <= kNarrow; };  // a row of one narrow unit
-  // What a unit costs that is not cut.  A narrow unit's parts have next to nothing to join, and the work ends more
-  // evenly with small ones behind the others.
-  uint32_t most = 0, most_narrow = 0;
-  float share = 0.0f, share_narrow = 0.0f;  // 1 / most
-  auto most_for = [&](const Cost& x) { return x.narrow ? most_narrow : most; };
-  auto parts_of = [&](const Cost& x) {  // (a rounding may make a part a little larger or smaller, the same for all who ask)
-    return x.cost <= most_for(x) ? 1u : (uint32_t)((float)(x.cost - 1) * (x.narrow ? share_narrow : share)) + 1;
-  };
+  PromptCut cut = {};
+  auto most_for = [&](const Cost& x) { return x.narrow ? cut.most_narrow : cut.most; };
+  auto parts_of = [&](const Cost& x) { return prompt_parts(cut, x.cost, x.narrow); };
   // items of a row's units from `unit` on: of the wide units only the last ones are cut
   auto items_from = [&](uint32_t unit, uint32_t units, uint32_t n, int32_t old) {
     uint32_t items = units - unit;
@@ -819,8 +814,8 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
   auto place_of = [&](const Row& r) {
     const Cost last = cost_of(r.units - 1, r.t.n, r.old);
     uint32_t cost = min(last.cost, most_for(last));
-    if (r.units > 1) cost = max(cost, min(cost_of(r.units - 2, r.t.n, r.old).cost, most));
-    const uint32_t from = (uint32_t)((float)(most - cost) * share * (kClasses / 2 - 1));
+    if (r.units > 1) cost = max(cost, min(cost_of(r.units - 2, r.t.n, r.old).cost, cut.most));
+    const uint32_t from = (uint32_t)((float)(cut.most - cost) * cut.share * (kClasses / 2 - 1));
     return atomicAdd(&s_class[from + (alone(r.t.n) ? kClasses / 2 : 0u)], items_from(0, r.units, r.t.n, r.old));
   };
   auto put = [&](uint32_t row, uint32_t place, uint32_t unit, const Cost& cost) {
@@ -830,8 +825,7 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
     const uint32_t at = s_at[place] + items_from(unit + 1, units_of(a, n), n, old);
     PromptItem y{row, unit, s_first[place], n, old, 0, tiles, kPromptWhole};
     if (parts > 1) {
-      const uint32_t places = cost.narrow ? 1u : kWidePlaces;
-      y.part = atomicAdd(&s_parts, parts * places);
+      y.part = atomicAdd(&s_parts, parts * prompt_places(cost.narrow));
       PromptItem z = y;
       z.beg = parts;
       const uint32_t split = atomicAdd(&s_splits, 1u);
@@ -841,7 +835,7 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       y.beg = p * each < tiles ? p * each : tiles;
       y.end = y.beg + each < tiles ? y.beg + each : tiles;
       if (at + p < a.max_items) a.items[at + p] = y;  // (always, but for rows that overlap; so above)
-      if (parts > 1) y.part += cost.narrow ? 1u : kWidePlaces;
+      if (parts > 1) y.part += prompt_places(cost.narrow);
     }
   };
   // Three times (pass: the costs' sum, the classes' sizes, the list) every row to a thread, 1024 at a time, and every
@@ -897,14 +891,7 @@ CATENA_DEV void attn_prompt_list(const AttnPromptArgs& a) {
       if (lane == 0 && mine) atomicAdd(&s_work, (unsigned long long)mine);
       if (lane == 0 && narrow) atomicAdd(&s_narrow, (unsigned long long)narrow);
       __syncthreads();
-      // (a cut unit costs more than the most of its kind, so the parts of all heads are fewer than 2 wide / most + 2
-      // narrow / most_narrow; that is 8 / 3 CUs' places for the wide ones' work, and with most_narrow >= 0.9 most / 4 no
-      // more than 12 for the narrow ones': fewer than kPromptParts)
-      const uint64_t work = s_work * a.kv.kv_heads, even = 3 * work / (4 * kPromptCus) + 1;
-      most = even < kPromptLeast ? kPromptLeast : even < 0x7FFFFFFFull ? (uint32_t)even : 0x7FFFFFFFu;
-      most_narrow = most / 4 < kPromptLeast / 2 ? kPromptLeast / 2 : most / 4;
-      share = 1.0f / (float)most;
-      share_narrow = 1.0f / (float)most_narrow;
+      cut = prompt_cut(s_work * a.kv.kv_heads);
     } else if (pass == 1) {
       if (tid < 64) {
         const uint32_t n = s_class[tid], upto = wave_prefix(n);
@@ -938,7 +925,7 @@ CATENA_DEV void attn_prompt_join(const AttnPromptArgs& a) {
     const PromptItem x = a.splits[split];
     constexpr uint32_t kLanes = D / 4, kAtOnce = 256 / kLanes;
     const uint32_t kvh = blockIdx.y, heads = a.group * a.kv.kv_heads, d = threadIdx.x % kLanes * 4;
-    const uint32_t places = x.n * a.group - x.unit * kRows <= kNarrow ? 1u : kWidePlaces;
+    const uint32_t places = prompt_places(x.n * a.group - x.unit * kRows <= kNarrow);
     for (uint32_t row = blockIdx.z * kAtOnce + threadIdx.x / kLanes; row < kRows; row += gridDim.z * kAtOnce) {
       const uint32_t m_row = x.unit * kRows + row, t = m_row / a.group;
       if (t >= x.n) break;

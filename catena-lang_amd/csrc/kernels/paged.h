@@ -201,6 +201,35 @@ constexpr uint32_t kPromptCus = 256;
 constexpr uint32_t kPromptRows = 256, kPromptNarrow = 64;  // query rows of a unit; of so many a narrow one
 constexpr uint32_t kPromptLeast = 32;              // what a unit costs that is not cut (two a tile of 64 slots)
 constexpr uint32_t kPromptParts = 16 * kPromptCus;  // places of kPromptNarrow query rows for the parts of all kv heads
+// What a unit costs that is not cut, in half tiles for a wide one (its tiles twice) and tiles for a narrow one: three
+// quarters of a CU's share of all the work, a quarter of that for a narrow one, whose parts have next to nothing to join.
+struct PromptCut {
+  uint32_t most, most_narrow;
+  float share, share_narrow;  // 1 / most
+};
+// work: the units' costs of all kv heads
+CATENA_HD PromptCut prompt_cut(uint64_t work) {
+  const uint64_t even = 3 * work / (4 * kPromptCus) + 1;
+  PromptCut c;
+  c.most = even < kPromptLeast ? kPromptLeast : even < 0x7FFFFFFFull ? (uint32_t)even : 0x7FFFFFFFu;
+  c.most_narrow = c.most / 4 < kPromptLeast / 2 ? kPromptLeast / 2 : c.most / 4;
+  c.share = 1.0f / (float)c.most;
+  c.share_narrow = 1.0f / (float)c.most_narrow;
+  return c;
+}
+// (a rounding may make a part a little larger or smaller, the same for all who ask)
+CATENA_HD uint32_t prompt_parts(const PromptCut& c, uint32_t cost, bool narrow) {
+  if (cost <= (narrow ? c.most_narrow : c.most)) return 1;
+  return (uint32_t)((float)(cost - 1) * (narrow ? c.share_narrow : c.share)) + 1;
+}
+// Places that one part takes for each kv head
+CATENA_HD uint32_t prompt_places(bool narrow) { return narrow ? 1 : kPromptRows / kPromptNarrow; }
+// Why kPromptParts places are enough.  A unit that is cut costs more than the most of its kind, so its parts are fewer
+// than 2 cost / most (both up to roundings of 2^-22).  With W the costs of all kv heads, most > 3 W / (4 CUs): wide
+// units take 4 places a part, so fewer than 8 W / most < 32 / 3 a CU; narrow ones one place, and most_narrow >= (most
+// - 3) / 4 >= 29 / 128 most, so fewer than 2 * 128 / 29 W / most < 11.8 a CU.  Whatever the mixture, no more than 12.
+static_assert(kPromptParts >= 12 * kPromptCus && kPromptRows == 4 * kPromptNarrow && kPromptLeast >= 32, "places for parts");
+
 // 256 query rows (unit `unit`) of a row's n new tokens, `old` slots in front of them: tiles [beg, end) of what they
 // see.  In the list of cut units: beg is the number of parts, `part` the first one.
 struct PromptItem {

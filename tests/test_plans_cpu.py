@@ -62,3 +62,62 @@ def test_every_tile_of_a_line_has_one_workgroup(tmp_path):
             args += [tiles, blocks, max(rows * kvh, parts)]
     args += [2 ** 31 - 1, 512, 512, 2 ** 31 - 1, 256, 512, 2 ** 31 - 1, 768, (1 << 24) - 1, 5, 3, 700, 1, 1, 1]
     on_host(tmp_path, STRETCHES, *args)
+
+
+PARTS = """
+    #include <algorithm>
+    #include <random>
+    #include <vector>
+    struct Units {
+      uint32_t cost;
+      bool narrow;
+      uint64_t n;
+    };
+    // parts of all kv heads of all units, at the places that the workspace has
+    bool fits(const std::vector<Units>& units, uint64_t kv_heads) {
+      uint64_t work = 0, places = 0, cut = 0;
+      for (const Units& u : units) work += u.n * u.cost;
+      const PromptCut c = prompt_cut(work * kv_heads);
+      for (const Units& u : units) {
+        const uint64_t parts = prompt_parts(c, u.cost, u.narrow);
+        if (parts < 1 || parts > std::max(1u, u.cost)) return false;
+        if (parts > 1) places += u.n * parts * prompt_places(u.narrow), cut += u.n;
+      }
+      return places * kv_heads <= kPromptParts && cut <= std::max<uint64_t>(1, kPromptParts / 2 / kv_heads);
+    }
+    int main() {
+      std::mt19937_64 r(1);
+      auto log_to = [&](double most) { return (uint64_t)std::exp(std::uniform_real_distribution<double>(0, std::log(most))(r)); };
+      uint64_t most_places = 0;
+      for (int i = 0; i < 300000; ++i) {
+        const uint64_t kv = log_to(512);
+        std::vector<Units> u;
+        for (int kinds = 1 + i % 5; kinds > 0; --kinds) u.push_back({(uint32_t)log_to(1 << 26), r() % 2 == 0, log_to(i % 3 ? 400 : 1 << 23)});
+        if (i % 2) {  // costs that are just above what is not cut
+          uint64_t work = 0;
+          for (const Units& x : u) work += x.n * x.cost;
+          const PromptCut c = prompt_cut(work * kv);
+          for (Units& x : u)  // (a unit has no more than 2^25 tiles)
+            x.cost = (uint32_t)std::min<uint64_t>(1u << 26, (x.narrow ? c.most_narrow : c.most) * (1 + r() % 3) + 1 + r() % 3);
+        }
+        CHECK(fits(u, kv));
+      }
+      // one cost for every number of units: the shares that one unit passes by the least
+      for (uint64_t n = 1; n <= 2100; ++n)
+        for (uint32_t cost = 1; cost < 3000; cost += 1 + cost / 40)
+          for (int narrow = 0; narrow < 2; ++narrow) {
+            CHECK(fits({{cost, narrow != 0, n}}, 1));
+            const PromptCut c = prompt_cut(n * cost);
+            const uint64_t parts = prompt_parts(c, cost, narrow != 0);
+            if (parts > 1) most_places = std::max(most_places, n * parts * prompt_places(narrow != 0));
+          }
+      CHECK(most_places > kPromptParts / 2);  // (so the bound is near)
+      CHECK(fits({{1u << 26, false, 1}}, 65535) && fits({{1u << 26, true, 1u << 23}}, 1));
+      std::puts("ok");
+      return 0;
+    }
+"""
+
+
+def test_parts_of_prompts_have_their_places(tmp_path):
+    on_host(tmp_path, "#include <cmath>\n" + textwrap.dedent(PARTS))
