@@ -40,8 +40,11 @@
 //
 // The maximum is raised only where a score passes it by more than 8 in base 2, by whole
 // numbers, so that what is there is scaled exactly.
-// Range: p enters the products times 2^-40 (and so does the sum, so that it leaves
-// again in the division): sums of finite values never overflow.
+// Range: p enters the products times a power of two (and so does the sum, so that it leaves
+// again in the division) that keeps those of a row's n slots below half the largest |v|:
+// sums of finite values never overflow.  2^-9 / n and not less of it: at the other end
+// products below 2^-126 may be lost, 6 n of them (two terms of p, sums between them), which
+// the division by 2^-10 / n or more makes n^2 2^-113 of o at most; and an infinity's p must not become 0.
 // p is rounded to bf16, as the products take it, and the sum is that of the rounded ones;
 // scores, sums and o are f32.
 // What a query row does not see has p = 0; an infinity or NaN in V there would still
@@ -56,7 +59,6 @@
 namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kEase = 40.0f;
 constexpr int kWaves = 8;
 constexpr uint32_t kRows = kPromptRows, kNarrow = kPromptNarrow;
 static_assert(kRows == 32 * kWaves, "a wave's query rows");
@@ -166,6 +168,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t heads = a.group * a.kv.kv_heads;
   const uint32_t len = (uint32_t)(it.old + (int32_t)it.n);  // slots in use
+  const float ease = (float)(41 - __builtin_clz(len | 1u));   // p's power of two: len of p <= 2^8 stay below 1/2
 
   // The lane's query row.  Up to 64 rows: one or two blocks of 32 (in turn over the waves, which share out the slots).
   const uint32_t rows_left = it.n * a.group - it.unit * kRows, rows = rows_left < kRows ? rows_left : kRows;
@@ -295,8 +298,8 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   }
   const uint32_t whole = upto <= it.beg ? 0u : upto < it.end ? upto - it.beg : count;
 
-  // The query row's exponents' reference point, a whole number (base 2), and from where on a score (in units of the
-  // products) raises it; l of the lane's half of the slots
+  // The query row's exponents' reference point (base 2; a whole number, with ease in it), and from where on a score (in
+  // units of the products) raises it; l of the lane's half of the slots
   float m = kNegInf, limit = kNegInf, l = 0.0f;
   f32x16_t acc[DB];
 #pragma unroll
@@ -331,12 +334,12 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   bf16x8_t pr[2][2];
   float top;
   auto raise = [&](bf16x8_t* pending) {
-    const float t = __builtin_ceilf(__builtin_fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2);
+    const float t = __builtin_ceilf(__builtin_fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2) + ease;
     const float m2 = __builtin_fmaxf(m, t);
     const int down = (int)__builtin_fmaxf(m - m2, -126.0f);  // (nothing is there yet where m is -inf)
     const float f = __uint_as_float((uint32_t)(127 + down) << 23);
     m = m2;
-    limit = (m2 + 8.0f) / a.scale_log2;
+    limit = (m2 + (8.0f - ease)) / a.scale_log2;
     l = l * f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -389,7 +392,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = larger(top, s[i]);
     if (passes()) raise(nullptr);
-    const float base = anchor(m) + kEase;
+    const float base = anchor(m);
     bf16x8_t p[2];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
@@ -559,7 +562,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   auto phase = [&](auto cur_, Block k, Block k_next, Block v, Block v_next) {
     constexpr int cur = cur_.value, nxt = 1 - cur;
     constexpr int kSteps = KS + kV, kEach = (16 + kSteps - 1) / kSteps;  // exponentials a step
-    const float base = anchor(m) + kEase;
+    const float base = anchor(m);
     u32x4_t w[2];
     float even = 0.0f;
 #pragma unroll
@@ -676,7 +679,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         *reinterpret_cast<f32x4_t*>(o + 32 * d + 2 * i) = f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
     return;
   }
-  const float by = 1.0f / (sees > 0 ? l : 1.0f);  // (l: p's sum times 2^-40, from 2^-48 on)
+  const float by = 1.0f / (sees > 0 ? l : 1.0f);  // (l: p's sum times 2^-ease, from 2^-42 on)
   uint16_t* o = a.o + q_at + 4 * h;
 #pragma unroll
   for (int d = 0; d < DB; ++d)

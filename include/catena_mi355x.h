@@ -540,7 +540,9 @@ int catena_mi355x_rope_packed_bf16(const catena_paged_kv_t *kv, const void *qkv,
  * slot gives 0; slots without a page are not seen, and a token whose slots all have none
  * gives NaN.  What lies in slots that a token does not see never reaches it, infinities
  * and NaN included.  Sums of finite values do not overflow (a mean within 2^-8 of the
- * type's largest may).  starts past `tokens` are cut there, rows that end before they
+ * type's largest may); of n slots that a token sees values below n^2 2^-105 lose bits (o is
+ * off by n^2 2^-113 more).  An infinity in v makes o infinite where its p is 2^-60 of the
+ * largest or more; a smaller p may be 0 beside it, which gives NaN.  starts past `tokens` are cut there, rows that end before they
  * begin have no tokens; places of q and o that belong to no row are not touched.
  * No two rows' tokens overlap.  o is not q, k or v.
  * workspace as for catena_mi355x_attn_paged_bf16, of attn_prompt_plan's size, which is
