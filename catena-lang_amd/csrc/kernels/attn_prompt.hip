@@ -45,8 +45,10 @@
 // sums of finite values never overflow.  2^-9 / n and not less of it: at the other end
 // products below 2^-126 may be lost, 6 n of them (two terms of p, sums between them), which
 // the division by 2^-10 / n or more makes n^2 2^-113 of o at most; and an infinity's p must not become 0.
-// p is rounded to bf16, as the products take it, and the sum is that of the rounded ones;
-// scores, sums and o are f32.
+// Rounding: scores, sums and o in f32.  p is rounded to bf16, as the products take it, and
+// the sum is that of the rounded ones.  Narrow units, whose products hide under their loads, take p
+// in two terms, the upper half of its bits and the rest (2^-16 of p), as attention of one
+// token does: a mixed step of chunks and single tokens 238 -> 239 us.
 // What a query row does not see has p = 0; an infinity or NaN in V there would still
 // reach it through the product, so tiles that are not seen whole are searched for
 // them, and where there are any they are taken out of the product and entered by
@@ -357,8 +359,8 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
   };
   auto passes = [&]() { return __any(top > limit) != 0; };
 
-  // A block of 32 slots from `slot` on by itself, in two halves: its scores, and the rest.  check: some rows may not
-  // see all of it.
+  // A block of 32 slots from `slot` on by itself, in two halves: its scores, and the rest.  fine: p in two terms.
+  // check: some rows may not see all of it.
   auto block_scores = [&](lds_char* k, int half) {
     f32x16_t s;
 #pragma unroll
@@ -367,7 +369,8 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int i = 0; i < KS; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(k, half, i), qf[i], s, 0, 0, 0);
     return s;
   };
-  auto block_rest = [&](f32x16_t s, lds_char* v, const uint16_t* v_rows, int half, uint32_t slot, bool check) {
+  auto block_rest = [&](auto fine_, f32x16_t s, lds_char* v, const uint16_t* v_rows, int half, uint32_t slot, bool check) {
+    constexpr bool fine = fine_.value;
     bool odd = false;
     if (check) {
       uint32_t found = 0;
@@ -393,17 +396,29 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int i = 1; i < 16; ++i) top = larger(top, s[i]);
     if (passes()) raise(nullptr);
     const float base = anchor(m);
-    bf16x8_t p[2];
+    bf16x8_t p[2], low[2];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      u32x4_t w;
+      u32x4_t w, r;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i], a.scale_log2, -base)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i + 1], a.scale_log2, -base)));
-        l = add_pair(w[i], l);
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i], a.scale_log2, -base));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + 2 * i + 1], a.scale_log2, -base));
+        if constexpr (fine) {
+          // the upper half, and what it leaves over, which is above 0 where p is (an infinity of V meets both)
+          const uint32_t b0 = __float_as_uint(e0), b1 = __float_as_uint(e1);
+          w[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+          r[i] = pack_bf16x2(__builtin_fmaxf(e0 - __uint_as_float(b0 & 0xFFFF0000u), e0 * 0x1p-20f),
+                             __builtin_fmaxf(e1 - __uint_as_float(b1 & 0xFFFF0000u), e1 * 0x1p-20f));
+          l = l + e0;
+          l = l + e1;
+        } else {
+          w[i] = pack_bf16x2(e0, e1);
+          l = add_pair(w[i], l);
+        }
       }
       p[y] = __builtin_bit_cast(bf16x8_t, w);
+      if constexpr (fine) low[y] = __builtin_bit_cast(bf16x8_t, r);
     }
     // V's values of one kind: the finite ones as they are (0), ones for inf (1), -inf (2), NaN (3)
     auto only = [&](int kind, int d, int x) {
@@ -425,11 +440,18 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int d = 0; d < DB; ++d) {
       if (!odd) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v_frag(v, d, 2 * half + x)), p[x], acc[d], 0, 0, 0);
+        for (int x = 0; x < 2; ++x) {
+          const bf16x8_t y = __builtin_bit_cast(bf16x8_t, v_frag(v, d, 2 * half + x));
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, p[x], acc[d], 0, 0, 0);
+          if constexpr (fine) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, low[x], acc[d], 0, 0, 0);
+        }
       } else {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(only(0, d, x), p[x], acc[d], 0, 0, 0);
+        for (int x = 0; x < 2; ++x) {
+          const bf16x8_t y = only(0, d, x);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, p[x], acc[d], 0, 0, 0);
+          if constexpr (fine) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, low[x], acc[d], 0, 0, 0);
+        }
 #pragma unroll 1
         for (int kind = 1; kind < 4; ++kind) {
           f32x16_t r;
@@ -492,7 +514,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
         __builtin_amdgcn_s_waitcnt(0x0F70);
       fence();
       // (a block inside `upto` tiles is seen by all rows)
-      block_rest(s, v, mine + kTile / 2, 0, slot_of(b), slot_of(b) + 32 > upto * kKeys);
+      block_rest(std::true_type{}, s, v, mine + kTile / 2, 0, slot_of(b), slot_of(b) + 32 > upto * kKeys);
       fence();
       __builtin_amdgcn_s_waitcnt(0xC07F);
       if (more) bring(pair, 1);
@@ -657,7 +679,7 @@ CATENA_DEV void attn_prompt_item(const AttnPromptArgs& a, const PromptItem& it, 
     for (int half = 0; half < 2; ++half) {
       const uint32_t slot = (it.beg + i) * kKeys + 32 * half;
       if ((int32_t)slot < w_most)
-        block_rest(block_scores(k_tile(i), half), v_tile(i), smem + (kStages + i % kStages) * kTile, half, slot, true);
+        block_rest(std::false_type{}, block_scores(k_tile(i), half), v_tile(i), smem + (kStages + i % kStages) * kTile, half, slot, true);
     }
     arrive();
   }

@@ -535,7 +535,9 @@ int catena_mi355x_rope_packed_bf16(const catena_paged_kv_t *kv, const void *qkv,
  * = 1 alone all of them, so prompts, later parts of prompts and single tokens may stand
  * beside each other.  Query head h reads kv head h / (heads / kv_heads).  o[tokens]
  * [heads][head_dim] bf16 RNE: scores, sums and o in f32, p rounded to bf16 (2^-8 of
- * it) in the sum over v and in its own.  The same call gives the same bits; where long
+ * it) in the sum over v and in its own; as catena_mi355x_attn_paged_bf16 has it, to
+ * 2^-16, where a row's n tokens are up to 64 query rows of a kv head (n * heads / kv_heads),
+ * or the last of them up to 64 behind a multiple of 256.  The same call gives the same bits; where long
  * rows are cut, a row's last bits depend on the rows beside it.  A token that sees no
  * slot gives 0; slots without a page are not seen, and a token whose slots all have none
  * gives NaN.  What lies in slots that a token does not see never reaches it, infinities
