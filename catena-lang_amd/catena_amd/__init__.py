@@ -621,7 +621,8 @@ def rope_packed_bf16(kv: PagedKV, qkv, qkv_f32: bool, rope_tab, table_positions:
 def rope_packed_q4(kv: PagedKV4, qkv, qkv_f32: bool, rope_tab, table_positions: int, rotary_dim: int,
                    interleaved: bool, token_pos, slot_map, q, tokens: int, heads: int, k_out=None,
                    v_out=None) -> None:
-    """rope_packed_bf16 into a cache in 4 bits; k_out / v_out: the values that it then holds."""
+    """rope_packed_bf16 into a cache in 4 bits; k_out / v_out: the values that it then
+    holds (v's rounded to bf16)."""
     check(lib().catena_mi355x_rope_packed_q4(kv, qkv, 1 if qkv_f32 else 0, rope_tab, table_positions,
                                              rotary_dim, 1 if interleaved else 0, token_pos, slot_map, q,
                                              tokens, heads, k_out, v_out))

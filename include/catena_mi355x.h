@@ -598,8 +598,11 @@ typedef struct catena_paged_kv4 {
  * codes: a block of keys counts the smallest power of two, 2^-127 at least, of which
  * its largest |x| is at most 6; a head's values count a sixth of their largest |x|,
  * rounded up to bf16; each code is the nearest, of two the even one.  A block with an
- * infinity or NaN becomes NaN.  k_out and v_out are the values that the codes stand for
- * (v's rounded to bf16), so that a prompt attends to what later steps will.
+ * infinity or NaN becomes NaN (and |k| above 3.5 * 2^126 counts 2^128, which bf16 does not
+ * hold: an infinity in k_out).  k_out and v_out are the values that the codes stand for, so that a prompt
+ * attends to what later steps will: k's exactly, v's, products of a code and a bf16
+ * scale, rounded to bf16 (2^-8 of them at most; catena_mi355x_attn_paged_q4 takes them
+ * whole).
  * kv_heads <= 128. */
 int catena_mi355x_rope_packed_q4(const catena_paged_kv4_t *kv, const void *qkv, int qkv_f32,
                                  const float *rope_tab, uint32_t table_positions,
