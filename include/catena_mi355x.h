@@ -452,8 +452,14 @@ int catena_mi355x_beam_reorder_paged_bf16(const catena_paged_kv_t *kv, uint16_t 
  * tokens asked for by the rows up to it are at most max_tokens, and it needs no page
  * or the pages asked for by the rows up to it are at most *free_count.  So the rows
  * that are refused are behind the admitted ones (but for rows that ask for no page, or
- * do not fit the table), and take nothing.  Admitted rows enter their pages into the table behind those that
- * they hold, the lowest row from the top of the stack.
+ * do not fit the table), and take nothing.  What a refused row asks for stays in the sums: one
+ * that asks for more pages than are free stops all rows behind it that need a page,
+ * step after step, until it asks for less; one that asks for more tokens than are left, all
+ * rows behind it that ask for any.  So requests that have begun stand in front of those
+ * that wait, or a want that is not met is taken back: starts[rows] below the sum
+ * of want says that there is one, lens_out[r] == lens[r] with want[r] > 0 which.
+ * Admitted rows enter their pages into the table behind those that they hold, the lowest row
+ * from the top of the stack.
  * Writes lens_out, held_out (both [rows]), starts[rows + 1], *free_count_out, and for
  * each of the max_tokens places of the list its position token_pos and its slot
  * slot_map = page * page_size + place in the page: token t of row r has position
