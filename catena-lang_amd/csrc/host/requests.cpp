@@ -40,7 +40,9 @@ int rope_packed_check(uint32_t kv_heads, uint32_t dim, const void* qkv, const fl
     return fail(CATENA_ERR_UNSUPPORTED, "rotary_dim %u is not a multiple of 16 up to head_dim %u", rot, dim);
   if ((k_out != nullptr) != (v_out != nullptr))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "copies of keys and values come together");
-  if (tokens > grid_most(256) || (uint64_t)heads + 2ull * kv_heads > 0xFFFFFFFFull / 8)
+  // (a workgroup's threads take runs of 16 values of a token in turn, up to 8 a head: their number, with a turn
+  // past it, stay below 2^32)
+  if (tokens > grid_most(256) || (uint64_t)heads + 2ull * kv_heads > (0xFFFFFFFFull - 256) / 8)
     return fail(CATENA_ERR_UNSUPPORTED, "packed rotation too large");
   if (tokens == 0) return CATENA_OK;
   if (!qkv || !rope_tab || !token_pos || !q) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");

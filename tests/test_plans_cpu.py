@@ -4,8 +4,12 @@ import os
 import subprocess
 import textwrap
 
+import pytest
+
 import catena_amd as ca
-from test_requests_cpu import geometry4
+from paged_util import geometry, refused
+from test_paged_cpu import UNSUPPORTED
+from test_requests_cpu import geometry4, rope
 
 KERNELS = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "catena-lang_amd", "csrc", "kernels")
 HEAD = """
@@ -121,3 +125,14 @@ PARTS = """
 
 def test_parts_of_prompts_have_their_places(tmp_path):
     on_host(tmp_path, "#include <cmath>\n" + textwrap.dedent(PARTS))
+
+
+@pytest.mark.parametrize("kv", [geometry(kv_heads=1), geometry4(kv_heads=1)])
+def test_rotation_counts_in_32_bits(kv):
+    """Threads go through a token's (heads + 2) * 8 runs of 16 values 256 apart: the number that ends
+    the walk may not lie within 256 of 2^32, where the walk would begin again."""
+    most = (2 ** 32 - 1 - 256) // 8 - 2
+    assert (most + 2) * 8 + 256 < 2 ** 32
+    for heads in (most + 1, 2 ** 29 - 3, 2 ** 32 - 1):
+        refused(UNSUPPORTED, rope, kv, heads=heads)
+    rope(kv, heads=most, tokens=0)
