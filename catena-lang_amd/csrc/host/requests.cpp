@@ -172,7 +172,9 @@ int catena_mi355x_kv_release_paged(const catena_paged_kv_t* kv, uint32_t* table,
   PagedKv c;
   const int st = paged_check(kv, false, &c);
   if (st) return st;
-  if (c.rows > 0x7FFFFFFFu) return fail(CATENA_ERR_UNSUPPORTED, "too many rows");
+  // (the pages given back are counted in 32 bits)
+  if (c.rows > 0x7FFFFFFFu || (uint64_t)c.rows * c.max_pages > 0xFFFFFFFFull)
+    return fail(CATENA_ERR_UNSUPPORTED, "too many rows and pages");
   if (!free_count || !free_count_out) return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");
   if (c.rows > 0 && (!table || !lens || !held || !finished || !free_pages || !lens_out || !held_out))
     return fail(CATENA_ERR_INVALID_ARGUMENT, "null operand");

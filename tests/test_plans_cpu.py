@@ -8,8 +8,8 @@ import pytest
 
 import catena_amd as ca
 from paged_util import geometry, refused
-from test_paged_cpu import UNSUPPORTED
-from test_requests_cpu import geometry4, rope
+from test_paged_cpu import INVALID, UNSUPPORTED
+from test_requests_cpu import geometry4, release, rope
 
 KERNELS = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "catena-lang_amd", "csrc", "kernels")
 HEAD = """
@@ -136,3 +136,11 @@ def test_rotation_counts_in_32_bits(kv):
     for heads in (most + 1, 2 ** 29 - 3, 2 ** 32 - 1):
         refused(UNSUPPORTED, rope, kv, heads=heads)
     rope(kv, heads=most, tokens=0)
+
+
+def test_release_counts_pages_in_32_bits():
+    """A table of 2^32 entries or more could give back more pages than its sums hold, and entries
+    behind them would stay."""
+    for rows, pages in ((1 << 20, 1 << 12), (1 << 12, 1 << 20), (1 << 31, 16)):
+        refused(UNSUPPORTED, release, geometry(rows=rows, max_pages=pages))
+    refused(INVALID, release, geometry(rows=1 << 20, max_pages=(1 << 12) - 1), held=0)  # not for its size
