@@ -144,3 +144,35 @@ def test_release_counts_pages_in_32_bits():
     for rows, pages in ((1 << 20, 1 << 12), (1 << 12, 1 << 20), (1 << 31, 16)):
         refused(UNSUPPORTED, release, geometry(rows=rows, max_pages=pages))
     refused(INVALID, release, geometry(rows=1 << 20, max_pages=(1 << 12) - 1), held=0)  # not for its size
+
+
+def _prompt_bytes(rows, tokens, heads, kvh, dim, slots):
+    """What prompt attention's list and parts take, in whole numbers of any size; None: refused."""
+    group = heads // kvh
+    units = tokens * group // 256 + min(rows, tokens)  # 256 query rows each, a row's last one any number
+    if tokens * group > 2 ** 31 - 1 or units * kvh > (2 ** 32 - 1) // 512:
+        return None
+    if slots <= 1024 and units <= 256:
+        return 0
+    places, at_once = 4096, min(64, tokens * group)
+    return 128 + 32 * (units + places) + 32 * min(units, max(1, places // 2 // kvh)) + places * at_once * (8 + 4 * dim)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_plans_up_to_the_largest_sizes(dim):
+    sizes = [(1, 2 ** 31 - 1, 1, 1), (1, 2 ** 31, 1, 1), (1, 2 ** 30, 2, 1), (1, 2 ** 30 - 1, 2, 1), (2 ** 31 - 1, 2 ** 23, 1, 1),
+             (2 ** 31 - 1, 2 ** 23 - 2 ** 16, 1, 1), (1, 1, 65535, 65535), (128, 256, 65535, 65535), (126, 256, 65535, 65535),
+             (8, 2 ** 28 - 1, 64, 8), (1000, 10 ** 6, 128, 8), (5, 3, 7, 7), (300, 300, 16, 8), (1, 12000, 32, 8)]
+    for rows, tokens, heads, kvh in sizes:
+        for max_pages in (1, 64, 65, 2 ** 27 - 1):
+            kv = geometry(rows=rows, kv_heads=kvh, head_dim=dim, max_pages=max_pages, page_size=16)
+            want = _prompt_bytes(rows, tokens, heads, kvh, dim, 16 * max_pages)
+            if tokens == 2 ** 31 or want is None:
+                refused(UNSUPPORTED, ca.attn_prompt_plan, kv, tokens, heads)
+            else:
+                assert ca.attn_prompt_plan(kv, tokens, heads) == want, (rows, tokens, heads, kvh, max_pages)
+        want = _prompt_bytes(rows, tokens, heads, kvh, dim, tokens)
+        if tokens == 2 ** 31 or want is None:
+            refused(UNSUPPORTED, ca.attn_packed_plan, rows, tokens, heads, kvh, dim)
+        else:
+            assert ca.attn_packed_plan(rows, tokens, heads, kvh, dim) == want
