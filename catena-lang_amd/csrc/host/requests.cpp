@@ -73,7 +73,8 @@ int prompt_plan(uint32_t rows, uint64_t tokens, uint32_t heads, uint32_t kv_head
   p->units = (uint32_t)units;
   // A list costs two more launches, and spares every workgroup of many the search for its unit: rows that may have no
   // more than 1024 slots, direct / listed, us: 8 prompts of up to 500 tokens 48 / 61, 32 of them 147 / 150, 6 beside 250
-  // single tokens 116 / 90; single tokens, 256 of them 109 / 68, 1024 454 / 204, 4096 2427 / 503.
+  // single tokens 116 / 90; single tokens, 256 of them 109 / 68, 1024 454 / 204, 4096 2427 / 503 (all with p in one term, 1 to 2 % less
+  // than single tokens take in two).
   p->list = slots > 1024 || units > 256;
   p->bytes = 0;
   if (!p->list) return CATENA_OK;

@@ -6,10 +6,11 @@
 // as attn_paged.hip has it for bf16: the same line of tiles, parts and join.
 //
 // Bound: the cache is read once, D + D / 32 + 2 bytes per (slot, kv head), so HBM, beside
-// about 1000 vector instructions of a wave for 128 slots of 128 columns, which keep the
-// SIMDs busy 40 % of the time.  64 rows x 4096 slots x 8 kv heads of 128 take 57 us (281
-// MB, 4.9 TB/s), 64 of 1 .. 8192 70 to 75 (as bf16 pages 88 for half the slots), one row of
-// 131072 of 64 columns 25 (6 the join), one of 640 and 16 heads 9.
+// about 1000 vector instructions of a wave for 128 slots of 128 columns (15800 a SIMD
+// in 121000 cycles of a ragged batch, half of its time by the counter of active ones).  64 rows x
+// 4096 slots x 8 kv heads of 128 take 57 us (281 MB, 4.9 TB/s), 64 of 1 .. 8192 62 to 75 by the lengths (as
+// bf16 pages 88 for half the slots), one row of 131072 of 64 columns 25 (6 the join), one of
+// 640 and 16 heads 9 to 10.
 //
 // A wave takes 128 slots at a time, its lane group g (lanes 16 g ..) slots 32 g ..
 // 32 g + 31 of them.

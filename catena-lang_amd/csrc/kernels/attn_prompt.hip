@@ -5,11 +5,13 @@
 //   s_j = scale * q . k_j,  o = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)
 //
 // Bound: the matrix cores: 4 D flop for each (query head, slot seen), against 4 D
-// bytes a slot and kv head that 256 query rows share.  They run at the chip's power limit:
-// 12000 tokens x 32 heads of 128 1000 to 1060 us (1.04 to 1.10 PFLOP/s; a large matrix
-// product of random values 1.2 to 1.36 on the same cards), 8 ragged prompts of up to
-// 4096 tokens 597 for 5.5e11 flop; 4 chunks of 500 tokens and 28 single ones over 8000
-// slots or fewer 230 (0.56 GB and 1.4e11 flop); 5 prompts of up to 130 tokens 7.7.
+// bytes a slot and kv head that 256 query rows share.  They run at the chip's power limit
+// (1.6 GHz of 2.4, matrix instructions in 55 % of the cycles): 11250 to 12000 tokens x 32 heads
+// of 128 980 to 1077 us (1.07 PFLOP/s; a large matrix product of random values 1.2 to 1.36 on
+// the same cards), 8 ragged prompts of 1024 to 4096 tokens 440 to 700 by their lengths (1.38 to
+// 1.49 times the operations' time at 1.31 PFLOP/s); 4 chunks of 469 to 500 tokens and 28
+// single ones over up to 8000 slots 203 to 314, half of them above 259 (2.0 to 2.5 times the
+// larger of operations and bytes); 5 prompts of up to 130 tokens 7.8 to 9.8.
 //
 // A workgroup takes 256 query rows of one row and kv head (a unit): query row m is token
 // m / group, head m % group of the kv head's, so that short sequences with grouped heads
@@ -31,7 +33,8 @@
 // takes four kv heads' at a time, since what a unit costs besides its loads is latency
 // (8 kv heads, 256 single tokens behind up to 400 slots 106 us with eight waves, 68 with
 // two, behind up to 4000 407 / 400; of fewer units the larger items end unevenly: 130
-// tokens behind up to 4000 251 us with eight waves, 281 with four).
+// tokens behind up to 4000 251 us with eight waves, 281 with four; p in one term, which was 1
+// to 2 % less than in two).
 //
 // Units are dealt out in one of two ways.  Few short ones: a workgroup each, which finds
 // it from the rows' lengths.  Else a kernel before lists them by length, long ones first,
@@ -48,7 +51,9 @@
 // Rounding: scores, sums and o in f32.  p is rounded to bf16, as the products take it, and
 // the sum is that of the rounded ones.  Narrow units, whose products hide under their loads, take p
 // in two terms, the upper half of its bits and the rest (2^-16 of p), as attention of one
-// token does: a mixed step of chunks and single tokens 238 -> 239 us.
+// token does (256 single tokens 68.8 -> 70.2 us, a mixed step 238 -> 239).  Wide ones would
+// take 1.45 times as long (12000 tokens 1102 -> 1611 us, with heads of 64 695 -> 1039), for o off by 1.6e-3
+// of itself instead of 2.2e-3, of which its own rounding is 1.6e-3.
 // What a query row does not see has p = 0; an infinity or NaN in V there would still
 // reach it through the product, so tiles that are not seen whole are searched for
 // them, and where there are any they are taken out of the product and entered by

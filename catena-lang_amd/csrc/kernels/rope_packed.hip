@@ -21,8 +21,9 @@
 // that a pair meets in one thread and both its halves are loads of 16 bytes.  Into 4 bits
 // a thread then takes 8 values from LDS (16, with half of the threads idle: 62 us).
 // 32 + 2 x 8 heads of 128, 8192 tokens: f32 in, bf16 pages 55 us (303 MB, 5.5 TB/s; 60
-// without the loads ahead), bf16 in, 4-bit pages and copies 56 us (211 MB, 3.8 TB/s: v's
-// bytes go out one by one); 56 tokens 4.7 us, of which 3.7 on the device.
+// without the loads ahead), bf16 in, 4-bit pages and copies 55 us (211 MB, 3.8 TB/s: v's
+// bytes go out one by one, and 140 MB are written for 110); 56 tokens 4.7 us, of which 3.9 on
+// the device.
 #include "common.h"
 #include "paged.h"
 

@@ -554,7 +554,9 @@ int catena_mi355x_rope_packed_bf16(const catena_paged_kv_t *kv, const void *qkv,
  * begin have no tokens; places of q and o that belong to no row are not touched.
  * No two rows' tokens overlap.  o is not q, k or v.
  * workspace as for catena_mi355x_attn_paged_bf16, of attn_prompt_plan's size, which is
- * a function of the sizes alone and needs no device.  q and o 16-byte aligned.
+ * a function of the sizes alone and needs no device (0 for few tokens over tables of up to
+ * 1024 slots, else up to 136 MB at 128 columns, 69 at 64, and 64 bytes for every row and
+ * 256 query rows).  q and o 16-byte aligned.
  * Allocates nothing; may be captured.  No reference counterpart. */
 int catena_mi355x_attn_prompt_plan(const catena_paged_kv_t *kv, uint64_t tokens, uint32_t heads,
                                    uint64_t *workspace_bytes);
